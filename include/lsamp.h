@@ -597,6 +597,187 @@ typedef struct lsamp_mask_assemble_args {
 lsamp_status lsamp_mask_assemble(lsamp_context* ctx, const lsamp_mask_assemble_args* args,
                                  void* stream);
 
+/* ---- the hidden-state side of the stage -----------------------------------
+ * What runs in front of the logits and what trains it: the linear blocks of a
+ * draft head, the vocabulary head's logits, its cross entropy straight from
+ * the hidden states, their gradients, and dropout.  The reference trains and
+ * runs these through MLX's Linear, crossEntropy and Dropout layers.
+ *
+ * Every matrix is rows of elements of `dtype` with its own distance between
+ * rows (`*_stride`, in elements); any distance and any element-aligned address
+ * is taken.  Products run on the matrix cores with float32 sums.  Rows that do
+ * not start at multiples of 16 bytes, or whose length is no multiple of 16
+ * bytes, are first copied to the workspace by the call.
+ *
+ * `workspace` is device memory of at least the bytes that the matching
+ * *_workspace function returns for the same arguments (its pointers included:
+ * their alignment counts), aligned to 256 bytes; its contents are scratch.
+ * A workspace function returns 0 where none is needed and a negative status
+ * for arguments that the call would refuse (last-error string set).
+ * Outputs may not overlap inputs, except that `out` may be the residual
+ * itself (same address and stride), and a dropout's `out` its `x`.  The calls
+ * use no other state, are ordered by their stream only, allocate nothing and
+ * may be captured into a HIP graph. */
+typedef enum lsamp_activation {
+  LSAMP_ACT_NONE = 0,
+  LSAMP_ACT_RELU = 1,
+  LSAMP_ACT_SILU = 2,      /* z / (1 + exp(-z))                                  */
+  LSAMP_ACT_GELU = 3,      /* z (1 + erf(z / sqrt 2)) / 2                        */
+  LSAMP_ACT_GELU_TANH = 4, /* its tanh form                                      */
+  LSAMP_ACT_SOFTCAP = 5    /* softcap * tanh(z / softcap)                        */
+} lsamp_activation;
+
+/* out = act(x weight^T + bias) + residual. */
+typedef struct lsamp_linear_args {
+  int32_t rows;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;      /* lsamp_dtype of x, weight, bias, residual                */
+  int32_t activation; /* lsamp_activation                                        */
+  float softcap;      /* > 0 with LSAMP_ACT_SOFTCAP, else ignored                */
+  int32_t out_dtype;  /* dtype, or LSAMP_DTYPE_F32                               */
+  const void* x;      /* [rows, in_features]                                     */
+  int64_t x_stride;
+  const void* weight; /* [out_features, in_features]                             */
+  int64_t weight_stride;
+  const void* bias;   /* [out_features] or NULL                                  */
+  const void* residual; /* [rows, out_features] or NULL                          */
+  int64_t residual_stride;
+  void* out;          /* [rows, out_features] of out_dtype                       */
+  int64_t out_stride;
+  float* pre;         /* [rows, out_features] float32 out or NULL: x weight^T +
+                         bias, which lsamp_linear_backward reads                 */
+  int64_t pre_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_linear_args;
+
+int64_t lsamp_linear_workspace(const lsamp_linear_args* args);
+lsamp_status lsamp_linear(lsamp_context* ctx, const lsamp_linear_args* args, void* stream);
+
+/* The gradients of lsamp_linear.  With dz = d_out * act'(pre), rounded to
+ * `dtype` for the two products (float32 stays as it is):
+ *   d_x = dz weight,  d_weight = dz^T x,  d_bias = column sums of dz.
+ * The residual's gradient is d_out itself. */
+typedef struct lsamp_linear_backward_args {
+  int32_t rows;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;      /* of every matrix but `pre`                               */
+  int32_t activation;
+  float softcap;
+  const void* x;      /* [rows, in_features]; needed for d_weight                */
+  int64_t x_stride;
+  const void* weight; /* [out_features, in_features]; needed for d_x             */
+  int64_t weight_stride;
+  const float* pre;   /* [rows, out_features] from lsamp_linear; not needed
+                         with LSAMP_ACT_NONE                                     */
+  int64_t pre_stride;
+  const void* d_out;  /* [rows, out_features]                                    */
+  int64_t d_out_stride;
+  void* d_x;          /* [rows, in_features] out or NULL                         */
+  int64_t d_x_stride;
+  void* d_weight;     /* [out_features, in_features] out or NULL                 */
+  int64_t d_weight_stride;
+  void* d_bias;       /* [out_features] out or NULL                              */
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_linear_backward_args;
+
+int64_t lsamp_linear_backward_workspace(const lsamp_linear_backward_args* args);
+lsamp_status lsamp_linear_backward(lsamp_context* ctx, const lsamp_linear_backward_args* args,
+                                   void* stream);
+
+/* The vocabulary head's cross entropy, without its logits in memory:
+ *   z = softcap(x weight^T + bias)  (softcap 0: none)
+ *   lse[r] = log sum_v exp(z[r][v]);  loss[r] = lse[r] - z[r][targets[r]].
+ * A row with a negative target is ignored: its loss is 0 (its lse is written).
+ * A bias of -inf takes an id out of the vocabulary.  A target >= vocab, or a
+ * row whose logits are all -inf, gives a NaN loss, a flag
+ * (LSAMP_ROW_TOKEN_RANGE, LSAMP_ROW_EMPTY) and no gradient; NaN or +inf logits
+ * give NaN and LSAMP_ROW_NONFINITE. */
+typedef struct lsamp_head_loss_args {
+  int32_t rows;
+  int32_t hidden;
+  int32_t vocab;
+  int32_t dtype;      /* of x, weight and bias                                   */
+  float softcap;      /* 0: none                                                 */
+  const void* x;      /* [rows, hidden]                                          */
+  int64_t x_stride;
+  const void* weight; /* [vocab, hidden]                                         */
+  int64_t weight_stride;
+  const void* bias;   /* [vocab] or NULL                                         */
+  const int32_t* targets; /* [rows]                                              */
+  float* loss;        /* [rows] out                                              */
+  float* lse;         /* [rows] out                                              */
+  uint32_t* row_flags; /* [rows] out or NULL                                     */
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_head_loss_args;
+
+int64_t lsamp_head_loss_workspace(const lsamp_head_loss_args* args);
+lsamp_status lsamp_head_loss(lsamp_context* ctx, const lsamp_head_loss_args* args, void* stream);
+
+/* Its gradients: with g[r][v] = d_loss[r] (exp(z[r][v] - lse[r]) - [v ==
+ * targets[r]]) softcap'(...), computed again from x and weight a piece of the
+ * vocabulary at a time and rounded to `dtype` for the two products,
+ *   d_x = g weight,  d_weight = g^T x,  d_bias = column sums of g.
+ * The workspace holds one piece of g (about 128 MiB) and the float32 sums of
+ * d_x. */
+typedef struct lsamp_head_loss_backward_args {
+  int32_t rows;
+  int32_t hidden;
+  int32_t vocab;
+  int32_t dtype;
+  float softcap;
+  const void* x;
+  int64_t x_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;
+  const int32_t* targets;
+  const float* lse;    /* [rows] from lsamp_head_loss                            */
+  const float* d_loss; /* [rows] the loss's gradient (1 / rows for a mean)       */
+  void* d_x;           /* [rows, hidden] out or NULL                             */
+  int64_t d_x_stride;
+  void* d_weight;      /* [vocab, hidden] out or NULL                            */
+  int64_t d_weight_stride;
+  void* d_bias;        /* [vocab] out or NULL                                    */
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_head_loss_backward_args;
+
+int64_t lsamp_head_loss_backward_workspace(const lsamp_head_loss_backward_args* args);
+lsamp_status lsamp_head_loss_backward(lsamp_context* ctx,
+                                      const lsamp_head_loss_backward_args* args, void* stream);
+
+/* Dropout whose mask is a function of (key, offset, row, column) and is never
+ * stored:
+ *   out = residual + (keep ? x / (1 - p') : 0),  p' = round(p 2^16) / 2^16.
+ * keep: 16 bits of Philox4x32-10 (Salmon et al., SC'11) are at least p' 2^16.
+ * Counter {column / 8, row, lo32(offset'), hi32(offset')}, key {lo32(key),
+ * hi32(key)}, offset' = offset + *step; element j = column % 8 takes bits
+ * 16 (j % 2) .. of word j / 2.  The backward pass is the same call on the
+ * gradient, without a residual.  A dropped element's x is not used. */
+typedef struct lsamp_dropout_args {
+  int32_t rows;
+  int32_t cols;
+  int32_t dtype;
+  float p;              /* [0, 1]                                                */
+  uint64_t key;
+  uint64_t offset;      /* another value for every layer and step                */
+  const uint64_t* step; /* device, or NULL: added to `offset` (a captured graph's
+                           counter)                                              */
+  const void* x;        /* [rows, cols]                                          */
+  int64_t x_stride;
+  const void* residual; /* [rows, cols] or NULL                                  */
+  int64_t residual_stride;
+  void* out;            /* [rows, cols]                                          */
+  int64_t out_stride;
+} lsamp_dropout_args;
+
+lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* args, void* stream);
+
 /* ---- host-side parameter resolution (no device work) ---------------------- */
 
 /* GenerateParameters subset that drives the mlx-lm sampler/processor factory

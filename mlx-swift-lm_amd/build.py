@@ -39,12 +39,13 @@ DEVICE = [
     "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-# compiled once per logits dtype (LSAMP_DT = 0, 1, 2), in parallel
-SOURCES_HIP_DT = ["lsamp_kernels.hip"]
+# compiled once per element type (LSAMP_DT = 0, 1, 2), in parallel
+SOURCES_HIP_DT = ["lsamp_kernels.hip", "lsamp_head.hip"]
 SOURCES_HIP = ["lsamp_topk.hip", "lsamp_rank.hip", "lsamp_commit.hip",
-               "lsamp_mask.hip", "lsamp_noalloc.hip", "lsamp_penalize.hip"]
-SOURCES_CPP = ["lsamp_api.cpp"]
-HEADERS = ["lsamp_internal.h", "lsamp_device.h"]
+               "lsamp_mask.hip", "lsamp_noalloc.hip", "lsamp_penalize.hip",
+               "lsamp_head_passes.hip", "lsamp_dropout.hip"]
+SOURCES_CPP = ["lsamp_api.cpp", "lsamp_head_api.cpp"]
+HEADERS = ["lsamp_internal.h", "lsamp_device.h", "lsamp_head.h", "lsamp_gemm.h"]
 
 
 def run(cmd):

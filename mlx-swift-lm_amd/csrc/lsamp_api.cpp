@@ -132,6 +132,8 @@ struct lsamp_context {
   } mstage;
 };
 
+int32_t lsamp::context_device(const lsamp_context* ctx) { return ctx->device; }
+
 namespace {
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -486,6 +488,13 @@ int64_t lsamp_abi_sizeof(const char* name) {
   if (!strcmp(name, "lsamp_mask_assemble_args")) return (int64_t)sizeof(lsamp_mask_assemble_args);
   if (!strcmp(name, "lsamp_logprobs_args")) return (int64_t)sizeof(lsamp_logprobs_args);
   if (!strcmp(name, "lsamp_penalize_args")) return (int64_t)sizeof(lsamp_penalize_args);
+  if (!strcmp(name, "lsamp_linear_args")) return (int64_t)sizeof(lsamp_linear_args);
+  if (!strcmp(name, "lsamp_linear_backward_args"))
+    return (int64_t)sizeof(lsamp_linear_backward_args);
+  if (!strcmp(name, "lsamp_head_loss_args")) return (int64_t)sizeof(lsamp_head_loss_args);
+  if (!strcmp(name, "lsamp_head_loss_backward_args"))
+    return (int64_t)sizeof(lsamp_head_loss_backward_args);
+  if (!strcmp(name, "lsamp_dropout_args")) return (int64_t)sizeof(lsamp_dropout_args);
   return -1;
 }
 

@@ -1,0 +1,159 @@
+// lsamp_head.h — plans of the hidden-state operators (linear blocks, the
+// vocabulary head's loss, dropout) shared by the C entry points, which build
+// them, and the kernels, which run them.
+#ifndef LSAMP_HEAD_H
+#define LSAMP_HEAD_H
+
+#include <stdint.h>
+
+#include "../../include/lsamp.h"
+
+namespace lsamp {
+
+// A matrix in HBM: `rows` rows of `cols` readable elements, `ld` elements
+// apart.  Products read 16-byte chunks: p and ld in bytes are multiples of 16,
+// cols of a chunk's elements.
+struct MatrixRef {
+  const void* p;
+  int64_t ld;
+  int32_t rows, cols;
+};
+
+struct GemmPlan {
+  MatrixRef a, b;
+  int32_t tiles_m, tiles_n, parts;
+  int32_t slabs, slabs_per_part;  // 128-byte slabs of the reduction
+};
+
+// Which operand is read along the reduction's rows (lsamp_gemm.h).
+enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
+// Tile shapes: 256 x 256, 128 x 128, 64 x 64.
+enum GemmTile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTiles = 3 };
+constexpr int kTileSide[kTiles] = {256, 128, 64};
+
+// Epilogues.  `m`, `n`: rows and columns that exist; `vec`: rows of every
+// matrix start at multiples of four elements, so four columns move at once.
+struct EpiLinear {
+  int32_t m, n;
+  int32_t activation, vec, wide;  // wide: out is float32
+  float softcap;
+  const void* bias;
+  const void* residual;
+  int64_t ld_residual;
+  void* out;
+  int64_t ld_out;
+  float* pre;
+  int64_t ld_pre;
+};
+struct EpiStore {  // out = sums * *scale, in the operands' type
+  int32_t m, n;
+  int32_t vec;
+  void* out;
+  int64_t ld_out;
+  const float* scale;  // device, or NULL for 1
+};
+struct EpiPartial {  // float32 sums of one part, added to what is there
+  int32_t m, n;
+  int32_t accumulate;
+  float* out;
+  int64_t ld;           // a multiple of 4
+  int64_t part_stride;
+};
+struct EpiStats {  // a tile's maximum and sum of exponentials of every row
+  int32_t m, n;
+  int32_t first_col, blocks, first_block;
+  float softcap;
+  const void* bias;
+  const int32_t* targets;
+  float* part;    // [m][blocks][2]
+  float* target;  // [m] the target's logit
+};
+struct EpiGrad {  // the loss's gradient at a piece of the logits
+  int32_t m, n;
+  int32_t first_col, n_pad;  // columns n .. n_pad - 1 are written as zero
+  float softcap;
+  const void* bias;
+  const int32_t* targets;
+  int32_t vocab;
+  const float* lse;
+  const float* d_loss;
+  const float* scale;  // [2] device: what the stored values are multiplied by, and its inverse
+  void* out;
+  int64_t ld_out;
+};
+
+struct PackPlan {  // rows copied to 16-byte aligned rows, zeros up to dst_cols
+  const void* src;
+  int64_t src_ld;
+  void* dst;
+  int64_t dst_ld;
+  int32_t rows, cols, dst_cols;
+};
+
+struct JoinStatsPlan {
+  int32_t rows, blocks, vocab;
+  const float* part;
+  const float* target;
+  const int32_t* targets;
+  float* loss;
+  float* lse;
+  uint32_t* row_flags;
+};
+
+struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial sum
+  int32_t rows, cols;
+  int32_t chunks, rows_per_chunk;
+  int32_t activation, vec;  // with `pre`: in * activation'(pre) is summed, and written to out
+  float softcap;
+  const void* in;
+  int64_t ld_in;
+  const float* pre;
+  int64_t ld_pre;
+  void* out;
+  int64_t ld_out;
+  int32_t out_cols;  // columns cols .. out_cols - 1 of out are written as zero
+  float* part;       // [chunks][ld_part], or NULL
+  int64_t ld_part;
+};
+
+struct DropoutPlan {
+  int32_t rows, cols;
+  uint32_t cut;  // an element is kept where its 16 bits are at least this
+  int32_t vec;
+  float scale;
+  uint64_t key, offset;
+  const uint64_t* step;
+  const void* x;
+  int64_t ld_x;
+  const void* residual;
+  int64_t ld_residual;
+  void* out;
+  int64_t ld_out;
+};
+
+// One set of these for each element type; 0 or a hipError_t.
+template <int DT>
+struct HeadOps {
+  static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
+  static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
+  static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
+  static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,
+                        void* stream);
+  static int gemm_partial(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiPartial& e,
+                          void* stream);
+  static int join_linear(const EpiPartial& from, int parts, const EpiLinear& e, void* stream);
+  static int join_store(const EpiPartial& from, int parts, const EpiStore& e, void* stream);
+  static int col_sum(const ColSumPlan& p, void* stream);
+  static int col_sum_join(const ColSumPlan& p, void* out, const float* scale, void* stream);
+};
+int launch_dropout(const DropoutPlan& p, int dtype, void* stream);
+// Element size 2 or 4.
+int launch_pack(const PackPlan& p, int element_bytes, void* stream);
+int launch_join_stats(const JoinStatsPlan& p, void* stream);
+// scale[0]: what a 16-bit gradient of the logits is multiplied by (1 where no
+// d_loss is finite and not 0), scale[1] = 1 / scale[0].
+int launch_grad_scale(const float* d_loss, int rows, float* scale, void* stream);
+
+}  // namespace lsamp
+
+#endif

@@ -1,0 +1,429 @@
+// lsamp_head.hip — the hidden-state operators: linear blocks, the vocabulary
+// head's cross entropy, and their gradients.  Compiled once per element type
+// (LSAMP_DT).  The matrix products are lsamp_gemm.h; this file holds what
+// happens to their sums, and the passes between them.
+#include <hip/hip_runtime.h>
+
+#include "lsamp_gemm.h"
+#include "lsamp_head.h"
+
+namespace lsamp {
+namespace gemm {
+namespace {
+
+constexpr int DT = LSAMP_DT;
+using S = El<DT>::S;
+typedef S v4e __attribute__((ext_vector_type(4)));
+
+// Four columns of a row: as one load where rows are aligned for it.
+__device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid, bool vec) {
+  const S* p = (const S*)base + i;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (vec && valid >= 4) {
+    const v4e e = *(const v4e*)p;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)e[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < valid) v[k] = (float)p[k];
+  }
+  return v;
+}
+__device__ __forceinline__ void store4(void* base, int64_t i, v4f v, int valid, bool vec) {
+  S* p = (S*)base + i;
+  if (vec && valid >= 4) {
+    v4e e;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = (S)v[k];
+    *(v4e*)p = e;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < valid) p[k] = (S)v[k];
+  }
+}
+__device__ __forceinline__ v4f load4f(const float* p, int valid, bool vec) {
+  if (vec && valid >= 4) return *(const v4f*)p;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < valid) v[k] = p[k];
+  return v;
+}
+__device__ __forceinline__ void store4f(float* p, v4f v, int valid, bool vec) {
+  if (vec && valid >= 4) {
+    *(v4f*)p = v;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < valid) p[k] = v[k];
+  }
+}
+
+// exp in float32 (a 16-bit result does not see the hardware exponential's last bits)
+__device__ __forceinline__ float expe(float x) {
+  if constexpr (DT == LSAMP_DTYPE_F32)
+    return expf(x);
+  else
+    return __expf(x);
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expe(-z)); }
+
+constexpr float kSqrtHalf = 0.70710678118654752f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
+constexpr float kGeluA = 0.79788456080286536f;  // sqrt(2 / pi)
+constexpr float kGeluB = 0.044715f;
+
+__device__ __forceinline__ float activate(int act, float cap, float z) {
+  switch (act) {
+    case LSAMP_ACT_RELU: return z < 0.f ? 0.f : z;  // (a NaN stays)
+    case LSAMP_ACT_SILU: return z * sigmoid(z);
+    case LSAMP_ACT_GELU: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case LSAMP_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(kGeluA * (z + kGeluB * z * z * z)));
+    case LSAMP_ACT_SOFTCAP: return cap * tanhf(z / cap);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float activate_slope(int act, float cap, float z) {
+  switch (act) {
+    case LSAMP_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case LSAMP_ACT_SILU: {
+      const float s = sigmoid(z);
+      return s * (1.f + z * (1.f - s));
+    }
+    case LSAMP_ACT_GELU:
+      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expe(-0.5f * z * z);
+    case LSAMP_ACT_GELU_TANH: {
+      const float t = tanhf(kGeluA * (z + kGeluB * z * z * z));
+      return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluA * (1.f + 3.f * kGeluB * z * z);
+    }
+    case LSAMP_ACT_SOFTCAP: {
+      const float t = tanhf(z / cap);
+      return 1.f - t * t;
+    }
+    default: return 1.f;
+  }
+}
+
+// ------------------------------------------------------------------ epilogues
+// put(r, c, v): four columns from c of row r.
+template <class E, int FM, int FN, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void put_all(const E& e, v4f (&acc)[FN][FM], int m0, int n0, int part,
+                                        int wm, int wn, int lane) {
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int r = m0 + wm * (FM * 16) + j * 16 + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
+      if (r < e.m && c < e.n) e.put(r, c, acc[i][j], part);
+    }
+  }
+}
+
+struct Linear : EpiLinear {
+  __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
+    const int valid = n - c;
+    if (bias) v += load4(bias, c, valid, vec);
+    if (pre) store4f(pre + (int64_t)r * ld_pre + c, v, valid, vec);
+    if (activation != LSAMP_ACT_NONE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = activate(activation, softcap, v[k]);
+    }
+    if (residual) v += load4(residual, (int64_t)r * ld_residual + c, valid, vec);
+    if (wide)
+      store4f((float*)out + (int64_t)r * ld_out + c, v, valid, vec);
+    else
+      store4(out, (int64_t)r * ld_out + c, v, valid, vec);
+  }
+  template <int FM, int FN, int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+                                      int lane, char*) const {
+    put_all<Linear, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+  }
+};
+
+struct Store : EpiStore {
+  __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
+    if (scale) v *= *scale;
+    store4(out, (int64_t)r * ld_out + c, v, n - c, vec);
+  }
+  template <int FM, int FN, int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+                                      int lane, char*) const {
+    put_all<Store, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+  }
+};
+
+struct Partial : EpiPartial {
+  __device__ __forceinline__ void put(int r, int c, v4f v, int part) const {
+    v4f* p = (v4f*)(out + part * part_stride + (int64_t)r * ld + c);
+    if (accumulate) v += *p;
+    *p = v;
+  }
+  template <int FM, int FN, int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+                                      int lane, char*) const {
+    put_all<Partial, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+  }
+};
+
+// z = softcap(sum + bias) of a piece's column; t = tanh(. / softcap).
+__device__ __forceinline__ v4f logits4(v4f v, const void* bias, int col, int valid, float softcap,
+                                       v4f* slope) {
+  if (bias) v += load4(bias, col, valid, false);
+  if (softcap > 0.f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float t = tanhf(v[k] / softcap);
+      v[k] = softcap * t;
+      if (slope) (*slope)[k] = 1.f - t * t;
+    }
+  }
+  return v;
+}
+
+// The forward pass keeps, of a tile's logits, each row's maximum and the sum of
+// exp(z - maximum): 4 columns x FN fragments in a lane, the four lanes of a row,
+// then the waves of the row through LDS.  A row whose logits here are all -inf
+// has maximum -inf and sum 0.
+struct Stats : EpiStats {
+  template <int FM, int FN, int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+                                      int lane, char* lds) const {
+    float* red = (float*)lds;  // [WN][BM][2]
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int rl = wm * (FM * 16) + j * 16 + (lane & 15);
+      const int r = m0 + rl;
+      const int t = r < m ? targets[r] - first_col : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
+        const int valid = n - c;
+        const v4f v = logits4(acc[i][j], bias, first_col + c, valid, softcap, nullptr);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool ok = k < valid;
+          acc[i][j][k] = ok ? v[k] : -INFINITY;
+          top = fmaxf(top, acc[i][j][k]);
+          if (ok && t == c + k) target[r] = v[k];
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      float sum = 0.f;
+      // (NaN logits are no maximum; they make the sum NaN)
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += expe(acc[i][j][k] - base);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (lane < 16) {
+        red[(wn * BM + rl) * 2] = top;
+        red[(wn * BM + rl) * 2 + 1] = sum;
+      }
+    }
+    __syncthreads();
+    for (int rl = threadIdx.x; rl < BM; rl += WM * WN * kWave) {
+      if (m0 + rl >= m) break;
+      float top = -INFINITY, sum = 0.f;
+      for (int w = 0; w < WN; ++w) top = fmaxf(top, red[(w * BM + rl) * 2]);
+      const float base = top == -INFINITY ? 0.f : top;
+      for (int w = 0; w < WN; ++w) {
+        const float t = red[(w * BM + rl) * 2], s = red[(w * BM + rl) * 2 + 1];
+        sum += t == -INFINITY ? s : s * expe(t - base);  // (a NaN sum stays)
+      }
+      float* o = part + ((int64_t)(m0 + rl) * blocks + first_block + at.n) * 2;
+      o[0] = top;
+      o[1] = sum;
+    }
+  }
+};
+
+// The gradient at the logits, d_loss[r] (softmax(z) - onehot(target)), from the
+// recomputed logits and the forward pass's log-sum-exp.  Rounded to the
+// operands' type because the two products that read it are matrix instructions
+// of that type; 16-bit values are scaled first (k_grad_scale).  A row without
+// a loss (target ignored or out of range, every logit -inf) is zero.
+struct Grad : EpiGrad {
+  template <int FM, int FN, int BM, int BN, int WM, int WN>
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
+                                      int lane, char*) const {
+    const float s = scale ? scale[0] : 1.f;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int r = m0 + wm * (FM * 16) + j * 16 + (lane & 15);
+      if (r >= m) continue;
+      const int target = targets[r];
+      const float l = lse[r];
+      const bool none = target < 0 || target >= vocab || l == -INFINITY;
+      const float w = d_loss[r] * s;
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
+        if (c >= n_pad) continue;
+        v4f slope = {1.f, 1.f, 1.f, 1.f}, g;
+        const int valid = n - c;
+        const v4f z = logits4(acc[i][j], bias, first_col + c, valid, softcap, &slope);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = expe(z[k] - l) - (first_col + c + k == target ? 1.f : 0.f);
+          g[k] = none || k >= valid ? 0.f : w * p * slope[k];
+        }
+        store4(out, (int64_t)r * ld_out + c, g, 4, true);
+      }
+    }
+  }
+};
+
+template <bool AK, bool BK, class E, class P>
+int launch(GemmTile tile, const GemmPlan& g, const P& plan, void* stream) {
+  E e;
+  static_cast<P&>(e) = plan;
+  const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  switch (tile) {
+    case kTile256:
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, E>), grid, dim3(512), 0, st, g, e);
+      break;
+    case kTile128:
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, E>), grid, dim3(256), 0, st, g, e);
+      break;
+    default:
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, E>), grid, dim3(256), 0, st, g, e);
+  }
+  return (int)hipGetLastError();
+}
+
+// ------------------------------------------------------------- passes between
+constexpr int kThreads = 256;
+
+// The parts of a split reduction, summed in their order, and the epilogue.
+template <class E>
+__global__ __launch_bounds__(kThreads) void k_join(EpiPartial from, int parts, E e) {
+  const int quads = (e.n + 3) / 4;
+  const int64_t total = (int64_t)e.m * quads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * kThreads) {
+    const int r = (int)(i / quads), c = (int)(i % quads) * 4;
+    const float* p = from.out + (int64_t)r * from.ld + c;
+    v4f v = *(const v4f*)p;
+    for (int k = 1; k < parts; ++k) v += *(const v4f*)(p + k * from.part_stride);
+    e.put(r, c, v, 0);
+  }
+}
+template <class E, class P>
+int launch_join(const EpiPartial& from, int parts, const P& plan, void* stream) {
+  E e;
+  static_cast<P&>(e) = plan;
+  const int64_t quads = (int64_t)e.m * ((e.n + 3) / 4);
+  int64_t blocks = (quads + kThreads - 1) / kThreads;
+  blocks = blocks < 8192 ? blocks : 8192;
+  hipLaunchKernelGGL((k_join<E>), dim3((unsigned)blocks), dim3(kThreads), 0,
+                     reinterpret_cast<hipStream_t>(stream), from, parts, e);
+  return (int)hipGetLastError();
+}
+
+// Column sums of a chunk of rows: 64 lanes x 4 columns, 4 waves taking rows in
+// turn and joined in LDS.  With `pre`: of in * activation'(pre), which is also
+// written out for the products that follow.
+__global__ __launch_bounds__(kThreads) void k_col_sum(ColSumPlan p) {
+  __shared__ v4f red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = ((int)blockIdx.x * 64 + lane) * 4;
+  const int valid = p.cols - c;
+  const int r0 = (int)blockIdx.y * p.rows_per_chunk;
+  const int r1 = min(p.rows, r0 + p.rows_per_chunk);
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  if (c < p.cols || (p.out && c < p.out_cols)) {
+    for (int r = r0 + wave; r < r1; r += 4) {
+      v4f v = load4(p.in, (int64_t)r * p.ld_in + c, valid, p.vec);
+      if (p.pre) {
+        const v4f z = load4f(p.pre + (int64_t)r * p.ld_pre + c, valid, p.vec);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = v[k] * activate_slope(p.activation, p.softcap, z[k]);
+          v[k] = k < valid ? d : 0.f;
+        }
+        store4(p.out, (int64_t)r * p.ld_out + c, v, p.out_cols - c, true);
+      }
+      sum += v;
+    }
+  }
+  if (!p.part) return;
+  red[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && c < p.ld_part) {
+    for (int w = 1; w < 4; ++w) sum += red[w][lane];
+    *(v4f*)(p.part + (int64_t)blockIdx.y * p.ld_part + c) = sum;
+  }
+}
+__global__ __launch_bounds__(kThreads) void k_col_sum_join(ColSumPlan p, S* out, const float* scale) {
+  const int c = (int)(blockIdx.x * kThreads + threadIdx.x);
+  if (c >= p.cols) return;
+  float s = 0.f;
+  for (int i = 0; i < p.chunks; ++i) s += p.part[(int64_t)i * p.ld_part + c];
+  out[c] = (S)(scale ? s * *scale : s);
+}
+
+}  // namespace
+}  // namespace gemm
+
+using namespace gemm;
+
+template <>
+int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& e, void* st) {
+  return launch<false, false, Linear>(t, g, e, st);
+}
+template <>
+int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& e, void* st) {
+  return launch<false, false, Stats>(t, g, e, st);
+}
+template <>
+int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& e, void* st) {
+  return launch<false, false, Grad>(t, g, e, st);
+}
+template <>
+int HeadOps<DT>::gemm_store(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiStore& e,
+                            void* st) {
+  return roles == kRolesNN ? launch<false, true, Store>(t, g, e, st)
+                           : launch<true, true, Store>(t, g, e, st);
+}
+template <>
+int HeadOps<DT>::gemm_partial(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiPartial& e,
+                              void* st) {
+  switch (roles) {
+    case kRolesNT: return launch<false, false, Partial>(t, g, e, st);
+    case kRolesNN: return launch<false, true, Partial>(t, g, e, st);
+    default: return launch<true, true, Partial>(t, g, e, st);
+  }
+}
+template <>
+int HeadOps<DT>::join_linear(const EpiPartial& from, int parts, const EpiLinear& e, void* st) {
+  return launch_join<Linear>(from, parts, e, st);
+}
+template <>
+int HeadOps<DT>::join_store(const EpiPartial& from, int parts, const EpiStore& e, void* st) {
+  return launch_join<Store>(from, parts, e, st);
+}
+template <>
+int HeadOps<DT>::col_sum(const ColSumPlan& p, void* stream) {
+  const int cols = p.out && p.out_cols > p.cols ? p.out_cols : p.cols;
+  const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)p.chunks);
+  hipLaunchKernelGGL(k_col_sum, grid, dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), p);
+  return (int)hipGetLastError();
+}
+template <>
+int HeadOps<DT>::col_sum_join(const ColSumPlan& p, void* out, const float* scale, void* stream) {
+  hipLaunchKernelGGL(k_col_sum_join, dim3((unsigned)((p.cols + kThreads - 1) / kThreads)),
+                     dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), p, (S*)out, scale);
+  return (int)hipGetLastError();
+}
+
+}  // namespace lsamp

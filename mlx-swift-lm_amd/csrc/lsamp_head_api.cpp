@@ -1,0 +1,790 @@
+// lsamp_head_api.cpp — the C entry points of the hidden-state operators:
+// argument checks, the choice of tiles, pieces and parts, and the launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "lsamp_head.h"
+#include "lsamp_internal.h"
+
+using namespace lsamp;
+
+namespace {
+
+constexpr int32_t kMaxDim = 1 << 27;
+constexpr int64_t kAlign = 256;
+// Work-groups of a launch: 512 threads each, below 2^32 threads in all.
+constexpr int64_t kMaxBlocks = (int64_t)1 << 22;
+
+struct OnDevice {
+  int prev = -1;
+  bool changed = false;
+  explicit OnDevice(int dev) {
+    if (hipGetDevice(&prev) == hipSuccess && prev != dev) changed = hipSetDevice(dev) == hipSuccess;
+  }
+  ~OnDevice() {
+    if (changed) (void)hipSetDevice(prev);
+  }
+};
+
+int element_bytes(int dtype) { return dtype == LSAMP_DTYPE_F32 ? 4 : 2; }
+int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+int64_t ceil_div(int64_t v, int64_t a) { return (v + a - 1) / a; }
+
+#define HEAD_OP(dtype, call)                                              \
+  ((dtype) == LSAMP_DTYPE_F32    ? HeadOps<LSAMP_DTYPE_F32>::call         \
+   : (dtype) == LSAMP_DTYPE_BF16 ? HeadOps<LSAMP_DTYPE_BF16>::call        \
+                                 : HeadOps<LSAMP_DTYPE_F16>::call)
+
+// Parts of the caller's workspace, in the order they are taken; with base NULL
+// only their sizes are added up.
+struct Arena {
+  char* base;
+  int64_t used = 0;
+  explicit Arena(void* p) : base((char*)p) {}
+  template <typename T = void>
+  T* take(int64_t bytes) {
+    T* p = (T*)(base ? base + used : nullptr);
+    used += round_up(bytes, kAlign);
+    return p;
+  }
+};
+
+bool chunked(const void* p, int64_t ld, int32_t cols, int eb) {
+  return (uintptr_t)p % 16 == 0 && ld * eb % 16 == 0 && (int64_t)cols * eb % 16 == 0;
+}
+
+// Whether four columns of a matrix's rows can be moved as one vector.
+bool quads(const void* p, int64_t ld, int eb) {
+  return !p || ((uintptr_t)p % (4 * eb) == 0 && ld % 4 == 0);
+}
+
+// A matrix as the products read it: itself, or a copy in the workspace.
+struct Operand {
+  MatrixRef ref;
+  bool packed;
+  PackPlan pack;
+};
+Operand operand(Arena& ws, const void* p, int64_t ld, int32_t rows, int32_t cols, int eb) {
+  Operand o{};
+  if (chunked(p, ld, cols, eb)) {
+    o.ref = MatrixRef{p, ld, rows, cols};
+    return o;
+  }
+  const int32_t wide = (int32_t)round_up(cols, 16 / eb);
+  void* dst = ws.take((int64_t)rows * wide * eb);
+  o.packed = true;
+  o.pack = PackPlan{p, ld, dst, wide, rows, cols, wide};
+  o.ref = MatrixRef{dst, wide, rows, wide};
+  return o;
+}
+int lay_out(const Operand& o, int eb, void* stream) {
+  return o.packed ? launch_pack(o.pack, eb, stream) : 0;
+}
+
+// Tile shape and number of parts of the reduction for an m x n product over
+// `slabs` 128-byte slabs, by the time that they take: a CU holds 1, 2 or 4
+// work-groups of the three shapes; a slab takes at least the latency of its
+// loads, and at least the time of its products shared among the CU's groups.
+// The times (microseconds) are fitted to products of 16-bit elements of 520 x
+// 776 x 1000 and 8192 x 4096 x 4096 (256: 1.4 a slab alone, 2.0 when every CU
+// is busy; 128: 0.65 and 0.52; 64: 0.42 and 0.18).
+struct Choice {
+  GemmTile tile;
+  int32_t parts;
+};
+Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
+  static const double kLatency[kTiles] = {1.4, 0.65, 0.42};
+  static const double kBusy16[kTiles] = {2.0, 0.52, 0.18};
+  static const double kBusy32[kTiles] = {7.0, 1.8, 0.5};
+  static const int kResident[kTiles] = {1, 2, 4};
+  constexpr int kCus = 256;
+  const double* busy = dtype == LSAMP_DTYPE_F32 ? kBusy32 : kBusy16;
+  Choice best{kTile64, 1};
+  double best_us = 1e300;
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t tiles = ceil_div(m, kTileSide[t]) * ceil_div(n, kTileSide[t]);
+    for (int parts = 1; parts <= (may_split ? 64 : 1) && parts <= slabs; parts *= 2) {
+      const int64_t each = ceil_div(tiles * parts, kCus);
+      const double per_slab = std::max((double)each * busy[t],
+                                       (double)ceil_div(each, kResident[t]) * kLatency[t]);
+      double us = per_slab * (double)ceil_div(slabs, parts);
+      if (parts > 1) us += 4.0 + (double)parts * (double)m * (double)n * 8e-6 / 4.0;
+      if (us < best_us) {
+        best_us = us;
+        best = Choice{(GemmTile)t, parts};
+      }
+    }
+  }
+  return best;
+}
+
+// `k`: elements of the reduction.
+GemmPlan plan_gemm(const Choice& c, const MatrixRef& a, const MatrixRef& b, int64_t m, int64_t n,
+                   int64_t k, int eb) {
+  GemmPlan g{};
+  g.a = a;
+  g.b = b;
+  g.tiles_m = (int32_t)ceil_div(m, kTileSide[c.tile]);
+  g.tiles_n = (int32_t)ceil_div(n, kTileSide[c.tile]);
+  g.slabs = (int32_t)ceil_div(k, 128 / eb);
+  g.slabs_per_part = (int32_t)ceil_div(g.slabs, c.parts);
+  g.parts = (int32_t)ceil_div(g.slabs, g.slabs_per_part);
+  return g;
+}
+bool too_many(const GemmPlan& g) {
+  return (int64_t)g.tiles_m * g.tiles_n * g.parts > kMaxBlocks;
+}
+
+int64_t slabs_of(int64_t k, int eb) { return ceil_div(k, 128 / eb); }
+
+// A product into `out`: straight, or in parts through float32 sums.
+EpiPartial take_partial(Arena& ws, int64_t m, int64_t n, int parts) {
+  EpiPartial p{};
+  p.m = (int32_t)m;
+  p.n = (int32_t)n;
+  p.ld = round_up(n, 4);
+  p.part_stride = m * p.ld;
+  p.out = ws.take<float>((int64_t)parts * p.part_stride * 4);
+  return p;
+}
+
+lsamp_status device_error(int err) {
+  return set_error(LSAMP_ERR_DEVICE, "kernel launch failed: %s", hipGetErrorString((hipError_t)err));
+}
+
+#define LSAMP_TRY(expr)                    \
+  do {                                     \
+    const int try_err = (expr);            \
+    if (try_err) return device_error(try_err); \
+  } while (0)
+
+// --------------------------------------------------------------------- checks
+lsamp_status check_dims(const char* what, int32_t v) {
+  if (v <= 0 || v > kMaxDim)
+    return set_error(LSAMP_ERR_SHAPE, "%s %d out of range [1, %d]", what, v, kMaxDim);
+  return LSAMP_OK;
+}
+lsamp_status check_dtype(int32_t dtype) {
+  if (dtype < LSAMP_DTYPE_F32 || dtype > LSAMP_DTYPE_F16)
+    return set_error(LSAMP_ERR_DTYPE, "dtype %d is not float32, bfloat16 or float16", dtype);
+  return LSAMP_OK;
+}
+// A matrix of the arguments: present, its elements aligned, its rows apart.
+lsamp_status check_matrix(const char* what, const void* p, int64_t ld, int32_t rows, int32_t cols,
+                          int eb) {
+  if (!p) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "%s is required", what);
+  if ((uintptr_t)p % eb)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "%s is not aligned to its elements", what);
+  if (rows > 1 && ld < cols)
+    return set_error(LSAMP_ERR_SHAPE, "%s stride %lld is below its %d columns", what, (long long)ld,
+                     cols);
+  if (ld < 0 || ld > ((int64_t)1 << 40))
+    return set_error(LSAMP_ERR_SHAPE, "%s stride %lld out of range", what, (long long)ld);
+  return LSAMP_OK;
+}
+// A vector (or a float output): present if required, aligned.
+lsamp_status check_vector(const char* what, const void* p, int eb, bool required) {
+  if (!p && required) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "%s is required", what);
+  if ((uintptr_t)p % eb)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "%s is not aligned to its elements", what);
+  return LSAMP_OK;
+}
+lsamp_status check_activation(int32_t act, float softcap) {
+  if (act < LSAMP_ACT_NONE || act > LSAMP_ACT_SOFTCAP)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "activation %d is unknown", act);
+  if (act == LSAMP_ACT_SOFTCAP && !(softcap > 0.f && std::isfinite(softcap)))
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "softcap %g must be positive and finite", softcap);
+  return LSAMP_OK;
+}
+lsamp_status check_workspace(const void* p, int64_t have, int64_t need) {
+  if (need == 0) return LSAMP_OK;
+  if (!p || have < need)
+    return set_error(LSAMP_ERR_CAPACITY, "the workspace holds %lld bytes, %lld are needed",
+                     p ? (long long)have : 0LL, (long long)need);
+  if ((uintptr_t)p % kAlign)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "the workspace is not aligned to %lld bytes",
+                     (long long)kAlign);
+  return LSAMP_OK;
+}
+// (a one-row matrix may carry any stride: its rows are taken as dense)
+int64_t stride_of(int64_t ld, int32_t rows, int32_t cols) { return rows > 1 ? ld : cols; }
+
+#define LSAMP_CHECK(expr)                     \
+  do {                                        \
+    const lsamp_status check_st = (expr);     \
+    if (check_st != LSAMP_OK) return check_st; \
+  } while (0)
+
+// ---------------------------------------------------------------------- linear
+struct LinearPlan {
+  Operand x, w;
+  Choice choice;
+  GemmPlan gemm;
+  EpiPartial partial;
+  EpiLinear epi;
+  int64_t bytes;
+};
+
+lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("in_features", a->in_features));
+  LSAMP_CHECK(check_dims("out_features", a->out_features));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  if (a->out_dtype != a->dtype && a->out_dtype != LSAMP_DTYPE_F32)
+    return set_error(LSAMP_ERR_DTYPE, "out_dtype %d must be the dtype %d or float32", a->out_dtype,
+                     a->dtype);
+  LSAMP_CHECK(check_activation(a->activation, a->softcap));
+  const int eb = element_bytes(a->dtype), ob = element_bytes(a->out_dtype);
+  const int32_t m = a->rows, n = a->out_features, k = a->in_features;
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, m, k, eb));
+  LSAMP_CHECK(check_matrix("weight", a->weight, a->weight_stride, n, k, eb));
+  LSAMP_CHECK(check_matrix("out", a->out, a->out_stride, m, n, ob));
+  LSAMP_CHECK(check_vector("bias", a->bias, eb, false));
+  if (a->residual)
+    LSAMP_CHECK(check_matrix("residual", a->residual, a->residual_stride, m, n, eb));
+  if (a->pre) LSAMP_CHECK(check_matrix("pre", a->pre, a->pre_stride, m, n, 4));
+
+  LinearPlan P{};
+  Arena ws(base);
+  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
+  P.choice = choose(m, n, slabs_of(k, eb), a->dtype, true);
+  P.gemm = plan_gemm(P.choice, P.x.ref, P.w.ref, m, n, k, eb);
+  if (too_many(P.gemm))
+    return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
+  if (P.gemm.parts > 1) P.partial = take_partial(ws, m, n, P.gemm.parts);
+  EpiLinear& e = P.epi;
+  e.m = m;
+  e.n = n;
+  e.activation = a->activation;
+  e.softcap = a->softcap;
+  e.wide = a->out_dtype == LSAMP_DTYPE_F32;
+  e.bias = a->bias;
+  e.residual = a->residual;
+  e.ld_residual = stride_of(a->residual_stride, m, n);
+  e.out = a->out;
+  e.ld_out = stride_of(a->out_stride, m, n);
+  e.pre = a->pre;
+  e.ld_pre = stride_of(a->pre_stride, m, n);
+  const bool one = m == 1;  // (the only row starts at its address)
+  e.vec = quads(e.bias, 4, eb) && quads(e.residual, one ? 4 : e.ld_residual, eb) &&
+          quads(e.out, one ? 4 : e.ld_out, ob) && quads(e.pre, one ? 4 : e.ld_pre, 4);
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+// ------------------------------------------------------------ linear, backward
+// Column sums in chunks of rows, enough of them to fill the device.
+void plan_col_sum(ColSumPlan& s, int32_t rows, int32_t cols) {
+  s.rows = rows;
+  s.cols = cols;
+  const int64_t across = ceil_div(cols, 256);
+  int64_t chunks = std::min(ceil_div(2048, across), ceil_div(rows, 16));
+  s.rows_per_chunk = (int32_t)ceil_div(rows, chunks);
+  s.chunks = (int32_t)ceil_div(rows, s.rows_per_chunk);
+}
+
+struct Product {  // one product of a backward pass
+  GemmRoles roles;
+  Choice choice;
+  GemmPlan gemm;
+  EpiPartial partial;
+  EpiStore store;
+};
+// out = A B in `roles`; `k` reduction elements.
+Product plan_product(Arena& ws, GemmRoles roles, const MatrixRef& a, const MatrixRef& b, int64_t m,
+                     int64_t n, int64_t k, int dtype, void* out, int64_t ld, const float* scale) {
+  const int eb = element_bytes(dtype);
+  Product p{};
+  p.roles = roles;
+  p.choice = choose(m, n, slabs_of(k, eb), dtype, true);
+  p.gemm = plan_gemm(p.choice, a, b, m, n, k, eb);
+  if (p.gemm.parts > 1) p.partial = take_partial(ws, m, n, p.gemm.parts);
+  p.store.m = (int32_t)m;
+  p.store.n = (int32_t)n;
+  p.store.out = out;
+  p.store.ld_out = ld;
+  p.store.scale = scale;
+  p.store.vec = quads(out, m == 1 ? 4 : ld, eb);
+  return p;
+}
+int run_product(const Product& p, int dtype, void* stream) {
+  if (p.gemm.parts == 1)
+    return HEAD_OP(dtype, gemm_store(p.roles, p.choice.tile, p.gemm, p.store, stream));
+  const int err =
+      HEAD_OP(dtype, gemm_partial(p.roles, p.choice.tile, p.gemm, p.partial, stream));
+  return err ? err : HEAD_OP(dtype, join_store(p.partial, p.gemm.parts, p.store, stream));
+}
+
+struct LinearBackwardPlan {
+  Operand x, w, d;
+  bool sum;  // the pass over d_out: d_bias, or dz for an activation
+  ColSumPlan col;
+  bool want_x, want_w;
+  Product dx, dw;
+  int64_t bytes;
+};
+
+lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* base,
+                                  LinearBackwardPlan* out) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("in_features", a->in_features));
+  LSAMP_CHECK(check_dims("out_features", a->out_features));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  LSAMP_CHECK(check_activation(a->activation, a->softcap));
+  const int eb = element_bytes(a->dtype);
+  const int32_t m = a->rows, n = a->out_features, k = a->in_features;
+  const bool act = a->activation != LSAMP_ACT_NONE;
+  if (!a->d_x && !a->d_weight && !a->d_bias)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  LSAMP_CHECK(check_matrix("d_out", a->d_out, a->d_out_stride, m, n, eb));
+  if (act) LSAMP_CHECK(check_matrix("pre", a->pre, a->pre_stride, m, n, 4));
+  if (a->d_x) {
+    LSAMP_CHECK(check_matrix("weight", a->weight, a->weight_stride, n, k, eb));
+    LSAMP_CHECK(check_matrix("d_x", a->d_x, a->d_x_stride, m, k, eb));
+  }
+  if (a->d_weight) {
+    LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, m, k, eb));
+    LSAMP_CHECK(check_matrix("d_weight", a->d_weight, a->d_weight_stride, n, k, eb));
+  }
+  LSAMP_CHECK(check_vector("d_bias", a->d_bias, eb, false));
+
+  LinearBackwardPlan P{};
+  Arena ws(base);
+  P.want_x = a->d_x != nullptr;
+  P.want_w = a->d_weight != nullptr;
+  const int64_t ld_d = stride_of(a->d_out_stride, m, n);
+  MatrixRef dz{};
+  if (act) {
+    const int32_t wide = (int32_t)round_up(n, 16 / eb);
+    dz = MatrixRef{ws.take((int64_t)m * wide * eb), wide, m, wide};
+  } else if (P.want_x || P.want_w) {
+    P.d = operand(ws, a->d_out, ld_d, m, n, eb);
+    dz = P.d.ref;
+  }
+  P.sum = act || a->d_bias;
+  if (P.sum) {
+    ColSumPlan& s = P.col;
+    plan_col_sum(s, m, n);
+    s.in = a->d_out;
+    s.ld_in = ld_d;
+    s.activation = a->activation;
+    s.softcap = a->softcap;
+    s.vec = quads(a->d_out, m == 1 ? 4 : ld_d, eb);
+    if (act) {
+      s.pre = a->pre;
+      s.ld_pre = stride_of(a->pre_stride, m, n);
+      s.vec = s.vec && quads(s.pre, m == 1 ? 4 : s.ld_pre, 4);
+      s.out = const_cast<void*>(dz.p);
+      s.ld_out = dz.ld;
+      s.out_cols = dz.cols;
+    }
+    if (a->d_bias) {
+      s.ld_part = round_up(n, 4);
+      s.part = ws.take<float>((int64_t)s.chunks * s.ld_part * 4);
+    }
+  }
+  if (P.want_x) {
+    P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
+    P.dx = plan_product(ws, kRolesNN, dz, P.w.ref, m, k, n, a->dtype, a->d_x,
+                        stride_of(a->d_x_stride, m, k), nullptr);
+  }
+  if (P.want_w) {
+    P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+    P.dw = plan_product(ws, kRolesTN, dz, P.x.ref, n, k, m, a->dtype, a->d_weight,
+                        stride_of(a->d_weight_stride, n, k), nullptr);
+  }
+  if ((P.want_x && too_many(P.dx.gemm)) || (P.want_w && too_many(P.dw.gemm)))
+    return set_error(LSAMP_ERR_SHAPE, "%d x %d x %d is too large for one call", m, n, k);
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+// ------------------------------------------------------------------- head loss
+// The checks that both directions share.
+template <typename A>
+lsamp_status check_head(const A* a) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("hidden", a->hidden));
+  LSAMP_CHECK(check_dims("vocab", a->vocab));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  if (!(a->softcap >= 0.f && std::isfinite(a->softcap)))
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "softcap %g must be finite and not negative",
+                     a->softcap);
+  const int eb = element_bytes(a->dtype);
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, a->rows, a->hidden, eb));
+  LSAMP_CHECK(check_matrix("weight", a->weight, a->weight_stride, a->vocab, a->hidden, eb));
+  LSAMP_CHECK(check_vector("bias", a->bias, eb, false));
+  LSAMP_CHECK(check_vector("targets", a->targets, 4, true));
+  LSAMP_CHECK(check_vector("lse", a->lse, 4, true));
+  return LSAMP_OK;
+}
+
+// A piece of the vocabulary is a multiple of the largest tile's columns, so that
+// the tiles of all pieces are those of the whole.
+constexpr int64_t kPieceStep = 256;
+int64_t piece_cols(int64_t vocab, int64_t most) {
+  most = std::max(kPieceStep, most / kPieceStep * kPieceStep);
+  const int64_t pieces = ceil_div(vocab, most);
+  return std::min(round_up(ceil_div(vocab, pieces), kPieceStep), round_up(vocab, kPieceStep));
+}
+// The weight rows of a piece: themselves, or their copy at `packed`.
+Operand weight_piece(const void* w, int64_t ld, int32_t first, int32_t rows, int32_t hidden, int eb,
+                     void* packed) {
+  const char* p = (const char*)w + (int64_t)first * ld * eb;
+  Operand o{};
+  if (!packed) {
+    o.ref = MatrixRef{p, ld, rows, hidden};
+    return o;
+  }
+  const int32_t wide = (int32_t)round_up(hidden, 16 / eb);
+  o.packed = true;
+  o.pack = PackPlan{p, ld, packed, wide, rows, hidden, wide};
+  o.ref = MatrixRef{packed, wide, rows, wide};
+  return o;
+}
+
+struct LossPlan {
+  Operand x;
+  Choice choice;
+  int64_t piece;  // vocabulary columns at a time
+  void* packed;
+  EpiStats epi;
+  JoinStatsPlan join;
+  int64_t bytes;
+};
+
+lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out) {
+  LSAMP_CHECK(check_head(a));
+  LSAMP_CHECK(check_vector("loss", a->loss, 4, true));
+  LSAMP_CHECK(check_vector("row_flags", a->row_flags, 4, false));
+  const int eb = element_bytes(a->dtype);
+  const int32_t m = a->rows, v = a->vocab, k = a->hidden;
+  LossPlan P{};
+  Arena ws(base);
+  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  const int64_t ld_w = stride_of(a->weight_stride, v, k);
+  P.piece = round_up(v, kPieceStep);
+  if (!chunked(a->weight, ld_w, k, eb)) {
+    const int64_t row = round_up(k, 16 / eb) * eb;
+    P.piece = piece_cols(v, ((int64_t)64 << 20) / row);
+    P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
+    if (!base) P.packed = (void*)1;  // (sizes only)
+  }
+  P.choice = choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, false);
+  const int64_t side = kTileSide[P.choice.tile];
+  if (ceil_div(m, side) * ceil_div(P.piece, side) > kMaxBlocks)
+    return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
+  EpiStats& e = P.epi;
+  e.m = m;
+  e.blocks = (int32_t)ceil_div(v, side);
+  e.softcap = a->softcap;
+  e.bias = a->bias;
+  e.targets = a->targets;
+  e.part = ws.take<float>((int64_t)m * e.blocks * 8);
+  e.target = ws.take<float>((int64_t)m * 4);
+  P.join = JoinStatsPlan{m, e.blocks, v, e.part, e.target, a->targets, a->loss, a->lse, a->row_flags};
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+struct LossBackwardPlan {
+  Operand x;
+  int64_t piece;
+  void* packed;
+  void* g;      // [rows, ld_g]: the gradient at a piece of the logits
+  int64_t ld_g;
+  float* scale;  // 16-bit types: {scale, 1 / scale}
+  Choice grad, dx, dw;
+  EpiPartial dx_sum, dw_sum;  // float32 sums of d_x (all pieces), of a piece's d_weight
+  bool dx_straight, dw_split;
+  ColSumPlan col;
+  int64_t bytes;
+};
+
+lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* base,
+                                LossBackwardPlan* out) {
+  LSAMP_CHECK(check_head(a));
+  LSAMP_CHECK(check_vector("d_loss", a->d_loss, 4, true));
+  const int eb = element_bytes(a->dtype);
+  const int32_t m = a->rows, v = a->vocab, k = a->hidden;
+  if (!a->d_x && !a->d_weight && !a->d_bias)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  if (a->d_x) LSAMP_CHECK(check_matrix("d_x", a->d_x, a->d_x_stride, m, k, eb));
+  if (a->d_weight)
+    LSAMP_CHECK(check_matrix("d_weight", a->d_weight, a->d_weight_stride, v, k, eb));
+  LSAMP_CHECK(check_vector("d_bias", a->d_bias, eb, false));
+
+  LossBackwardPlan P{};
+  Arena ws(base);
+  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  // A piece's gradient stays in the 256 MB last-level cache between the pass
+  // that writes it and the products that read it.
+  P.piece = piece_cols(v, ((int64_t)128 << 20) / ((int64_t)m * eb));
+  const int64_t ld_w = stride_of(a->weight_stride, v, k);
+  if (!chunked(a->weight, ld_w, k, eb)) {
+    const int64_t row = round_up(k, 16 / eb) * eb;
+    P.piece = std::min(P.piece, piece_cols(v, ((int64_t)128 << 20) / row));
+    P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
+    if (!base) P.packed = (void*)1;  // (sizes only)
+  }
+  const int64_t cols = std::min(P.piece, (int64_t)v);
+  P.ld_g = round_up(cols, 64);
+  P.g = ws.take((int64_t)m * P.ld_g * eb);
+  if (eb == 2) P.scale = ws.take<float>(8);
+  P.grad = choose(m, cols, slabs_of(k, eb), a->dtype, false);
+  const int64_t side = kTileSide[P.grad.tile];
+  if (ceil_div(m, side) * ceil_div(cols, side) > kMaxBlocks)
+    return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
+  if (a->d_x) {
+    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, true);
+    const GemmPlan g = plan_gemm(P.dx, MatrixRef{}, MatrixRef{}, m, k, cols, eb);
+    if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", m, k);
+    P.dx_straight = g.parts == 1 && cols == v;
+    if (!P.dx_straight) P.dx_sum = take_partial(ws, m, k, g.parts);
+  }
+  if (a->d_weight) {
+    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, true);
+    const GemmPlan g = plan_gemm(P.dw, MatrixRef{}, MatrixRef{}, cols, k, m, eb);
+    if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", v, k);
+    P.dw_split = g.parts > 1;
+    if (P.dw_split) P.dw_sum = take_partial(ws, cols, k, g.parts);
+  }
+  if (a->d_bias) {
+    plan_col_sum(P.col, m, (int32_t)cols);
+    P.col.ld_part = round_up(cols, 4);
+    P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
+  }
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+int64_t needed(lsamp_status st, int64_t bytes) {
+  if (st != LSAMP_OK) return st;
+  clear_error();
+  return bytes;
+}
+
+}  // namespace
+
+int64_t lsamp_linear_workspace(const lsamp_linear_args* a) {
+  LinearPlan P;
+  const lsamp_status st = plan_linear(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_linear(lsamp_context* ctx, const lsamp_linear_args* a, void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  LinearPlan P;
+  LSAMP_CHECK(plan_linear(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  const int eb = element_bytes(a->dtype);
+  LSAMP_TRY(lay_out(P.x, eb, stream));
+  LSAMP_TRY(lay_out(P.w, eb, stream));
+  if (P.gemm.parts == 1) {
+    LSAMP_TRY(HEAD_OP(a->dtype, gemm_linear(P.choice.tile, P.gemm, P.epi, stream)));
+  } else {
+    LSAMP_TRY(HEAD_OP(a->dtype, gemm_partial(kRolesNT, P.choice.tile, P.gemm, P.partial, stream)));
+    LSAMP_TRY(HEAD_OP(a->dtype, join_linear(P.partial, P.gemm.parts, P.epi, stream)));
+  }
+  return clear_error();
+}
+
+int64_t lsamp_linear_backward_workspace(const lsamp_linear_backward_args* a) {
+  LinearBackwardPlan P;
+  const lsamp_status st = plan_linear_backward(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_linear_backward(lsamp_context* ctx, const lsamp_linear_backward_args* a,
+                                   void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  LinearBackwardPlan P;
+  LSAMP_CHECK(plan_linear_backward(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  const int eb = element_bytes(a->dtype);
+  LSAMP_TRY(lay_out(P.d, eb, stream));
+  if (P.sum) LSAMP_TRY(HEAD_OP(a->dtype, col_sum(P.col, stream)));
+  if (a->d_bias) LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(P.col, a->d_bias, nullptr, stream)));
+  if (P.want_x) {
+    LSAMP_TRY(lay_out(P.w, eb, stream));
+    LSAMP_TRY(run_product(P.dx, a->dtype, stream));
+  }
+  if (P.want_w) {
+    LSAMP_TRY(lay_out(P.x, eb, stream));
+    LSAMP_TRY(run_product(P.dw, a->dtype, stream));
+  }
+  return clear_error();
+}
+
+int64_t lsamp_head_loss_workspace(const lsamp_head_loss_args* a) {
+  LossPlan P;
+  const lsamp_status st = plan_loss(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_head_loss(lsamp_context* ctx, const lsamp_head_loss_args* a, void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  LossPlan P;
+  LSAMP_CHECK(plan_loss(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  const int eb = element_bytes(a->dtype);
+  const int32_t v = a->vocab, k = a->hidden;
+  LSAMP_TRY(lay_out(P.x, eb, stream));
+  for (int64_t first = 0; first < v; first += P.piece) {
+    const int32_t n = (int32_t)std::min(P.piece, v - first);
+    const Operand w = weight_piece(a->weight, stride_of(a->weight_stride, v, k), (int32_t)first, n,
+                                   k, eb, P.packed);
+    LSAMP_TRY(lay_out(w, eb, stream));
+    EpiStats e = P.epi;
+    e.n = n;
+    e.first_col = (int32_t)first;
+    e.first_block = (int32_t)(first / kTileSide[P.choice.tile]);
+    const GemmPlan g = plan_gemm(P.choice, P.x.ref, w.ref, a->rows, n, k, eb);
+    LSAMP_TRY(HEAD_OP(a->dtype, gemm_stats(P.choice.tile, g, e, stream)));
+  }
+  LSAMP_TRY(launch_join_stats(P.join, stream));
+  return clear_error();
+}
+
+int64_t lsamp_head_loss_backward_workspace(const lsamp_head_loss_backward_args* a) {
+  LossBackwardPlan P;
+  const lsamp_status st = plan_loss_backward(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_backward_args* a,
+                                      void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  LossBackwardPlan P;
+  LSAMP_CHECK(plan_loss_backward(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  const int eb = element_bytes(a->dtype);
+  const int32_t m = a->rows, v = a->vocab, k = a->hidden;
+  const float* inverse = P.scale ? P.scale + 1 : nullptr;
+  LSAMP_TRY(lay_out(P.x, eb, stream));
+  if (P.scale) LSAMP_TRY(launch_grad_scale(a->d_loss, m, P.scale, stream));
+  EpiStore dx{};
+  dx.m = m;
+  dx.n = k;
+  dx.out = a->d_x;
+  dx.ld_out = stride_of(a->d_x_stride, m, k);
+  dx.vec = quads(dx.out, m == 1 ? 4 : dx.ld_out, eb);
+  dx.scale = inverse;
+  int dx_parts = 0;
+  for (int64_t first = 0; first < v; first += P.piece) {
+    const int32_t n = (int32_t)std::min(P.piece, v - first);
+    const Operand w = weight_piece(a->weight, stride_of(a->weight_stride, v, k), (int32_t)first, n,
+                                   k, eb, P.packed);
+    LSAMP_TRY(lay_out(w, eb, stream));
+    EpiGrad e{};
+    e.m = m;
+    e.n = n;
+    e.n_pad = (int32_t)round_up(n, 16 / eb);
+    e.first_col = (int32_t)first;
+    e.softcap = a->softcap;
+    e.bias = a->bias;
+    e.targets = a->targets;
+    e.vocab = v;
+    e.lse = a->lse;
+    e.d_loss = a->d_loss;
+    e.scale = P.scale;
+    e.out = P.g;
+    e.ld_out = P.ld_g;
+    LSAMP_TRY(HEAD_OP(a->dtype, gemm_grad(P.grad.tile,
+                                          plan_gemm(P.grad, P.x.ref, w.ref, m, n, k, eb), e, stream)));
+    const MatrixRef g{P.g, P.ld_g, m, e.n_pad};
+    if (a->d_x) {
+      const GemmPlan plan = plan_gemm(P.dx, g, w.ref, m, k, n, eb);
+      if (P.dx_straight) {
+        LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesNN, P.dx.tile, plan, dx, stream)));
+      } else {
+        EpiPartial sum = P.dx_sum;
+        sum.accumulate = first > 0;
+        if (first == 0) dx_parts = plan.parts;
+        LSAMP_TRY(HEAD_OP(a->dtype, gemm_partial(kRolesNN, P.dx.tile, plan, sum, stream)));
+      }
+    }
+    if (a->d_weight) {
+      EpiStore dw{};
+      dw.m = n;
+      dw.n = k;
+      dw.ld_out = stride_of(a->d_weight_stride, v, k);
+      dw.out = (char*)a->d_weight + first * dw.ld_out * eb;
+      dw.vec = quads(dw.out, v == 1 ? 4 : dw.ld_out, eb);
+      dw.scale = inverse;
+      const GemmPlan plan = plan_gemm(P.dw, g, P.x.ref, n, k, m, eb);
+      if (!P.dw_split) {
+        LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesTN, P.dw.tile, plan, dw, stream)));
+      } else {
+        EpiPartial sum = P.dw_sum;
+        sum.m = n;
+        LSAMP_TRY(HEAD_OP(a->dtype, gemm_partial(kRolesTN, P.dw.tile, plan, sum, stream)));
+        LSAMP_TRY(HEAD_OP(a->dtype, join_store(sum, plan.parts, dw, stream)));
+      }
+    }
+    if (a->d_bias) {
+      ColSumPlan s = P.col;
+      s.cols = n;
+      s.in = P.g;
+      s.ld_in = P.ld_g;
+      s.vec = 1;
+      LSAMP_TRY(HEAD_OP(a->dtype, col_sum(s, stream)));
+      LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
+    }
+  }
+  if (a->d_x && !P.dx_straight)
+    LSAMP_TRY(HEAD_OP(a->dtype, join_store(P.dx_sum, dx_parts, dx, stream)));
+  return clear_error();
+}
+
+lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* a, void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  if (!(a->p >= 0.f && a->p <= 1.f))
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "p %g out of range [0, 1]", a->p);
+  const int eb = element_bytes(a->dtype);
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, a->rows, a->cols, eb));
+  LSAMP_CHECK(check_matrix("out", a->out, a->out_stride, a->rows, a->cols, eb));
+  if (a->residual)
+    LSAMP_CHECK(check_matrix("residual", a->residual, a->residual_stride, a->rows, a->cols, eb));
+  LSAMP_CHECK(check_vector("step", a->step, 8, false));
+  DropoutPlan P{};
+  P.rows = a->rows;
+  P.cols = a->cols;
+  P.cut = (uint32_t)std::lrint((double)a->p * 65536.0);
+  P.scale = P.cut == 65536u ? 0.f : (float)(65536.0 / (65536.0 - (double)P.cut));
+  P.key = a->key;
+  P.offset = a->offset;
+  P.step = a->step;
+  P.x = a->x;
+  P.ld_x = stride_of(a->x_stride, a->rows, a->cols);
+  P.residual = a->residual;
+  P.ld_residual = stride_of(a->residual_stride, a->rows, a->cols);
+  P.out = a->out;
+  P.ld_out = stride_of(a->out_stride, a->rows, a->cols);
+  const auto vec = [&](const void* p, int64_t ld) {
+    return !p || ((uintptr_t)p % 16 == 0 && (a->rows == 1 || ld * eb % 16 == 0));
+  };
+  P.vec = vec(P.x, P.ld_x) && vec(P.residual, P.ld_residual) && vec(P.out, P.ld_out);
+  OnDevice guard(context_device(ctx));
+  LSAMP_TRY(launch_dropout(P, a->dtype, stream));
+  return clear_error();
+}

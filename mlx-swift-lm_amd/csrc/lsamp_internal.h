@@ -594,6 +594,8 @@ lsamp_status sample_step(const WorkspaceViews& v, const DeviceShape& d, int32_t 
 // The thread's last-error string (xgrammar_c.h:63-69 convention).
 lsamp_status set_error(lsamp_status st, const char* fmt, ...);
 lsamp_status clear_error();
+// The device that a context was made on.
+int32_t context_device(const lsamp_context* ctx);
 // Zero `bytes` (a multiple of 4) at `p` on `stream` with a fill kernel (no
 // memset node, so the call can be captured in a HIP graph).
 int launch_zero_words(void* p, size_t bytes, void* stream);

@@ -40,6 +40,8 @@ STATUS_PENALTY_CAPACITY = 2
 MASK_ID_RANGE = 1
 MASK_MAX_WORDS = 16000
 
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_SOFTCAP = range(6)
+
 
 class RowParams(Structure):
     _fields_ = [
@@ -289,6 +291,121 @@ class LogprobsArgs(Structure):
     ]
 
 
+class LinearArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("in_features", c_int32),
+        ("out_features", c_int32),
+        ("dtype", c_int32),
+        ("activation", c_int32),
+        ("softcap", c_float),
+        ("out_dtype", c_int32),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("bias", c_void_p),
+        ("residual", c_void_p),
+        ("residual_stride", c_int64),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("pre", c_void_p),
+        ("pre_stride", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class LinearBackwardArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("in_features", c_int32),
+        ("out_features", c_int32),
+        ("dtype", c_int32),
+        ("activation", c_int32),
+        ("softcap", c_float),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("pre", c_void_p),
+        ("pre_stride", c_int64),
+        ("d_out", c_void_p),
+        ("d_out_stride", c_int64),
+        ("d_x", c_void_p),
+        ("d_x_stride", c_int64),
+        ("d_weight", c_void_p),
+        ("d_weight_stride", c_int64),
+        ("d_bias", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class HeadLossArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("hidden", c_int32),
+        ("vocab", c_int32),
+        ("dtype", c_int32),
+        ("softcap", c_float),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("bias", c_void_p),
+        ("targets", c_void_p),
+        ("loss", c_void_p),
+        ("lse", c_void_p),
+        ("row_flags", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class HeadLossBackwardArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("hidden", c_int32),
+        ("vocab", c_int32),
+        ("dtype", c_int32),
+        ("softcap", c_float),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("bias", c_void_p),
+        ("targets", c_void_p),
+        ("lse", c_void_p),
+        ("d_loss", c_void_p),
+        ("d_x", c_void_p),
+        ("d_x_stride", c_int64),
+        ("d_weight", c_void_p),
+        ("d_weight_stride", c_int64),
+        ("d_bias", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class DropoutArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("dtype", c_int32),
+        ("p", c_float),
+        ("key", c_uint64),
+        ("offset", c_uint64),
+        ("step", c_void_p),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("residual", c_void_p),
+        ("residual_stride", c_int64),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+    ]
+
+
 class LibraryMissing(RuntimeError):
     pass
 
@@ -346,6 +463,16 @@ def load_library(path: str | None = None):
     lib.lsamp_top2.restype = c_int32
     lib.lsamp_logprobs.argtypes = [c_void_p, POINTER(LogprobsArgs), c_void_p]
     lib.lsamp_logprobs.restype = c_int32
+    for name, args in (("lsamp_linear", LinearArgs),
+                       ("lsamp_linear_backward", LinearBackwardArgs),
+                       ("lsamp_head_loss", HeadLossArgs),
+                       ("lsamp_head_loss_backward", HeadLossBackwardArgs)):
+        getattr(lib, name).argtypes = [c_void_p, POINTER(args), c_void_p]
+        getattr(lib, name).restype = c_int32
+        getattr(lib, name + "_workspace").argtypes = [POINTER(args)]
+        getattr(lib, name + "_workspace").restype = c_int64
+    lib.lsamp_dropout.argtypes = [c_void_p, POINTER(DropoutArgs), c_void_p]
+    lib.lsamp_dropout.restype = c_int32
     lib.lsamp_resolve_generate_parameters.argtypes = [
         POINTER(GenerateParameters), POINTER(RowParams), POINTER(c_int32)]
     lib.lsamp_resolve_generate_parameters.restype = c_int32

@@ -12,7 +12,7 @@ from typing import Iterable, Optional, Sequence
 import numpy as np
 import torch
 
-from . import _ffi
+from . import _ffi, head
 
 PENALTY_DTYPE = np.dtype([("token", "<i4"), ("count", "<i4"), ("flags", "<u4"), ("bias", "<f4")])
 PARAMS_DTYPE = np.dtype([
@@ -306,6 +306,53 @@ class Context:
         prep = self.prepare_verify(target, draft, draft_tokens, params, uniforms, **kw)
         prep.launch()
         return prep.outputs()
+
+    # ----------------------------------------------- hidden states (lsamp/head.py)
+    def prepare_linear(self, x: torch.Tensor, weight: torch.Tensor, **kw) -> "head.PreparedLinear":
+        """act(x weight^T + bias) + residual: a draft head's block, or the
+        vocabulary head's logits (lsamp_linear).  Keywords: bias, residual,
+        activation, softcap, out_dtype, want_pre, out."""
+        return head.PreparedLinear(self, x, weight, **kw)
+
+    def linear(self, x: torch.Tensor, weight: torch.Tensor, **kw) -> torch.Tensor:
+        p = self.prepare_linear(x, weight, **kw)
+        p.launch()
+        return p.out
+
+    def prepare_linear_backward(self, d_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                                **kw) -> "head.PreparedLinearBackward":
+        """Its gradients.  Keywords: pre, activation, softcap, want_x,
+        want_weight, want_bias."""
+        return head.PreparedLinearBackward(self, d_out, x, weight, **kw)
+
+    def prepare_head_loss(self, x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                          **kw) -> "head.PreparedHeadLoss":
+        """Cross entropy of the vocabulary head straight from hidden states
+        (lsamp_head_loss).  Keywords: bias, softcap."""
+        return head.PreparedHeadLoss(self, x, weight, targets, **kw)
+
+    def head_loss(self, x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, **kw) -> dict:
+        p = self.prepare_head_loss(x, weight, targets, **kw)
+        p.launch()
+        return p.outputs()
+
+    def prepare_head_loss_backward(self, d_loss: torch.Tensor, x: torch.Tensor,
+                                   weight: torch.Tensor, targets: torch.Tensor,
+                                   **kw) -> "head.PreparedHeadLossBackward":
+        """Its gradients.  Keywords: lse, bias, softcap, want_x, want_weight,
+        want_bias."""
+        return head.PreparedHeadLossBackward(self, d_loss, x, weight, targets, **kw)
+
+    def prepare_dropout(self, x: torch.Tensor, *, p: float, key: int,
+                        **kw) -> "head.PreparedDropout":
+        """residual + dropout(x) (lsamp_dropout).  Keywords: offset, residual,
+        step, out."""
+        return head.PreparedDropout(self, x, p=p, key=key, **kw)
+
+    def dropout(self, x: torch.Tensor, **kw) -> torch.Tensor:
+        p = self.prepare_dropout(x, **kw)
+        p.launch()
+        return p.out
 
 
 class PreparedSample:
