@@ -48,6 +48,15 @@ __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
 constexpr int kSlabBytes = 128;
 constexpr int kWave = 64;
 
+// Waits until at most `N` of this wave's vector memory operations (in the order
+// of their issue) and none of its LDS operations are under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "six bits");
+  // vmcnt in bits 3:0 and 15:14, expcnt 6:4 (unused: 7), lgkmcnt 11:8
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
+}
+
 template <int DT>
 struct El;
 template <>
@@ -113,58 +122,58 @@ struct Side {
   static constexpr int kBytes = ROWS * kSlabBytes;
   static_assert(ROWS % (8 * WAVES) == 0, "whole units a wave");
 
-  const char* p[kUnits];
-  int64_t step;
-  int koff;  // row-major: the lane's chunk's first step of the slab
+  const char* base;         // the slab's first element (the same for every lane)
+  int64_t step;             // bytes from slab to slab
+  uint32_t off[kUnits];     // the lane's chunk of each unit, from base
+  int koff;                 // row-major: the lane's chunk's first step of the slab
 
   // slab row of this lane in unit i (k-major)
   static __device__ __forceinline__ int slab_row(int wave, int lane, int i) {
     return ((wave * kUnits + i) % (kSlab / 8)) * 8 + (lane >> 3);
   }
 
+  // `first`: the tile's first output row (column); it exists.
   __device__ __forceinline__ void init(const MatrixRef& o, int first, int slab0, int wave, int lane) {
     if constexpr (!KMAJ) {
       koff = ((lane & 7) ^ (lane >> 3)) * kChunk;
       step = kSlabBytes;
+      base = (const char*)o.p + ((int64_t)first * o.ld + (int64_t)slab0 * kSlab) * kEb;
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        int r = first + (wave * kUnits + i) * 8 + (lane >> 3);
-        r = r < o.rows ? r : o.rows - 1;  // (rows past the end repeat the last: never stored)
-        p[i] = (const char*)o.p + (int64_t)r * o.ld * kEb +
-               ((int64_t)slab0 * kSlab + koff) * kEb;
+        // (rows past the end repeat the last: what they give is never stored)
+        const int r = min((wave * kUnits + i) * 8 + (lane >> 3), o.rows - 1 - first);
+        off[i] = ((uint32_t)r * (uint32_t)o.ld + (uint32_t)koff) * kEb;
       }
     } else {
       koff = 0;
       step = (int64_t)kSlab * o.ld * kEb;
+      base = (const char*)o.p + ((int64_t)slab0 * kSlab * o.ld + first) * kEb;
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int u = wave * kUnits + i;
         const int r = slab_row(wave, lane, i);
-        int c = first + (u / (kSlab / 8)) * kSlab + kmajor_place<DT>(r, lane & 7) * kChunk;
-        c = c < o.cols ? c : o.cols - kChunk;
-        p[i] = (const char*)o.p + ((int64_t)(slab0 * (int64_t)kSlab + r) * o.ld + c) * kEb;
+        const int c = min((u / (kSlab / 8)) * kSlab + kmajor_place<DT>(r, lane & 7) * kChunk,
+                          o.cols - kChunk - first);
+        off[i] = ((uint32_t)r * (uint32_t)o.ld + (uint32_t)c) * kEb;
       }
     }
   }
 
-  // One slab to LDS.  `left`: reduction steps from this slab on; the chunks (rows)
+  // One slab to LDS.  TAIL: only `left` reduction steps remain; the chunks (rows)
   // past them come from a zeroed buffer.
-  __device__ __forceinline__ void load(char* lds, int left, const char* zero, int wave, int lane) {
-    if (left >= kSlab) {
+  template <bool TAIL>
+  __device__ __forceinline__ void load(char* lds, int left, int wave, int lane) {
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i)
-        __builtin_amdgcn_global_load_lds(LSAMP_GLOBAL(p[i]),
-                                         LSAMP_LDS(lds + (wave * kUnits + i) * 1024), 16, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
+      const char* p = base + off[i];
+      if constexpr (TAIL) {
         const int k = KMAJ ? slab_row(wave, lane, i) : koff;
-        __builtin_amdgcn_global_load_lds(LSAMP_GLOBAL(k < left ? p[i] : zero),
-                                         LSAMP_LDS(lds + (wave * kUnits + i) * 1024), 16, 0, 0);
+        p = k < left ? p : (const char*)kZeros;
       }
+      __builtin_amdgcn_global_load_lds(LSAMP_GLOBAL(p),
+                                       LSAMP_LDS(lds + (wave * kUnits + i) * 1024), 16, 0, 0);
     }
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) p[i] += step;
+    base += step;
   }
 
   // The fragment of 16 output rows from `row0` (a multiple of 16), half `kk` of the slab.
@@ -224,33 +233,49 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
 }
 
 // One tile.  Epi: what happens to the sums; called once per work-group with
-//   run(acc, m0, n0, part, lane, wave-in-M, wave-in-N, lds)
+//   run(acc, m0, n0, at, wave-in-M, wave-in-N, lane, lds)
 // where acc[fn][fm][i] is row m0 + fm * 16 + (lane & 15), column
-// n0 + fn * 16 + (lane >> 4) * 4 + i.
-template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, class Epi>
-__global__ __launch_bounds__(WM* WN* kWave) void k_gemm(GemmPlan g, Epi epi) {
+// n0 + fn * 16 + (lane >> 4) * 4 + i of the wave's part.
+//
+// STAGES 2: two slabs in LDS, one on its way while the other is multiplied; a
+// barrier a slab.  Work-groups that share a CU hide each other's waits.  (More
+// stages change nothing: a slab's time is its barrier, its LDS reads and its
+// products one after the other, 0.4 us on a 64 x 64 tile, not the loads.)
+// GROUPS: so many slabs are multiplied at a time, each by its own WM x WN waves,
+// and the groups' sums joined through LDS at the end: for products with fewer
+// tiles than the device has CUs, whose time is the length of the reduction.
+// STAGES 0 (the 256 x 256 tile, one work-group a CU): two slabs in two halves.
+// While the products of one half run, the fragments of the next are read from
+// LDS.  In the middle of slab t every wave has its last fragments of the slab in
+// registers: after that barrier slab t + 2 may overwrite it, and slab t + 1
+// (loaded a whole slab ago) is complete.
+template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, int STAGES, int GROUPS, class Epi>
+__global__ __launch_bounds__(WM* WN* GROUPS* kWave) void k_gemm(GemmPlan g, Epi epi) {
   constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   using A = Side<DT, AK, BM, kWaves>;
   using B = Side<DT, BK, BN, kWaves>;
   constexpr int kStage = A::kBytes + B::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * GROUPS * kStage];
 
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave = wave_all % kWaves, group = wave_all / kWaves;
   const TileAt at = tile_at((int)blockIdx.x, g.tiles_m, g.tiles_n, g.parts);
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int slab0 = at.part * g.slabs_per_part;
   const int slabs = min(g.slabs_per_part, g.slabs - slab0);
   const int wm = wave % WM, wn = wave / WM;
-  const char* zero = (const char*)kZeros;
 
   A a;
   B b;
-  a.init(g.a, m0, slab0, wave, lane);
-  b.init(g.b, n0, slab0, wave, lane);
-  int left_a = (AK ? g.a.rows : g.a.cols) - slab0 * kSlabOf<DT>;
-  int left_b = (BK ? g.b.rows : g.b.cols) - slab0 * kSlabOf<DT>;
+  a.init(g.a, m0, slab0 + group, wave, lane);
+  b.init(g.b, n0, slab0 + group, wave, lane);
+  a.step *= GROUPS;
+  b.step *= GROUPS;
+  // reduction steps of this part's last slab
+  const int last_a = (AK ? g.a.rows : g.a.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
+  const int last_b = (BK ? g.b.rows : g.b.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
 
   v4f acc[FN][FM];
 #pragma unroll
@@ -258,33 +283,111 @@ __global__ __launch_bounds__(WM* WN* kWave) void k_gemm(GemmPlan g, Epi epi) {
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  a.load(lds, left_a, zero, wave, lane);
-  b.load(lds + A::kBytes, left_b, zero, wave, lane);
-  __syncthreads();
-  for (int t = 0; t < slabs; ++t) {
-    const char* cur = lds + (t & 1) * kStage;
-    if (t + 1 < slabs) {
-      char* next = lds + ((t + 1) & 1) * kStage;
-      left_a -= kSlabOf<DT>;
-      left_b -= kSlabOf<DT>;
-      a.load(next, left_a, zero, wave, lane);
-      b.load(next + A::kBytes, left_b, zero, wave, lane);
+  const auto fetch_full = [&](int buffer) {
+    char* dst = lds + buffer * kStage;
+    a.template load<false>(dst, 0, wave, lane);
+    b.template load<false>(dst + A::kBytes, 0, wave, lane);
+  };
+  const auto fetch = [&](int slab, int buffer) {
+    if (slab + 1 < slabs) {
+      fetch_full(buffer);
+    } else {
+      char* dst = lds + buffer * kStage;
+      a.template load<true>(dst, last_a, wave, lane);
+      b.template load<true>(dst + A::kBytes, last_b, wave, lane);
     }
+  };
+  const auto read = [&](v4i (&fa)[FM], v4i (&fb)[FN], int buffer, int kk) {
+    const char* cur = lds + buffer * kStage;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4i fa[FM], fb[FN];
+    for (int i = 0; i < FN; ++i)
+      fb[i] = B::frag(cur + A::kBytes, wn * (FN * 16) + i * 16, kk, lane);
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-        fb[i] = B::frag(cur + A::kBytes, wn * (FN * 16) + i * 16, kk, lane);
+    for (int i = 0; i < FM; ++i) fa[i] = A::frag(cur, wm * (FM * 16) + i * 16, kk, lane);
+  };
+  const auto multiply = [&](const v4i (&fa)[FM], const v4i (&fb)[FN]) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = A::frag(cur, wm * (FM * 16) + i * 16, kk, lane);
+    for (int j = 0; j < FM; ++j)
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) mma<DT>(acc[i][j], fb[i], fa[j]);
+      for (int i = 0; i < FN; ++i) mma<DT>(acc[i][j], fb[i], fa[j]);
+  };
+
+  if constexpr (STAGES == 0) {
+    const auto settle = [] {
+      __builtin_amdgcn_sched_barrier(0);
+      wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    v4i fa[2][FM], fb[2][FN];
+    fetch(0, 0);
+    settle();
+    if (slabs > 1) fetch(1, 1);
+    read(fa[0], fb[0], 0, 0);
+    int t = 0;
+    for (; t + 3 < slabs; ++t) {
+      read(fa[1], fb[1], t & 1, 1);
+      multiply(fa[0], fb[0]);
+      settle();
+      fetch_full(t & 1);
+      read(fa[0], fb[0], (t + 1) & 1, 0);
+      multiply(fa[1], fb[1]);
     }
-    __syncthreads();
+    for (; t < slabs; ++t) {
+      read(fa[1], fb[1], t & 1, 1);
+      multiply(fa[0], fb[0]);
+      settle();
+      if (t + 2 < slabs) fetch(t + 2, t & 1);
+      if (t + 1 < slabs) read(fa[0], fb[0], (t + 1) & 1, 0);
+      multiply(fa[1], fb[1]);
+    }
+  } else {
+    // buffer: (parity of the step) * GROUPS + group
+    if (group < slabs) fetch(group, group);
+    int buffer = group;
+    for (int t = group; t - group < slabs; t += GROUPS) {
+      __builtin_amdgcn_sched_barrier(0);
+      wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      const int other = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
+      // (the slab that the other buffer held was multiplied before the barrier)
+      if (t + GROUPS < slabs) fetch(t + GROUPS, other);
+      if (GROUPS == 1 || t < slabs) {
+        v4i fa[2][FM], fb[2][FN];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) read(fa[kk], fb[kk], buffer, kk);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) multiply(fa[kk], fb[kk]);
+      }
+      buffer = other;
+    }
+    if constexpr (GROUPS > 1) {
+      // [group - 1][fragment][lane] of every wave; the first group adds them up in order
+      constexpr int kFrags = FM * FN;
+      __syncthreads();
+      v4f* sums = (v4f*)lds;
+      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 <= (int)sizeof(lds), "fits");
+      if (group > 0) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            sums[(((group - 1) * kWaves + wave) * kFrags + i * FM + j) * kWave + lane] = acc[i][j];
+      }
+      __syncthreads();
+      if (group > 0) return;
+      for (int k = 0; k < GROUPS - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            acc[i][j] += sums[((k * kWaves + wave) * kFrags + i * FM + j) * kWave + lane];
+      epi.template run<FM, FN, BM, BN, WM, WN>(acc, m0, n0, at, wm, wn, lane, nullptr);
+      return;
+    }
   }
+  __syncthreads();
   epi.template run<FM, FN, BM, BN, WM, WN>(acc, m0, n0, at, wm, wn, lane, lds);
 }
 

@@ -27,9 +27,21 @@ struct GemmPlan {
 
 // Which operand is read along the reduction's rows (lsamp_gemm.h).
 enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
-// Tile shapes: 256 x 256, 128 x 128, 64 x 64.
-enum GemmTile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTiles = 3 };
-constexpr int kTileSide[kTiles] = {256, 128, 64};
+// Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
+// slabs of the reduction at a time, for launches of at most a tile a CU; and the
+// products of at most 16, 32 or 64 rows (lsamp_skinny.h), 64 or 16 columns a
+// work-group.
+enum GemmTile {
+  kTile256,
+  kTile128,
+  kTile64,
+  kTile128x2,
+  kTile64x4,
+  kSkinny64,
+  kSkinny16,
+};
+constexpr int kTileSide[] = {256, 128, 64, 128, 64, 64, 16};
+constexpr int kSkinnyRows = 64;
 
 // Epilogues.  `m`, `n`: rows and columns that exist; `vec`: rows of every
 // matrix start at multiples of four elements, so four columns move at once.
@@ -135,10 +147,13 @@ struct DropoutPlan {
 template <int DT>
 struct HeadOps {
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
+  // (the loss's epilogues: the first three shapes and kSkinny64)
   static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
   static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
+  // (the first five shapes)
   static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,
                         void* stream);
+  // (the first three shapes)
   static int gemm_partial(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiPartial& e,
                           void* stream);
   static int join_linear(const EpiPartial& from, int parts, const EpiLinear& e, void* stream);

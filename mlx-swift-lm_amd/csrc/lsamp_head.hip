@@ -6,6 +6,7 @@
 
 #include "lsamp_gemm.h"
 #include "lsamp_head.h"
+#include "lsamp_skinny.h"
 
 namespace lsamp {
 namespace gemm {
@@ -282,22 +283,56 @@ struct Grad : EpiGrad {
   }
 };
 
-template <bool AK, bool BK, class E, class P>
-int launch(GemmTile tile, const GemmPlan& g, const P& plan, void* stream) {
+template <class E, class P>
+E with(const P& plan) {
   E e;
   static_cast<P&>(e) = plan;
+  return e;
+}
+
+// GROUPED: the shapes that take several slabs at a time too.
+template <bool AK, bool BK, bool GROUPED, class E>
+int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (tile) {
     case kTile256:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, E>), grid, dim3(512), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, E>), grid, dim3(512), 0, st, g, e);
       break;
     case kTile128:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, E>), grid, dim3(256), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
       break;
+    case kTile64:
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
+      break;
+    case kTile128x2:
+      if constexpr (GROUPED) {
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, E>), grid, dim3(512), 0, st, g, e);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
+    case kTile64x4:
+      if constexpr (GROUPED) {
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, E>), grid, dim3(1024), 0, st, g, e);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
     default:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, E>), grid, dim3(256), 0, st, g, e);
+      return (int)hipErrorInvalidValue;
   }
+  return (int)hipGetLastError();
+}
+
+template <int NF, int WK, bool ROWWISE, class E>
+int launch_skinny(const GemmPlan& g, const E& e, void* stream) {
+  const dim3 grid((unsigned)g.tiles_n), threads(WK * kWave);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (g.a.rows <= 16)
+    hipLaunchKernelGGL((k_skinny<DT, 1, NF, WK, ROWWISE, E>), grid, threads, 0, st, g, e);
+  else if (g.a.rows <= 32)
+    hipLaunchKernelGGL((k_skinny<DT, 2, NF, WK, ROWWISE, E>), grid, threads, 0, st, g, e);
+  else
+    hipLaunchKernelGGL((k_skinny<DT, 4, NF, WK, ROWWISE, E>), grid, threads, 0, st, g, e);
   return (int)hipGetLastError();
 }
 
@@ -320,8 +355,7 @@ __global__ __launch_bounds__(kThreads) void k_join(EpiPartial from, int parts, E
 }
 template <class E, class P>
 int launch_join(const EpiPartial& from, int parts, const P& plan, void* stream) {
-  E e;
-  static_cast<P&>(e) = plan;
+  const E e = with<E>(plan);
   const int64_t quads = (int64_t)e.m * ((e.n + 3) / 4);
   int64_t blocks = (quads + kThreads - 1) / kThreads;
   blocks = blocks < 8192 ? blocks : 8192;
@@ -378,30 +412,39 @@ __global__ __launch_bounds__(kThreads) void k_col_sum_join(ColSumPlan p, S* out,
 using namespace gemm;
 
 template <>
-int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& e, void* st) {
-  return launch<false, false, Linear>(t, g, e, st);
+int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& p, void* st) {
+  const Linear e = with<Linear>(p);
+  if (t == kSkinny64) return launch_skinny<4, 4, true>(g, e, st);
+  if (t == kSkinny16) return launch_skinny<1, 8, true>(g, e, st);
+  return launch<false, false, true>(t, g, e, st);
 }
 template <>
-int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& e, void* st) {
-  return launch<false, false, Stats>(t, g, e, st);
+int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& p, void* st) {
+  const Stats e = with<Stats>(p);
+  if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
+  return launch<false, false, false>(t, g, e, st);
 }
 template <>
-int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& e, void* st) {
-  return launch<false, false, Grad>(t, g, e, st);
+int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& p, void* st) {
+  const Grad e = with<Grad>(p);
+  if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
+  return launch<false, false, false>(t, g, e, st);
 }
 template <>
-int HeadOps<DT>::gemm_store(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiStore& e,
+int HeadOps<DT>::gemm_store(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiStore& p,
                             void* st) {
-  return roles == kRolesNN ? launch<false, true, Store>(t, g, e, st)
-                           : launch<true, true, Store>(t, g, e, st);
+  const Store e = with<Store>(p);
+  return roles == kRolesNN ? launch<false, true, true>(t, g, e, st)
+                           : launch<true, true, true>(t, g, e, st);
 }
 template <>
-int HeadOps<DT>::gemm_partial(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiPartial& e,
+int HeadOps<DT>::gemm_partial(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiPartial& p,
                               void* st) {
+  const Partial e = with<Partial>(p);
   switch (roles) {
-    case kRolesNT: return launch<false, false, Partial>(t, g, e, st);
-    case kRolesNN: return launch<false, true, Partial>(t, g, e, st);
-    default: return launch<true, true, Partial>(t, g, e, st);
+    case kRolesNT: return launch<false, false, false>(t, g, e, st);
+    case kRolesNN: return launch<false, true, false>(t, g, e, st);
+    default: return launch<true, true, false>(t, g, e, st);
   }
 }
 template <>

@@ -52,8 +52,11 @@ struct Arena {
   }
 };
 
+// Whether the tiled products read a matrix as it is: rows of whole aligned
+// chunks, and a tile's rows within 32 bits of its first.
 bool chunked(const void* p, int64_t ld, int32_t cols, int eb) {
-  return (uintptr_t)p % 16 == 0 && ld * eb % 16 == 0 && (int64_t)cols * eb % 16 == 0;
+  return (uintptr_t)p % 16 == 0 && ld * eb % 16 == 0 && (int64_t)cols * eb % 16 == 0 &&
+         ld * eb <= ((int64_t)1 << 32) / 512;
 }
 
 // Whether four columns of a matrix's rows can be moved as one vector.
@@ -61,15 +64,17 @@ bool quads(const void* p, int64_t ld, int eb) {
   return !p || ((uintptr_t)p % (4 * eb) == 0 && ld % 4 == 0);
 }
 
-// A matrix as the products read it: itself, or a copy in the workspace.
+// A matrix as the products read it: itself, or a copy in the workspace (`any`:
+// the product takes any row).
 struct Operand {
   MatrixRef ref;
   bool packed;
   PackPlan pack;
 };
-Operand operand(Arena& ws, const void* p, int64_t ld, int32_t rows, int32_t cols, int eb) {
+Operand operand(Arena& ws, const void* p, int64_t ld, int32_t rows, int32_t cols, int eb,
+                bool any = false) {
   Operand o{};
-  if (chunked(p, ld, cols, eb)) {
+  if (any || chunked(p, ld, cols, eb)) {
     o.ref = MatrixRef{p, ld, rows, cols};
     return o;
   }
@@ -85,40 +90,59 @@ int lay_out(const Operand& o, int eb, void* stream) {
 }
 
 // Tile shape and number of parts of the reduction for an m x n product over
-// `slabs` 128-byte slabs, by the time that they take: a CU holds 1, 2 or 4
-// work-groups of the three shapes; a slab takes at least the latency of its
-// loads, and at least the time of its products shared among the CU's groups.
-// The times (microseconds) are fitted to products of 16-bit elements of 520 x
-// 776 x 1000 and 8192 x 4096 x 4096 (256: 1.4 a slab alone, 2.0 when every CU
-// is busy; 128: 0.65 and 0.52; 64: 0.42 and 0.18).
+// `slabs` 128-byte slabs, by the time that they take.  A CU holds 1, 2 or 4
+// work-groups of the three shapes; a slab takes at least its barrier, its LDS
+// reads and its products in turn, and at least the time of the products of all
+// groups on the CU.  Measured in microseconds (16-bit elements): alone on a CU
+// 1.5, 0.65 and 0.25 (304 x 2048 x 1536, 1024 x 4096 x 2048), in company 1.65,
+// 0.5 and 0.18 (8192 x 4096 x 4096); two or four slabs at a time alone 0.5 and
+// 0.16.  A split reduction is another launch, and its sums' traffic.
 struct Choice {
   GemmTile tile;
   int32_t parts;
 };
-Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
-  static const double kLatency[kTiles] = {1.4, 0.65, 0.42};
-  static const double kBusy16[kTiles] = {2.0, 0.52, 0.18};
-  static const double kBusy32[kTiles] = {7.0, 1.8, 0.5};
-  static const int kResident[kTiles] = {1, 2, 4};
+// What may share a tile's reduction: nothing, work-groups (parts), or these and
+// groups of waves.
+enum Splitting { kWhole, kParts, kAny };
+Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, Splitting split) {
+  struct Shape {
+    GemmTile tile, grouped;
+    int resident;
+    double alone, alone_grouped, busy16, busy32;
+  };
+  static const Shape kShapes[] = {{kTile256, kTile256, 1, 1.5, 1.5, 1.65, 7.0},
+                                  {kTile128, kTile128x2, 2, 0.65, 0.5, 0.5, 1.8},
+                                  {kTile64, kTile64x4, 4, 0.25, 0.16, 0.18, 0.5}};
   constexpr int kCus = 256;
-  const double* busy = dtype == LSAMP_DTYPE_F32 ? kBusy32 : kBusy16;
   Choice best{kTile64, 1};
   double best_us = 1e300;
-  for (int t = 0; t < kTiles; ++t) {
-    const int64_t tiles = ceil_div(m, kTileSide[t]) * ceil_div(n, kTileSide[t]);
-    for (int parts = 1; parts <= (may_split ? 64 : 1) && parts <= slabs; parts *= 2) {
+  for (const Shape& s : kShapes) {
+    const int64_t tiles = ceil_div(m, kTileSide[s.tile]) * ceil_div(n, kTileSide[s.tile]);
+    for (int parts = 1; parts <= (split == kWhole ? 1 : 64) && parts <= slabs; parts *= 2) {
       const int64_t each = ceil_div(tiles * parts, kCus);
-      const double per_slab = std::max((double)each * busy[t],
-                                       (double)ceil_div(each, kResident[t]) * kLatency[t]);
+      const double busy = dtype == LSAMP_DTYPE_F32 ? s.busy32 : s.busy16;
+      const bool grouped = split == kAny && parts == 1 && each == 1;
+      const double per_slab =
+          std::max((double)each * busy,
+                   (double)ceil_div(each, s.resident) * (grouped ? s.alone_grouped : s.alone));
       double us = per_slab * (double)ceil_div(slabs, parts);
       if (parts > 1) us += 4.0 + (double)parts * (double)m * (double)n * 8e-6 / 4.0;
       if (us < best_us) {
         best_us = us;
-        best = Choice{(GemmTile)t, parts};
+        best = Choice{grouped ? s.grouped : s.tile, parts};
       }
     }
   }
   return best;
+}
+// At most 64 rows are bound by reading the other operand, which the kernels of
+// lsamp_skinny.h do without a detour: 64 columns a work-group where that leaves
+// none of the device idle, else 16 (64 x 16384 x 4096: 31 us and 54; 64 x 4096 x
+// 4096: 26 and 14; 8 x 4096 x 4096: 13 and 9).  They take any rows of the other
+// operand, and of x up to kLooseRows.
+constexpr int kLooseRows = 16;
+Choice choose_skinny(int64_t m, int64_t n, bool whole_rows) {
+  return Choice{whole_rows || n >= (m > kLooseRows ? 8192 : 16384) ? kSkinny64 : kSkinny16, 1};
 }
 
 // `k`: elements of the reduction.
@@ -127,7 +151,8 @@ GemmPlan plan_gemm(const Choice& c, const MatrixRef& a, const MatrixRef& b, int6
   GemmPlan g{};
   g.a = a;
   g.b = b;
-  g.tiles_m = (int32_t)ceil_div(m, kTileSide[c.tile]);
+  const bool skinny = c.tile == kSkinny64 || c.tile == kSkinny16;
+  g.tiles_m = skinny ? 1 : (int32_t)ceil_div(m, kTileSide[c.tile]);
   g.tiles_n = (int32_t)ceil_div(n, kTileSide[c.tile]);
   g.slabs = (int32_t)ceil_div(k, 128 / eb);
   g.slabs_per_part = (int32_t)ceil_div(g.slabs, c.parts);
@@ -250,9 +275,10 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
 
   LinearPlan P{};
   Arena ws(base);
-  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
-  P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
-  P.choice = choose(m, n, slabs_of(k, eb), a->dtype, true);
+  const bool skinny = m <= kSkinnyRows;
+  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb, m <= kLooseRows);
+  P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb, skinny);
+  P.choice = skinny ? choose_skinny(m, n, false) : choose(m, n, slabs_of(k, eb), a->dtype, kAny);
   P.gemm = plan_gemm(P.choice, P.x.ref, P.w.ref, m, n, k, eb);
   if (too_many(P.gemm))
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
@@ -302,7 +328,7 @@ Product plan_product(Arena& ws, GemmRoles roles, const MatrixRef& a, const Matri
   const int eb = element_bytes(dtype);
   Product p{};
   p.roles = roles;
-  p.choice = choose(m, n, slabs_of(k, eb), dtype, true);
+  p.choice = choose(m, n, slabs_of(k, eb), dtype, kAny);
   p.gemm = plan_gemm(p.choice, a, b, m, n, k, eb);
   if (p.gemm.parts > 1) p.partial = take_partial(ws, m, n, p.gemm.parts);
   p.store.m = (int32_t)m;
@@ -470,16 +496,18 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
   const int32_t m = a->rows, v = a->vocab, k = a->hidden;
   LossPlan P{};
   Arena ws(base);
-  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  const bool skinny = m <= kSkinnyRows;
+  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb, m <= kLooseRows);
   const int64_t ld_w = stride_of(a->weight_stride, v, k);
   P.piece = round_up(v, kPieceStep);
-  if (!chunked(a->weight, ld_w, k, eb)) {
+  if (!skinny && !chunked(a->weight, ld_w, k, eb)) {
     const int64_t row = round_up(k, 16 / eb) * eb;
     P.piece = piece_cols(v, ((int64_t)64 << 20) / row);
     P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
     if (!base) P.packed = (void*)1;  // (sizes only)
   }
-  P.choice = choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, false);
+  P.choice = skinny ? choose_skinny(m, v, true)
+                    : choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, kWhole);
   const int64_t side = kTileSide[P.choice.tile];
   if (ceil_div(m, side) * ceil_div(P.piece, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
@@ -541,19 +569,21 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   P.ld_g = round_up(cols, 64);
   P.g = ws.take((int64_t)m * P.ld_g * eb);
   if (eb == 2) P.scale = ws.take<float>(8);
-  P.grad = choose(m, cols, slabs_of(k, eb), a->dtype, false);
+  P.grad = m <= kSkinnyRows ? choose_skinny(m, cols, true)
+                            : choose(m, cols, slabs_of(k, eb), a->dtype, kWhole);
   const int64_t side = kTileSide[P.grad.tile];
   if (ceil_div(m, side) * ceil_div(cols, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
   if (a->d_x) {
-    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, true);
+    // (the sums of all pieces are added in float32, unless there is one)
+    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, cols == v ? kAny : kParts);
     const GemmPlan g = plan_gemm(P.dx, MatrixRef{}, MatrixRef{}, m, k, cols, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", m, k);
     P.dx_straight = g.parts == 1 && cols == v;
     if (!P.dx_straight) P.dx_sum = take_partial(ws, m, k, g.parts);
   }
   if (a->d_weight) {
-    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, true);
+    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, kAny);
     const GemmPlan g = plan_gemm(P.dw, MatrixRef{}, MatrixRef{}, cols, k, m, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", v, k);
     P.dw_split = g.parts > 1;

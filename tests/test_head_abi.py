@@ -68,11 +68,14 @@ def test_linear_refusals(lib):
 
 def test_linear_workspace_counts_alignment(lib):
     f = lambda **kw: lib.lsamp_linear_workspace(ctypes.byref(linear(**kw)))  # noqa: E731
-    base = f()
-    assert f(x=P + 2) >= base + 4 * 64 * 2  # rows that start between 16-byte chunks are copied
-    assert f(x_stride=65) >= base + 4 * 64 * 2
-    assert f(x_stride=72) == base
-    assert f(rows=1, x_stride=1) >= 0  # (a one-row matrix carries any stride)
+    base = f(rows=100)
+    # rows that start between 16-byte chunks are copied; so are rows too far apart
+    assert f(rows=100, x=P + 2) >= base + 100 * 64 * 2
+    assert f(rows=100, x_stride=65) >= base + 100 * 64 * 2
+    assert f(rows=100, x_stride=1 << 30) >= base + 100 * 64 * 2
+    assert f(rows=100, x_stride=72) == base
+    assert f(x=P + 2, x_stride=65) == 0  # (few rows are read as they are)
+    assert f(rows=1, x_stride=1) == 0  # (a one-row matrix carries any stride)
 
 
 @pytest.mark.parametrize("cls,entry", [
