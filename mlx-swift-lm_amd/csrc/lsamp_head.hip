@@ -70,7 +70,27 @@ __device__ __forceinline__ float expe(float x) {
     return __expf(x);
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expe(-z)); }
+// 1 / (1 + exp(-z)) and tanh.  For 16-bit elements with the hardware's
+// reciprocal (1 ulp) in place of a division of some ten instructions, and tanh
+// as 1 - 2 / (exp(2 |x|) + 1), a polynomial below 0.3 where that cancels: off by
+// less than 6 2^-24, far below the result's own rounding.  (The library's tanhf
+// took a third of the time of a soft-capped head of 333 x 1000 x 40003.)
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (DT == LSAMP_DTYPE_F32)
+    return 1.f / (1.f + expe(-z));
+  else
+    return __builtin_amdgcn_rcpf(1.f + expe(-z));
+}
+__device__ __forceinline__ float tanhe(float x) {
+  if constexpr (DT == LSAMP_DTYPE_F32) {
+    return tanhf(x);
+  } else {
+    const float a = fabsf(x), q = x * x;
+    const float near = a + a * q * (-1.f / 3 + q * (2.f / 15 + q * (-17.f / 315 + q * (62.f / 2835))));
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(expe(2.f * a) + 1.f);
+    return copysignf(a < 0.3f ? near : far, x);
+  }
+}
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
@@ -82,8 +102,8 @@ __device__ __forceinline__ float activate(int act, float cap, float z) {
     case LSAMP_ACT_RELU: return z < 0.f ? 0.f : z;  // (a NaN stays)
     case LSAMP_ACT_SILU: return z * sigmoid(z);
     case LSAMP_ACT_GELU: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
-    case LSAMP_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(kGeluA * (z + kGeluB * z * z * z)));
-    case LSAMP_ACT_SOFTCAP: return cap * tanhf(z / cap);
+    case LSAMP_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhe(kGeluA * (z + kGeluB * z * z * z)));
+    case LSAMP_ACT_SOFTCAP: return cap * tanhe(z / cap);
     default: return z;
   }
 }
@@ -97,11 +117,11 @@ __device__ __forceinline__ float activate_slope(int act, float cap, float z) {
     case LSAMP_ACT_GELU:
       return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expe(-0.5f * z * z);
     case LSAMP_ACT_GELU_TANH: {
-      const float t = tanhf(kGeluA * (z + kGeluB * z * z * z));
+      const float t = tanhe(kGeluA * (z + kGeluB * z * z * z));
       return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluA * (1.f + 3.f * kGeluB * z * z);
     }
     case LSAMP_ACT_SOFTCAP: {
-      const float t = tanhf(z / cap);
+      const float t = tanhe(z / cap);
       return 1.f - t * t;
     }
     default: return 1.f;
@@ -125,24 +145,55 @@ __device__ __forceinline__ void put_all(const E& e, v4f (&acc)[FN][FM], int m0, 
 }
 
 struct Linear : EpiLinear {
-  __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
+  __device__ __forceinline__ v4f bias_at(int c) const {
+    return bias ? load4(bias, c, n - c, vec) : v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ v4f residual_at(int r, int c) const {
+    return residual && r < m ? load4(residual, (int64_t)r * ld_residual + c, n - c, vec)
+                             : v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void finish(int r, int c, v4f v, v4f b, v4f res) const {
     const int valid = n - c;
-    if (bias) v += load4(bias, c, valid, vec);
+    v += b;
     if (pre) store4f(pre + (int64_t)r * ld_pre + c, v, valid, vec);
     if (activation != LSAMP_ACT_NONE) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = activate(activation, softcap, v[k]);
     }
-    if (residual) v += load4(residual, (int64_t)r * ld_residual + c, valid, vec);
+    if (residual) v += res;
     if (wide)
       store4f((float*)out + (int64_t)r * ld_out + c, v, valid, vec);
     else
       store4(out, (int64_t)r * ld_out + c, v, valid, vec);
   }
+  __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
+    finish(r, c, v, bias_at(c), residual_at(r, c));
+  }
+  // A row's residual is on its way while the row before is stored (which may be
+  // the residual's own memory, so the compiler keeps the order as written).
   template <int FM, int FN, int BM, int BN, int WM, int WN>
-  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
                                       int lane, char*) const {
-    put_all<Linear, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+    const int r0 = m0 + wm * (FM * 16) + (lane & 15);
+    const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
+    v4f b[FN], res[2][FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      b[i] = bias_at(c0 + i * 16);
+      res[0][i] = residual_at(r0, c0 + i * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int r = r0 + j * 16;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+        if (j + 1 < FM) res[(j + 1) & 1][i] = residual_at(r + 16, c0 + i * 16);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int c = c0 + i * 16;
+        if (r < m && c < n) finish(r, c, acc[i][j], b[i], res[j & 1][i]);
+      }
+    }
   }
 };
 
@@ -154,36 +205,61 @@ struct Store : EpiStore {
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char*) const {
-    put_all<Store, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+    if (scale) {  // (once: the stores may be to its memory for all the compiler knows)
+      const float s = *scale;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] *= s;
+    }
+    Store plain = *this;
+    plain.scale = nullptr;
+    put_all<Store, FM, FN, BM, BN, WM, WN>(plain, acc, m0, n0, at.part, wm, wn, lane);
   }
 };
 
 struct Partial : EpiPartial {
+  __device__ __forceinline__ v4f* at(int r, int c, int part) const {
+    return (v4f*)(out + part * part_stride + (int64_t)r * ld + c);
+  }
   __device__ __forceinline__ void put(int r, int c, v4f v, int part) const {
-    v4f* p = (v4f*)(out + part * part_stride + (int64_t)r * ld + c);
+    v4f* p = at(r, c, part);
     if (accumulate) v += *p;
     *p = v;
   }
   template <int FM, int FN, int BM, int BN, int WM, int WN>
-  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt tile, int wm, int wn,
                                       int lane, char*) const {
-    put_all<Partial, FM, FN, BM, BN, WM, WN>(*this, acc, m0, n0, at.part, wm, wn, lane);
+    if (accumulate) {  // all reads before the first store
+      const int r0 = m0 + wm * (FM * 16) + (lane & 15);
+      const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+          if (r0 + j * 16 < m && c0 + i * 16 < n) acc[i][j] += *at(r0 + j * 16, c0 + i * 16, tile.part);
+    }
+    Partial plain = *this;
+    plain.accumulate = 0;
+    put_all<Partial, FM, FN, BM, BN, WM, WN>(plain, acc, m0, n0, tile.part, wm, wn, lane);
   }
 };
 
-// z = softcap(sum + bias) of a piece's column; t = tanh(. / softcap).
-__device__ __forceinline__ v4f logits4(v4f v, const void* bias, int col, int valid, float softcap,
-                                       v4f* slope) {
-  if (bias) v += load4(bias, col, valid, false);
+// z = softcap(sum + bias) of four columns, and the slope of the cap.
+__device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float inverse, v4f* slope) {
+  v += b;
   if (softcap > 0.f) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float t = tanhf(v[k] / softcap);
+      const float t = tanhe(v[k] * inverse);
       v[k] = softcap * t;
       if (slope) (*slope)[k] = 1.f - t * t;
     }
   }
   return v;
+}
+__device__ __forceinline__ v4f head_bias(const void* bias, int col, int valid) {
+  return bias ? load4(bias, col, valid, false) : v4f{0.f, 0.f, 0.f, 0.f};
 }
 
 // The forward pass keeps, of a tile's logits, each row's maximum and the sum of
@@ -195,6 +271,13 @@ struct Stats : EpiStats {
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char* lds) const {
     float* red = (float*)lds;  // [WN][BM][2]
+    const float inverse = softcap > 0.f ? 1.f / softcap : 0.f;
+    v4f b[FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
+      b[i] = head_bias(bias, first_col + c, n - c);
+    }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       const int rl = wm * (FM * 16) + j * 16 + (lane & 15);
@@ -205,7 +288,7 @@ struct Stats : EpiStats {
       for (int i = 0; i < FN; ++i) {
         const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
         const int valid = n - c;
-        const v4f v = logits4(acc[i][j], bias, first_col + c, valid, softcap, nullptr);
+        const v4f v = logits4(acc[i][j], b[i], softcap, inverse, nullptr);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const bool ok = k < valid;
@@ -257,25 +340,37 @@ struct Grad : EpiGrad {
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
                                       int lane, char*) const {
     const float s = scale ? scale[0] : 1.f;
+    const float inverse = softcap > 0.f ? 1.f / softcap : 0.f;
+    const int r0 = m0 + wm * (FM * 16) + (lane & 15);
+    const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
+    v4f b[FN];
+    int target[FM];
+    float l[FM], w[FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) b[i] = head_bias(bias, first_col + c0 + i * 16, n - c0 - i * 16);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const int r = m0 + wm * (FM * 16) + j * 16 + (lane & 15);
+      const int r = min(r0 + j * 16, m - 1);
+      target[j] = targets[r];
+      l[j] = lse[r];
+      w[j] = d_loss[r] * s;
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int r = r0 + j * 16;
       if (r >= m) continue;
-      const int target = targets[r];
-      const float l = lse[r];
-      const bool none = target < 0 || target >= vocab || l == -INFINITY;
-      const float w = d_loss[r] * s;
+      const bool none = target[j] < 0 || target[j] >= vocab || l[j] == -INFINITY;
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
+        const int c = c0 + i * 16;
         if (c >= n_pad) continue;
         v4f slope = {1.f, 1.f, 1.f, 1.f}, g;
         const int valid = n - c;
-        const v4f z = logits4(acc[i][j], bias, first_col + c, valid, softcap, &slope);
+        const v4f z = logits4(acc[i][j], b[i], softcap, inverse, &slope);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float p = expe(z[k] - l) - (first_col + c + k == target ? 1.f : 0.f);
-          g[k] = none || k >= valid ? 0.f : w * p * slope[k];
+          const float p = expe(z[k] - l[j]) - (first_col + c + k == target[j] ? 1.f : 0.f);
+          g[k] = none || k >= valid ? 0.f : w[j] * p * slope[k];
         }
         store4(out, (int64_t)r * ld_out + c, g, 4, true);
       }
@@ -398,11 +493,20 @@ __global__ __launch_bounds__(kThreads) void k_col_sum(ColSumPlan p) {
     *(v4f*)(p.part + (int64_t)blockIdx.y * p.ld_part + c) = sum;
   }
 }
+// 64 columns a work-group, its waves taking chunks in turn.
 __global__ __launch_bounds__(kThreads) void k_col_sum_join(ColSumPlan p, S* out, const float* scale) {
-  const int c = (int)(blockIdx.x * kThreads + threadIdx.x);
-  if (c >= p.cols) return;
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (int)blockIdx.x * 64 + lane;
   float s = 0.f;
-  for (int i = 0; i < p.chunks; ++i) s += p.part[(int64_t)i * p.ld_part + c];
+  if (c < p.cols) {
+#pragma unroll 8
+    for (int i = wave; i < p.chunks; i += 4) s += p.part[(int64_t)i * p.ld_part + c];
+  }
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= p.cols) return;
+  s = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
   out[c] = (S)(scale ? s * *scale : s);
 }
 
@@ -464,8 +568,7 @@ int HeadOps<DT>::col_sum(const ColSumPlan& p, void* stream) {
 }
 template <>
 int HeadOps<DT>::col_sum_join(const ColSumPlan& p, void* out, const float* scale, void* stream) {
-  hipLaunchKernelGGL(k_col_sum_join, dim3((unsigned)((p.cols + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), p, (S*)out, scale);
+  hipLaunchKernelGGL(k_col_sum_join, dim3((unsigned)((p.cols + 63) / 64)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), p, (S*)out, scale);
   return (int)hipGetLastError();
 }
 

@@ -29,6 +29,13 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
+def _stream_of(device: torch.device) -> int:
+    """The current torch stream's handle (without the 2 us of building a
+    torch.cuda.Stream, as long as a small launch itself)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
 class PreparedCall:
     """One bound C call; `keep_alive` holds every tensor whose pointer it has."""
 
@@ -41,7 +48,7 @@ class PreparedCall:
             raise ValueError(f"tensors are on {device}, the context on cuda:{ctx.device}")
         self.keep_alive = []
         self.args = None
-        self.stream = torch.cuda.current_stream(device).cuda_stream
+        self.stream = _stream_of(device)
 
     # ------------------------------------------------------------- arguments
     def _matrix(self, name: str, t: torch.Tensor, rows: Optional[int] = None,
@@ -90,7 +97,7 @@ class PreparedCall:
                 args.workspace_bytes = need
 
     def launch(self, stream: Optional[int] = None) -> None:
-        s = stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
+        s = stream if stream is not None else _stream_of(self.device)
         if s != self.stream:
             # the allocator must not hand these out while this stream reads them
             ext = torch.cuda.ExternalStream(s, device=self.device)
