@@ -28,6 +28,8 @@
 
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "lsamp_head.h"
 
 namespace lsamp {
@@ -79,7 +81,7 @@ constexpr int kChunkOf = 16 / El<DT>::kBytes;  // elements of a 16-byte chunk
 template <int DT>
 constexpr int kSlabOf = kSlabBytes / El<DT>::kBytes;  // reduction steps of a slab
 
-// acc += 16 x 16 outer products over the reduction steps of one chunk per lane
+// acc += 16 x 16 products over the reduction steps of one chunk per lane
 // (32 steps of 16-bit elements, 16 of float32).  Lane l holds row l & 15 and the
 // chunk of steps l >> 4.  The float32 instruction takes one step of a lane at a
 // time: step j of every lane's chunk, which is a different set of reduction steps
@@ -100,6 +102,65 @@ __device__ __forceinline__ void mma(v4f& acc, const v4i& b, const v4i& a) {
   }
 }
 
+// Float32 products on the bfloat16 matrix instructions.  A value is split into
+// three bfloat16 parts, a = h + m + l, h its first 8 bits (cut off, so that it is
+// finite), m and l the rest rounded; a b = hh + hm + mh + mm + hl + lh, and what
+// is left out is below 2^-23 |a b|, 2^-25 in the mean, so the sums are those of
+// float32.  Six instructions of 16 cycles take 32 steps of a 16 x 16 tile, the
+// float32 instruction takes 256 cycles.
+//
+// An infinity or a NaN has no remainder: it turns its row or column of the tile
+// into NaN.  A tile that ends with one is computed again with such values left
+// out of the products of remainders (`hx`).  The products of finite values are
+// the same ones in the same order, so no other row of the result changes.
+struct Split {
+  v8bf h, m, l;
+};
+struct SplitAny {
+  v8bf h, hx, m, l;
+};
+__device__ __forceinline__ Split split8(const v4i& a, const v4i& b) {
+  Split s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int bits = i < 4 ? a[i] : b[i - 4];
+    const float h = __builtin_bit_cast(float, bits & (int)0xffff0000);
+    const float r = __builtin_bit_cast(float, bits) - h;
+    const __bf16 m = (__bf16)r;
+    s.h[i] = __builtin_bit_cast(__bf16, (short)(bits >> 16));
+    s.m[i] = m;
+    s.l[i] = (__bf16)(r - (float)m);
+  }
+  return s;
+}
+__device__ __forceinline__ SplitAny split8_any(const v4i& a, const v4i& b) {
+  SplitAny s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int bits = i < 4 ? a[i] : b[i - 4];
+    const float v = __builtin_bit_cast(float, bits);
+    const bool finite = (bits & 0x7f800000) != 0x7f800000;
+    const float h = __builtin_bit_cast(float, bits & (int)0xffff0000);
+    const float r = finite ? v - h : 0.f;
+    const __bf16 m = (__bf16)r;
+    s.h[i] = (__bf16)(finite ? h : v);
+    s.hx[i] = (__bf16)(finite ? h : 0.f);
+    s.m[i] = m;
+    s.l[i] = (__bf16)(r - (float)m);
+  }
+  return s;
+}
+__device__ __forceinline__ void mma_split(v4f& acc, const v8bf& bh, const v8bf& bx, const v8bf& bm,
+                                          const v8bf& bl, const v8bf& ah, const v8bf& ax,
+                                          const v8bf& am, const v8bf& al) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bl, ax, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bx, al, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bm, am, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bm, ax, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bx, am, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bh, ah, acc, 0, 0, 0);
+}
+
 // Where chunk `c` of slab row `r` of a k-major slab is kept.  16-bit: a fragment
 // is a 32-byte pair of chunks of the rows 8 g + j (g, j = 0..3), and the pair
 // moves with bits of j and g; float32: a 64-byte half of the rows 4 g + j.
@@ -109,6 +170,26 @@ __device__ __forceinline__ int kmajor_place(int r, int c) {
     return c ^ ((((r >> 1) & 1) | (((r >> 3) & 1) << 1)) << 1);
   else
     return c ^ (((r >> 2) & 1) << 2);
+}
+
+// 16 bytes a lane from memory to LDS, lane after lane from LDS address `lds` (the
+// same for the wave).  Written out because the compiler makes every later LDS
+// read wait for such loads, also a read of the other buffer; here the wave waits
+// where it must (wait_loads) and nowhere else.  No register is written.
+__device__ __forceinline__ uint32_t lds_address(char* lds) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+}
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(p)
+               : "memory", "m0");
 }
 
 // One operand's side of a work-group's tile: ROWS output rows (or columns), read
@@ -162,7 +243,22 @@ struct Side {
   // One slab to LDS.  TAIL: only `left` reduction steps remain; the chunks (rows)
   // past them come from a zeroed buffer.
   template <bool TAIL>
-  __device__ __forceinline__ void load(char* lds, int left, int wave, int lane) {
+  __device__ __forceinline__ void load(uint32_t lds, int left, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const uint32_t dst = lds + (wave * kUnits + i) * 1024;
+      if constexpr (TAIL) {
+        const int k = KMAJ ? slab_row(wave, lane, i) : koff;
+        load_to_lds(dst, k < left ? base + off[i] : (const char*)kZeros);
+      } else {
+        load_to_lds(dst, base, off[i]);
+      }
+    }
+    base += step;
+  }
+  // The same, known to the compiler: among loads whose results it waits for.
+  template <bool TAIL>
+  __device__ __forceinline__ void load_counted(char* lds, int left, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const char* p = base + off[i];
@@ -250,7 +346,7 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
 // registers: after that barrier slab t + 2 may overwrite it, and slab t + 1
 // (loaded a whole slab ago) is complete.
 template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, int STAGES, int GROUPS, class Epi>
-__global__ __launch_bounds__(WM* WN* GROUPS* kWave) void k_gemm(GemmPlan g, Epi epi) {
+__global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, Epi epi) {
   constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   using A = Side<DT, AK, BM, kWaves>;
@@ -283,8 +379,9 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave) void k_gemm(GemmPlan g, Epi 
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
+  const uint32_t lds0 = lds_address(lds);
   const auto fetch_full = [&](int buffer) {
-    char* dst = lds + buffer * kStage;
+    const uint32_t dst = lds0 + buffer * kStage;
     a.template load<false>(dst, 0, wave, lane);
     b.template load<false>(dst + A::kBytes, 0, wave, lane);
   };
@@ -292,7 +389,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave) void k_gemm(GemmPlan g, Epi 
     if (slab + 1 < slabs) {
       fetch_full(buffer);
     } else {
-      char* dst = lds + buffer * kStage;
+      const uint32_t dst = lds0 + buffer * kStage;
       a.template load<true>(dst, last_a, wave, lane);
       b.template load<true>(dst + A::kBytes, last_b, wave, lane);
     }
@@ -342,25 +439,72 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave) void k_gemm(GemmPlan g, Epi 
       multiply(fa[1], fb[1]);
     }
   } else {
-    // buffer: (parity of the step) * GROUPS + group
-    if (group < slabs) fetch(group, group);
-    int buffer = group;
-    for (int t = group; t - group < slabs; t += GROUPS) {
-      __builtin_amdgcn_sched_barrier(0);
-      wait_loads<0>();
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      const int other = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
-      // (the slab that the other buffer held was multiplied before the barrier)
-      if (t + GROUPS < slabs) fetch(t + GROUPS, other);
-      if (GROUPS == 1 || t < slabs) {
-        v4i fa[2][FM], fb[2][FN];
+    // ANY: float32 values that may not be finite.
+    const auto reduce = [&](auto any) {
+      // buffer: (parity of the step) * GROUPS + group
+      if (group < slabs) fetch(group, group);
+      int buffer = group;
+      for (int t = group; t - group < slabs; t += GROUPS) {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        const int other = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
+        // (the slab that the other buffer held was multiplied before the barrier)
+        if (t + GROUPS < slabs) fetch(t + GROUPS, other);
+        if (GROUPS == 1 || t < slabs) {
+          v4i fa[2][FM], fb[2][FN];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) read(fa[kk], fb[kk], buffer, kk);
+          for (int kk = 0; kk < 2; ++kk) read(fa[kk], fb[kk], buffer, kk);
+          if constexpr (DT != LSAMP_DTYPE_F32) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) multiply(fa[kk], fb[kk]);
+            for (int kk = 0; kk < 2; ++kk) multiply(fa[kk], fb[kk]);
+          } else if constexpr (!decltype(any)::value) {
+            Split sb[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) sb[i] = split8(fb[0][i], fb[1][i]);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+              __builtin_amdgcn_sched_barrier(0);  // (one split fragment of A at a time)
+              const Split sa = split8(fa[0][j], fa[1][j]);
+#pragma unroll
+              for (int i = 0; i < FN; ++i)
+                mma_split(acc[i][j], sb[i].h, sb[i].h, sb[i].m, sb[i].l, sa.h, sa.h, sa.m, sa.l);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+#pragma unroll
+              for (int i = 0; i < FN; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                const SplitAny sb = split8_any(fb[0][i], fb[1][i]), sa = split8_any(fa[0][j], fa[1][j]);
+                mma_split(acc[i][j], sb.h, sb.hx, sb.m, sb.l, sa.h, sa.hx, sa.m, sa.l);
+              }
+          }
+        }
+        buffer = other;
       }
-      buffer = other;
+    };
+    reduce(std::false_type{});
+    if constexpr (DT == LSAMP_DTYPE_F32) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) nan |= acc[i][j][k] != acc[i][j][k];
+      if (__syncthreads_or(nan)) {
+        a.init(g.a, m0, slab0 + group, wave, lane);
+        b.init(g.b, n0, slab0 + group, wave, lane);
+        a.step *= GROUPS;
+        b.step *= GROUPS;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        reduce(std::true_type{});
+      }
     }
     if constexpr (GROUPS > 1) {
       // [group - 1][fragment][lane] of every wave; the first group adds them up in order

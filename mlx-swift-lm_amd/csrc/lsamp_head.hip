@@ -385,15 +385,19 @@ E with(const P& plan) {
   return e;
 }
 
-// GROUPED: the shapes that take several slabs at a time too.
+// GROUPED: the shapes that take several slabs at a time too.  (float32 tiles go up
+// to 128 x 128: a wave's split fragments need the registers.)
 template <bool AK, bool BK, bool GROUPED, class E>
 int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (tile) {
     case kTile256:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, E>), grid, dim3(512), 0, st, g, e);
-      break;
+      if constexpr (DT != LSAMP_DTYPE_F32) {
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, E>), grid, dim3(512), 0, st, g, e);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
     case kTile128:
       hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
       break;

@@ -108,11 +108,14 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, Splitting split) {
   struct Shape {
     GemmTile tile, grouped;
     int resident;
-    double alone, alone_grouped, busy16, busy32;
+    struct {
+      double alone, alone_grouped, busy;
+    } us[2];  // 16-bit elements, float32
   };
-  static const Shape kShapes[] = {{kTile256, kTile256, 1, 1.5, 1.5, 1.65, 7.0},
-                                  {kTile128, kTile128x2, 2, 0.65, 0.5, 0.5, 1.8},
-                                  {kTile64, kTile64x4, 4, 0.25, 0.16, 0.18, 0.5}};
+  static const Shape kShapes[] = {
+      {kTile256, kTile256, 1, {{1.5, 1.5, 1.65}, {1e30, 1e30, 1e30}}},
+      {kTile128, kTile128x2, 2, {{0.65, 0.5, 0.5}, {0.95, 0.8, 0.8}}},
+      {kTile64, kTile64x4, 4, {{0.25, 0.16, 0.18}, {0.5, 0.38, 0.38}}}};
   constexpr int kCus = 256;
   Choice best{kTile64, 1};
   double best_us = 1e300;
@@ -120,11 +123,11 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, Splitting split) {
     const int64_t tiles = ceil_div(m, kTileSide[s.tile]) * ceil_div(n, kTileSide[s.tile]);
     for (int parts = 1; parts <= (split == kWhole ? 1 : 64) && parts <= slabs; parts *= 2) {
       const int64_t each = ceil_div(tiles * parts, kCus);
-      const double busy = dtype == LSAMP_DTYPE_F32 ? s.busy32 : s.busy16;
+      const auto& us_of = s.us[dtype == LSAMP_DTYPE_F32];
       const bool grouped = split == kAny && parts == 1 && each == 1;
       const double per_slab =
-          std::max((double)each * busy,
-                   (double)ceil_div(each, s.resident) * (grouped ? s.alone_grouped : s.alone));
+          std::max((double)each * us_of.busy, (double)ceil_div(each, s.resident) *
+                                                  (grouped ? us_of.alone_grouped : us_of.alone));
       double us = per_slab * (double)ceil_div(slabs, parts);
       if (parts > 1) us += 4.0 + (double)parts * (double)m * (double)n * 8e-6 / 4.0;
       if (us < best_us) {

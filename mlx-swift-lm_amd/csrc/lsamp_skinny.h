@@ -92,7 +92,7 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
   const auto load = [&](Step& s, int slab, int buffer) {
     if constexpr (kStaged) {
       x.base = x_base + (int64_t)slab * kSlabBytes;
-      x.template load<false>(mine + buffer * X::kBytes, 0, 0, lane);
+      x.template load_counted<false>(mine + buffer * X::kBytes, 0, 0, lane);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
       wait_loads<0>();
       __builtin_amdgcn_sched_barrier(0);
       x.base = x_base + (int64_t)whole * kSlabBytes;
-      x.template load<true>(mine, g.a.cols - whole * kSlab, 0, lane);
+      x.template load_counted<true>(mine, g.a.cols - whole * kSlab, 0, lane);
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
