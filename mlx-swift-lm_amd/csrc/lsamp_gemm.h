@@ -175,7 +175,8 @@ __device__ __forceinline__ int kmajor_place(int r, int c) {
 // 16 bytes a lane from memory to LDS, lane after lane from LDS address `lds` (the
 // same for the wave).  Written out because the compiler makes every later LDS
 // read wait for such loads, also a read of the other buffer; here the wave waits
-// where it must (wait_loads) and nowhere else.  No register is written.
+// where it must (wait_loads) and nowhere else.  No vector register is written;
+// M0 is the compiler's only around single instructions that it sets it for.
 __device__ __forceinline__ uint32_t lds_address(char* lds) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 }
@@ -183,13 +184,13 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* base, uint
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(p)
-               : "memory", "m0");
+               : "memory");
 }
 
 // One operand's side of a work-group's tile: ROWS output rows (or columns), read
@@ -328,7 +329,8 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
   return t;
 }
 
-// One tile.  Epi: what happens to the sums; called once per work-group with
+// One tile.  Epi: what happens to the sums, with kBarriers barriers; called by the
+// waves that hold them with
 //   run(acc, m0, n0, at, wave-in-M, wave-in-N, lane, lds)
 // where acc[fn][fm][i] is row m0 + fm * 16 + (lane & 15), column
 // n0 + fn * 16 + (lane >> 4) * 4 + i of the wave's part.
@@ -511,7 +513,8 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
       constexpr int kFrags = FM * FN;
       __syncthreads();
       v4f* sums = (v4f*)lds;
-      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 <= (int)sizeof(lds), "fits");
+      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + WN * BM * 8 <= (int)sizeof(lds),
+                    "the sums and an epilogue's pair of floats for every row and wave");
       if (group > 0) {
 #pragma unroll
         for (int i = 0; i < FN; ++i)
@@ -520,14 +523,19 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
             sums[(((group - 1) * kWaves + wave) * kFrags + i * FM + j) * kWave + lane] = acc[i][j];
       }
       __syncthreads();
-      if (group > 0) return;
+      if (group > 0) {
+        for (int k = 0; k < Epi::kBarriers; ++k) __syncthreads();  // (those of the epilogue)
+        return;
+      }
       for (int k = 0; k < GROUPS - 1; ++k)
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
           for (int j = 0; j < FM; ++j)
             acc[i][j] += sums[((k * kWaves + wave) * kFrags + i * FM + j) * kWave + lane];
-      epi.template run<FM, FN, BM, BN, WM, WN>(acc, m0, n0, at, wm, wn, lane, nullptr);
+      epi.template run<FM, FN, BM, BN, WM, WN>(
+          acc, m0, n0, at, wm, wn, lane,
+          lds + (GROUPS - 1) * kWaves * kFrags * kWave * 16);
       return;
     }
   }

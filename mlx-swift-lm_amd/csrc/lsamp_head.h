@@ -147,13 +147,11 @@ struct DropoutPlan {
 template <int DT>
 struct HeadOps {
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
-  // (the loss's epilogues: the first three shapes and kSkinny64)
+  // (kSkinny16: gemm_linear only, kSkinny64 not gemm_store and gemm_partial)
   static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
   static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
-  // (the first five shapes)
   static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,
                         void* stream);
-  // (the first three shapes)
   static int gemm_partial(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiPartial& e,
                           void* stream);
   static int join_linear(const EpiPartial& from, int parts, const EpiLinear& e, void* stream);

@@ -145,6 +145,7 @@ __device__ __forceinline__ void put_all(const E& e, v4f (&acc)[FN][FM], int m0, 
 }
 
 struct Linear : EpiLinear {
+  static constexpr int kBarriers = 0;
   __device__ __forceinline__ v4f bias_at(int c) const {
     return bias ? load4(bias, c, n - c, vec) : v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -198,6 +199,7 @@ struct Linear : EpiLinear {
 };
 
 struct Store : EpiStore {
+  static constexpr int kBarriers = 0;
   __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
     if (scale) v *= *scale;
     store4(out, (int64_t)r * ld_out + c, v, n - c, vec);
@@ -219,6 +221,7 @@ struct Store : EpiStore {
 };
 
 struct Partial : EpiPartial {
+  static constexpr int kBarriers = 0;
   __device__ __forceinline__ v4f* at(int r, int c, int part) const {
     return (v4f*)(out + part * part_stride + (int64_t)r * ld + c);
   }
@@ -267,6 +270,7 @@ __device__ __forceinline__ v4f head_bias(const void* bias, int col, int valid) {
 // then the waves of the row through LDS.  A row whose logits here are all -inf
 // has maximum -inf and sum 0.
 struct Stats : EpiStats {
+  static constexpr int kBarriers = 1;
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char* lds) const {
@@ -336,6 +340,7 @@ struct Stats : EpiStats {
 // of that type; 16-bit values are scaled first (k_grad_scale).  A row without
 // a loss (target ignored or out of range, every logit -inf) is zero.
 struct Grad : EpiGrad {
+  static constexpr int kBarriers = 0;
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
                                       int lane, char*) const {
@@ -385,9 +390,8 @@ E with(const P& plan) {
   return e;
 }
 
-// GROUPED: the shapes that take several slabs at a time too.  (float32 tiles go up
-// to 128 x 128: a wave's split fragments need the registers.)
-template <bool AK, bool BK, bool GROUPED, class E>
+// (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
+template <bool AK, bool BK, class E>
 int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -405,17 +409,11 @@ int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
       hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
       break;
     case kTile128x2:
-      if constexpr (GROUPED) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, E>), grid, dim3(512), 0, st, g, e);
-        break;
-      }
-      return (int)hipErrorInvalidValue;
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, E>), grid, dim3(512), 0, st, g, e);
+      break;
     case kTile64x4:
-      if constexpr (GROUPED) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, E>), grid, dim3(1024), 0, st, g, e);
-        break;
-      }
-      return (int)hipErrorInvalidValue;
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, E>), grid, dim3(1024), 0, st, g, e);
+      break;
     default:
       return (int)hipErrorInvalidValue;
   }
@@ -438,25 +436,37 @@ int launch_skinny(const GemmPlan& g, const E& e, void* stream) {
 // ------------------------------------------------------------- passes between
 constexpr int kThreads = 256;
 
-// The parts of a split reduction, summed in their order, and the epilogue.
+// The parts of a split reduction, summed, and the epilogue: 64 quads of columns a
+// work-group, each wave a quarter of the parts, always in the same order.
 template <class E>
 __global__ __launch_bounds__(kThreads) void k_join(EpiPartial from, int parts, E e) {
+  __shared__ v4f red[3][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int quads = (e.n + 3) / 4;
   const int64_t total = (int64_t)e.m * quads;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * kThreads) {
+  for (int64_t first = (int64_t)blockIdx.x * 64; first < total; first += (int64_t)gridDim.x * 64) {
+    const int64_t i = first + lane;
     const int r = (int)(i / quads), c = (int)(i % quads) * 4;
-    const float* p = from.out + (int64_t)r * from.ld + c;
-    v4f v = *(const v4f*)p;
-    for (int k = 1; k < parts; ++k) v += *(const v4f*)(p + k * from.part_stride);
-    e.put(r, c, v, 0);
+    v4f v = {0.f, 0.f, 0.f, 0.f};
+    if (i < total) {
+      const float* p = from.out + (int64_t)r * from.ld + c;
+#pragma unroll 8
+      for (int k = wave; k < parts; k += 4) v += *(const v4f*)(p + k * from.part_stride);
+    }
+    if (wave > 0) red[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave == 0 && i < total) {
+      for (int k = 0; k < 3; ++k) v += red[k][lane];
+      e.put(r, c, v, 0);
+    }
+    __syncthreads();
   }
 }
 template <class E, class P>
 int launch_join(const EpiPartial& from, int parts, const P& plan, void* stream) {
   const E e = with<E>(plan);
   const int64_t quads = (int64_t)e.m * ((e.n + 3) / 4);
-  int64_t blocks = (quads + kThreads - 1) / kThreads;
+  int64_t blocks = (quads + 63) / 64;
   blocks = blocks < 8192 ? blocks : 8192;
   hipLaunchKernelGGL((k_join<E>), dim3((unsigned)blocks), dim3(kThreads), 0,
                      reinterpret_cast<hipStream_t>(stream), from, parts, e);
@@ -524,35 +534,35 @@ int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& p, 
   const Linear e = with<Linear>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, true>(g, e, st);
   if (t == kSkinny16) return launch_skinny<1, 8, true>(g, e, st);
-  return launch<false, false, true>(t, g, e, st);
+  return launch<false, false>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& p, void* st) {
   const Stats e = with<Stats>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
-  return launch<false, false, false>(t, g, e, st);
+  return launch<false, false>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& p, void* st) {
   const Grad e = with<Grad>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
-  return launch<false, false, false>(t, g, e, st);
+  return launch<false, false>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_store(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiStore& p,
                             void* st) {
   const Store e = with<Store>(p);
-  return roles == kRolesNN ? launch<false, true, true>(t, g, e, st)
-                           : launch<true, true, true>(t, g, e, st);
+  return roles == kRolesNN ? launch<false, true>(t, g, e, st)
+                           : launch<true, true>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_partial(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiPartial& p,
                               void* st) {
   const Partial e = with<Partial>(p);
   switch (roles) {
-    case kRolesNT: return launch<false, false, false>(t, g, e, st);
-    case kRolesNN: return launch<false, true, false>(t, g, e, st);
-    default: return launch<true, true, false>(t, g, e, st);
+    case kRolesNT: return launch<false, false>(t, g, e, st);
+    case kRolesNN: return launch<false, true>(t, g, e, st);
+    default: return launch<true, true>(t, g, e, st);
   }
 }
 template <>

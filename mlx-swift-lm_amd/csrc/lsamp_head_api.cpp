@@ -101,10 +101,7 @@ struct Choice {
   GemmTile tile;
   int32_t parts;
 };
-// What may share a tile's reduction: nothing, work-groups (parts), or these and
-// groups of waves.
-enum Splitting { kWhole, kParts, kAny };
-Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, Splitting split) {
+Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
   struct Shape {
     GemmTile tile, grouped;
     int resident;
@@ -121,10 +118,10 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, Splitting split) {
   double best_us = 1e300;
   for (const Shape& s : kShapes) {
     const int64_t tiles = ceil_div(m, kTileSide[s.tile]) * ceil_div(n, kTileSide[s.tile]);
-    for (int parts = 1; parts <= (split == kWhole ? 1 : 64) && parts <= slabs; parts *= 2) {
+    for (int parts = 1; parts <= (may_split ? 64 : 1) && parts <= slabs; parts *= 2) {
       const int64_t each = ceil_div(tiles * parts, kCus);
       const auto& us_of = s.us[dtype == LSAMP_DTYPE_F32];
-      const bool grouped = split == kAny && parts == 1 && each == 1;
+      const bool grouped = each == 1;
       const double per_slab =
           std::max((double)each * us_of.busy, (double)ceil_div(each, s.resident) *
                                                   (grouped ? us_of.alone_grouped : us_of.alone));
@@ -281,7 +278,7 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
   const bool skinny = m <= kSkinnyRows;
   P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb, m <= kLooseRows);
   P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb, skinny);
-  P.choice = skinny ? choose_skinny(m, n, false) : choose(m, n, slabs_of(k, eb), a->dtype, kAny);
+  P.choice = skinny ? choose_skinny(m, n, false) : choose(m, n, slabs_of(k, eb), a->dtype, true);
   P.gemm = plan_gemm(P.choice, P.x.ref, P.w.ref, m, n, k, eb);
   if (too_many(P.gemm))
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
@@ -331,7 +328,7 @@ Product plan_product(Arena& ws, GemmRoles roles, const MatrixRef& a, const Matri
   const int eb = element_bytes(dtype);
   Product p{};
   p.roles = roles;
-  p.choice = choose(m, n, slabs_of(k, eb), dtype, kAny);
+  p.choice = choose(m, n, slabs_of(k, eb), dtype, true);
   p.gemm = plan_gemm(p.choice, a, b, m, n, k, eb);
   if (p.gemm.parts > 1) p.partial = take_partial(ws, m, n, p.gemm.parts);
   p.store.m = (int32_t)m;
@@ -510,7 +507,7 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
     if (!base) P.packed = (void*)1;  // (sizes only)
   }
   P.choice = skinny ? choose_skinny(m, v, true)
-                    : choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, kWhole);
+                    : choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, false);
   const int64_t side = kTileSide[P.choice.tile];
   if (ceil_div(m, side) * ceil_div(P.piece, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
@@ -573,20 +570,20 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   P.g = ws.take((int64_t)m * P.ld_g * eb);
   if (eb == 2) P.scale = ws.take<float>(8);
   P.grad = m <= kSkinnyRows ? choose_skinny(m, cols, true)
-                            : choose(m, cols, slabs_of(k, eb), a->dtype, kWhole);
+                            : choose(m, cols, slabs_of(k, eb), a->dtype, false);
   const int64_t side = kTileSide[P.grad.tile];
   if (ceil_div(m, side) * ceil_div(cols, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
   if (a->d_x) {
     // (the sums of all pieces are added in float32, unless there is one)
-    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, cols == v ? kAny : kParts);
+    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, true);
     const GemmPlan g = plan_gemm(P.dx, MatrixRef{}, MatrixRef{}, m, k, cols, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", m, k);
     P.dx_straight = g.parts == 1 && cols == v;
     if (!P.dx_straight) P.dx_sum = take_partial(ws, m, k, g.parts);
   }
   if (a->d_weight) {
-    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, kAny);
+    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, true);
     const GemmPlan g = plan_gemm(P.dw, MatrixRef{}, MatrixRef{}, cols, k, m, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", v, k);
     P.dw_split = g.parts > 1;
