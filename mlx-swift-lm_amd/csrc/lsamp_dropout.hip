@@ -42,14 +42,19 @@ template <typename E>
 struct Vec8 {
   E v[8];
 };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename E>
+struct __attribute__((packed, aligned(sizeof(E)))) Any16 {  // 16 bytes of any alignment
+  u32x4 v;
+};
 
 template <typename E>
-__device__ __forceinline__ Vec8<E> load8(const E* p, int valid, bool vec) {
+__device__ __forceinline__ Vec8<E> load8(const E* p, int valid) {
   Vec8<E> o;
-  if (vec && valid >= 8) {
+  if (valid >= 8) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
-      const uint4 q = ((const uint4*)p)[i];
+      const u32x4 q = ((const Any16<E>*)p)[i].v;
       __builtin_memcpy((char*)o.v + 16 * i, &q, 16);
     }
   } else {
@@ -70,9 +75,9 @@ __global__ __launch_bounds__(kThreads) void k_dropout(DropoutPlan p, int log_x) 
   const int valid = p.cols - g * 8;
   for (int64_t r = (int64_t)blockIdx.y * per_block + (threadIdx.x >> log_x); r < p.rows;
        r += (int64_t)gridDim.y * per_block) {
-    const Vec8<E> x = load8((const E*)p.x + r * p.ld_x + g * 8, valid, p.vec);
+    const Vec8<E> x = load8((const E*)p.x + r * p.ld_x + g * 8, valid);
     Vec8<E> y;
-    if (p.residual) y = load8((const E*)p.residual + r * p.ld_residual + g * 8, valid, p.vec);
+    if (p.residual) y = load8((const E*)p.residual + r * p.ld_residual + g * 8, valid);
     const Words w = philox((uint32_t)g, (uint32_t)r, (uint32_t)offset, (uint32_t)(offset >> 32),
                            (uint32_t)p.key, (uint32_t)(p.key >> 32));
 #pragma unroll
@@ -83,12 +88,12 @@ __global__ __launch_bounds__(kThreads) void k_dropout(DropoutPlan p, int log_x) 
       y.v[k] = (E)v;
     }
     E* out = (E*)p.out + r * p.ld_out + g * 8;
-    if (p.vec && valid >= 8) {
+    if (valid >= 8) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
-        uint4 q;
+        u32x4 q;
         __builtin_memcpy(&q, (const char*)y.v + 16 * i, 16);
-        ((uint4*)out)[i] = q;
+        ((Any16<E>*)out)[i].v = q;
       }
     } else {
 #pragma unroll

@@ -81,6 +81,16 @@ constexpr int kChunkOf = 16 / El<DT>::kBytes;  // elements of a 16-byte chunk
 template <int DT>
 constexpr int kSlabOf = kSlabBytes / El<DT>::kBytes;  // reduction steps of a slab
 
+// Every wave's barrier, with no memory access moved across it by the compiler
+// (and no wait: what has to be done by then is waited for by wait_loads).
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // acc += 16 x 16 products over the reduction steps of one chunk per lane
 // (32 steps of 16-bit elements, 16 of float32).  Lane l holds row l & 15 and the
 // chunk of steps l >> 4.  The float32 instruction takes one step of a lane at a
@@ -191,6 +201,28 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
                :
                : "s"(lds), "v"(p)
                : "memory");
+}
+
+// 16 bytes from an address aligned to elements only.
+template <int DT>
+__device__ __forceinline__ v4i load_chunk(const char* p) {
+  struct __attribute__((packed, aligned(El<DT>::kBytes))) Any {
+    v4i v;
+  };
+  return ((const Any*)p)->v;
+}
+// The chunk at element k of a row of `cols` elements, zero past its end.
+template <int DT>
+__device__ __forceinline__ v4i load_chunk_end(const char* row, int k, int cols) {
+  using S = typename El<DT>::S;
+  constexpr int N = kChunkOf<DT>;
+  if (k + N <= cols) return load_chunk<DT>(row + (int64_t)k * El<DT>::kBytes);
+  S e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = k + i < cols ? ((const S*)row)[k + i] : (S)0.f;
+  v4i v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
 }
 
 // One operand's side of a work-group's tile: ROWS output rows (or columns), read
@@ -308,6 +340,57 @@ struct Side {
   }
 };
 
+// The same for a matrix whose rows lie anywhere and end anywhere (`cols` exact):
+// chunks go through registers, taken by elements where a row or the reduction
+// ends, and are written to the same places of LDS.
+template <int DT, bool KMAJ, int ROWS, int WAVES>
+struct LooseSide : Side<DT, KMAJ, ROWS, WAVES> {
+  using Base = Side<DT, KMAJ, ROWS, WAVES>;
+  static constexpr int kEb = Base::kEb, kSlab = Base::kSlab, kChunk = Base::kChunk;
+  static constexpr int kUnits = Base::kUnits;
+  const char* row[kUnits];  // row-major: the row; k-major: the slab's first row
+  int col[kUnits];          // k-major: the chunk's first column
+  int64_t ld;
+  int cols;
+  v4i held[kUnits];
+
+  __device__ __forceinline__ void init(const MatrixRef& o, int first, int slab0, int wave, int lane) {
+    ld = o.ld * kEb;
+    cols = o.cols;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u = wave * kUnits + i;
+      if constexpr (!KMAJ) {
+        const int r = min(first + u * 8 + (lane >> 3), o.rows - 1);
+        row[i] = (const char*)o.p + (int64_t)r * ld;
+      } else {
+        row[i] = (const char*)o.p;
+        col[i] = first + (u / (kSlab / 8)) * kSlab +
+                 kmajor_place<DT>(Base::slab_row(wave, lane, i), lane & 7) * kChunk;
+      }
+    }
+  }
+  // Slab `slab` to registers; `rows`: k-major rows in all.
+  __device__ __forceinline__ void hold(int slab, int rows, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      if constexpr (!KMAJ) {
+        const int k = slab * kSlab + ((lane & 7) ^ (lane >> 3)) * kChunk;
+        held[i] = load_chunk_end<DT>(row[i], k, cols);
+      } else {
+        const int r = slab * kSlab + Base::slab_row(wave, lane, i);
+        held[i] = r < rows ? load_chunk_end<DT>(row[i] + (int64_t)r * ld, col[i], cols)
+                           : v4i{0, 0, 0, 0};
+      }
+    }
+  }
+  __device__ __forceinline__ void place(char* lds, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i)
+      *(v4i*)(lds + (wave * kUnits + i) * 1024 + lane * 16) = held[i];
+  }
+};
+
 // Work-group -> (tile row, tile column, part of the reduction).  Consecutive
 // work-groups go to the 8 XCDs in turn, so each XCD is given a contiguous range
 // of the order; in the order, 8 tile rows by tile columns run together, so that
@@ -342,17 +425,20 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
 // GROUPS: so many slabs are multiplied at a time, each by its own WM x WN waves,
 // and the groups' sums joined through LDS at the end: for products with fewer
 // tiles than the device has CUs, whose time is the length of the reduction.
+// LOOSE: operands that are no 16-byte chunks, through registers.
 // STAGES 0 (the 256 x 256 tile, one work-group a CU): two slabs in two halves.
 // While the products of one half run, the fragments of the next are read from
 // LDS.  In the middle of slab t every wave has its last fragments of the slab in
 // registers: after that barrier slab t + 2 may overwrite it, and slab t + 1
 // (loaded a whole slab ago) is complete.
-template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, int STAGES, int GROUPS, class Epi>
+template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, int STAGES, int GROUPS, bool LOOSE,
+          class Epi>
 __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, Epi epi) {
   constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-  using A = Side<DT, AK, BM, kWaves>;
-  using B = Side<DT, BK, BN, kWaves>;
+  using A = std::conditional_t<LOOSE, LooseSide<DT, AK, BM, kWaves>, Side<DT, AK, BM, kWaves>>;
+  using B = std::conditional_t<LOOSE, LooseSide<DT, BK, BN, kWaves>, Side<DT, BK, BN, kWaves>>;
+  static_assert(!LOOSE || STAGES == 2, "two buffers");
   constexpr int kStage = A::kBytes + B::kBytes;
   __shared__ __attribute__((aligned(1024))) char lds[2 * GROUPS * kStage];
 
@@ -367,10 +453,15 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
 
   A a;
   B b;
-  a.init(g.a, m0, slab0 + group, wave, lane);
-  b.init(g.b, n0, slab0 + group, wave, lane);
-  a.step *= GROUPS;
-  b.step *= GROUPS;
+  const auto start = [&] {
+    a.init(g.a, m0, slab0 + group, wave, lane);
+    b.init(g.b, n0, slab0 + group, wave, lane);
+    if constexpr (!LOOSE) {
+      a.step *= GROUPS;
+      b.step *= GROUPS;
+    }
+  };
+  start();
   // reduction steps of this part's last slab
   const int last_a = (AK ? g.a.rows : g.a.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
   const int last_b = (BK ? g.b.rows : g.b.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
@@ -383,17 +474,28 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
 
   const uint32_t lds0 = lds_address(lds);
   const auto fetch_full = [&](int buffer) {
-    const uint32_t dst = lds0 + buffer * kStage;
-    a.template load<false>(dst, 0, wave, lane);
-    b.template load<false>(dst + A::kBytes, 0, wave, lane);
+    if constexpr (!LOOSE) {
+      const uint32_t dst = lds0 + buffer * kStage;
+      a.template load<false>(dst, 0, wave, lane);
+      b.template load<false>(dst + A::kBytes, 0, wave, lane);
+    }
   };
   const auto fetch = [&](int slab, int buffer) {
-    if (slab + 1 < slabs) {
+    if constexpr (LOOSE) {
+      a.hold(slab0 + slab, g.a.rows, wave, lane);
+      b.hold(slab0 + slab, g.b.rows, wave, lane);
+    } else if (slab + 1 < slabs) {
       fetch_full(buffer);
     } else {
       const uint32_t dst = lds0 + buffer * kStage;
       a.template load<true>(dst, last_a, wave, lane);
       b.template load<true>(dst + A::kBytes, last_b, wave, lane);
+    }
+  };
+  const auto land = [&](int buffer) {  // LOOSE: what fetch() holds
+    if constexpr (LOOSE) {
+      a.place(lds + buffer * kStage, wave, lane);
+      b.place(lds + buffer * kStage + A::kBytes, wave, lane);
     }
   };
   const auto read = [&](v4i (&fa)[FM], v4i (&fb)[FN], int buffer, int kk) {
@@ -415,8 +517,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
     const auto settle = [] {
       __builtin_amdgcn_sched_barrier(0);
       wait_loads<0>();
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
+      barrier();
     };
     v4i fa[2][FM], fb[2][FN];
     fetch(0, 0);
@@ -444,13 +545,15 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
     // ANY: float32 values that may not be finite.
     const auto reduce = [&](auto any) {
       // buffer: (parity of the step) * GROUPS + group
-      if (group < slabs) fetch(group, group);
+      if (group < slabs) {
+        fetch(group, group);
+        land(group);
+      }
       int buffer = group;
       for (int t = group; t - group < slabs; t += GROUPS) {
         __builtin_amdgcn_sched_barrier(0);
         wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        barrier();
         const int other = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
         // (the slab that the other buffer held was multiplied before the barrier)
         if (t + GROUPS < slabs) fetch(t + GROUPS, other);
@@ -484,6 +587,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
               }
           }
         }
+        if (t + GROUPS < slabs) land(other);
         buffer = other;
       }
     };
@@ -497,10 +601,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
 #pragma unroll
           for (int k = 0; k < 4; ++k) nan |= acc[i][j][k] != acc[i][j][k];
       if (__syncthreads_or(nan)) {
-        a.init(g.a, m0, slab0 + group, wave, lane);
-        b.init(g.b, n0, slab0 + group, wave, lane);
-        a.step *= GROUPS;
-        b.step *= GROUPS;
+        start();
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll

@@ -13,6 +13,8 @@ namespace lsamp {
 // A matrix in HBM: `rows` rows of `cols` readable elements, `ld` elements
 // apart.  Products read 16-byte chunks: p and ld in bytes are multiples of 16,
 // cols of a chunk's elements.
+// (Loose shapes and the kernels of few rows read rows of any address, distance
+// and length.)
 struct MatrixRef {
   const void* p;
   int64_t ld;
@@ -28,26 +30,27 @@ struct GemmPlan {
 // Which operand is read along the reduction's rows (lsamp_gemm.h).
 enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
 // Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
-// slabs of the reduction at a time, for launches of at most a tile a CU; and the
-// products of at most 16, 32 or 64 rows (lsamp_skinny.h), 64 or 16 columns a
-// work-group.
+// slabs of the reduction at a time, for launches of at most a tile a CU; the last
+// two for operands whose rows are no 16-byte chunks; and the products of at most
+// 16, 32 or 64 rows (lsamp_skinny.h), 64 or 16 columns a work-group.
 enum GemmTile {
   kTile256,
   kTile128,
   kTile64,
   kTile128x2,
   kTile64x4,
+  kLoose64,
+  kLoose64x4,
   kSkinny64,
   kSkinny16,
 };
-constexpr int kTileSide[] = {256, 128, 64, 128, 64, 64, 16};
+constexpr int kTileSide[] = {256, 128, 64, 128, 64, 64, 64, 64, 16};
 constexpr int kSkinnyRows = 64;
 
-// Epilogues.  `m`, `n`: rows and columns that exist; `vec`: rows of every
-// matrix start at multiples of four elements, so four columns move at once.
+// Epilogues.  `m`, `n`: rows and columns that exist.
 struct EpiLinear {
   int32_t m, n;
-  int32_t activation, vec, wide;  // wide: out is float32
+  int32_t activation, wide;  // wide: out is float32
   float softcap;
   const void* bias;
   const void* residual;
@@ -59,7 +62,6 @@ struct EpiLinear {
 };
 struct EpiStore {  // out = sums * *scale, in the operands' type
   int32_t m, n;
-  int32_t vec;
   void* out;
   int64_t ld_out;
   const float* scale;  // device, or NULL for 1
@@ -115,7 +117,7 @@ struct JoinStatsPlan {
 struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial sum
   int32_t rows, cols;
   int32_t chunks, rows_per_chunk;
-  int32_t activation, vec;  // with `pre`: in * activation'(pre) is summed, and written to out
+  int32_t activation;  // with `pre`: in * activation'(pre) is summed, and written to out
   float softcap;
   const void* in;
   int64_t ld_in;
@@ -131,7 +133,6 @@ struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial s
 struct DropoutPlan {
   int32_t rows, cols;
   uint32_t cut;  // an element is kept where its 16 bits are at least this
-  int32_t vec;
   float scale;
   uint64_t key, offset;
   const uint64_t* step;
@@ -147,7 +148,8 @@ struct DropoutPlan {
 template <int DT>
 struct HeadOps {
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
-  // (kSkinny16: gemm_linear only, kSkinny64 not gemm_store and gemm_partial)
+  // (kSkinny16: gemm_linear only; kSkinny64: not gemm_store and gemm_partial;
+  // loose shapes: not the loss's)
   static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
   static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
   static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,

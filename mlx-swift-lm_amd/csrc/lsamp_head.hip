@@ -16,12 +16,17 @@ constexpr int DT = LSAMP_DT;
 using S = El<DT>::S;
 typedef S v4e __attribute__((ext_vector_type(4)));
 
-// Four columns of a row: as one load where rows are aligned for it.
-__device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid, bool vec) {
+// Four columns of a row, `valid` of them in it: one access of any alignment, or
+// by elements at a row's end.
+template <typename V, typename E>
+struct __attribute__((packed, aligned(sizeof(E)))) Any {
+  V v;
+};
+__device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid) {
   const S* p = (const S*)base + i;
   v4f v = {0.f, 0.f, 0.f, 0.f};
-  if (vec && valid >= 4) {
-    const v4e e = *(const v4e*)p;
+  if (valid >= 4) {
+    const v4e e = ((const Any<v4e, S>*)p)->v;
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = (float)e[k];
   } else {
@@ -31,30 +36,30 @@ __device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid, boo
   }
   return v;
 }
-__device__ __forceinline__ void store4(void* base, int64_t i, v4f v, int valid, bool vec) {
+__device__ __forceinline__ void store4(void* base, int64_t i, v4f v, int valid) {
   S* p = (S*)base + i;
-  if (vec && valid >= 4) {
+  if (valid >= 4) {
     v4e e;
 #pragma unroll
     for (int k = 0; k < 4; ++k) e[k] = (S)v[k];
-    *(v4e*)p = e;
+    ((Any<v4e, S>*)p)->v = e;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (k < valid) p[k] = (S)v[k];
   }
 }
-__device__ __forceinline__ v4f load4f(const float* p, int valid, bool vec) {
-  if (vec && valid >= 4) return *(const v4f*)p;
+__device__ __forceinline__ v4f load4f(const float* p, int valid) {
+  if (valid >= 4) return ((const Any<v4f, float>*)p)->v;
   v4f v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < valid) v[k] = p[k];
   return v;
 }
-__device__ __forceinline__ void store4f(float* p, v4f v, int valid, bool vec) {
-  if (vec && valid >= 4) {
-    *(v4f*)p = v;
+__device__ __forceinline__ void store4f(float* p, v4f v, int valid) {
+  if (valid >= 4) {
+    ((Any<v4f, float>*)p)->v = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -62,12 +67,18 @@ __device__ __forceinline__ void store4f(float* p, v4f v, int valid, bool vec) {
   }
 }
 
-// exp in float32 (a 16-bit result does not see the hardware exponential's last bits)
+// exp(x).  For 16-bit elements exp2(x log2 e), relatively off by |x| 2^-24 from
+// the product's rounding; for float32 that rounding is put back.
 __device__ __forceinline__ float expe(float x) {
-  if constexpr (DT == LSAMP_DTYPE_F32)
-    return expf(x);
-  else
+  if constexpr (DT == LSAMP_DTYPE_F32) {
+    constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+    x = x < -150.f ? -150.f : x;  // (0 either way; -inf has no remainder)
+    const float t = x * kLog2e;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return x > 88.f ? __expf(x) : fmaf(e, fmaf(x, kLog2e, -t) * kLn2, e);
+  } else {
     return __expf(x);
+  }
 }
 
 // 1 / (1 + exp(-z)) and tanh.  For 16-bit elements with the hardware's
@@ -97,34 +108,51 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluA = 0.79788456080286536f;  // sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
-__device__ __forceinline__ float activate(int act, float cap, float z) {
+#define LSAMP_EACH(expr)                                 \
+  do {                                                   \
+    _Pragma("unroll") for (int k = 0; k < 4; ++k) {      \
+      const float z = v[k];                              \
+      v[k] = (expr);                                     \
+    }                                                    \
+    return v;                                            \
+  } while (0)
+
+// act(z) and act'(z) of four columns (one branch for them: it costs as much as
+// the arithmetic of one).
+__device__ __forceinline__ v4f activate(int act, float cap, v4f v) {
   switch (act) {
-    case LSAMP_ACT_RELU: return z < 0.f ? 0.f : z;  // (a NaN stays)
-    case LSAMP_ACT_SILU: return z * sigmoid(z);
-    case LSAMP_ACT_GELU: return 0.5f * z * (1.f + erff(z * kSqrtHalf));
-    case LSAMP_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhe(kGeluA * (z + kGeluB * z * z * z)));
-    case LSAMP_ACT_SOFTCAP: return cap * tanhe(z / cap);
-    default: return z;
+    case LSAMP_ACT_RELU: LSAMP_EACH(z < 0.f ? 0.f : z);  // (a NaN stays)
+    case LSAMP_ACT_SILU: LSAMP_EACH(z * sigmoid(z));
+    case LSAMP_ACT_GELU: LSAMP_EACH(0.5f * z * (1.f + erff(z * kSqrtHalf)));
+    case LSAMP_ACT_GELU_TANH:
+      LSAMP_EACH(0.5f * z * (1.f + tanhe(kGeluA * (z + kGeluB * z * z * z))));
+    case LSAMP_ACT_SOFTCAP: {
+      const float inverse = 1.f / cap;
+      LSAMP_EACH(cap * tanhe(z * inverse));
+    }
+    default: return v;
   }
 }
-__device__ __forceinline__ float activate_slope(int act, float cap, float z) {
+__device__ __forceinline__ float silu_slope(float z) {
+  const float s = sigmoid(z);
+  return s * (1.f + z * (1.f - s));
+}
+__device__ __forceinline__ float gelu_tanh_slope(float z) {
+  const float t = tanhe(kGeluA * (z + kGeluB * z * z * z));
+  return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluA * (1.f + 3.f * kGeluB * z * z);
+}
+__device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
   switch (act) {
-    case LSAMP_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case LSAMP_ACT_SILU: {
-      const float s = sigmoid(z);
-      return s * (1.f + z * (1.f - s));
-    }
+    case LSAMP_ACT_RELU: LSAMP_EACH(z > 0.f ? 1.f : 0.f);
+    case LSAMP_ACT_SILU: LSAMP_EACH(silu_slope(z));
     case LSAMP_ACT_GELU:
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expe(-0.5f * z * z);
-    case LSAMP_ACT_GELU_TANH: {
-      const float t = tanhe(kGeluA * (z + kGeluB * z * z * z));
-      return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluA * (1.f + 3.f * kGeluB * z * z);
-    }
+      LSAMP_EACH(0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expe(-0.5f * z * z));
+    case LSAMP_ACT_GELU_TANH: LSAMP_EACH(gelu_tanh_slope(z));
     case LSAMP_ACT_SOFTCAP: {
-      const float t = tanhe(z / cap);
-      return 1.f - t * t;
+      const float inverse = 1.f / cap;
+      LSAMP_EACH(1.f - tanhe(z * inverse) * tanhe(z * inverse));
     }
-    default: return 1.f;
+    default: return v4f{1.f, 1.f, 1.f, 1.f};
   }
 }
 
@@ -147,25 +175,22 @@ __device__ __forceinline__ void put_all(const E& e, v4f (&acc)[FN][FM], int m0, 
 struct Linear : EpiLinear {
   static constexpr int kBarriers = 0;
   __device__ __forceinline__ v4f bias_at(int c) const {
-    return bias ? load4(bias, c, n - c, vec) : v4f{0.f, 0.f, 0.f, 0.f};
+    return bias ? load4(bias, c, n - c) : v4f{0.f, 0.f, 0.f, 0.f};
   }
   __device__ __forceinline__ v4f residual_at(int r, int c) const {
-    return residual && r < m ? load4(residual, (int64_t)r * ld_residual + c, n - c, vec)
+    return residual && r < m ? load4(residual, (int64_t)r * ld_residual + c, n - c)
                              : v4f{0.f, 0.f, 0.f, 0.f};
   }
   __device__ __forceinline__ void finish(int r, int c, v4f v, v4f b, v4f res) const {
     const int valid = n - c;
     v += b;
-    if (pre) store4f(pre + (int64_t)r * ld_pre + c, v, valid, vec);
-    if (activation != LSAMP_ACT_NONE) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = activate(activation, softcap, v[k]);
-    }
+    if (pre) store4f(pre + (int64_t)r * ld_pre + c, v, valid);
+    v = activate(activation, softcap, v);
     if (residual) v += res;
     if (wide)
-      store4f((float*)out + (int64_t)r * ld_out + c, v, valid, vec);
+      store4f((float*)out + (int64_t)r * ld_out + c, v, valid);
     else
-      store4(out, (int64_t)r * ld_out + c, v, valid, vec);
+      store4(out, (int64_t)r * ld_out + c, v, valid);
   }
   __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
     finish(r, c, v, bias_at(c), residual_at(r, c));
@@ -202,7 +227,7 @@ struct Store : EpiStore {
   static constexpr int kBarriers = 0;
   __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
     if (scale) v *= *scale;
-    store4(out, (int64_t)r * ld_out + c, v, n - c, vec);
+    store4(out, (int64_t)r * ld_out + c, v, n - c);
   }
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
@@ -262,7 +287,7 @@ __device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float invers
   return v;
 }
 __device__ __forceinline__ v4f head_bias(const void* bias, int col, int valid) {
-  return bias ? load4(bias, col, valid, false) : v4f{0.f, 0.f, 0.f, 0.f};
+  return bias ? load4(bias, col, valid) : v4f{0.f, 0.f, 0.f, 0.f};
 }
 
 // The forward pass keeps, of a tile's logits, each row's maximum and the sum of
@@ -377,7 +402,7 @@ struct Grad : EpiGrad {
           const float p = expe(z[k] - l[j]) - (first_col + c + k == target[j] ? 1.f : 0.f);
           g[k] = none || k >= valid ? 0.f : w[j] * p * slope[k];
         }
-        store4(out, (int64_t)r * ld_out + c, g, 4, true);
+        store4(out, (int64_t)r * ld_out + c, g, 4);
       }
     }
   }
@@ -390,29 +415,41 @@ E with(const P& plan) {
   return e;
 }
 
-// (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
-template <bool AK, bool BK, class E>
+// LOOSE: the shapes that take any rows too.  (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
+template <bool AK, bool BK, bool LOOSE, class E>
 int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (tile) {
     case kTile256:
       if constexpr (DT != LSAMP_DTYPE_F32) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, E>), grid, dim3(512), 0, st, g, e);
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, false, E>), grid, dim3(512), 0, st, g, e);
         break;
       }
       return (int)hipErrorInvalidValue;
     case kTile128:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, false, E>), grid, dim3(256), 0, st, g, e);
       break;
     case kTile64:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, E>), grid, dim3(256), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, false, E>), grid, dim3(256), 0, st, g, e);
       break;
     case kTile128x2:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, E>), grid, dim3(512), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, false, E>), grid, dim3(512), 0, st, g, e);
       break;
+    case kLoose64:
+      if constexpr (LOOSE) {
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, true, E>), grid, dim3(256), 0, st, g, e);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
+    case kLoose64x4:
+      if constexpr (LOOSE) {
+        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, true, E>), grid, dim3(1024), 0, st, g, e);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
     case kTile64x4:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, E>), grid, dim3(1024), 0, st, g, e);
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, false, E>), grid, dim3(1024), 0, st, g, e);
       break;
     default:
       return (int)hipErrorInvalidValue;
@@ -486,15 +523,13 @@ __global__ __launch_bounds__(kThreads) void k_col_sum(ColSumPlan p) {
   v4f sum = {0.f, 0.f, 0.f, 0.f};
   if (c < p.cols || (p.out && c < p.out_cols)) {
     for (int r = r0 + wave; r < r1; r += 4) {
-      v4f v = load4(p.in, (int64_t)r * p.ld_in + c, valid, p.vec);
+      v4f v = load4(p.in, (int64_t)r * p.ld_in + c, valid);
       if (p.pre) {
-        const v4f z = load4f(p.pre + (int64_t)r * p.ld_pre + c, valid, p.vec);
+        const v4f z = load4f(p.pre + (int64_t)r * p.ld_pre + c, valid);
+        const v4f slope = activate_slope(p.activation, p.softcap, z);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float d = v[k] * activate_slope(p.activation, p.softcap, z[k]);
-          v[k] = k < valid ? d : 0.f;
-        }
-        store4(p.out, (int64_t)r * p.ld_out + c, v, p.out_cols - c, true);
+        for (int k = 0; k < 4; ++k) v[k] = k < valid ? v[k] * slope[k] : 0.f;
+        store4(p.out, (int64_t)r * p.ld_out + c, v, p.out_cols - c);
       }
       sum += v;
     }
@@ -534,35 +569,35 @@ int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& p, 
   const Linear e = with<Linear>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, true>(g, e, st);
   if (t == kSkinny16) return launch_skinny<1, 8, true>(g, e, st);
-  return launch<false, false>(t, g, e, st);
+  return launch<false, false, true>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& p, void* st) {
   const Stats e = with<Stats>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
-  return launch<false, false>(t, g, e, st);
+  return launch<false, false, false>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& p, void* st) {
   const Grad e = with<Grad>(p);
   if (t == kSkinny64) return launch_skinny<4, 4, false>(g, e, st);
-  return launch<false, false>(t, g, e, st);
+  return launch<false, false, false>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_store(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiStore& p,
                             void* st) {
   const Store e = with<Store>(p);
-  return roles == kRolesNN ? launch<false, true>(t, g, e, st)
-                           : launch<true, true>(t, g, e, st);
+  return roles == kRolesNN ? launch<false, true, true>(t, g, e, st)
+                           : launch<true, true, true>(t, g, e, st);
 }
 template <>
 int HeadOps<DT>::gemm_partial(GemmRoles roles, GemmTile t, const GemmPlan& g, const EpiPartial& p,
                               void* st) {
   const Partial e = with<Partial>(p);
   switch (roles) {
-    case kRolesNT: return launch<false, false>(t, g, e, st);
-    case kRolesNN: return launch<false, true>(t, g, e, st);
-    default: return launch<true, true>(t, g, e, st);
+    case kRolesNT: return launch<false, false, true>(t, g, e, st);
+    case kRolesNN: return launch<false, true, true>(t, g, e, st);
+    default: return launch<true, true, true>(t, g, e, st);
   }
 }
 template <>

@@ -59,31 +59,28 @@ bool chunked(const void* p, int64_t ld, int32_t cols, int eb) {
          ld * eb <= ((int64_t)1 << 32) / 512;
 }
 
-// Whether four columns of a matrix's rows can be moved as one vector.
-bool quads(const void* p, int64_t ld, int eb) {
-  return !p || ((uintptr_t)p % (4 * eb) == 0 && ld % 4 == 0);
-}
-
-// A matrix as the products read it: itself, or a copy in the workspace (`any`:
-// the product takes any row).
+// A matrix of the arguments, and what the products read: itself, or a copy in
+// the workspace that is made before the first of them.
 struct Operand {
   MatrixRef ref;
-  bool packed;
+  bool chunked, packed;
   PackPlan pack;
 };
-Operand operand(Arena& ws, const void* p, int64_t ld, int32_t rows, int32_t cols, int eb,
-                bool any = false) {
+Operand operand(const void* p, int64_t ld, int32_t rows, int32_t cols, int eb) {
   Operand o{};
-  if (any || chunked(p, ld, cols, eb)) {
-    o.ref = MatrixRef{p, ld, rows, cols};
-    return o;
-  }
-  const int32_t wide = (int32_t)round_up(cols, 16 / eb);
-  void* dst = ws.take((int64_t)rows * wide * eb);
-  o.packed = true;
-  o.pack = PackPlan{p, ld, dst, wide, rows, cols, wide};
-  o.ref = MatrixRef{dst, wide, rows, wide};
+  o.ref = MatrixRef{p, ld, rows, cols};
+  o.chunked = chunked(p, ld, cols, eb);
   return o;
+}
+// Lays the operand out, if it has to be.
+MatrixRef packed(Arena& ws, Operand& o, int eb) {
+  if (!o.chunked && !o.packed) {
+    const int32_t wide = (int32_t)round_up(o.ref.cols, 16 / eb);
+    void* dst = ws.take((int64_t)o.ref.rows * wide * eb);
+    o.packed = true;
+    o.pack = PackPlan{o.ref.p, o.ref.ld, dst, wide, o.ref.rows, o.ref.cols, wide};
+  }
+  return o.packed ? MatrixRef{o.pack.dst, o.pack.dst_ld, o.pack.rows, o.pack.dst_cols} : o.ref;
 }
 int lay_out(const Operand& o, int eb, void* stream) {
   return o.packed ? launch_pack(o.pack, eb, stream) : 0;
@@ -100,8 +97,9 @@ int lay_out(const Operand& o, int eb, void* stream) {
 struct Choice {
   GemmTile tile;
   int32_t parts;
+  double us;
 };
-Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
+Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split, bool loose = false) {
   struct Shape {
     GemmTile tile, grouped;
     int resident;
@@ -114,9 +112,9 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
       {kTile128, kTile128x2, 2, {{0.65, 0.5, 0.5}, {0.95, 0.8, 0.8}}},
       {kTile64, kTile64x4, 4, {{0.25, 0.16, 0.18}, {0.5, 0.38, 0.38}}}};
   constexpr int kCus = 256;
-  Choice best{kTile64, 1};
-  double best_us = 1e300;
+  Choice best{kTile64, 1, 1e300};
   for (const Shape& s : kShapes) {
+    if (loose && s.tile != kTile64) continue;
     const int64_t tiles = ceil_div(m, kTileSide[s.tile]) * ceil_div(n, kTileSide[s.tile]);
     for (int parts = 1; parts <= (may_split ? 64 : 1) && parts <= slabs; parts *= 2) {
       const int64_t each = ceil_div(tiles * parts, kCus);
@@ -127,13 +125,31 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
                                                   (grouped ? us_of.alone_grouped : us_of.alone));
       double us = per_slab * (double)ceil_div(slabs, parts);
       if (parts > 1) us += 4.0 + (double)parts * (double)m * (double)n * 8e-6 / 4.0;
-      if (us < best_us) {
-        best_us = us;
-        best = Choice{grouped ? s.grouped : s.tile, parts};
-      }
+      if (us < best.us) best = Choice{grouped ? s.grouped : s.tile, parts, us};
     }
   }
+  if (loose) best.tile = best.tile == kTile64 ? kLoose64 : kLoose64x4;
   return best;
+}
+// What laying a matrix out for the tiled products takes: a launch and, at the
+// rate that its element-wise reads reach, its bytes.
+double pack_us(int64_t rows, int64_t cols, int eb) {
+  return 4.0 + (double)rows * (double)cols * eb * 2.0 / 2e6;
+}
+double pack_all(const Operand& a, const Operand& b, int eb) {
+  double us = 0.0;
+  for (const Operand* o : {&a, &b})
+    if (!o->chunked && !o->packed) us += pack_us(o->ref.rows, o->ref.cols, eb);
+  return us;
+}
+bool is_loose(const Choice& c) { return c.tile == kLoose64 || c.tile == kLoose64x4; }
+// For operands of which some are no chunks: the loose 64 x 64 tiles (about 1.3
+// times an aligned one's time), or any tile after `pack` microseconds of copies.
+Choice choose_rows(int64_t m, int64_t n, int64_t slabs, int dtype, double pack) {
+  const Choice best = choose(m, n, slabs, dtype, true);
+  if (pack == 0.0) return best;
+  const Choice any = choose(m, n, slabs, dtype, true, true);
+  return any.us * 1.3 < best.us + pack ? any : best;
 }
 // At most 64 rows are bound by reading the other operand, which the kernels of
 // lsamp_skinny.h do without a detour: 64 columns a work-group where that leaves
@@ -142,7 +158,7 @@ Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split) {
 // operand, and of x up to kLooseRows.
 constexpr int kLooseRows = 16;
 Choice choose_skinny(int64_t m, int64_t n, bool whole_rows) {
-  return Choice{whole_rows || n >= (m > kLooseRows ? 8192 : 16384) ? kSkinny64 : kSkinny16, 1};
+  return Choice{whole_rows || n >= (m > kLooseRows ? 8192 : 16384) ? kSkinny64 : kSkinny16, 1, 0.0};
 }
 
 // `k`: elements of the reduction.
@@ -275,11 +291,20 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
 
   LinearPlan P{};
   Arena ws(base);
-  const bool skinny = m <= kSkinnyRows;
-  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb, m <= kLooseRows);
-  P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb, skinny);
-  P.choice = skinny ? choose_skinny(m, n, false) : choose(m, n, slabs_of(k, eb), a->dtype, true);
-  P.gemm = plan_gemm(P.choice, P.x.ref, P.w.ref, m, n, k, eb);
+  P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.w = operand(a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
+  MatrixRef x = P.x.ref, w = P.w.ref;
+  if (m <= kSkinnyRows) {
+    P.choice = choose_skinny(m, n, false);
+    if (m > kLooseRows) x = packed(ws, P.x, eb);
+  } else {
+    P.choice = choose_rows(m, n, slabs_of(k, eb), a->dtype, pack_all(P.x, P.w, eb));
+    if (!is_loose(P.choice)) {
+      x = packed(ws, P.x, eb);
+      w = packed(ws, P.w, eb);
+    }
+  }
+  P.gemm = plan_gemm(P.choice, x, w, m, n, k, eb);
   if (too_many(P.gemm))
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
   if (P.gemm.parts > 1) P.partial = take_partial(ws, m, n, P.gemm.parts);
@@ -296,9 +321,6 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
   e.ld_out = stride_of(a->out_stride, m, n);
   e.pre = a->pre;
   e.ld_pre = stride_of(a->pre_stride, m, n);
-  const bool one = m == 1;  // (the only row starts at its address)
-  e.vec = quads(e.bias, 4, eb) && quads(e.residual, one ? 4 : e.ld_residual, eb) &&
-          quads(e.out, one ? 4 : e.ld_out, ob) && quads(e.pre, one ? 4 : e.ld_pre, 4);
   P.bytes = ws.used;
   *out = P;
   return LSAMP_OK;
@@ -323,20 +345,20 @@ struct Product {  // one product of a backward pass
   EpiStore store;
 };
 // out = A B in `roles`; `k` reduction elements.
-Product plan_product(Arena& ws, GemmRoles roles, const MatrixRef& a, const MatrixRef& b, int64_t m,
-                     int64_t n, int64_t k, int dtype, void* out, int64_t ld, const float* scale) {
+Product plan_product(Arena& ws, GemmRoles roles, Operand& a, Operand& b, int64_t m, int64_t n,
+                     int64_t k, int dtype, void* out, int64_t ld) {
   const int eb = element_bytes(dtype);
   Product p{};
   p.roles = roles;
-  p.choice = choose(m, n, slabs_of(k, eb), dtype, true);
-  p.gemm = plan_gemm(p.choice, a, b, m, n, k, eb);
+  p.choice = choose_rows(m, n, slabs_of(k, eb), dtype, pack_all(a, b, eb));
+  const bool loose = is_loose(p.choice);
+  p.gemm = plan_gemm(p.choice, loose ? a.ref : packed(ws, a, eb), loose ? b.ref : packed(ws, b, eb),
+                     m, n, k, eb);
   if (p.gemm.parts > 1) p.partial = take_partial(ws, m, n, p.gemm.parts);
   p.store.m = (int32_t)m;
   p.store.n = (int32_t)n;
   p.store.out = out;
   p.store.ld_out = ld;
-  p.store.scale = scale;
-  p.store.vec = quads(out, m == 1 ? 4 : ld, eb);
   return p;
 }
 int run_product(const Product& p, int dtype, void* stream) {
@@ -349,7 +371,7 @@ int run_product(const Product& p, int dtype, void* stream) {
 
 struct LinearBackwardPlan {
   Operand x, w, d;
-  bool sum;  // the pass over d_out: d_bias, or dz for an activation
+  bool sum;  // the pass over d_out: d_bias, or dz (then `d`) for an activation
   ColSumPlan col;
   bool want_x, want_w;
   Product dx, dw;
@@ -386,13 +408,12 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
   P.want_x = a->d_x != nullptr;
   P.want_w = a->d_weight != nullptr;
   const int64_t ld_d = stride_of(a->d_out_stride, m, n);
-  MatrixRef dz{};
   if (act) {
     const int32_t wide = (int32_t)round_up(n, 16 / eb);
-    dz = MatrixRef{ws.take((int64_t)m * wide * eb), wide, m, wide};
-  } else if (P.want_x || P.want_w) {
-    P.d = operand(ws, a->d_out, ld_d, m, n, eb);
-    dz = P.d.ref;
+    P.d = operand(ws.take((int64_t)m * wide * eb), wide, m, wide, eb);
+    P.d.chunked = true;
+  } else {
+    P.d = operand(a->d_out, ld_d, m, n, eb);
   }
   P.sum = act || a->d_bias;
   if (P.sum) {
@@ -402,14 +423,12 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
     s.ld_in = ld_d;
     s.activation = a->activation;
     s.softcap = a->softcap;
-    s.vec = quads(a->d_out, m == 1 ? 4 : ld_d, eb);
     if (act) {
       s.pre = a->pre;
       s.ld_pre = stride_of(a->pre_stride, m, n);
-      s.vec = s.vec && quads(s.pre, m == 1 ? 4 : s.ld_pre, 4);
-      s.out = const_cast<void*>(dz.p);
-      s.ld_out = dz.ld;
-      s.out_cols = dz.cols;
+      s.out = const_cast<void*>(P.d.ref.p);
+      s.ld_out = P.d.ref.ld;
+      s.out_cols = P.d.ref.cols;
     }
     if (a->d_bias) {
       s.ld_part = round_up(n, 4);
@@ -417,14 +436,14 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
     }
   }
   if (P.want_x) {
-    P.w = operand(ws, a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
-    P.dx = plan_product(ws, kRolesNN, dz, P.w.ref, m, k, n, a->dtype, a->d_x,
-                        stride_of(a->d_x_stride, m, k), nullptr);
+    P.w = operand(a->weight, stride_of(a->weight_stride, n, k), n, k, eb);
+    P.dx = plan_product(ws, kRolesNN, P.d, P.w, m, k, n, a->dtype, a->d_x,
+                        stride_of(a->d_x_stride, m, k));
   }
   if (P.want_w) {
-    P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
-    P.dw = plan_product(ws, kRolesTN, dz, P.x.ref, n, k, m, a->dtype, a->d_weight,
-                        stride_of(a->d_weight_stride, n, k), nullptr);
+    P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
+    P.dw = plan_product(ws, kRolesTN, P.d, P.x, n, k, m, a->dtype, a->d_weight,
+                        stride_of(a->d_weight_stride, n, k));
   }
   if ((P.want_x && too_many(P.dx.gemm)) || (P.want_w && too_many(P.dw.gemm)))
     return set_error(LSAMP_ERR_SHAPE, "%d x %d x %d is too large for one call", m, n, k);
@@ -480,6 +499,7 @@ Operand weight_piece(const void* w, int64_t ld, int32_t first, int32_t rows, int
 
 struct LossPlan {
   Operand x;
+  MatrixRef x_ref;
   Choice choice;
   int64_t piece;  // vocabulary columns at a time
   void* packed;
@@ -497,7 +517,8 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
   LossPlan P{};
   Arena ws(base);
   const bool skinny = m <= kSkinnyRows;
-  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb, m <= kLooseRows);
+  P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.x_ref = m <= kLooseRows ? P.x.ref : packed(ws, P.x, eb);
   const int64_t ld_w = stride_of(a->weight_stride, v, k);
   P.piece = round_up(v, kPieceStep);
   if (!skinny && !chunked(a->weight, ld_w, k, eb)) {
@@ -527,6 +548,7 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
 
 struct LossBackwardPlan {
   Operand x;
+  MatrixRef x_ref;
   int64_t piece;
   void* packed;
   void* g;      // [rows, ld_g]: the gradient at a piece of the logits
@@ -554,7 +576,8 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
 
   LossBackwardPlan P{};
   Arena ws(base);
-  P.x = operand(ws, a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.x_ref = packed(ws, P.x, eb);
   // A piece's gradient stays in the 256 MB last-level cache between the pass
   // that writes it and the products that read it.
   P.piece = piece_cols(v, ((int64_t)128 << 20) / ((int64_t)m * eb));
@@ -683,7 +706,7 @@ lsamp_status lsamp_head_loss(lsamp_context* ctx, const lsamp_head_loss_args* a, 
     e.n = n;
     e.first_col = (int32_t)first;
     e.first_block = (int32_t)(first / kTileSide[P.choice.tile]);
-    const GemmPlan g = plan_gemm(P.choice, P.x.ref, w.ref, a->rows, n, k, eb);
+    const GemmPlan g = plan_gemm(P.choice, P.x_ref, w.ref, a->rows, n, k, eb);
     LSAMP_TRY(HEAD_OP(a->dtype, gemm_stats(P.choice.tile, g, e, stream)));
   }
   LSAMP_TRY(launch_join_stats(P.join, stream));
@@ -713,7 +736,6 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   dx.n = k;
   dx.out = a->d_x;
   dx.ld_out = stride_of(a->d_x_stride, m, k);
-  dx.vec = quads(dx.out, m == 1 ? 4 : dx.ld_out, eb);
   dx.scale = inverse;
   int dx_parts = 0;
   for (int64_t first = 0; first < v; first += P.piece) {
@@ -736,7 +758,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
     e.out = P.g;
     e.ld_out = P.ld_g;
     LSAMP_TRY(HEAD_OP(a->dtype, gemm_grad(P.grad.tile,
-                                          plan_gemm(P.grad, P.x.ref, w.ref, m, n, k, eb), e, stream)));
+                                          plan_gemm(P.grad, P.x_ref, w.ref, m, n, k, eb), e, stream)));
     const MatrixRef g{P.g, P.ld_g, m, e.n_pad};
     if (a->d_x) {
       const GemmPlan plan = plan_gemm(P.dx, g, w.ref, m, k, n, eb);
@@ -755,9 +777,8 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
       dw.n = k;
       dw.ld_out = stride_of(a->d_weight_stride, v, k);
       dw.out = (char*)a->d_weight + first * dw.ld_out * eb;
-      dw.vec = quads(dw.out, v == 1 ? 4 : dw.ld_out, eb);
       dw.scale = inverse;
-      const GemmPlan plan = plan_gemm(P.dw, g, P.x.ref, n, k, m, eb);
+      const GemmPlan plan = plan_gemm(P.dw, g, P.x_ref, n, k, m, eb);
       if (!P.dw_split) {
         LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesTN, P.dw.tile, plan, dw, stream)));
       } else {
@@ -772,7 +793,6 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
       s.cols = n;
       s.in = P.g;
       s.ld_in = P.ld_g;
-      s.vec = 1;
       LSAMP_TRY(HEAD_OP(a->dtype, col_sum(s, stream)));
       LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
     }
@@ -810,10 +830,6 @@ lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* a, void
   P.ld_residual = stride_of(a->residual_stride, a->rows, a->cols);
   P.out = a->out;
   P.ld_out = stride_of(a->out_stride, a->rows, a->cols);
-  const auto vec = [&](const void* p, int64_t ld) {
-    return !p || ((uintptr_t)p % 16 == 0 && (a->rows == 1 || ld * eb % 16 == 0));
-  };
-  P.vec = vec(P.x, P.ld_x) && vec(P.residual, P.ld_residual) && vec(P.out, P.ld_out);
   OnDevice guard(context_device(ctx));
   LSAMP_TRY(launch_dropout(P, a->dtype, stream));
   return clear_error();

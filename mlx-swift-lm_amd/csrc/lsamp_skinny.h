@@ -17,28 +17,6 @@
 namespace lsamp {
 namespace gemm {
 
-// 16 bytes from an address aligned to elements only.
-template <int DT>
-__device__ __forceinline__ v4i load_chunk(const char* p) {
-  struct __attribute__((packed, aligned(El<DT>::kBytes))) Any {
-    v4i v;
-  };
-  return ((const Any*)p)->v;
-}
-// The chunk at element k of a row of `cols` elements, zero past its end.
-template <int DT>
-__device__ __forceinline__ v4i load_chunk_end(const char* row, int k, int cols) {
-  using S = typename El<DT>::S;
-  constexpr int N = kChunkOf<DT>;
-  if (k + N <= cols) return load_chunk<DT>(row + (int64_t)k * El<DT>::kBytes);
-  S e[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) e[i] = k + i < cols ? ((const S*)row)[k + i] : (S)0.f;
-  v4i v;
-  __builtin_memcpy(&v, e, 16);
-  return v;
-}
-
 // NF x 16 columns and MF x 16 rows a work-group of WK waves.
 //
 // One wave's 16 rows of x come straight from L2.  With more (MF > 1) those reads

@@ -68,13 +68,17 @@ def test_linear_refusals(lib):
 
 def test_linear_workspace_counts_alignment(lib):
     f = lambda **kw: lib.lsamp_linear_workspace(ctypes.byref(linear(**kw)))  # noqa: E731
-    base = f(rows=100)
+    big = dict(rows=8192, in_features=4096, out_features=4096, weight_stride=4096,
+               out_stride=4096, x_stride=4096)
+    base, copy = f(**big), 8192 * 4096 * 2
     # rows that start between 16-byte chunks are copied; so are rows too far apart
-    assert f(rows=100, x=P + 2) >= base + 100 * 64 * 2
-    assert f(rows=100, x_stride=65) >= base + 100 * 64 * 2
-    assert f(rows=100, x_stride=1 << 30) >= base + 100 * 64 * 2
-    assert f(rows=100, x_stride=72) == base
-    assert f(x=P + 2, x_stride=65) == 0  # (few rows are read as they are)
+    assert f(**dict(big, x=P + 2)) >= base + copy
+    assert f(**dict(big, x_stride=4097)) >= base + copy
+    assert f(**dict(big, x_stride=1 << 30)) >= base + copy
+    assert f(**dict(big, x_stride=4104)) == base
+    # small and few rows are read as they are
+    assert f(rows=100, x=P + 2, x_stride=65) == f(rows=100)
+    assert f(x=P + 2, x_stride=65) == 0
     assert f(rows=1, x_stride=1) == 0  # (a one-row matrix carries any stride)
 
 
