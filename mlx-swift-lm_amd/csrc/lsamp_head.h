@@ -30,8 +30,8 @@ struct GemmPlan {
 // Which operand is read along the reduction's rows (lsamp_gemm.h).
 enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
 // Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
-// slabs of the reduction at a time, for launches of at most a tile a CU; the last
-// two for operands whose rows are no 16-byte chunks; and the products of at most
+// slabs of the reduction at a time, for launches of at most a tile a CU; loose ones
+// for operands whose rows are no 16-byte chunks; and the products of at most
 // 16, 32 or 64 rows (lsamp_skinny.h), 64 or 16 columns a work-group.
 enum GemmTile {
   kTile256,
@@ -39,12 +39,13 @@ enum GemmTile {
   kTile64,
   kTile128x2,
   kTile64x4,
+  kLoose128,
   kLoose64,
   kLoose64x4,
   kSkinny64,
   kSkinny16,
 };
-constexpr int kTileSide[] = {256, 128, 64, 128, 64, 64, 64, 64, 16};
+constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16};
 constexpr int kSkinnyRows = 64;
 
 // Epilogues.  `m`, `n`: rows and columns that exist.
@@ -128,6 +129,8 @@ struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial s
   int32_t out_cols;  // columns cols .. out_cols - 1 of out are written as zero
   float* part;       // [chunks][ld_part], or NULL
   int64_t ld_part;
+  void* sums;        // one chunk: the sums themselves, times *scale
+  const float* scale;
 };
 
 struct DropoutPlan {
@@ -149,7 +152,7 @@ template <int DT>
 struct HeadOps {
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
   // (kSkinny16: gemm_linear only; kSkinny64: not gemm_store and gemm_partial;
-  // loose shapes: not the loss's)
+  // kLoose64 and kLoose64x4: not the loss's)
   static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
   static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
   static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,

@@ -307,24 +307,32 @@ struct Stats : EpiStats {
       const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
       b[i] = head_bias(bias, first_col + c, n - c);
     }
+    const bool inside = n0 + BN <= n;  // (every column of the tile exists)
+    int t[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int r = m0 + wm * (FM * 16) + j * 16 + (lane & 15);
+      t[j] = r < m ? targets[r] - first_col : -1;
+    }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       const int rl = wm * (FM * 16) + j * 16 + (lane & 15);
       const int r = m0 + rl;
-      const int t = r < m ? targets[r] - first_col : -1;
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
-        const int valid = n - c;
-        const v4f v = logits4(acc[i][j], b[i], softcap, inverse, nullptr);
+        v4f v = logits4(acc[i][j], b[i], softcap, inverse, nullptr);
+        if (!inside) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool ok = k < valid;
-          acc[i][j][k] = ok ? v[k] : -INFINITY;
-          top = fmaxf(top, acc[i][j][k]);
-          if (ok && t == c + k) target[r] = v[k];
+          for (int k = 0; k < 4; ++k) v[k] = c + k < n ? v[k] : -INFINITY;
         }
+        if ((unsigned)(t[j] - c) < 4u && t[j] < n) {
+          const int k = t[j] - c;
+          target[r] = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3];
+        }
+        top = fmaxf(fmaxf(fmaxf(top, v[0]), fmaxf(v[1], v[2])), v[3]);
+        acc[i][j] = v;
       }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -398,9 +406,17 @@ struct Grad : EpiGrad {
         const int valid = n - c;
         const v4f z = logits4(acc[i][j], b[i], softcap, inverse, &slope);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float p = expe(z[k] - l[j]) - (first_col + c + k == target[j] ? 1.f : 0.f);
-          g[k] = none || k >= valid ? 0.f : w[j] * p * slope[k];
+        for (int k = 0; k < 4; ++k) g[k] = expe(z[k] - l[j]);
+        const int at = target[j] - first_col - c;
+        if ((unsigned)at < 4u) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) g[k] -= k == at ? 1.f : 0.f;
+        }
+        g *= w[j];
+        if (softcap > 0.f) g *= slope;
+        if (none || valid < 4) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) g[k] = none || k >= valid ? 0.f : g[k];
         }
         store4(out, (int64_t)r * ld_out + c, g, 4);
       }
@@ -415,7 +431,7 @@ E with(const P& plan) {
   return e;
 }
 
-// LOOSE: the shapes that take any rows too.  (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
+// LOOSE: the small shapes that take any rows too.  (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
 template <bool AK, bool BK, bool LOOSE, class E>
 int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
@@ -442,6 +458,9 @@ int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
         break;
       }
       return (int)hipErrorInvalidValue;
+    case kLoose128:
+      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, true, E>), grid, dim3(256), 0, st, g, e);
+      break;
     case kLoose64x4:
       if constexpr (LOOSE) {
         hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, true, E>), grid, dim3(1024), 0, st, g, e);
@@ -534,11 +553,14 @@ __global__ __launch_bounds__(kThreads) void k_col_sum(ColSumPlan p) {
       sum += v;
     }
   }
-  if (!p.part) return;
+  if (!p.part && !p.sums) return;
   red[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && c < p.ld_part) {
-    for (int w = 1; w < 4; ++w) sum += red[w][lane];
+  if (wave != 0) return;
+  for (int w = 1; w < 4; ++w) sum += red[w][lane];
+  if (p.sums) {  // (the only chunk)
+    if (c < p.cols) store4(p.sums, c, p.scale ? sum * *p.scale : sum, valid);
+  } else if (c < p.ld_part) {
     *(v4f*)(p.part + (int64_t)blockIdx.y * p.ld_part + c) = sum;
   }
 }

@@ -91,50 +91,62 @@ int lay_out(const Operand& o, int eb, void* stream) {
 // work-groups of the three shapes; a slab takes at least its barrier, its LDS
 // reads and its products in turn, and at least the time of the products of all
 // groups on the CU.  Measured in microseconds (16-bit elements): alone on a CU
-// 1.5, 0.65 and 0.25 (304 x 2048 x 1536, 1024 x 4096 x 2048), in company 1.65,
-// 0.5 and 0.18 (8192 x 4096 x 4096); two or four slabs at a time alone 0.5 and
-// 0.16.  A split reduction is another launch, and its sums' traffic.
+// 1.5, 0.63 and 0.2 (304 x 2048 x 1536, 1024 x 4096 x 2048), in company 1.6, 0.46
+// and 0.18 (8192 x 4096 x 4096); two or four slabs at a time alone 0.57 and 0.15.
+// A tile ends with its epilogue's `bytes` an element at the CU's share of the
+// memory rate, hidden behind other work-groups' products where a CU has some
+// (151936 x 4096 gradients of few rows: 513 us on 256 x 256 tiles, 230 on 128 x
+// 128).  A split reduction is another launch, and its sums' traffic.
 struct Choice {
   GemmTile tile;
   int32_t parts;
   double us;
 };
-Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, bool may_split, bool loose = false) {
+enum Rows { kChunked, kLooseSmall, kLooseAny };  // kLooseAny: under every epilogue
+Choice choose(int64_t m, int64_t n, int64_t slabs, int dtype, double bytes, bool may_split,
+              Rows rows = kChunked) {
   struct Shape {
-    GemmTile tile, grouped;
+    GemmTile tile, grouped, loose, loose_grouped;
     int resident;
+    double exposed, fixed;
     struct {
       double alone, alone_grouped, busy;
     } us[2];  // 16-bit elements, float32
   };
   static const Shape kShapes[] = {
-      {kTile256, kTile256, 1, {{1.5, 1.5, 1.65}, {1e30, 1e30, 1e30}}},
-      {kTile128, kTile128x2, 2, {{0.65, 0.5, 0.5}, {0.95, 0.8, 0.8}}},
-      {kTile64, kTile64x4, 4, {{0.25, 0.16, 0.18}, {0.5, 0.38, 0.38}}}};
+      {kTile256, kTile256, kTile256, kTile256, 1, 1.0, 2.0, {{1.5, 1.5, 1.6}, {1e30, 1e30, 1e30}}},
+      {kTile128, kTile128x2, kLoose128, kLoose128, 2, 0.6, 1.0, {{0.63, 0.57, 0.46}, {0.95, 0.8, 0.8}}},
+      {kTile64, kTile64x4, kLoose64, kLoose64x4, 4, 0.5, 0.5, {{0.2, 0.15, 0.18}, {0.5, 0.38, 0.38}}}};
   constexpr int kCus = 256;
-  Choice best{kTile64, 1, 1e300};
+  constexpr double kBytesPerUs = 5e6;  // of the device
+  Choice best{rows == kChunked ? kTile64 : kLoose128, 1, 1e300};
   for (const Shape& s : kShapes) {
-    if (loose && s.tile != kTile64) continue;
-    const int64_t tiles = ceil_div(m, kTileSide[s.tile]) * ceil_div(n, kTileSide[s.tile]);
+    if (rows != kChunked && s.tile == kTile256) continue;
+    if (rows == kLooseAny && s.tile == kTile64) continue;
+    const int64_t side = kTileSide[s.tile], tiles = ceil_div(m, side) * ceil_div(n, side);
+    const auto& us_of = s.us[dtype == LSAMP_DTYPE_F32];
     for (int parts = 1; parts <= (may_split ? 64 : 1) && parts <= slabs; parts *= 2) {
-      const int64_t each = ceil_div(tiles * parts, kCus);
-      const auto& us_of = s.us[dtype == LSAMP_DTYPE_F32];
+      const int64_t each = ceil_div(tiles * parts, kCus), rounds = ceil_div(each, s.resident);
       const bool grouped = each == 1;
-      const double per_slab =
-          std::max((double)each * us_of.busy, (double)ceil_div(each, s.resident) *
-                                                  (grouped ? us_of.alone_grouped : us_of.alone));
-      double us = per_slab * (double)ceil_div(slabs, parts);
-      if (parts > 1) us += 4.0 + (double)parts * (double)m * (double)n * 8e-6 / 4.0;
-      if (us < best.us) best = Choice{grouped ? s.grouped : s.tile, parts, us};
+      const double per_slab = std::max((double)each * us_of.busy,
+                                       (double)rounds * (grouped ? us_of.alone_grouped : us_of.alone));
+      const double out = parts > 1 ? 4.0 : bytes;
+      double us = per_slab * (double)ceil_div(slabs, parts) + (double)rounds * s.fixed +
+                  (double)each * (double)(side * side) * out * s.exposed * kCus / kBytesPerUs;
+      us = std::max(us, (double)parts * (double)m * (double)n * out / kBytesPerUs);
+      if (parts > 1) us += 4.0 + (double)m * (double)n * ((double)parts * 4.0 + bytes) / kBytesPerUs;
+      if (us < best.us)
+        best = Choice{rows == kChunked ? (grouped ? s.grouped : s.tile)
+                                       : (grouped ? s.loose_grouped : s.loose),
+                      parts, us};
     }
   }
-  if (loose) best.tile = best.tile == kTile64 ? kLoose64 : kLoose64x4;
   return best;
 }
-// What laying a matrix out for the tiled products takes: a launch and, at the
-// rate that its element-wise reads reach, its bytes.
+// What laying a matrix out for the tiled products takes: a launch, and its bytes
+// read and written.
 double pack_us(int64_t rows, int64_t cols, int eb) {
-  return 4.0 + (double)rows * (double)cols * eb * 2.0 / 2e6;
+  return 4.0 + (double)rows * (double)cols * eb * 2.0 / 4e6;
 }
 double pack_all(const Operand& a, const Operand& b, int eb) {
   double us = 0.0;
@@ -142,14 +154,16 @@ double pack_all(const Operand& a, const Operand& b, int eb) {
     if (!o->chunked && !o->packed) us += pack_us(o->ref.rows, o->ref.cols, eb);
   return us;
 }
-bool is_loose(const Choice& c) { return c.tile == kLoose64 || c.tile == kLoose64x4; }
-// For operands of which some are no chunks: the loose 64 x 64 tiles (about 1.3
-// times an aligned one's time), or any tile after `pack` microseconds of copies.
-Choice choose_rows(int64_t m, int64_t n, int64_t slabs, int dtype, double pack) {
-  const Choice best = choose(m, n, slabs, dtype, true);
+bool is_loose(const Choice& c) {
+  return c.tile == kLoose128 || c.tile == kLoose64 || c.tile == kLoose64x4;
+}
+// For operands of which some are no chunks: loose tiles (about 1.4 times an
+// aligned one's time), or any tile after `pack` microseconds of copies.
+Choice choose_rows(int64_t m, int64_t n, int64_t slabs, int dtype, double bytes, double pack) {
+  const Choice best = choose(m, n, slabs, dtype, bytes, true);
   if (pack == 0.0) return best;
-  const Choice any = choose(m, n, slabs, dtype, true, true);
-  return any.us * 1.3 < best.us + pack ? any : best;
+  const Choice any = choose(m, n, slabs, dtype, bytes, true, kLooseSmall);
+  return any.us * 1.4 < best.us + pack ? any : best;
 }
 // At most 64 rows are bound by reading the other operand, which the kernels of
 // lsamp_skinny.h do without a detour: 64 columns a work-group where that leaves
@@ -298,7 +312,8 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
     P.choice = choose_skinny(m, n, false);
     if (m > kLooseRows) x = packed(ws, P.x, eb);
   } else {
-    P.choice = choose_rows(m, n, slabs_of(k, eb), a->dtype, pack_all(P.x, P.w, eb));
+    P.choice = choose_rows(m, n, slabs_of(k, eb), a->dtype,
+                           ob + (a->residual ? eb : 0) + (a->pre ? 4 : 0), pack_all(P.x, P.w, eb));
     if (!is_loose(P.choice)) {
       x = packed(ws, P.x, eb);
       w = packed(ws, P.w, eb);
@@ -332,7 +347,8 @@ void plan_col_sum(ColSumPlan& s, int32_t rows, int32_t cols) {
   s.rows = rows;
   s.cols = cols;
   const int64_t across = ceil_div(cols, 256);
-  int64_t chunks = std::min(ceil_div(2048, across), ceil_div(rows, 16));
+  // (up to 128 rows one chunk: its sums need no second pass)
+  int64_t chunks = rows <= 128 ? 1 : std::min(ceil_div(2048, across), ceil_div(rows, 16));
   s.rows_per_chunk = (int32_t)ceil_div(rows, chunks);
   s.chunks = (int32_t)ceil_div(rows, s.rows_per_chunk);
 }
@@ -350,7 +366,7 @@ Product plan_product(Arena& ws, GemmRoles roles, Operand& a, Operand& b, int64_t
   const int eb = element_bytes(dtype);
   Product p{};
   p.roles = roles;
-  p.choice = choose_rows(m, n, slabs_of(k, eb), dtype, pack_all(a, b, eb));
+  p.choice = choose_rows(m, n, slabs_of(k, eb), dtype, eb, pack_all(a, b, eb));
   const bool loose = is_loose(p.choice);
   p.gemm = plan_gemm(p.choice, loose ? a.ref : packed(ws, a, eb), loose ? b.ref : packed(ws, b, eb),
                      m, n, k, eb);
@@ -432,7 +448,10 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
     }
     if (a->d_bias) {
       s.ld_part = round_up(n, 4);
-      s.part = ws.take<float>((int64_t)s.chunks * s.ld_part * 4);
+      if (s.chunks > 1)
+        s.part = ws.take<float>((int64_t)s.chunks * s.ld_part * 4);
+      else
+        s.sums = a->d_bias;
     }
   }
   if (P.want_x) {
@@ -497,6 +516,14 @@ Operand weight_piece(const void* w, int64_t ld, int32_t first, int32_t rows, int
   return o;
 }
 
+// Weight rows that are no chunks are read as they are up to so many rows of x,
+// where that costs less than copying them (a copy moves 4 bytes an element, a
+// loose product takes some 40% longer); backward, with three products, half.
+constexpr int kLooseLossRows = 1024;
+// The loss's epilogues as bytes an element: some ten instructions, and what the
+// gradient's stores.
+constexpr double kStatsBytes = 2.0, kGradBytes = 3.0;
+
 struct LossPlan {
   Operand x;
   MatrixRef x_ref;
@@ -517,18 +544,20 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
   LossPlan P{};
   Arena ws(base);
   const bool skinny = m <= kSkinnyRows;
-  P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
-  P.x_ref = m <= kLooseRows ? P.x.ref : packed(ws, P.x, eb);
   const int64_t ld_w = stride_of(a->weight_stride, v, k);
+  const bool loose = !chunked(a->weight, ld_w, k, eb) && m <= kLooseLossRows;
+  P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
+  P.x_ref = m <= kLooseRows || (loose && !skinny) ? P.x.ref : packed(ws, P.x, eb);
   P.piece = round_up(v, kPieceStep);
-  if (!skinny && !chunked(a->weight, ld_w, k, eb)) {
+  if (!loose && !chunked(a->weight, ld_w, k, eb)) {
     const int64_t row = round_up(k, 16 / eb) * eb;
-    P.piece = piece_cols(v, ((int64_t)64 << 20) / row);
+    P.piece = piece_cols(v, ((int64_t)128 << 20) / row);
     P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
     if (!base) P.packed = (void*)1;  // (sizes only)
   }
   P.choice = skinny ? choose_skinny(m, v, true)
-                    : choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, false);
+                    : choose(m, std::min(P.piece, (int64_t)v), slabs_of(k, eb), a->dtype, kStatsBytes,
+                             false, loose ? kLooseAny : kChunked);
   const int64_t side = kTileSide[P.choice.tile];
   if (ceil_div(m, side) * ceil_div(P.piece, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
@@ -549,6 +578,7 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
 struct LossBackwardPlan {
   Operand x;
   MatrixRef x_ref;
+  bool loose;  // weight rows and x are read as they are
   int64_t piece;
   void* packed;
   void* g;      // [rows, ld_g]: the gradient at a piece of the logits
@@ -577,12 +607,14 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   LossBackwardPlan P{};
   Arena ws(base);
   P.x = operand(a->x, stride_of(a->x_stride, m, k), m, k, eb);
-  P.x_ref = packed(ws, P.x, eb);
+  const int64_t ld_w = stride_of(a->weight_stride, v, k);
+  P.loose = !chunked(a->weight, ld_w, k, eb) && m <= kLooseLossRows / 2;
+  const Rows rows = P.loose ? kLooseAny : kChunked, rows2 = P.loose ? kLooseSmall : kChunked;
+  P.x_ref = P.loose && m > kSkinnyRows ? P.x.ref : packed(ws, P.x, eb);
   // A piece's gradient stays in the 256 MB last-level cache between the pass
   // that writes it and the products that read it.
   P.piece = piece_cols(v, ((int64_t)128 << 20) / ((int64_t)m * eb));
-  const int64_t ld_w = stride_of(a->weight_stride, v, k);
-  if (!chunked(a->weight, ld_w, k, eb)) {
+  if (!P.loose && !chunked(a->weight, ld_w, k, eb)) {
     const int64_t row = round_up(k, 16 / eb) * eb;
     P.piece = std::min(P.piece, piece_cols(v, ((int64_t)128 << 20) / row));
     P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
@@ -593,20 +625,20 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   P.g = ws.take((int64_t)m * P.ld_g * eb);
   if (eb == 2) P.scale = ws.take<float>(8);
   P.grad = m <= kSkinnyRows ? choose_skinny(m, cols, true)
-                            : choose(m, cols, slabs_of(k, eb), a->dtype, false);
+                            : choose(m, cols, slabs_of(k, eb), a->dtype, kGradBytes, false, rows);
   const int64_t side = kTileSide[P.grad.tile];
   if (ceil_div(m, side) * ceil_div(cols, side) > kMaxBlocks)
     return set_error(LSAMP_ERR_SHAPE, "%d rows of %d logits are too many for one call", m, v);
   if (a->d_x) {
     // (the sums of all pieces are added in float32, unless there is one)
-    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, true);
+    P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, cols == v ? eb : 8, true, rows2);
     const GemmPlan g = plan_gemm(P.dx, MatrixRef{}, MatrixRef{}, m, k, cols, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", m, k);
     P.dx_straight = g.parts == 1 && cols == v;
     if (!P.dx_straight) P.dx_sum = take_partial(ws, m, k, g.parts);
   }
   if (a->d_weight) {
-    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, true);
+    P.dw = choose(cols, k, slabs_of(m, eb), a->dtype, eb, true, rows2);
     const GemmPlan g = plan_gemm(P.dw, MatrixRef{}, MatrixRef{}, cols, k, m, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", v, k);
     P.dw_split = g.parts > 1;
@@ -615,7 +647,7 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   if (a->d_bias) {
     plan_col_sum(P.col, m, (int32_t)cols);
     P.col.ld_part = round_up(cols, 4);
-    P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
+    if (P.col.chunks > 1) P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
   }
   P.bytes = ws.used;
   *out = P;
@@ -670,7 +702,7 @@ lsamp_status lsamp_linear_backward(lsamp_context* ctx, const lsamp_linear_backwa
   const int eb = element_bytes(a->dtype);
   LSAMP_TRY(lay_out(P.d, eb, stream));
   if (P.sum) LSAMP_TRY(HEAD_OP(a->dtype, col_sum(P.col, stream)));
-  if (a->d_bias) LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(P.col, a->d_bias, nullptr, stream)));
+  if (P.col.part) LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(P.col, a->d_bias, nullptr, stream)));
   if (P.want_x) {
     LSAMP_TRY(lay_out(P.w, eb, stream));
     LSAMP_TRY(run_product(P.dx, a->dtype, stream));
@@ -793,8 +825,13 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
       s.cols = n;
       s.in = P.g;
       s.ld_in = P.ld_g;
+      if (!s.part) {
+        s.sums = (char*)a->d_bias + first * eb;
+        s.scale = inverse;
+      }
       LSAMP_TRY(HEAD_OP(a->dtype, col_sum(s, stream)));
-      LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
+      if (s.part)
+        LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
     }
   }
   if (a->d_x && !P.dx_straight)

@@ -13,7 +13,13 @@ constexpr int kThreads = 256;
 
 // Rows whose start, distance or length keeps them from being read as 16-byte
 // chunks are copied once to rows that can, zero-filled to whole chunks.  A
-// thread writes one chunk; bound by HBM, one read and one write.
+// thread writes one chunk, read by one access of any alignment; bound by HBM,
+// one read and one write.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename U>
+struct __attribute__((packed, aligned(sizeof(U)))) Any16 {
+  u32x4 v;
+};
 template <typename U>
 __global__ __launch_bounds__(kThreads) void k_pack(PackPlan p) {
   constexpr int N = 16 / (int)sizeof(U);
@@ -23,12 +29,16 @@ __global__ __launch_bounds__(kThreads) void k_pack(PackPlan p) {
     U* dst = (U*)p.dst + (int64_t)r * p.dst_ld;
     for (int c = (int)(blockIdx.x * kThreads + threadIdx.x); c < chunks;
          c += (int)gridDim.x * kThreads) {
-      U v[N];
+      u32x4 o;
+      if (c * N + N <= p.cols) {
+        o = ((const Any16<U>*)(src + c * N))->v;
+      } else {
+        U v[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = c * N + k < p.cols ? src[c * N + k] : (U)0;
-      uint4 o;
-      __builtin_memcpy(&o, v, 16);
-      *(uint4*)(dst + c * N) = o;
+        for (int k = 0; k < N; ++k) v[k] = c * N + k < p.cols ? src[c * N + k] : (U)0;
+        __builtin_memcpy(&o, v, 16);
+      }
+      *(u32x4*)(dst + c * N) = o;
     }
   }
 }
