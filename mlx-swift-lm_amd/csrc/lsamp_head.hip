@@ -196,28 +196,35 @@ struct Linear : EpiLinear {
     finish(r, c, v, bias_at(c), residual_at(r, c));
   }
   // A row's residual is on its way while the row before is stored (which may be
-  // the residual's own memory, so the compiler keeps the order as written).
+  // the residual's own memory, so the compiler keeps the order as written).  One
+  // copy of the code for all rows, the sums moved down to it: unrolled, the
+  // activations are 150 KB of instructions that no cache holds (silu over 8192 x
+  // 4096 x 4096 took 40 us).
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
                                       int lane, char*) const {
     const int r0 = m0 + wm * (FM * 16) + (lane & 15);
     const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
-    v4f b[FN], res[2][FN];
+    v4f b[FN], res[FN], next[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       b[i] = bias_at(c0 + i * 16);
-      res[0][i] = residual_at(r0, c0 + i * 16);
+      next[i] = residual_at(r0, c0 + i * 16);
     }
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < FM; ++j) {
       const int r = r0 + j * 16;
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-        if (j + 1 < FM) res[(j + 1) & 1][i] = residual_at(r + 16, c0 + i * 16);
+      for (int i = 0; i < FN; ++i) {
+        res[i] = next[i];
+        next[i] = residual_at(j + 1 < FM ? r + 16 : m, c0 + i * 16);
+      }
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int c = c0 + i * 16;
-        if (r < m && c < n) finish(r, c, acc[i][j], b[i], res[j & 1][i]);
+        if (r < m && c < n) finish(r, c, acc[i][0], b[i], res[i]);
+#pragma unroll
+        for (int k = 0; k + 1 < FM; ++k) acc[i][k] = acc[i][k + 1];
       }
     }
   }
