@@ -104,31 +104,39 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
     at_step = at_step + 1 == steps ? 0 : at_step + 1;
     return slab;
   };
-  // Step u: the next step's loads, then u's products once only those are under
+  // A step: the next one's loads, then its own products once only those are under
   // way.  The LDS reads of the step before are done by then (wait_loads), so its
-  // buffer may be filled.
-  const auto step = [&](Step& now, Step& then, int u, int buffer) {
+  // buffer may be filled.  MORE is known when it is compiled: where the loads are
+  // in doubt the compiler waits for all of them.
+  const auto step = [&](Step& now, Step& then, int buffer, auto more) {
+    constexpr bool MORE = decltype(more)::value;
     if constexpr (kStaged) {
       __builtin_amdgcn_sched_barrier(0);
       wait_loads<kLoads>();
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (u + 1 < steps) load(then, next(), buffer ^ 1);
+    if constexpr (MORE) load(then, next(), buffer ^ 1);
     if constexpr (kStaged) {
       __builtin_amdgcn_sched_barrier(0);
-      if (u + 1 < steps)
-        wait_loads<kLoads>();
-      else
-        wait_loads<0>();
+      wait_loads<MORE ? kLoads : 0>();
       __builtin_amdgcn_sched_barrier(0);
     }
     multiply(now, buffer);
   };
   Step s0, s1;
-  if (steps > 0) load(s0, next(), 0);
-  for (int u = 0; u < steps; u += 2) {
-    step(s0, s1, u, 0);
-    if (u + 1 < steps) step(s1, s0, u + 1, 1);
+  if (steps > 0) {
+    load(s0, next(), 0);
+    int u = 0;
+    for (; u + 2 < steps; u += 2) {
+      step(s0, s1, 0, std::true_type{});
+      step(s1, s0, 1, std::true_type{});
+    }
+    if (u + 1 < steps) {
+      step(s0, s1, 0, std::true_type{});
+      step(s1, s0, 1, std::false_type{});
+    } else {
+      step(s0, s1, 0, std::false_type{});
+    }
   }
   if (whole * kSlab < k_all && wave == whole % WK) {  // the last slab, where it ends
     if constexpr (kStaged) {
