@@ -14,6 +14,10 @@ using namespace lsamp;
 namespace {
 
 constexpr int32_t kMaxDim = 1 << 27;
+// Columns of a matrix: a tile's rows lie within 32 bits of its first (256 rows of
+// 16-bit elements, 128 of float32).
+constexpr int32_t kMaxFeatures = 1 << 22;
+constexpr int32_t kMaxLossRows = 1 << 23;  // (a work-group a row)
 constexpr int64_t kAlign = 256;
 // Work-groups of a launch: 512 threads each, below 2^32 threads in all.
 constexpr int64_t kMaxBlocks = (int64_t)1 << 22;
@@ -217,9 +221,9 @@ lsamp_status device_error(int err) {
   } while (0)
 
 // --------------------------------------------------------------------- checks
-lsamp_status check_dims(const char* what, int32_t v) {
-  if (v <= 0 || v > kMaxDim)
-    return set_error(LSAMP_ERR_SHAPE, "%s %d out of range [1, %d]", what, v, kMaxDim);
+lsamp_status check_dims(const char* what, int32_t v, int32_t most = kMaxFeatures) {
+  if (v <= 0 || v > most)
+    return set_error(LSAMP_ERR_SHAPE, "%s %d out of range [1, %d]", what, v, most);
   return LSAMP_OK;
 }
 lsamp_status check_dtype(int32_t dtype) {
@@ -285,7 +289,7 @@ struct LinearPlan {
 
 lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out) {
   if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
-  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
   LSAMP_CHECK(check_dims("in_features", a->in_features));
   LSAMP_CHECK(check_dims("out_features", a->out_features));
   LSAMP_CHECK(check_dtype(a->dtype));
@@ -397,7 +401,7 @@ struct LinearBackwardPlan {
 lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* base,
                                   LinearBackwardPlan* out) {
   if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
-  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
   LSAMP_CHECK(check_dims("in_features", a->in_features));
   LSAMP_CHECK(check_dims("out_features", a->out_features));
   LSAMP_CHECK(check_dtype(a->dtype));
@@ -427,7 +431,6 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
   if (act) {
     const int32_t wide = (int32_t)round_up(n, 16 / eb);
     P.d = operand(ws.take((int64_t)m * wide * eb), wide, m, wide, eb);
-    P.d.chunked = true;
   } else {
     P.d = operand(a->d_out, ld_d, m, n, eb);
   }
@@ -476,7 +479,7 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
 template <typename A>
 lsamp_status check_head(const A* a) {
   if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
-  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxLossRows));
   LSAMP_CHECK(check_dims("hidden", a->hidden));
   LSAMP_CHECK(check_dims("vocab", a->vocab));
   LSAMP_CHECK(check_dtype(a->dtype));
@@ -842,8 +845,8 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
 lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* a, void* stream) {
   if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
   if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
-  LSAMP_CHECK(check_dims("rows", a->rows));
-  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
+  LSAMP_CHECK(check_dims("cols", a->cols, kMaxDim));
   LSAMP_CHECK(check_dtype(a->dtype));
   if (!(a->p >= 0.f && a->p <= 1.f))
     return set_error(LSAMP_ERR_INVALID_ARGUMENT, "p %g out of range [0, 1]", a->p);

@@ -220,6 +220,26 @@ def test_head_loss_in_pieces(ctx, dtype):
             H.check(got, want[name], name)
 
 
+@pytest.mark.parametrize("dtype,case", [
+    ("bf16", (1030, 8193, 8200, 0.0, True, "odd")), ("f32", (1030, 4101, 8200, 0.0, False, "odd"))])
+def test_head_loss_weight_copied_in_pieces(ctx, dtype, case):
+    """Weight rows of odd lengths under many rows of x are laid out a piece of
+    the vocabulary at a time, in both directions; here two pieces."""
+    print(f"copied pieces {case} {dtype}", flush=True)
+    x, w, b, t, d, cap = _loss_inputs(case, dtype)
+    f = ctx.prepare_head_loss(x, w, t, bias=b, softcap=cap)
+    f.launch()
+    want = H.loss64(x, w, t, b, cap)
+    H.check(f.lse, want["lse"], "lse")
+    H.check(f.loss, want["loss"], "loss")
+    p = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, bias=b, softcap=cap, want_bias=True)
+    p.launch()
+    print("the 64-bit gradients", flush=True)
+    want = H.loss_grads64(d, x, w, t, f.lse, b, cap)
+    for name, got in p.outputs().items():
+        H.check(got, want[name], name)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_head_loss_masked_vocabulary(ctx, dtype):
     """Ids with a bias of -inf or the type's lowest value have no mass; whole

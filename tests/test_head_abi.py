@@ -124,3 +124,23 @@ def test_calls_without_a_context(lib):
     for entry in ("lsamp_linear_backward", "lsamp_head_loss", "lsamp_head_loss_backward",
                   "lsamp_dropout"):
         assert getattr(lib, entry)(None, None, None) == _ffi.LSAMP_ERR_INVALID_ARGUMENT
+
+
+def test_limits_of_sizes(lib):
+    """A tile's rows lie within 32 bits of its first: features end at 2^22; a
+    loss has a work-group a row: 2^23 rows."""
+    wide = 1 << 22
+    f = lambda **kw: lib.lsamp_linear_workspace(ctypes.byref(linear(**kw)))  # noqa: E731
+    S = _ffi.LSAMP_ERR_SHAPE
+    for dtype in (_ffi.DTYPE_F32, _ffi.DTYPE_BF16):
+        kw = dict(rows=100, dtype=dtype, out_dtype=dtype)
+        assert f(in_features=wide, x_stride=wide, weight_stride=wide, **kw) >= 0
+        assert f(in_features=wide + 1, x_stride=wide + 1, weight_stride=wide + 1, **kw) == S
+        assert f(out_features=wide, out_stride=wide, **kw) >= 0
+        assert f(out_features=wide + 1, out_stride=wide + 1, **kw) == S
+    for cls, entry in ((_ffi.HeadLossArgs, lib.lsamp_head_loss_workspace),
+                       (_ffi.HeadLossBackwardArgs, lib.lsamp_head_loss_backward_workspace)):
+        assert entry(ctypes.byref(loss(cls, rows=1 << 23))) > 0
+        assert entry(ctypes.byref(loss(cls, rows=(1 << 23) + 1))) == S
+        assert b"rows" in lib.lsamp_last_error()
+        assert entry(ctypes.byref(loss(cls, vocab=wide + 1))) == S
