@@ -11,10 +11,9 @@
 namespace lsamp {
 
 // A matrix in HBM: `rows` rows of `cols` readable elements, `ld` elements
-// apart.  Products read 16-byte chunks: p and ld in bytes are multiples of 16,
-// cols of a chunk's elements.
-// (Loose shapes and the kernels of few rows read rows of any address, distance
-// and length.)
+// apart.  The tiled products read 16-byte chunks: p and ld in bytes are multiples
+// of 16, cols of a chunk's elements.  Loose shapes take rows of any address,
+// distance and length, as the kernels of few rows do of W (and of x up to 16 rows).
 struct MatrixRef {
   const void* p;
   int64_t ld;
@@ -150,9 +149,9 @@ struct DropoutPlan {
 // One set of these for each element type; 0 or a hipError_t.
 template <int DT>
 struct HeadOps {
+  // kSkinny16: gemm_linear only; kSkinny64: not gemm_store and gemm_partial;
+  // kLoose64 and kLoose64x4: not gemm_stats and gemm_grad; kTile256: not float32.
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinear& e, void* stream);
-  // (kSkinny16: gemm_linear only; kSkinny64: not gemm_store and gemm_partial;
-  // kLoose64 and kLoose64x4: not the loss's)
   static int gemm_stats(GemmTile tile, const GemmPlan& g, const EpiStats& e, void* stream);
   static int gemm_grad(GemmTile tile, const GemmPlan& g, const EpiGrad& e, void* stream);
   static int gemm_store(GemmRoles roles, GemmTile tile, const GemmPlan& g, const EpiStore& e,

@@ -36,18 +36,18 @@ __device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid) {
   }
   return v;
 }
-__device__ __forceinline__ void store4(void* base, int64_t i, v4f v, int valid) {
+__device__ __forceinline__ void store4e(void* base, int64_t i, v4e v, int valid) {
   S* p = (S*)base + i;
   if (valid >= 4) {
-    v4e e;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) e[k] = (S)v[k];
-    ((Any<v4e, S>*)p)->v = e;
+    ((Any<v4e, S>*)p)->v = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < valid) p[k] = (S)v[k];
+      if (k < valid) p[k] = v[k];
   }
+}
+__device__ __forceinline__ void store4(void* base, int64_t i, v4f v, int valid) {
+  store4e(base, i, __builtin_convertvector(v, v4e), valid);
 }
 __device__ __forceinline__ v4f load4f(const float* p, int valid) {
   if (valid >= 4) return ((const Any<v4f, float>*)p)->v;
@@ -84,14 +84,14 @@ __device__ __forceinline__ float expe(float x) {
 // 1 / (1 + exp(-z)) and tanh.  For 16-bit elements with the hardware's
 // reciprocal (1 ulp) in place of a division of some ten instructions, and tanh
 // as 1 - 2 / (exp(2 |x|) + 1), a polynomial below 0.3 where that cancels: off by
-// less than 6 2^-24, far below the result's own rounding.  (The library's tanhf
-// took a third of the time of a soft-capped head of 333 x 1000 x 40003.)
-__device__ __forceinline__ float sigmoid(float z) {
+// less than 6 2^-24, far below the result's own rounding.
+__device__ __forceinline__ float reciprocal(float v) {
   if constexpr (DT == LSAMP_DTYPE_F32)
-    return 1.f / (1.f + expe(-z));
+    return 1.f / v;
   else
-    return __builtin_amdgcn_rcpf(1.f + expe(-z));
+    return __builtin_amdgcn_rcpf(v);
 }
+__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + expe(-z)); }
 __device__ __forceinline__ float tanhe(float x) {
   if constexpr (DT == LSAMP_DTYPE_F32) {
     return tanhf(x);
@@ -117,6 +117,16 @@ constexpr float kGeluB = 0.044715f;
     return v;                                            \
   } while (0)
 
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)): nothing cancels, and no tanh.  Past 1e4
+// it is 0 or 1 all the same, and the cube finite.
+__device__ __forceinline__ float clamped(float z) { return fminf(fmaxf(z, -1e4f), 1e4f); }
+__device__ __forceinline__ float gelu_gate(float z) {
+  const float c = clamped(z);
+  return sigmoid(2.f * kGeluA * (c + kGeluB * c * c * c));
+}
+__device__ __forceinline__ float gelu_tanh(float z) {
+  return z * gelu_gate(z);
+}
 // act(z) and act'(z) of four columns (one branch for them: it costs as much as
 // the arithmetic of one).
 __device__ __forceinline__ v4f activate(int act, float cap, v4f v) {
@@ -124,8 +134,7 @@ __device__ __forceinline__ v4f activate(int act, float cap, v4f v) {
     case LSAMP_ACT_RELU: LSAMP_EACH(z < 0.f ? 0.f : z);  // (a NaN stays)
     case LSAMP_ACT_SILU: LSAMP_EACH(z * sigmoid(z));
     case LSAMP_ACT_GELU: LSAMP_EACH(0.5f * z * (1.f + erff(z * kSqrtHalf)));
-    case LSAMP_ACT_GELU_TANH:
-      LSAMP_EACH(0.5f * z * (1.f + tanhe(kGeluA * (z + kGeluB * z * z * z))));
+    case LSAMP_ACT_GELU_TANH: LSAMP_EACH(gelu_tanh(z));
     case LSAMP_ACT_SOFTCAP: {
       const float inverse = 1.f / cap;
       LSAMP_EACH(cap * tanhe(z * inverse));
@@ -138,8 +147,8 @@ __device__ __forceinline__ float silu_slope(float z) {
   return s * (1.f + z * (1.f - s));
 }
 __device__ __forceinline__ float gelu_tanh_slope(float z) {
-  const float t = tanhe(kGeluA * (z + kGeluB * z * z * z));
-  return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluA * (1.f + 3.f * kGeluB * z * z);
+  const float s = gelu_gate(z), c = clamped(z);
+  return s + 2.f * kGeluA * z * (s * (1.f - s)) * (1.f + 3.f * kGeluB * c * c);
 }
 __device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
   switch (act) {
@@ -157,19 +166,27 @@ __device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
 }
 
 // ------------------------------------------------------------------ epilogues
-// put(r, c, v): four columns from c of row r.
-template <class E, int FM, int FN, int BM, int BN, int WM, int WN>
-__device__ __forceinline__ void put_all(const E& e, v4f (&acc)[FN][FM], int m0, int n0, int part,
-                                        int wm, int wn, int lane) {
+// A wave's sums lie with 16 lanes down a column of rows; stored like that, an
+// instruction writes 16 rows of 32 bytes, and rows a power of two apart meet in
+// the same few channels (4096 x 16384 x 4096: 490 us, 371 without its stores).
+// So the quads of columns of 16 rows change lanes through LDS, a KB a quad of
+// columns and wave: 4 FN lanes then lie along a row, 16 / FN rows a quad.
+template <int FN>
+struct Along {
+  static constexpr int kLanes = 4 * FN, kRows = 16 / FN;
+  int row, col;  // of the 16 rows, of the wave's columns
+  __device__ __forceinline__ explicit Along(int lane) : row(lane / kLanes), col(lane % kLanes * 4) {}
+};
+template <int FN, class V>
+__device__ __forceinline__ void exchange(V (&v)[FN], char* lds, int lane) {
+  constexpr int kLanes = 4 * FN;
+  V* const rows = (V*)lds;
+  // (permuted within the row: 16 rows' writes fall on different banks)
+  const auto place = [](int r, int q) { return r * kLanes + (q ^ (r / (4 / FN))); };
 #pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int r = m0 + wm * (FM * 16) + j * 16 + (lane & 15);
+  for (int i = 0; i < FN; ++i) rows[place(lane & 15, i * 4 + (lane >> 4))] = v[i];
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
-      if (r < e.m && c < e.n) e.put(r, c, acc[i][j], part);
-    }
-  }
+  for (int i = 0; i < FN; ++i) v[i] = rows[place(i * (16 / FN) + lane / kLanes, lane % kLanes)];
 }
 
 struct Linear : EpiLinear {
@@ -195,37 +212,37 @@ struct Linear : EpiLinear {
   __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
     finish(r, c, v, bias_at(c), residual_at(r, c));
   }
-  // A row's residual is on its way while the row before is stored (which may be
+  // The next rows' residual is on its way while these are stored (which may be
   // the residual's own memory, so the compiler keeps the order as written).  One
   // copy of the code for all rows, the sums moved down to it: unrolled, the
   // activations are 150 KB of instructions that no cache holds (silu over 8192 x
   // 4096 x 4096 took 40 us).
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
-                                      int lane, char*) const {
-    const int r0 = m0 + wm * (FM * 16) + (lane & 15);
-    const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
-    v4f b[FN], res[FN], next[FN];
+                                      int lane, char* lds) const {
+    const Along<FN> at(lane);
+    char* const mine = lds + (wn * WM + wm) * (FN * 1024);
+    const int r0 = m0 + wm * (FM * 16) + at.row, c = n0 + wn * (FN * 16) + at.col;
+    const v4f b = bias_at(c);
+    v4f res[FN], next[FN];
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      b[i] = bias_at(c0 + i * 16);
-      next[i] = residual_at(r0, c0 + i * 16);
-    }
+    for (int i = 0; i < FN; ++i) next[i] = residual_at(r0 + i * at.kRows, c);
 #pragma unroll 1
     for (int j = 0; j < FM; ++j) {
       const int r = r0 + j * 16;
+      v4f v[FN];
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        res[i] = next[i];
-        next[i] = residual_at(j + 1 < FM ? r + 16 : m, c0 + i * 16);
-      }
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const int c = c0 + i * 16;
-        if (r < m && c < n) finish(r, c, acc[i][0], b[i], res[i]);
+        v[i] = acc[i][0];
 #pragma unroll
         for (int k = 0; k + 1 < FM; ++k) acc[i][k] = acc[i][k + 1];
+        res[i] = next[i];
+        next[i] = residual_at(j + 1 < FM ? r + 16 + i * at.kRows : m, c);
       }
+      exchange<FN>(v, mine, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+        if (r + i * at.kRows < m && c < n) finish(r + i * at.kRows, c, v[i], b, res[i]);
     }
   }
 };
@@ -237,18 +254,25 @@ struct Store : EpiStore {
     store4(out, (int64_t)r * ld_out + c, v, n - c);
   }
   template <int FM, int FN, int BM, int BN, int WM, int WN>
-  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
-                                      int lane, char*) const {
-    if (scale) {  // (once: the stores may be to its memory for all the compiler knows)
-      const float s = *scale;
+  __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
+                                      int lane, char* lds) const {
+    // (once: the stores may be to its memory for all the compiler knows)
+    const float s = scale ? *scale : 1.f;
+    const Along<FN> at(lane);
+    char* const mine = lds + (wn * WM + wm) * (FN * 1024);
+    const int r0 = m0 + wm * (FM * 16) + at.row, c = n0 + wn * (FN * 16) + at.col;
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
+    for (int j = 0; j < FM; ++j) {
+      v4e v[FN];
 #pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] *= s;
+      for (int i = 0; i < FN; ++i) v[i] = __builtin_convertvector(acc[i][j] * s, v4e);
+      exchange<FN>(v, mine, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int r = r0 + j * 16 + i * at.kRows;
+        if (r < m && c < n) store4e(out, (int64_t)r * ld_out + c, v[i], n - c);
+      }
     }
-    Store plain = *this;
-    plain.scale = nullptr;
-    put_all<Store, FM, FN, BM, BN, WM, WN>(plain, acc, m0, n0, at.part, wm, wn, lane);
   }
 };
 
@@ -264,31 +288,50 @@ struct Partial : EpiPartial {
   }
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt tile, int wm, int wn,
-                                      int lane, char*) const {
+                                      int lane, char* lds) const {
+    const Along<FN> along(lane);
+    char* const mine = lds + (wn * WM + wm) * (FN * 1024);
+    const int r0 = m0 + wm * (FM * 16) + along.row, c = n0 + wn * (FN * 16) + along.col;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      v4f v[FN];
+#pragma unroll
+      for (int i = 0; i < FN; ++i) v[i] = acc[i][j];
+      exchange<FN>(v, mine, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) acc[i][j] = v[i];
+    }
+    if (c >= n) return;
     if (accumulate) {  // all reads before the first store
-      const int r0 = m0 + wm * (FM * 16) + (lane & 15);
-      const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
 #pragma unroll
       for (int j = 0; j < FM; ++j)
 #pragma unroll
-        for (int i = 0; i < FN; ++i)
-          if (r0 + j * 16 < m && c0 + i * 16 < n) acc[i][j] += *at(r0 + j * 16, c0 + i * 16, tile.part);
+        for (int i = 0; i < FN; ++i) {
+          const int r = r0 + j * 16 + i * along.kRows;
+          if (r < m) acc[i][j] += *at(r, c, tile.part);
+        }
     }
-    Partial plain = *this;
-    plain.accumulate = 0;
-    put_all<Partial, FM, FN, BM, BN, WM, WN>(plain, acc, m0, n0, tile.part, wm, wn, lane);
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int r = r0 + j * 16 + i * along.kRows;
+        if (r < m) *at(r, c, tile.part) = acc[i][j];
+      }
   }
 };
 
-// z = softcap(sum + bias) of four columns, and the slope of the cap.
-__device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float inverse, v4f* slope) {
+// z = softcap(sum + bias) of four columns, and the slope of the cap: with r = 1 /
+// (exp(2 t) + 1), tanh t = 1 - 2 r and its slope is 4 r (1 - r).  Absolutely that is
+// as near as the logit's own sum (some 2^-24 of the cap); the slope does not cancel.
+__device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float twice, v4f* slope) {
   v += b;
   if (softcap > 0.f) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float t = tanhe(v[k] * inverse);
-      v[k] = softcap * t;
-      if (slope) (*slope)[k] = 1.f - t * t;
+      const float r = reciprocal(1.f + expe(v[k] * twice));
+      v[k] = fmaf(-2.f * softcap, r, softcap);
+      if (slope) (*slope)[k] = 4.f * r * (1.f - r);
     }
   }
   return v;
@@ -307,7 +350,7 @@ struct Stats : EpiStats {
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char* lds) const {
     float* red = (float*)lds;  // [WN][BM][2]
-    const float inverse = softcap > 0.f ? 1.f / softcap : 0.f;
+    const float twice = softcap > 0.f ? 2.f / softcap : 0.f;
     v4f b[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
@@ -329,7 +372,7 @@ struct Stats : EpiStats {
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
-        v4f v = logits4(acc[i][j], b[i], softcap, inverse, nullptr);
+        v4f v = logits4(acc[i][j], b[i], softcap, twice, nullptr);
         if (!inside) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = c + k < n ? v[k] : -INFINITY;
@@ -383,9 +426,12 @@ struct Grad : EpiGrad {
   static constexpr int kBarriers = 0;
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt, int wm, int wn,
-                                      int lane, char*) const {
+                                      int lane, char* lds) const {
+    const Along<FN> along(lane);
+    char* const mine = lds + (wn * WM + wm) * (FN * 1024);
+    const int out_col = n0 + wn * (FN * 16) + along.col;
     const float s = scale ? scale[0] : 1.f;
-    const float inverse = softcap > 0.f ? 1.f / softcap : 0.f;
+    const float twice = softcap > 0.f ? 2.f / softcap : 0.f;
     const int r0 = m0 + wm * (FM * 16) + (lane & 15);
     const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
     v4f b[FN];
@@ -402,16 +448,14 @@ struct Grad : EpiGrad {
     }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const int r = r0 + j * 16;
-      if (r >= m) continue;
       const bool none = target[j] < 0 || target[j] >= vocab || l[j] == -INFINITY;
+      v4e q[FN];
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int c = c0 + i * 16;
-        if (c >= n_pad) continue;
         v4f slope = {1.f, 1.f, 1.f, 1.f}, g;
         const int valid = n - c;
-        const v4f z = logits4(acc[i][j], b[i], softcap, inverse, &slope);
+        const v4f z = logits4(acc[i][j], b[i], softcap, twice, &slope);
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] = expe(z[k] - l[j]);
         const int at = target[j] - first_col - c;
@@ -425,7 +469,13 @@ struct Grad : EpiGrad {
 #pragma unroll
           for (int k = 0; k < 4; ++k) g[k] = none || k >= valid ? 0.f : g[k];
         }
-        store4(out, (int64_t)r * ld_out + c, g, 4);
+        q[i] = __builtin_convertvector(g, v4e);
+      }
+      exchange<FN>(q, mine, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int r = m0 + wm * (FM * 16) + j * 16 + i * along.kRows + along.row;
+        if (r < m && out_col < n_pad) store4e(out, (int64_t)r * ld_out + out_col, q[i], 4);
       }
     }
   }
@@ -438,7 +488,11 @@ E with(const P& plan) {
   return e;
 }
 
-// LOOSE: the small shapes that take any rows too.  (float32 tiles go up to 128 x 128: a wave's split fragments need the registers)
+#define LSAMP_TILE(THREADS, ...)                                                               \
+  hipLaunchKernelGGL((k_gemm<DT, AK, BK, __VA_ARGS__, E>), grid, dim3(THREADS), 0, st, g, e)
+
+// LOOSE: the 64 x 64 shapes that take any rows too.  Float32 tiles go up to 128 x
+// 128: a wave's split fragments need the registers.
 template <bool AK, bool BK, bool LOOSE, class E>
 int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.parts));
@@ -446,36 +500,36 @@ int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
   switch (tile) {
     case kTile256:
       if constexpr (DT != LSAMP_DTYPE_F32) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 256, 256, 2, 4, 0, 1, false, E>), grid, dim3(512), 0, st, g, e);
+        LSAMP_TILE(512, 256, 256, 2, 4, 0, 1, false);
         break;
       }
       return (int)hipErrorInvalidValue;
     case kTile128:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, false, E>), grid, dim3(256), 0, st, g, e);
+      LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, false);
       break;
     case kTile64:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, false, E>), grid, dim3(256), 0, st, g, e);
+      LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, false);
       break;
     case kTile128x2:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 2, false, E>), grid, dim3(512), 0, st, g, e);
+      LSAMP_TILE(512, 128, 128, 2, 2, 2, 2, false);
       break;
     case kLoose64:
       if constexpr (LOOSE) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 1, true, E>), grid, dim3(256), 0, st, g, e);
+        LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, true);
         break;
       }
       return (int)hipErrorInvalidValue;
     case kLoose128:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 128, 128, 2, 2, 2, 1, true, E>), grid, dim3(256), 0, st, g, e);
+      LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, true);
       break;
     case kLoose64x4:
       if constexpr (LOOSE) {
-        hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, true, E>), grid, dim3(1024), 0, st, g, e);
+        LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, true);
         break;
       }
       return (int)hipErrorInvalidValue;
     case kTile64x4:
-      hipLaunchKernelGGL((k_gemm<DT, AK, BK, 64, 64, 2, 2, 2, 4, false, E>), grid, dim3(1024), 0, st, g, e);
+      LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, false);
       break;
     default:
       return (int)hipErrorInvalidValue;
@@ -646,7 +700,8 @@ int HeadOps<DT>::col_sum(const ColSumPlan& p, void* stream) {
 }
 template <>
 int HeadOps<DT>::col_sum_join(const ColSumPlan& p, void* out, const float* scale, void* stream) {
-  hipLaunchKernelGGL(k_col_sum_join, dim3((unsigned)((p.cols + 63) / 64)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream), p, (S*)out, scale);
+  hipLaunchKernelGGL(k_col_sum_join, dim3((unsigned)((p.cols + 63) / 64)), dim3(kThreads), 0,
+                     reinterpret_cast<hipStream_t>(stream), p, (S*)out, scale);
   return (int)hipGetLastError();
 }
 

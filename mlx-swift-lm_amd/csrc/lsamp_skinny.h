@@ -35,7 +35,8 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
   using X = Side<DT, false, MF * 16, 1>;
   constexpr int kStageBytes = kStaged ? WK * 2 * X::kBytes : 0;
   constexpr int kSumBytes = WK * kFrags * kWave * 16;
-  constexpr int kRedBytes = ROWWISE ? 0 : WK * MF * 16 * 8;
+  // (an epilogue's pair of floats a row and wave, or its 16 rows of 16 columns a wave)
+  constexpr int kRedBytes = ROWWISE ? 0 : WK * (MF * 128 > 1024 ? MF * 128 : 1024);
   constexpr int kLds = kStageBytes > kSumBytes + kRedBytes ? kStageBytes : kSumBytes + kRedBytes;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   static_assert(ROWWISE || NF == WK, "a wave for every 16 columns");
