@@ -51,6 +51,7 @@ constexpr int kSkinnyRows = 64;
 struct EpiLinear {
   int32_t m, n;
   int32_t activation, wide;  // wide: out is float32
+  int32_t stream;            // out (and pre) are stored past the caches
   float softcap;
   const void* bias;
   const void* residual;
@@ -65,6 +66,7 @@ struct EpiStore {  // out = sums * *scale, in the operands' type
   void* out;
   int64_t ld_out;
   const float* scale;  // device, or NULL for 1
+  int32_t stream;      // stored past the caches
 };
 struct EpiPartial {  // float32 sums of one part, added to what is there
   int32_t m, n;

@@ -36,10 +36,16 @@ __device__ __forceinline__ v4f load4(const void* base, int64_t i, int valid) {
   }
   return v;
 }
+// STREAM: past the caches (an output that is larger than they are).
+template <bool STREAM = false>
 __device__ __forceinline__ void store4e(void* base, int64_t i, v4e v, int valid) {
+  typedef S v4u __attribute__((ext_vector_type(4), aligned(sizeof(S))));
   S* p = (S*)base + i;
   if (valid >= 4) {
-    ((Any<v4e, S>*)p)->v = v;
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(v, (v4u*)p);
+    else
+      *(v4u*)p = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -57,9 +63,14 @@ __device__ __forceinline__ v4f load4f(const float* p, int valid) {
     if (k < valid) v[k] = p[k];
   return v;
 }
+template <bool STREAM = false>
 __device__ __forceinline__ void store4f(float* p, v4f v, int valid) {
+  typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
   if (valid >= 4) {
-    ((Any<v4f, float>*)p)->v = v;
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(v, (v4u*)p);
+    else
+      *(v4u*)p = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -201,13 +212,24 @@ struct Linear : EpiLinear {
   __device__ __forceinline__ void finish(int r, int c, v4f v, v4f b, v4f res) const {
     const int valid = n - c;
     v += b;
-    if (pre) store4f(pre + (int64_t)r * ld_pre + c, v, valid);
+    if (pre) {
+      float* p = pre + (int64_t)r * ld_pre + c;
+      if (stream)
+        store4f<true>(p, v, valid);
+      else
+        store4f(p, v, valid);
+    }
     v = activate(activation, softcap, v);
     if (residual) v += res;
-    if (wide)
+    if (wide) {
       store4f((float*)out + (int64_t)r * ld_out + c, v, valid);
-    else
-      store4(out, (int64_t)r * ld_out + c, v, valid);
+    } else {
+      const v4e e = __builtin_convertvector(v, v4e);
+      if (stream)
+        store4e<true>(out, (int64_t)r * ld_out + c, e, valid);
+      else
+        store4e(out, (int64_t)r * ld_out + c, e, valid);
+    }
   }
   __device__ __forceinline__ void put(int r, int c, v4f v, int) const {
     finish(r, c, v, bias_at(c), residual_at(r, c));
@@ -270,7 +292,12 @@ struct Store : EpiStore {
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int r = r0 + j * 16 + i * at.kRows;
-        if (r < m && c < n) store4e(out, (int64_t)r * ld_out + c, v[i], n - c);
+        if (r < m && c < n) {
+          if (stream)
+            store4e<true>(out, (int64_t)r * ld_out + c, v[i], n - c);
+          else
+            store4e(out, (int64_t)r * ld_out + c, v[i], n - c);
+        }
       }
     }
   }

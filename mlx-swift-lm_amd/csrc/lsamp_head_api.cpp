@@ -197,6 +197,12 @@ bool too_many(const GemmPlan& g) {
   return (int64_t)g.tiles_m * g.tiles_n * g.parts > kMaxBlocks;
 }
 
+// An output larger than the L2s (8 x 4 MB) only pushes the operands out of them:
+// 4096 x 2048 x 32000 (262 MB) 490 us, 437 stored past them; 8192 x 4096 x 4096's
+// gradients 452 and 442.  A smaller one is there for the next call (a gradient of
+// 2048 x 4096 that the next two products read: 69 us and 83).
+bool streams(int64_t m, int64_t n, int eb) { return m * n * eb > (int64_t)32 << 20; }
+
 int64_t slabs_of(int64_t k, int eb) { return ceil_div(k, 128 / eb); }
 
 // A product into `out`: straight, or in parts through float32 sums.
@@ -333,6 +339,7 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
   e.activation = a->activation;
   e.softcap = a->softcap;
   e.wide = a->out_dtype == LSAMP_DTYPE_F32;
+  e.stream = streams(m, n, ob);
   e.bias = a->bias;
   e.residual = a->residual;
   e.ld_residual = stride_of(a->residual_stride, m, n);
@@ -379,6 +386,7 @@ Product plan_product(Arena& ws, GemmRoles roles, Operand& a, Operand& b, int64_t
   p.store.n = (int32_t)n;
   p.store.out = out;
   p.store.ld_out = ld;
+  p.store.stream = streams(m, n, eb);
   return p;
 }
 int run_product(const Product& p, int dtype, void* stream) {
@@ -772,6 +780,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   dx.out = a->d_x;
   dx.ld_out = stride_of(a->d_x_stride, m, k);
   dx.scale = inverse;
+  dx.stream = streams(m, k, eb);
   int dx_parts = 0;
   for (int64_t first = 0; first < v; first += P.piece) {
     const int32_t n = (int32_t)std::min(P.piece, v - first);
@@ -813,6 +822,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
       dw.ld_out = stride_of(a->d_weight_stride, v, k);
       dw.out = (char*)a->d_weight + first * dw.ld_out * eb;
       dw.scale = inverse;
+      dw.stream = streams(v, k, eb);
       const GemmPlan plan = plan_gemm(P.dw, g, P.x_ref, n, k, m, eb);
       if (!P.dw_split) {
         LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesTN, P.dw.tile, plan, dw, stream)));
