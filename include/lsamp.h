@@ -617,7 +617,7 @@ lsamp_status lsamp_mask_assemble(lsamp_context* ctx, const lsamp_mask_assemble_a
  * A workspace function returns 0 where none is needed and a negative status
  * for arguments that the call would refuse (last-error string set).
  * Outputs may not overlap inputs, except that `out` may be the residual
- * itself (same address and stride), and a dropout's `out` its `x`.  The calls
+ * itself (same address, stride and type), and a dropout's `out` its `x`.  The calls
  * use no other state, are ordered by their stream only, allocate nothing and
  * may be captured into a HIP graph. */
 typedef enum lsamp_activation {

@@ -76,13 +76,19 @@ Operand operand(const void* p, int64_t ld, int32_t rows, int32_t cols, int eb) {
   o.chunked = chunked(p, ld, cols, eb);
   return o;
 }
+// Rows in the workspace: whole chunks, and 128-byte lines apart, since a slab of a
+// row that lies across two lines reads both (2000 x 4097 x 4097 with its copies: 164
+// us with rows 8,208 bytes apart, 128 with rows 8,320 apart).
+int64_t row_chunks(int64_t cols, int eb) { return round_up(cols, 16 / eb); }
+int64_t row_pitch(int64_t cols, int eb) { return round_up(cols, 128 / eb); }
 // Lays the operand out, if it has to be.
 MatrixRef packed(Arena& ws, Operand& o, int eb) {
   if (!o.chunked && !o.packed) {
-    const int32_t wide = (int32_t)round_up(o.ref.cols, 16 / eb);
-    void* dst = ws.take((int64_t)o.ref.rows * wide * eb);
+    const int64_t pitch = row_pitch(o.ref.cols, eb);
+    void* dst = ws.take((int64_t)o.ref.rows * pitch * eb);
     o.packed = true;
-    o.pack = PackPlan{o.ref.p, o.ref.ld, dst, wide, o.ref.rows, o.ref.cols, wide};
+    o.pack = PackPlan{o.ref.p,    o.ref.ld,   dst, pitch, o.ref.rows,
+                      o.ref.cols, (int32_t)row_chunks(o.ref.cols, eb)};
   }
   return o.packed ? MatrixRef{o.pack.dst, o.pack.dst_ld, o.pack.rows, o.pack.dst_cols} : o.ref;
 }
@@ -197,11 +203,12 @@ bool too_many(const GemmPlan& g) {
   return (int64_t)g.tiles_m * g.tiles_n * g.parts > kMaxBlocks;
 }
 
-// An output larger than the L2s (8 x 4 MB) only pushes the operands out of them:
-// 4096 x 2048 x 32000 (262 MB) 490 us, 437 stored past them; 8192 x 4096 x 4096's
-// gradients 452 and 442.  A smaller one is there for the next call (a gradient of
-// 2048 x 4096 that the next two products read: 69 us and 83).
-bool streams(int64_t m, int64_t n, int eb) { return m * n * eb > (int64_t)32 << 20; }
+// Outputs of more than half the last-level cache (256 MB) only push the operands
+// out of it and are stored past it: 8192 x 4096 x 4096 with kept pre-activations
+// (201 MB) 287 us and 246, 4096 x 2048 x 32000 (262 MB) 490 and 458.  Smaller ones
+// are found there by what reads them next: the head's gradients of 333 x 1000 x
+// 40003 (80 MB) take 138 us, stored past it 152.
+bool streams(int64_t bytes) { return bytes > (int64_t)128 << 20; }
 
 int64_t slabs_of(int64_t k, int eb) { return ceil_div(k, 128 / eb); }
 
@@ -339,7 +346,7 @@ lsamp_status plan_linear(const lsamp_linear_args* a, void* base, LinearPlan* out
   e.activation = a->activation;
   e.softcap = a->softcap;
   e.wide = a->out_dtype == LSAMP_DTYPE_F32;
-  e.stream = streams(m, n, ob);
+  e.stream = streams((int64_t)m * n * (ob + (a->pre ? 4 : 0)));
   e.bias = a->bias;
   e.residual = a->residual;
   e.ld_residual = stride_of(a->residual_stride, m, n);
@@ -386,7 +393,7 @@ Product plan_product(Arena& ws, GemmRoles roles, Operand& a, Operand& b, int64_t
   p.store.n = (int32_t)n;
   p.store.out = out;
   p.store.ld_out = ld;
-  p.store.stream = streams(m, n, eb);
+  p.store.stream = streams(m * n * eb);
   return p;
 }
 int run_product(const Product& p, int dtype, void* stream) {
@@ -437,8 +444,8 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
   P.want_w = a->d_weight != nullptr;
   const int64_t ld_d = stride_of(a->d_out_stride, m, n);
   if (act) {
-    const int32_t wide = (int32_t)round_up(n, 16 / eb);
-    P.d = operand(ws.take((int64_t)m * wide * eb), wide, m, wide, eb);
+    const int64_t pitch = row_pitch(n, eb);
+    P.d = operand(ws.take((int64_t)m * pitch * eb), pitch, m, (int32_t)row_chunks(n, eb), eb);
   } else {
     P.d = operand(a->d_out, ld_d, m, n, eb);
   }
@@ -520,10 +527,11 @@ Operand weight_piece(const void* w, int64_t ld, int32_t first, int32_t rows, int
     o.ref = MatrixRef{p, ld, rows, hidden};
     return o;
   }
-  const int32_t wide = (int32_t)round_up(hidden, 16 / eb);
+  const int32_t wide = (int32_t)row_chunks(hidden, eb);
+  const int64_t pitch = row_pitch(hidden, eb);
   o.packed = true;
-  o.pack = PackPlan{p, ld, packed, wide, rows, hidden, wide};
-  o.ref = MatrixRef{packed, wide, rows, wide};
+  o.pack = PackPlan{p, ld, packed, pitch, rows, hidden, wide};
+  o.ref = MatrixRef{packed, pitch, rows, wide};
   return o;
 }
 
@@ -561,7 +569,7 @@ lsamp_status plan_loss(const lsamp_head_loss_args* a, void* base, LossPlan* out)
   P.x_ref = m <= kLooseRows || (loose && !skinny) ? P.x.ref : packed(ws, P.x, eb);
   P.piece = round_up(v, kPieceStep);
   if (!loose && !chunked(a->weight, ld_w, k, eb)) {
-    const int64_t row = round_up(k, 16 / eb) * eb;
+    const int64_t row = row_pitch(k, eb) * eb;
     P.piece = piece_cols(v, ((int64_t)128 << 20) / row);
     P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
     if (!base) P.packed = (void*)1;  // (sizes only)
@@ -626,7 +634,7 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   // that writes it and the products that read it.
   P.piece = piece_cols(v, ((int64_t)128 << 20) / ((int64_t)m * eb));
   if (!P.loose && !chunked(a->weight, ld_w, k, eb)) {
-    const int64_t row = round_up(k, 16 / eb) * eb;
+    const int64_t row = row_pitch(k, eb) * eb;
     P.piece = std::min(P.piece, piece_cols(v, ((int64_t)128 << 20) / row));
     P.packed = ws.take(std::min(P.piece, (int64_t)v) * row);
     if (!base) P.packed = (void*)1;  // (sizes only)
@@ -780,7 +788,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   dx.out = a->d_x;
   dx.ld_out = stride_of(a->d_x_stride, m, k);
   dx.scale = inverse;
-  dx.stream = streams(m, k, eb);
+  dx.stream = streams((int64_t)m * k * eb);
   int dx_parts = 0;
   for (int64_t first = 0; first < v; first += P.piece) {
     const int32_t n = (int32_t)std::min(P.piece, v - first);
@@ -822,7 +830,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
       dw.ld_out = stride_of(a->d_weight_stride, v, k);
       dw.out = (char*)a->d_weight + first * dw.ld_out * eb;
       dw.scale = inverse;
-      dw.stream = streams(v, k, eb);
+      dw.stream = streams((int64_t)v * k * eb);
       const GemmPlan plan = plan_gemm(P.dw, g, P.x_ref, n, k, m, eb);
       if (!P.dw_split) {
         LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesTN, P.dw.tile, plan, dw, stream)));
