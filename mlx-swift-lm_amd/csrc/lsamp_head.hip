@@ -179,7 +179,7 @@ __device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
 // ------------------------------------------------------------------ epilogues
 // A wave's sums lie with 16 lanes down a column of rows; stored like that, an
 // instruction writes 16 rows of 32 bytes, and rows a power of two apart meet in
-// the same few channels (4096 x 16384 x 4096: 490 us, 371 without its stores).
+// the same few channels (4096 x 4096 x 16384: 490 us, 371 without its stores).
 // So the quads of columns of 16 rows change lanes through LDS, a KB a quad of
 // columns and wave: 4 FN lanes then lie along a row, 16 / FN rows a quad.  (Float32
 // parts, whose quads are 64 bytes of a row, gain nothing by it.)
