@@ -197,8 +197,10 @@ __device__ __forceinline__ void exchange(V (&v)[FN], char* lds, int lane) {
   const auto place = [](int r, int q) { return r * kLanes + (q ^ (r / (4 / FN))); };
 #pragma unroll
   for (int i = 0; i < FN; ++i) rows[place(lane & 15, i * 4 + (lane >> 4))] = v[i];
+  __builtin_amdgcn_wave_barrier();  // (other lanes' quads: a wave's LDS accesses stay in order)
 #pragma unroll
   for (int i = 0; i < FN; ++i) v[i] = rows[place(i * (16 / FN) + lane / kLanes, lane % kLanes)];
+  __builtin_amdgcn_wave_barrier();
 }
 
 struct Linear : EpiLinear {
