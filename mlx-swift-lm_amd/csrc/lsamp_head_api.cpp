@@ -185,9 +185,11 @@ Choice choose_skinny(int64_t m, int64_t n, bool whole_rows) {
   return Choice{whole_rows || n >= (m > kLooseRows ? 8192 : 16384) ? kSkinny64 : kSkinny16, 1, 0.0};
 }
 
-// `k`: elements of the reduction.
+// `k`: elements of the reduction.  `slabs_per_part`: of an earlier plan whose parts
+// these are added to.  (Parts of equal shares of a shorter reduction can be more:
+// 680 slabs in 32 shares are 31 parts of 22, 668 are 32 of 21.)
 GemmPlan plan_gemm(const Choice& c, const MatrixRef& a, const MatrixRef& b, int64_t m, int64_t n,
-                   int64_t k, int eb) {
+                   int64_t k, int eb, int32_t slabs_per_part = 0) {
   GemmPlan g{};
   g.a = a;
   g.b = b;
@@ -195,7 +197,7 @@ GemmPlan plan_gemm(const Choice& c, const MatrixRef& a, const MatrixRef& b, int6
   g.tiles_m = skinny ? 1 : (int32_t)ceil_div(m, kTileSide[c.tile]);
   g.tiles_n = (int32_t)ceil_div(n, kTileSide[c.tile]);
   g.slabs = (int32_t)ceil_div(k, 128 / eb);
-  g.slabs_per_part = (int32_t)ceil_div(g.slabs, c.parts);
+  g.slabs_per_part = slabs_per_part ? slabs_per_part : (int32_t)ceil_div(g.slabs, c.parts);
   g.parts = (int32_t)ceil_div(g.slabs, g.slabs_per_part);
   return g;
 }
@@ -605,6 +607,7 @@ struct LossBackwardPlan {
   float* scale;  // 16-bit types: {scale, 1 / scale}
   Choice grad, dx, dw;
   EpiPartial dx_sum, dw_sum;  // float32 sums of d_x (all pieces), of a piece's d_weight
+  int32_t dx_parts, dx_slabs_per_part;  // of the first piece, the longest
   bool dx_straight, dw_split;
   ColSumPlan col;
   int64_t bytes;
@@ -653,6 +656,8 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
     P.dx = choose(m, k, slabs_of(cols, eb), a->dtype, cols == v ? eb : 8, true, rows2);
     const GemmPlan g = plan_gemm(P.dx, MatrixRef{}, MatrixRef{}, m, k, cols, eb);
     if (too_many(g)) return set_error(LSAMP_ERR_SHAPE, "%d x %d is too large for one call", m, k);
+    P.dx_parts = g.parts;
+    P.dx_slabs_per_part = g.slabs_per_part;
     P.dx_straight = g.parts == 1 && cols == v;
     if (!P.dx_straight) P.dx_sum = take_partial(ws, m, k, g.parts);
   }
@@ -789,7 +794,6 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   dx.ld_out = stride_of(a->d_x_stride, m, k);
   dx.scale = inverse;
   dx.stream = streams((int64_t)m * k * eb);
-  int dx_parts = 0;
   for (int64_t first = 0; first < v; first += P.piece) {
     const int32_t n = (int32_t)std::min(P.piece, v - first);
     const Operand w = weight_piece(a->weight, stride_of(a->weight_stride, v, k), (int32_t)first, n,
@@ -813,13 +817,12 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
                                           plan_gemm(P.grad, P.x_ref, w.ref, m, n, k, eb), e, stream)));
     const MatrixRef g{P.g, P.ld_g, m, e.n_pad};
     if (a->d_x) {
-      const GemmPlan plan = plan_gemm(P.dx, g, w.ref, m, k, n, eb);
+      const GemmPlan plan = plan_gemm(P.dx, g, w.ref, m, k, n, eb, P.dx_slabs_per_part);
       if (P.dx_straight) {
         LSAMP_TRY(HEAD_OP(a->dtype, gemm_store(kRolesNN, P.dx.tile, plan, dx, stream)));
       } else {
         EpiPartial sum = P.dx_sum;
         sum.accumulate = first > 0;
-        if (first == 0) dx_parts = plan.parts;
         LSAMP_TRY(HEAD_OP(a->dtype, gemm_partial(kRolesNN, P.dx.tile, plan, sum, stream)));
       }
     }
@@ -856,7 +859,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
     }
   }
   if (a->d_x && !P.dx_straight)
-    LSAMP_TRY(HEAD_OP(a->dtype, join_store(P.dx_sum, dx_parts, dx, stream)));
+    LSAMP_TRY(HEAD_OP(a->dtype, join_store(P.dx_sum, P.dx_parts, dx, stream)));
   return clear_error();
 }
 

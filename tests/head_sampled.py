@@ -1,0 +1,109 @@
+"""Sampled rows and columns of the hidden-state operators in 64 bits, with bounds
+derived as in head_common.py, for sizes whose whole results are too large for
+the CPU.  A row of d_x needs its own row of x and all of the weight, a row of
+d_weight its own row of the weight and all of x."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+import head_common as H
+
+
+def sample(rng, n, count, *also):
+    """Some of 0 .. n - 1: both ends, both sides of multiples of 256, `also`,
+    and others at random."""
+    at = {0, n - 1, *[i for i in (63, 64, 127, 128, 255, 256, n // 256 * 256 - 1, n // 256 * 256)
+                      if 0 <= i < n], *[int(i) for i in also]}
+    at |= {int(i) for i in rng.integers(0, n, count)}
+    return torch.tensor(sorted(at))
+
+
+def rounded(y, err, dt):
+    return y, err + H.U[dt] * (y.abs() + err) + H.TINY[dt] * H.U[dt]
+
+
+def product(a, a_err, b, count, dt):
+    y = a @ b
+    return rounded(y, a_err @ b.abs() + H.sum_bound(count, (a.abs() + a_err) @ b.abs()), dt)
+
+
+def linear_grads(d_out, x, w, pre, act, cap, rows, outs):
+    """d_x at `rows`, d_weight and d_bias at the outputs `outs`."""
+    dt = d_out.dtype
+    X, W = H.d64(x), H.d64(w)
+
+    def dz(sl):
+        D = H.d64(d_out[sl])
+        if act == "none":
+            return D, torch.zeros_like(D), torch.zeros_like(D)
+        z = H.d64(pre[sl])
+        y = D * H.act64(act, z, cap)[1]
+        own = D.abs() * 24 * H.E * (z.abs() + 1)  # of the slope, in float32
+        return y, own, own + H.U[dt] * y.abs() + H.TINY[dt] * H.U[dt]
+
+    dev = d_out.device
+    r, _, r_err = dz(rows.to(dev))
+    o, o_own, o_err = dz((slice(None), outs.to(dev)))
+    db_err = o_own.sum(0) + H.sum_bound(x.shape[0], (o.abs() + o_own).sum(0))
+    return {"d_x": product(r, r_err, W, w.shape[0], dt),
+            "d_weight": product(o.t(), o_err.t(), X, x.shape[0], dt),
+            "d_bias": rounded(o.sum(0), db_err, dt)}
+
+
+def loss_grad(d_loss, x, w, targets, lse, bias, cap, ids, top):
+    """The gradient at the logits of the ids `ids` (whose rows `w` holds), and what
+    it may be off by in float32 and as it is stored.  `top`: the largest |d_loss| of
+    a row with a loss, which the scale of a 16-bit gradient goes by."""
+    dt = x.dtype
+    X, W = H.d64(x), H.d64(w)
+    z = X @ W.t()
+    mags = X.abs() @ W.abs().t()
+    if bias is not None:
+        b = H.d64(bias)
+        z, mags = z + b, mags + b.abs().masked_fill(torch.isinf(b), 0)
+    err = H.sum_bound(x.shape[1], mags)
+    slope, slope_rel = torch.ones_like(z), torch.zeros_like(z)
+    if cap:
+        t = z / cap
+        e = torch.exp(-2 * t.abs())
+        # (relatively: twice the argument's own error, and some roundings of a function)
+        slope, slope_rel = 4 * e / (1 + e) ** 2, 4 * err / cap + H.E * (16 + 8 * t.abs())
+        slope_rel = slope_rel.nan_to_num(posinf=0)  # (a slope of 0)
+        z, err = cap * torch.tanh(t), err + 8 * H.E * cap
+    L = H.d64(lse)[:, None]
+    t = targets.cpu().long()
+    ok = (t >= 0) & ~torch.isneginf(L[:, 0])
+    onehot = (t[:, None] == ids[None, :]).double()
+    p = torch.exp(z - L)
+    wt = torch.where(ok, H.d64(d_loss), torch.zeros(1, dtype=torch.float64))[:, None]
+    dead = ~ok[:, None].expand_as(z)
+    g = (wt * (p - onehot) * slope).masked_fill(dead, 0)
+    arg = z.abs().masked_fill(torch.isinf(z), 0) + L.abs().nan_to_num()
+    p_err = p * (err + 4 * H.E * (arg + 4)) + H.E
+    own = (wt.abs() * p_err * slope + g.abs() * (16 * H.E + slope_rel)).masked_fill(dead, 0)
+    stored = own
+    if dt != torch.float32:  # rounded once; half of float16's last step, unscaled
+        stored = own + H.U[dt] * g.abs() + (top * 2.0 ** -39 * ok.double())[:, None]
+    return g, own, stored
+
+
+def head_grads(d_loss, x, w, targets, lse, bias, cap, rows, ids):
+    """d_x at `rows`, d_weight and d_bias at the ids `ids`, from the kernel's own lse."""
+    dt = x.dtype
+    dev = x.device
+    t = targets.cpu().long()
+    live = (t >= 0) & (t < w.shape[0]) & ~torch.isneginf(H.d64(lse))
+    t = torch.where(live, t, torch.full_like(t, -1))
+    d = H.d64(d_loss)[live].abs()
+    d = d[torch.isfinite(d)]
+    top = float(d.max()) if len(d) else 0.0
+    ri, ci = rows.to(dev), ids.to(dev)
+    every = torch.arange(w.shape[0])
+    r, _, r_err = loss_grad(d_loss[ri], x[ri], w, t[rows], lse[ri], bias, cap, every, top)
+    c, c_own, c_err = loss_grad(d_loss, x, w[ci], t, lse, None if bias is None else bias[ci], cap,
+                                ids, top)
+    db_err = c_err.sum(0) + H.sum_bound(x.shape[0], (c.abs() + c_err).sum(0))
+    return {"d_x": product(r, r_err, H.d64(w), w.shape[0], dt),
+            "d_weight": product(c.t(), c_err.t(), H.d64(x), x.shape[0], dt),
+            "d_bias": rounded(c.sum(0), db_err, dt)}
