@@ -116,6 +116,16 @@ struct JoinStatsPlan {
   uint32_t* row_flags;
 };
 
+// scale[0]: what a 16-bit gradient of the logits is multiplied by (1 where no
+// d_loss of a row with a gradient is finite and not 0), scale[1] = 1 / scale[0].
+struct GradScalePlan {
+  int32_t rows, vocab;
+  const float* d_loss;
+  const float* lse;
+  const int32_t* targets;
+  float* scale;
+};
+
 struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial sum
   int32_t rows, cols;
   int32_t chunks, rows_per_chunk;
@@ -169,9 +179,7 @@ int launch_dropout(const DropoutPlan& p, int dtype, void* stream);
 // Element size 2 or 4.
 int launch_pack(const PackPlan& p, int element_bytes, void* stream);
 int launch_join_stats(const JoinStatsPlan& p, void* stream);
-// scale[0]: what a 16-bit gradient of the logits is multiplied by (1 where no
-// d_loss is finite and not 0), scale[1] = 1 / scale[0].
-int launch_grad_scale(const float* d_loss, int rows, float* scale, void* stream);
+int launch_grad_scale(const GradScalePlan& p, void* stream);
 
 }  // namespace lsamp
 

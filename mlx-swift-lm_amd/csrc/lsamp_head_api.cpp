@@ -786,7 +786,8 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   const int32_t m = a->rows, v = a->vocab, k = a->hidden;
   const float* inverse = P.scale ? P.scale + 1 : nullptr;
   LSAMP_TRY(lay_out(P.x, eb, stream));
-  if (P.scale) LSAMP_TRY(launch_grad_scale(a->d_loss, m, P.scale, stream));
+  if (P.scale)
+    LSAMP_TRY(launch_grad_scale(GradScalePlan{m, v, a->d_loss, a->lse, a->targets, P.scale}, stream));
   EpiStore dx{};
   dx.m = m;
   dx.n = k;

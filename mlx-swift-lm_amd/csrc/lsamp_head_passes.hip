@@ -94,24 +94,30 @@ __global__ __launch_bounds__(kThreads) void k_join_stats(JoinStatsPlan p) {
 // itself where the target is unlikely.  The scale brings the largest |d_loss|
 // to 32640 = 255 x 2^7: exact in bfloat16 and float16 and just below a power of
 // two, where a rounding is relatively smallest; small probabilities stay
-// normal numbers of float16 down to 2^-29.
+// normal numbers of float16 down to 2^-29.  Only rows that have a gradient count
+// (the epilogue that writes it leaves the same ones out), and only finite values:
+// what a caller keeps at ignored rows must not shrink the others'.
 constexpr float kGradTop = 32640.f;
 
-__global__ __launch_bounds__(1024) void k_grad_scale(const float* d_loss, int rows, float* scale) {
+__global__ __launch_bounds__(1024) void k_grad_scale(GradScalePlan p) {
   __shared__ float red[16];
   float top = 0.f;
-  for (int r = (int)threadIdx.x; r < rows; r += 1024) top = fmaxf(top, fabsf(d_loss[r]));
+  for (int r = (int)threadIdx.x; r < p.rows; r += 1024) {
+    const int target = p.targets[r];
+    const float d = fabsf(p.d_loss[r]);
+    if (target >= 0 && target < p.vocab && p.lse[r] != -INFINITY && d < INFINITY) top = fmaxf(top, d);
+  }
   for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
   float s = 1.f;
-  if (top > 0.f && top < INFINITY) s = kGradTop / top;
+  if (top > 0.f) s = kGradTop / top;
   if (!(s < 1e30f)) s = 1e30f;
   if (s < 1e-30f) s = 1e-30f;
-  scale[0] = s;
-  scale[1] = 1.f / s;
+  p.scale[0] = s;
+  p.scale[1] = 1.f / s;
 }
 
 }  // namespace
@@ -134,9 +140,8 @@ int launch_join_stats(const JoinStatsPlan& p, void* stream) {
   return (int)hipGetLastError();
 }
 
-int launch_grad_scale(const float* d_loss, int rows, float* scale, void* stream) {
-  hipLaunchKernelGGL(k_grad_scale, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream),
-                     d_loss, rows, scale);
+int launch_grad_scale(const GradScalePlan& p, void* stream) {
+  hipLaunchKernelGGL(k_grad_scale, dim3(1), dim3(1024), 0, reinterpret_cast<hipStream_t>(stream), p);
   return (int)hipGetLastError();
 }
 

@@ -157,10 +157,10 @@ int launch_join_stats(const JoinStatsPlan& p, void*) {
   writes(&l, p.loss, 1, p.rows, 1, 4);
   return put(l);
 }
-int launch_grad_scale(const float* d_loss, int rows, float* scale, void*) {
+int launch_grad_scale(const GradScalePlan& p, void*) {
   Launch l{};
-  l.kind = kGradScale, l.m = rows, l.a = at(d_loss);
-  writes(&l, scale, 1, 2, 1, 4);
+  l.kind = kGradScale, l.m = p.rows, l.n = p.vocab, l.a = at(p.d_loss);
+  writes(&l, p.scale, 1, 2, 1, 4);
   return put(l);
 }
 

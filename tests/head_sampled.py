@@ -80,11 +80,13 @@ def loss_grad(d_loss, x, w, targets, lse, bias, cap, ids, top):
     dead = ~ok[:, None].expand_as(z)
     g = (wt * (p - onehot) * slope).masked_fill(dead, 0)
     arg = z.abs().masked_fill(torch.isinf(z), 0) + L.abs().nan_to_num()
-    p_err = p * (err + 4 * H.E * (arg + 4)) + H.E
+    p_err = p * (err + 4 * H.E * (arg + 4)) + H.E * onehot  # (the target's difference, rounded)
     own = (wt.abs() * p_err * slope + g.abs() * (16 * H.E + slope_rel)).masked_fill(dead, 0)
     stored = own
-    if dt != torch.float32:  # rounded once; half of float16's last step, unscaled
-        stored = own + H.U[dt] * g.abs() + (top * 2.0 ** -39 * ok.double())[:, None]
+    if dt != torch.float32:  # rounded once
+        stored = own + H.U[dt] * g.abs()
+    if dt == torch.float16:  # half of its last step, unscaled
+        stored = stored + (top * 2.0 ** -39 * ok.double())[:, None]
     return g, own, stored
 
 
