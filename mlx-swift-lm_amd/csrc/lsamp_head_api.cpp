@@ -448,6 +448,9 @@ lsamp_status plan_linear_backward(const lsamp_linear_backward_args* a, void* bas
   if (act) {
     const int64_t pitch = row_pitch(n, eb);
     P.d = operand(ws.take((int64_t)m * pitch * eb), pitch, m, (int32_t)row_chunks(n, eb), eb);
+    // (written by the pass below, after any copy: read as it lies, as copies themselves
+    // are.  float32 rows of up to 16 MiB: a tile of them has at most 128, 2^31 bytes)
+    P.d.chunked = true;
   } else {
     P.d = operand(a->d_out, ld_d, m, n, eb);
   }

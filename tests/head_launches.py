@@ -144,11 +144,15 @@ def head_loss_backward(dtype, m, k, v, layout="dense", *, bias=False, want_x=Tru
 
 
 def check_workspace(need, launches):
-    """Every write to the workspace ends inside it, and buffers there do not
-    overlap.  Sums of parts: what is added to was written before, every part
-    written is joined, and the parts cover the reduction."""
+    """Every write to the workspace ends inside it, buffers there do not overlap,
+    and none is read before it was written.  Sums of parts: what is added to was
+    written before, every part written is joined, and the parts cover the
+    reduction."""
     extent, written = {}, {}
     for l in launches:
+        for p in (l.a, l.b):
+            if WORKSPACE <= p < min(AT.values()):
+                assert p in extent, f"launch of kind {l.kind} reads what nothing has written"
         for p, size in ((l.out, l.out_bytes), (l.out2, l.out2_bytes)):
             if size and WORKSPACE <= p < min(AT.values()):
                 assert p + size <= WORKSPACE + need, (l.kind, p + size - WORKSPACE, need)

@@ -57,3 +57,18 @@ def test_parts_of_later_pieces(ctx, case):
     H.check(p.d_x[rows.cuda()], want["d_x"], "d_x")
     H.check(p.d_weight[ids.cuda()], want["d_weight"], "d_weight")
     H.check(p.d_bias[ids.cuda()], want["d_bias"], "d_bias")
+
+
+def test_gradients_of_rows_past_8_mib(ctx):
+    """float32 rows of more than 8 MiB: the gradient at the pre-activations is as long."""
+    rng = np.random.default_rng(41)
+    m, k, n = 130, 64, (1 << 21) + 1
+    x, w = matrix(rng, m, k, torch.float32), matrix(rng, n, k, torch.float32, 1 / 8)
+    d, pre = matrix(rng, m, n, torch.float32), matrix(rng, m, n, torch.float32)
+    p = ctx.prepare_linear_backward(d, x, w, pre=pre, activation="silu", want_bias=True)
+    p.launch()
+    rows, outs = S.sample(rng, m, 3), S.sample(rng, n, 200)
+    want = S.linear_grads(d, x, w, pre, "silu", 0.0, rows, outs)
+    H.check(p.d_x[rows.cuda()], want["d_x"], "d_x")
+    H.check(p.d_weight[outs.cuda()], want["d_weight"], "d_weight")
+    H.check(p.d_bias[outs.cuda()], want["d_bias"], "d_bias")

@@ -26,6 +26,19 @@ def test_parts_of_later_pieces(case):
         HL.check_workspace(need, launches)
 
 
+@pytest.mark.parametrize("m,n", [(1, (1 << 21) + 1), (40, 3000001), (700, 1 << 22)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_products_follow_the_pass_that_writes_what_they_read(m, n, bias):
+    """The gradient at the pre-activations is written by the pass over d_out and
+    read where it lies, however long its rows are."""
+    for dtype in HL.DTYPES:
+        need, launches = HL.linear_backward(dtype, m, 64, n, activation=2, bias=bias)
+        HL.check_workspace(need, launches)
+        dz = next(l.out for l in launches if l.kind == HL.COL_SUM)
+        read = [l.a for l in launches if l.kind in (HL.STORE, HL.PARTIAL)]
+        assert len(read) == 2 and all(p == dz for p in read)
+
+
 def _log_int(rng, low, high):
     return int(round(low * (high / low) ** rng.random()))
 
