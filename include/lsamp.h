@@ -605,7 +605,8 @@ lsamp_status lsamp_mask_assemble(lsamp_context* ctx, const lsamp_mask_assemble_a
  *
  * Every matrix is rows of elements of `dtype` with its own distance between
  * rows (`*_stride`, in elements); any distance and any element-aligned address
- * is taken.  Products run on the matrix cores with float32 sums.  Rows that do
+ * is taken.  Products run on the matrix cores with float32 sums (float32 operands
+ * of more than 64 rows to 24 bits or 2^-134, whichever is larger).  Rows that do
  * not start at multiples of 16 bytes, or whose length is no multiple of 16
  * bytes, are read as they are in small products; where it is quicker they are
  * first copied to the workspace by the call.  Up to 2^27 rows (a loss: 2^23)
@@ -724,9 +725,9 @@ lsamp_status lsamp_head_loss(lsamp_context* ctx, const lsamp_head_loss_args* arg
  * targets[r]]) softcap'(...), computed again from x and weight a piece of the
  * vocabulary at a time and rounded to `dtype` for the two products,
  *   d_x = g weight,  d_weight = g^T x,  d_bias = column sums of g.
- * A 16-bit g is rounded times one scale, which brings the largest finite |d_loss|
- * of the rows that have a gradient near float16's largest value; what d_loss holds
- * at other rows does not count.  (A float16 row whose d_loss is below 2^-29 of
+ * g is held times one scale (float32: a power of two), which brings the largest
+ * finite |d_loss| of the rows that have a gradient near float16's largest value;
+ * what d_loss holds at other rows does not count.  (A float16 row whose d_loss is below 2^-29 of
  * that one loses bits.)
  * The workspace holds one piece of g (about 128 MiB) and the float32 sums of
  * d_x. */

@@ -117,7 +117,9 @@ __device__ __forceinline__ void mma(v4f& acc, const v4i& b, const v4i& a) {
 // finite), m and l the rest rounded; a b = hh + hm + mh + mm + hl + lh, and what
 // is left out is below 2^-23 |a b|, 2^-25 in the mean, so the sums are those of
 // float32.  Six instructions of 16 cycles take 32 steps of a 16 x 16 tile, the
-// float32 instruction takes 256 cycles.
+// float32 instruction takes 256 cycles.  The parts end at bfloat16's last step,
+// 2^-133: a value is kept to 24 bits or to 2^-134, whichever is larger, so below
+// 2^-110 it has fewer bits than float32.
 //
 // An infinity or a NaN has no remainder: it turns its row or column of the tile
 // into NaN.  A tile that ends with one is computed again with such values left

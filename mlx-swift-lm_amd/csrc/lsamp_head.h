@@ -116,10 +116,11 @@ struct JoinStatsPlan {
   uint32_t* row_flags;
 };
 
-// scale[0]: what a 16-bit gradient of the logits is multiplied by (1 where no
-// d_loss of a row with a gradient is finite and not 0), scale[1] = 1 / scale[0].
+// scale[0]: what the gradient at the logits is multiplied by (1 where no d_loss of
+// a row with a gradient is finite and not 0), scale[1] = 1 / scale[0].
 struct GradScalePlan {
   int32_t rows, vocab;
+  int32_t exact;  // a power of two (float32)
   const float* d_loss;
   const float* lse;
   const int32_t* targets;

@@ -437,7 +437,7 @@ struct Stats : EpiStats {
 // The gradient at the logits, d_loss[r] (softmax(z) - onehot(target)), from the
 // recomputed logits and the forward pass's log-sum-exp.  Rounded to the
 // operands' type because the two products that read it are matrix instructions
-// of that type; 16-bit values are scaled first (k_grad_scale).  A row without
+// of that type, and scaled first (k_grad_scale).  A row without
 // a loss (target ignored or out of range, every logit -inf) is zero.  4096 x 4096 x
 // 151936 in ten pieces: 4.16 ms (1.22 PFLOP/s), the plain product 3.84.
 struct Grad : EpiGrad {
@@ -448,7 +448,7 @@ struct Grad : EpiGrad {
     const Along<FN> along(lane);
     char* const mine = lds + (wn * WM + wm) * (FN * 1024);
     const int out_col = n0 + wn * (FN * 16) + along.col;
-    const float s = scale ? scale[0] : 1.f;
+    const float s = scale[0];
     const float twice = softcap > 0.f ? 2.f / softcap : 0.f;
     const int r0 = m0 + wm * (FM * 16) + (lane & 15);
     const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;

@@ -607,7 +607,7 @@ struct LossBackwardPlan {
   void* packed;
   void* g;      // [rows, ld_g]: the gradient at a piece of the logits
   int64_t ld_g;
-  float* scale;  // 16-bit types: {scale, 1 / scale}
+  float* scale;  // {scale, 1 / scale} of g
   Choice grad, dx, dw;
   EpiPartial dx_sum, dw_sum;  // float32 sums of d_x (all pieces), of a piece's d_weight
   int32_t dx_parts, dx_slabs_per_part;  // of the first piece, the longest
@@ -648,7 +648,7 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   const int64_t cols = std::min(P.piece, (int64_t)v);
   P.ld_g = round_up(cols, 64);
   P.g = ws.take((int64_t)m * P.ld_g * eb);
-  if (eb == 2) P.scale = ws.take<float>(8);
+  P.scale = ws.take<float>(8);
   P.grad = m <= kSkinnyRows ? choose_skinny(m, cols, true)
                             : choose(m, cols, slabs_of(k, eb), a->dtype, kGradBytes, false, rows);
   const int64_t side = kTileSide[P.grad.tile];
@@ -787,10 +787,11 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
   OnDevice guard(context_device(ctx));
   const int eb = element_bytes(a->dtype);
   const int32_t m = a->rows, v = a->vocab, k = a->hidden;
-  const float* inverse = P.scale ? P.scale + 1 : nullptr;
+  const float* inverse = P.scale + 1;
   LSAMP_TRY(lay_out(P.x, eb, stream));
-  if (P.scale)
-    LSAMP_TRY(launch_grad_scale(GradScalePlan{m, v, a->d_loss, a->lse, a->targets, P.scale}, stream));
+  LSAMP_TRY(launch_grad_scale(
+      GradScalePlan{m, v, a->dtype == LSAMP_DTYPE_F32, a->d_loss, a->lse, a->targets, P.scale},
+      stream));
   EpiStore dx{};
   dx.m = m;
   dx.n = k;

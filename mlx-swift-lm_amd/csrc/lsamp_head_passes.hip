@@ -97,6 +97,11 @@ __global__ __launch_bounds__(kThreads) void k_join_stats(JoinStatsPlan p) {
 // normal numbers of float16 down to 2^-29.  Only rows that have a gradient count
 // (the epilogue that writes it leaves the same ones out), and only finite values:
 // what a caller keeps at ignored rows must not shrink the others'.
+//
+// Float32 gradients are multiplied by a power of two, which changes no bit of the
+// result, to a largest |d_loss| of 2^14 to 2^15: the products split them into
+// bfloat16 parts, whose last step is 2^-133, so that values below 2^-110 would
+// keep fewer than 24 bits (a loss times 2^-106: d_weight off by 2^-19).
 constexpr float kGradTop = 32640.f;
 
 __global__ __launch_bounds__(1024) void k_grad_scale(GradScalePlan p) {
@@ -113,9 +118,13 @@ __global__ __launch_bounds__(1024) void k_grad_scale(GradScalePlan p) {
   if (threadIdx.x != 0) return;
   for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
   float s = 1.f;
-  if (top > 0.f) s = kGradTop / top;
-  if (!(s < 1e30f)) s = 1e30f;
-  if (s < 1e-30f) s = 1e-30f;
+  if (p.exact) {
+    if (top > 0.f) s = ldexpf(1.f, max(-100, min(100, 14 - ilogbf(top))));
+  } else {
+    if (top > 0.f) s = kGradTop / top;
+    if (!(s < 1e30f)) s = 1e30f;
+    if (s < 1e-30f) s = 1e-30f;
+  }
   p.scale[0] = s;
   p.scale[1] = 1.f / s;
 }

@@ -79,3 +79,25 @@ def test_an_infinite_gradient_stays_in_its_row(ctx, dtype):
     rest[[9, 40]] = False
     assert torch.equal(p.d_x[rest.cuda()], want.d_x[rest.cuda()])
     assert not torch.isfinite(p.d_x[[9, 40]].float()).any()
+
+
+def test_small_float32_gradients_keep_their_bits(ctx):
+    """A loss times a power of two has its gradients times that power, bit for bit,
+    as long as they are normal numbers: also where bfloat16 parts of the gradient
+    at the logits would not be."""
+    m, k, v = 200, 64, 900
+    rng = np.random.default_rng(35)
+    x, w, t, d = _inputs(rng, "f32", m, k, v)
+    f = ctx.prepare_head_loss(x, w, t)
+    f.launch()
+    p = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, want_bias=True)
+    p.launch()
+    one = {n: g.clone() for n, g in p.outputs().items()}
+    for e in (-106, -60, 60, 110):
+        d.mul_(2.0 ** e)
+        p.launch()
+        d.mul_(2.0 ** -e)
+        for n, g in p.outputs().items():
+            normal = one[n].abs() > 2.0 ** -18
+            assert normal.any()
+            assert torch.equal(g[normal] * 2.0 ** -e, one[n][normal]), (n, e)
