@@ -94,8 +94,8 @@ __device__ __forceinline__ float expe(float x) {
 
 // 1 / (1 + exp(-z)) and tanh.  For 16-bit elements with the hardware's
 // reciprocal (1 ulp) in place of a division of some ten instructions, and tanh
-// as 1 - 2 / (exp(2 |x|) + 1), a polynomial below 0.3 where that cancels: off by
-// less than 6 2^-24, far below the result's own rounding.
+// as (1 - e) / (1 + e) with e = exp(-2 |x|), a polynomial below 0.3 where that
+// cancels: off by less than 8 2^-24, far below the result's own rounding.
 __device__ __forceinline__ float reciprocal(float v) {
   if constexpr (DT == LSAMP_DTYPE_F32)
     return 1.f / v;
@@ -103,16 +103,27 @@ __device__ __forceinline__ float reciprocal(float v) {
     return __builtin_amdgcn_rcpf(v);
 }
 __device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + expe(-z)); }
-__device__ __forceinline__ float tanhe(float x) {
+// tanh(x) from e = exp(-2 |x|) and r = 1 / (1 + e).
+__device__ __forceinline__ float tanh_of(float x, float e, float r) {
   if constexpr (DT == LSAMP_DTYPE_F32) {
     return tanhf(x);
   } else {
     const float a = fabsf(x), q = x * x;
-    const float near = a + a * q * (-1.f / 3 + q * (2.f / 15 + q * (-17.f / 315 + q * (62.f / 2835))));
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(expe(2.f * a) + 1.f);
-    return copysignf(a < 0.3f ? near : far, x);
+    const float p = fmaf(q, fmaf(q, fmaf(q, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3);
+    return copysignf(a < 0.3f ? fmaf(a * q, p, a) : (1.f - e) * r, x);
   }
 }
+// cap tanh(z / cap), given 1 / cap (see inverse_cap), and its slope 4 e / (1 + e)^2,
+// of which nothing cancels on either side.  Both are relatively right: a cap far
+// above the logits takes nothing from them.
+__device__ __forceinline__ float soft_cap(float z, float cap, float inverse, float* slope) {
+  const float t = z * inverse;
+  const float e = expe(-2.f * fabsf(t)), r = reciprocal(1.f + e);
+  if (slope) *slope = 4.f * e * r * r;
+  return cap * tanh_of(t, e, r);
+}
+// (finite, so that a logit of 0 stays 0 under the smallest caps)
+__device__ __forceinline__ float inverse_cap(float cap) { return fminf(1.f / cap, 3.4e38f); }
 
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
@@ -147,8 +158,8 @@ __device__ __forceinline__ v4f activate(int act, float cap, v4f v) {
     case LSAMP_ACT_GELU: LSAMP_EACH(0.5f * z * (1.f + erff(z * kSqrtHalf)));
     case LSAMP_ACT_GELU_TANH: LSAMP_EACH(gelu_tanh(z));
     case LSAMP_ACT_SOFTCAP: {
-      const float inverse = 1.f / cap;
-      LSAMP_EACH(cap * tanhe(z * inverse));
+      const float inverse = inverse_cap(cap);
+      LSAMP_EACH(soft_cap(z, cap, inverse, nullptr));
     }
     default: return v;
   }
@@ -161,6 +172,11 @@ __device__ __forceinline__ float gelu_tanh_slope(float z) {
   const float s = gelu_gate(z), c = clamped(z);
   return s + 2.f * kGeluA * z * (s * (1.f - s)) * (1.f + 3.f * kGeluB * c * c);
 }
+__device__ __forceinline__ float cap_slope(float z, float cap, float inverse) {
+  float slope;
+  soft_cap(z, cap, inverse, &slope);
+  return slope;
+}
 __device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
   switch (act) {
     case LSAMP_ACT_RELU: LSAMP_EACH(z > 0.f ? 1.f : 0.f);
@@ -169,8 +185,8 @@ __device__ __forceinline__ v4f activate_slope(int act, float cap, v4f v) {
       LSAMP_EACH(0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * expe(-0.5f * z * z));
     case LSAMP_ACT_GELU_TANH: LSAMP_EACH(gelu_tanh_slope(z));
     case LSAMP_ACT_SOFTCAP: {
-      const float inverse = 1.f / cap;
-      LSAMP_EACH(1.f - tanhe(z * inverse) * tanhe(z * inverse));
+      const float inverse = inverse_cap(cap);
+      LSAMP_EACH(cap_slope(z, cap, inverse));
     }
     default: return v4f{1.f, 1.f, 1.f, 1.f};
   }
@@ -336,17 +352,15 @@ struct Partial : EpiPartial {
   }
 };
 
-// z = softcap(sum + bias) of four columns, and the slope of the cap: with r = 1 /
-// (exp(2 t) + 1), tanh t = 1 - 2 r and its slope is 4 r (1 - r).  Absolutely that is
-// as near as the logit's own sum (some 2^-24 of the cap); the slope does not cancel.
-__device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float twice, v4f* slope) {
+// z = softcap(sum + bias) of four columns, and the slope of the cap.
+__device__ __forceinline__ v4f logits4(v4f v, v4f b, float softcap, float inverse, v4f* slope) {
   v += b;
   if (softcap > 0.f) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float r = reciprocal(1.f + expe(v[k] * twice));
-      v[k] = fmaf(-2.f * softcap, r, softcap);
-      if (slope) (*slope)[k] = 4.f * r * (1.f - r);
+      float s;
+      v[k] = soft_cap(v[k], softcap, inverse, &s);
+      if (slope) (*slope)[k] = s;
     }
   }
   return v;
@@ -367,7 +381,7 @@ struct Stats : EpiStats {
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char* lds) const {
     float* red = (float*)lds;  // [WN][BM][2]
-    const float twice = softcap > 0.f ? 2.f / softcap : 0.f;
+    const float inverse = softcap > 0.f ? inverse_cap(softcap) : 0.f;
     v4f b[FN];
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
@@ -389,7 +403,7 @@ struct Stats : EpiStats {
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int c = n0 + wn * (FN * 16) + i * 16 + (lane >> 4) * 4;
-        v4f v = logits4(acc[i][j], b[i], softcap, twice, nullptr);
+        v4f v = logits4(acc[i][j], b[i], softcap, inverse, nullptr);
         if (!inside) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = c + k < n ? v[k] : -INFINITY;
@@ -449,7 +463,7 @@ struct Grad : EpiGrad {
     char* const mine = lds + (wn * WM + wm) * (FN * 1024);
     const int out_col = n0 + wn * (FN * 16) + along.col;
     const float s = scale[0];
-    const float twice = softcap > 0.f ? 2.f / softcap : 0.f;
+    const float inverse = softcap > 0.f ? inverse_cap(softcap) : 0.f;
     const int r0 = m0 + wm * (FM * 16) + (lane & 15);
     const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
     v4f b[FN];
@@ -473,7 +487,7 @@ struct Grad : EpiGrad {
         const int c = c0 + i * 16;
         v4f slope = {1.f, 1.f, 1.f, 1.f}, g;
         const int valid = n - c;
-        const v4f z = logits4(acc[i][j], b[i], softcap, twice, &slope);
+        const v4f z = logits4(acc[i][j], b[i], softcap, inverse, &slope);
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] = expe(z[k] - l[j]);
         const int at = target[j] - first_col - c;

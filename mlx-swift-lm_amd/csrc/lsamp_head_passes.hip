@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void k_join_stats(JoinStatsPlan p) {
 // Float32 gradients are multiplied by a power of two, which changes no bit of the
 // result, to a largest |d_loss| of 2^14 to 2^15: the products split them into
 // bfloat16 parts, whose last step is 2^-133, so that values below 2^-110 would
-// keep fewer than 24 bits (a loss times 2^-106: d_weight off by 2^-19).
+// keep fewer than 24 bits (a loss times 2^-106: its gradients were off by 2^-17 in the norm).
 constexpr float kGradTop = 32640.f;
 
 __global__ __launch_bounds__(1024) void k_grad_scale(GradScalePlan p) {

@@ -1,5 +1,6 @@
 """What the hidden-state operators' functions and scales may be off by, on the GPU
-against 64 bits: rows without a loss beside a float16 gradient's scale."""
+against 64 bits: rows without a loss beside a float16 gradient's scale, and soft
+caps near and far from saturation."""
 from __future__ import annotations
 
 import numpy as np
@@ -79,6 +80,74 @@ def test_an_infinite_gradient_stays_in_its_row(ctx, dtype):
     rest[[9, 40]] = False
     assert torch.equal(p.d_x[rest.cuda()], want.d_x[rest.cuda()])
     assert not torch.isfinite(p.d_x[[9, 40]].float()).any()
+
+
+# ------------------------------------------------------------------------- soft caps
+def _capped(dtype, cap):
+    """One row of one feature: the logits are the weights themselves, t = z / cap
+    from -12 to 12, and the target another id."""
+    dt = H.DT[dtype]
+    z = (torch.linspace(-12, 12, 385) * cap).to(dt)
+    w = torch.cat([z, z[:1] * 0])[:, None].cuda()
+    return torch.ones(1, 1, dtype=dt, device="cuda"), w, torch.tensor([385], dtype=torch.int32).cuda()
+
+
+@pytest.mark.parametrize("cap", [0.5, 30.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_slope_of_a_capped_logit(ctx, dtype, cap):
+    """softcap' = 4 e / (1 + e)^2, e = exp(-2 |t|), is relatively right at both signs,
+    down to 1e-10 at t = -12 as at 12."""
+    x, w, t = _capped(dtype, cap)
+    d = torch.ones(1, device="cuda")
+    f = ctx.prepare_head_loss(x, w, t, softcap=cap)
+    f.launch()
+    p = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, softcap=cap, want_bias=True)
+    p.launch()
+    want = S.head_grads(d, x, w, t, f.lse, None, cap, torch.arange(1), torch.arange(386))
+    for n, g in p.outputs().items():
+        H.check(g, want[n], n)
+    y, err = want["d_weight"]
+    if dtype != "f16":  # (float16 holds no 1e-10)
+        assert float((err / y.abs())[:385].max()) < 2.0 ** -6, "the bound has become empty"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_slope_of_a_capped_activation(ctx, dtype):
+    """The same of a linear block whose activation is a soft cap, from `pre`."""
+    cap = 5.0
+    pre = (torch.linspace(-12, 12, 385) * cap)[None, :].cuda()
+    dt = H.DT[dtype]
+    one = torch.ones(1, 385, dtype=dt, device="cuda")
+    p = ctx.prepare_linear_backward(one, one[:, :1], one.t().contiguous(), pre=pre,
+                                    activation="softcap", softcap=cap, want_x=False, want_bias=True)
+    p.launch()
+    t = H.d64(pre)[0] / cap
+    e = torch.exp(-2 * t.abs())
+    y = 4 * e / (1 + e) ** 2
+    want = S.rounded(y, y * H.E * (16 + 8 * t.abs()), dt)
+    H.check(p.d_bias, want, "d_bias")
+    H.check(p.d_weight[:, 0], want, "d_weight")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_small_logits_under_a_large_cap(ctx, dtype):
+    """cap tanh(z / cap) of logits far below the cap is as near as the logits' own
+    sums: a cap of 10^4 or 10^6 loses nothing."""
+    m, k, v = 40, 64, 900
+    rng = np.random.default_rng(33)
+    x, w, t, d = _inputs(rng, dtype, m, k, v)
+    X, W = H.d64(x), H.d64(w)
+    raw = X @ W.t()
+    for cap in (1e4, 1e6, 1e38):
+        f = ctx.prepare_head_loss(x, w, t, softcap=cap)
+        f.launch()
+        z = cap * torch.tanh(raw / cap)
+        err = (H.sum_bound(k, X.abs() @ W.abs().t()) + 16 * H.E * z.abs()).amax(1)
+        lse = torch.logsumexp(z, 1)
+        zt = z.gather(1, t.cpu().long()[:, None])[:, 0]
+        e = err + H.E * (64 + 2 * (z.amax(1) - z.amin(1)) + 2 * lse.abs())
+        H.check(f.lse, (lse, e), f"lse, cap {cap:g}")
+        H.check(f.loss, (lse - zt, 2 * e + 2 * H.E * zt.abs()), f"loss, cap {cap:g}")
 
 
 def test_small_float32_gradients_keep_their_bits(ctx):
