@@ -695,10 +695,11 @@ lsamp_status lsamp_linear_backward(lsamp_context* ctx, const lsamp_linear_backwa
  *   z = softcap(x weight^T + bias)  (softcap 0: none)
  *   lse[r] = log sum_v exp(z[r][v]);  loss[r] = lse[r] - z[r][targets[r]].
  * A row with a negative target is ignored: its loss is 0 (its lse is written).
- * A bias of -inf takes an id out of the vocabulary.  A target >= vocab, or a
- * row whose logits are all -inf, gives a NaN loss, a flag
- * (LSAMP_ROW_TOKEN_RANGE, LSAMP_ROW_EMPTY) and no gradient; NaN or +inf logits
- * give NaN and LSAMP_ROW_NONFINITE. */
+ * Without a soft cap a bias of -inf takes an id out of the vocabulary; with one its
+ * logit is -softcap, and the id keeps that mass.  A target >= vocab, or a row whose
+ * logits are all -inf, gives a NaN loss, a flag (LSAMP_ROW_TOKEN_RANGE,
+ * LSAMP_ROW_EMPTY) and no gradient; NaN or +inf logits give NaN and
+ * LSAMP_ROW_NONFINITE. */
 typedef struct lsamp_head_loss_args {
   int32_t rows;
   int32_t hidden;

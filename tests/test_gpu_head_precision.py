@@ -170,3 +170,25 @@ def test_small_float32_gradients_keep_their_bits(ctx):
             normal = one[n].abs() > 2.0 ** -18
             assert normal.any()
             assert torch.equal(g[normal] * 2.0 ** -e, one[n][normal]), (n, e)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_bias_of_minus_infinity_under_a_cap(ctx, dtype):
+    """A capped logit is at least -softcap, also where the bias is -inf: the id keeps
+    that mass, and has no gradient."""
+    m, k, v, cap = 70, 64, 900, 2.0
+    rng = np.random.default_rng(34)
+    x, w, t, d = _inputs(rng, dtype, m, k, v)
+    b = H.matrix(rng, 1, v, H.DT[dtype], 0.5)[0]
+    b[::3] = float("-inf")
+    f = ctx.prepare_head_loss(x, w, t, bias=b, softcap=cap)
+    f.launch()
+    want = H.loss64(x, w, t, b, cap)
+    H.check(f.lse, want["lse"], "lse")
+    H.check(f.loss, want["loss"], "loss")
+    p = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, bias=b, softcap=cap, want_bias=True)
+    p.launch()
+    want = S.head_grads(d, x, w, t, f.lse, b, cap, torch.arange(m), torch.arange(v))
+    for n, g in p.outputs().items():
+        H.check(g, want[n], n)
+    assert (p.d_weight[::3] == 0).all()
