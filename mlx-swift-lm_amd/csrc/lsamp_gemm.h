@@ -187,23 +187,29 @@ __device__ __forceinline__ int kmajor_place(int r, int c) {
 // 16 bytes a lane from memory to LDS, lane after lane from LDS address `lds` (the
 // same for the wave).  Written out because the compiler makes every later LDS
 // read wait for such loads, also a read of the other buffer; here the wave waits
-// where it must (wait_loads) and nowhere else.  No vector register is written;
-// M0 is the compiler's only around single instructions that it sets it for.
+// where it must (wait_loads) and nowhere else.  No vector register is written.  M0
+// is named as overwritten: the compiler allocates it to nothing and sets it ahead
+// of what reads it, but it joins settings of equal values, which an unnamed one
+// between them would break.  (It warns that it does not preserve the register for
+// us: nothing here expects that.)
 __device__ __forceinline__ uint32_t lds_address(char* lds) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* base, uint32_t off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds), "v"(off), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(p)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // 16 bytes from an address aligned to elements only.
 template <int DT>
