@@ -725,11 +725,11 @@ lsamp_status lsamp_head_loss(lsamp_context* ctx, const lsamp_head_loss_args* arg
 /* Its gradients: with g[r][v] = d_loss[r] (exp(z[r][v] - lse[r]) - [v ==
  * targets[r]]) softcap'(...), computed again from x and weight a piece of the
  * vocabulary at a time and rounded to `dtype` for the two products,
- *   d_x = g weight,  d_weight = g^T x,  d_bias = column sums of g.
+ *   d_x = g weight,  d_weight = g^T x,  d_bias = column sums of g before rounding.
  * g is held times one scale (float32: a power of two), which brings the largest
  * finite |d_loss| of the rows that have a gradient near float16's largest value;
- * what d_loss holds at other rows does not count.  (A float16 row whose d_loss is below 2^-29 of
- * that one loses bits.)
+ * what d_loss holds at other rows does not count.  (A float16 row whose d_loss is
+ * below 2^-29 of that one loses bits.)
  * The workspace holds one piece of g (about 128 MiB) and the float32 sums of
  * d_x. */
 typedef struct lsamp_head_loss_backward_args {

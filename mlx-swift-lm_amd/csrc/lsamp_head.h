@@ -45,6 +45,7 @@ enum GemmTile {
   kSkinny16,
 };
 constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16};
+constexpr int kTileWavesM[] = {2, 2, 2, 2, 2, 2, 2, 2, 1, 1};  // waves that share a tile's rows
 constexpr int kSkinnyRows = 64;
 
 // Epilogues.  `m`, `n`: rows and columns that exist.
@@ -96,6 +97,8 @@ struct EpiGrad {  // the loss's gradient at a piece of the logits
   const float* scale;  // [2] device: what the stored values are multiplied by, and its inverse
   void* out;
   int64_t ld_out;
+  float* sums;  // [rows of tiles x their waves][ld_sums] column sums before rounding, or NULL
+  int64_t ld_sums;
 };
 
 struct PackPlan {  // rows copied to 16-byte aligned rows, zeros up to dst_cols
@@ -141,8 +144,7 @@ struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial s
   int32_t out_cols;  // columns cols .. out_cols - 1 of out are written as zero
   float* part;       // [chunks][ld_part], or NULL
   int64_t ld_part;
-  void* sums;        // one chunk: the sums themselves, times *scale
-  const float* scale;
+  void* sums;        // one chunk: the sums themselves
 };
 
 struct DropoutPlan {

@@ -452,8 +452,10 @@ struct Stats : EpiStats {
 // recomputed logits and the forward pass's log-sum-exp.  Rounded to the
 // operands' type because the two products that read it are matrix instructions
 // of that type, and scaled first (k_grad_scale).  A row without
-// a loss (target ignored or out of range, every logit -inf) is zero.  4096 x 4096 x
-// 151936 in ten pieces: 4.16 ms (1.22 PFLOP/s), the plain product 3.84.
+// a loss (target ignored or out of range, every logit -inf) is zero.  The columns'
+// sums for d_bias are taken here, in float32 and before the rounding: a wave's rows
+// in registers, joined later in a fixed order.  4096 x 4096 x 151936 in ten pieces:
+// 4.16 ms (1.22 PFLOP/s), the plain product 3.84.
 struct Grad : EpiGrad {
   static constexpr int kBarriers = 0;
   template <int FM, int FN, int BM, int BN, int WM, int WN>
@@ -478,9 +480,12 @@ struct Grad : EpiGrad {
       l[j] = lse[r];
       w[j] = d_loss[r] * s;
     }
+    v4f sum[FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) sum[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const bool none = target[j] < 0 || target[j] >= vocab || l[j] == -INFINITY;
+      const bool none = target[j] < 0 || target[j] >= vocab || l[j] == -INFINITY || r0 + j * 16 >= m;
       v4e q[FN];
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
@@ -501,6 +506,7 @@ struct Grad : EpiGrad {
 #pragma unroll
           for (int k = 0; k < 4; ++k) g[k] = none || k >= valid ? 0.f : g[k];
         }
+        sum[i] += g;
         q[i] = __builtin_convertvector(g, v4e);
       }
       exchange<FN>(q, mine, lane);
@@ -508,6 +514,18 @@ struct Grad : EpiGrad {
       for (int i = 0; i < FN; ++i) {
         const int r = m0 + wm * (FM * 16) + j * 16 + i * along.kRows + along.row;
         if (r < m && out_col < n_pad) store4e(out, (int64_t)r * ld_out + out_col, q[i], 4);
+      }
+    }
+    if (sums) {
+      float* const to = sums + (int64_t)(m0 / BM * WM + wm) * ld_sums;
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int d = 1; d < 16; d *= 2) sum[i][k] += __shfl_xor(sum[i][k], d);
+        // (columns n .. are zero, and lie within the row)
+        if ((lane & 15) == 0 && c0 + i * 16 < n) *(v4f*)(to + c0 + i * 16) = sum[i];
       }
     }
   }
@@ -655,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void k_col_sum(ColSumPlan p) {
   if (wave != 0) return;
   for (int w = 1; w < 4; ++w) sum += red[w][lane];
   if (p.sums) {  // (the only chunk)
-    if (c < p.cols) store4(p.sums, c, p.scale ? sum * *p.scale : sum, valid);
+    if (c < p.cols) store4(p.sums, c, sum, valid);
   } else if (c < p.ld_part) {
     *(v4f*)(p.part + (int64_t)blockIdx.y * p.ld_part + c) = sum;
   }

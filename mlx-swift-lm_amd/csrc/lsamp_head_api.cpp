@@ -612,7 +612,7 @@ struct LossBackwardPlan {
   EpiPartial dx_sum, dw_sum;  // float32 sums of d_x (all pieces), of a piece's d_weight
   int32_t dx_parts, dx_slabs_per_part;  // of the first piece, the longest
   bool dx_straight, dw_split;
-  ColSumPlan col;
+  ColSumPlan col;  // d_bias: the joint of the tiles' column sums
   int64_t bytes;
 };
 
@@ -672,9 +672,9 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
     if (P.dw_split) P.dw_sum = take_partial(ws, cols, k, g.parts);
   }
   if (a->d_bias) {
-    plan_col_sum(P.col, m, (int32_t)cols);
+    P.col.chunks = (int32_t)ceil_div(m, side) * kTileWavesM[P.grad.tile];
     P.col.ld_part = round_up(cols, 4);
-    if (P.col.chunks > 1) P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
+    P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
   }
   P.bytes = ws.used;
   *out = P;
@@ -818,6 +818,8 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
     e.scale = P.scale;
     e.out = P.g;
     e.ld_out = P.ld_g;
+    e.sums = P.col.part;
+    e.ld_sums = P.col.ld_part;
     LSAMP_TRY(HEAD_OP(a->dtype, gemm_grad(P.grad.tile,
                                           plan_gemm(P.grad, P.x_ref, w.ref, m, n, k, eb), e, stream)));
     const MatrixRef g{P.g, P.ld_g, m, e.n_pad};
@@ -852,15 +854,7 @@ lsamp_status lsamp_head_loss_backward(lsamp_context* ctx, const lsamp_head_loss_
     if (a->d_bias) {
       ColSumPlan s = P.col;
       s.cols = n;
-      s.in = P.g;
-      s.ld_in = P.ld_g;
-      if (!s.part) {
-        s.sums = (char*)a->d_bias + first * eb;
-        s.scale = inverse;
-      }
-      LSAMP_TRY(HEAD_OP(a->dtype, col_sum(s, stream)));
-      if (s.part)
-        LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
+      LSAMP_TRY(HEAD_OP(a->dtype, col_sum_join(s, (char*)a->d_bias + first * eb, inverse, stream)));
     }
   }
   if (a->d_x && !P.dx_straight)

@@ -88,6 +88,9 @@ int32_t context_device(const lsamp_context*) { return 0; }
     Launch l = product(kGrad, t, g);                                                               \
     l.m = e.m, l.n = e.n, l.first_col = e.first_col;                                               \
     writes(&l, e.out, e.ld_out, e.m, e.n_pad, EB);                                                 \
+    l.out2 = at(e.sums);                                                                           \
+    l.chunks = e.sums ? g.tiles_m * kTileWavesM[t] : 0;                                            \
+    if (e.sums) l.out2_bytes = ((l.chunks - 1) * e.ld_sums + (e.n + 3) / 4 * 4) * 4;               \
     return put(l);                                                                                 \
   }                                                                                                \
   template <>                                                                                      \

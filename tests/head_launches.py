@@ -148,7 +148,7 @@ def check_workspace(need, launches):
     and none is read before it was written.  Sums of parts: what is added to was
     written before, every part written is joined, and the parts cover the
     reduction."""
-    extent, written = {}, {}
+    extent, written, chunks = {}, {}, {}
     for l in launches:
         for p in (l.a, l.b):
             if WORKSPACE <= p < min(AT.values()):
@@ -157,6 +157,10 @@ def check_workspace(need, launches):
             if size and WORKSPACE <= p < min(AT.values()):
                 assert p + size <= WORKSPACE + need, (l.kind, p + size - WORKSPACE, need)
                 extent[p] = max(extent.get(p, 0), size)
+        if l.kind in (COL_SUM, GRAD) and l.out2:
+            chunks[l.out2] = l.chunks
+        if l.kind == COL_SUM_JOIN:
+            assert l.chunks == chunks[l.a], "column sums left out"
         if l.kind == PARTIAL:
             assert l.parts * l.slabs_per_part >= l.slabs > (l.parts - 1) * l.slabs_per_part
             if l.accumulate:

@@ -1,6 +1,6 @@
 """What the hidden-state operators' functions and scales may be off by, on the GPU
-against 64 bits: rows without a loss beside a float16 gradient's scale, and soft
-caps near and far from saturation."""
+against 64 bits: rows without a loss beside a float16 gradient's scale, soft
+caps near and far from saturation, and column sums before rounding."""
 from __future__ import annotations
 
 import numpy as np
@@ -192,3 +192,31 @@ def test_a_bias_of_minus_infinity_under_a_cap(ctx, dtype):
     for n, g in p.outputs().items():
         H.check(g, want[n], n)
     assert (p.d_weight[::3] == 0).all()
+
+
+# ------------------------------------------------------------------------ column sums
+@pytest.mark.parametrize("m,v,layout", [(1, 300, "dense"), (40, 1003, "dense"), (64, 777, "odd"),
+                                        (300, 2100, "dense"), (1100, 5000, "dense"),
+                                        (300, 1999, "odd"), (2050, 70001, "dense")])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_head_bias_gradient_sums_in_float32(ctx, dtype, m, v, layout):
+    """d_bias adds up the gradient at the logits before it is rounded for the products."""
+    rng = np.random.default_rng(m + v)
+    k = 72
+    dt = H.DT[dtype]
+    x, w = H.matrix(rng, m, k, dt, layout=layout), H.matrix(rng, v, k, dt, 3 / np.sqrt(k), layout)
+    # (few targets: their columns' sums nearly cancel against their probabilities)
+    t = torch.from_numpy(rng.integers(0, min(v, 20), m).astype(np.int32)).cuda()
+    d = torch.from_numpy(rng.uniform(0.5, 2.0, m).astype(np.float32)).cuda() / m
+    f = ctx.prepare_head_loss(x, w, t)
+    f.launch()
+    p = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, want_bias=True)
+    p.launch()
+    ids = S.sample(rng, v, 100, *range(min(v, 20)))
+    c, own, _ = S.loss_grad(d, x, w[ids.cuda()], t.cpu().long(), f.lse, None, 0.0, ids, 0.0)
+    err = own.sum(0) + H.sum_bound(m, (c.abs() + own).sum(0))
+    H.check(p.d_bias[ids.cuda()], S.rounded(c.sum(0), err, dt), "d_bias")
+    only = ctx.prepare_head_loss_backward(d, x, w, t, lse=f.lse, want_x=False, want_weight=False,
+                                          want_bias=True)
+    only.launch()
+    assert torch.equal(only.d_bias, p.d_bias)
