@@ -7,6 +7,7 @@ import random
 import pytest
 
 import head_launches as HL
+import head_shapes as SH
 
 
 # rows, hidden, vocabulary whose last piece is split into more parts than the
@@ -64,3 +65,87 @@ def test_workspace_of_any_size():
                 HL.check_workspace(need, launches)
             except AssertionError as e:
                 raise AssertionError(f"{f.__name__} {dtype} {args} {layout} {more}: {e}") from None
+
+
+# every product of an operator (operator, launch, roles of the operands) and the
+# shapes that SHAPES has to reach for it.  "parts": a reduction split over work-groups.
+ALL = "256 128 64 128x2 64x4 loose128 loose64 loose64x4"
+F32 = ALL[4:]
+TAKEN = {
+    ("head", "16", "gradient", "NT"): "256 128 64 128x2 64x4 loose128",
+    ("head", "16", "parts", "NN"): "128 64 64x4 loose128 loose64 loose64x4",
+    ("head", "16", "parts", "TN"): "128 64 64x4",
+    ("head", "16", "statistics", "NT"): "256 128 64 128x2 64x4 loose128",
+    ("head", "16", "store", "NN"): "256 128 64 128x2 64x4 loose64",
+    ("head", "16", "store", "TN"): ALL,
+    ("head", "f32", "gradient", "NT"): "128 64 128x2 64x4 loose128",
+    ("head", "f32", "parts", "NN"): "128 64 128x2 64x4 loose128 loose64x4",
+    ("head", "f32", "parts", "TN"): "128 64 128x2 64x4 loose64x4",
+    ("head", "f32", "statistics", "NT"): "128 64 128x2 64x4 loose128",
+    ("head", "f32", "store", "NN"): "128 64 128x2 64x4 loose128 loose64",
+    ("head", "f32", "store", "TN"): "128 64 128x2 loose128 loose64 loose64x4",
+    ("linear", "16", "out", "NT"): "256 128 64 128x2 loose128 loose64",
+    ("linear", "16", "parts", "NT"): "64 64x4 loose64 loose64x4",
+    ("linear", "f32", "out", "NT"): "128 64 128x2 loose128 loose64",
+    ("linear", "f32", "parts", "NT"): "128 128x2 64x4 loose128 loose64x4",
+    ("linear_backward", "16", "parts", "NN"): "128 64 64x4 loose128 loose64 loose64x4",
+    ("linear_backward", "16", "parts", "TN"): "128 64 64x4 loose128 loose64 loose64x4",
+    ("linear_backward", "16", "store", "NN"): "256 128 64 128x2 64x4 loose128 loose64",
+    ("linear_backward", "16", "store", "TN"): "256 128 64 128x2 loose128 loose64 loose64x4",
+    ("linear_backward", "f32", "parts", "NN"): "128 64 128x2 64x4 loose128 loose64x4",
+    ("linear_backward", "f32", "parts", "TN"): "128 64 128x2 64x4 loose128 loose64x4",
+    ("linear_backward", "f32", "store", "NN"): "128 64 128x2 loose128 loose64",
+    ("linear_backward", "f32", "store", "TN"): "128 64 128x2 64x4 loose128 loose64",
+}
+
+
+def _products(op, dtype, m, k, n, layout):
+    """The products of a case: (operator, dtype, launch, roles), shape and launch."""
+    kinds = {HL.LINEAR: "out", HL.STATS: "statistics", HL.GRAD: "gradient", HL.STORE: "store",
+             HL.PARTIAL: "parts"}
+    calls = {"linear": [(HL.linear, {})], "linear_backward": [(HL.linear_backward, {"activation": 2})],
+             "head": [(HL.head_loss, {}), (HL.head_loss_backward, {"bias": True})]}[op]
+    for f, kw in calls:
+        need, launches = f("bf16" if dtype == "16" else dtype, m, k, n, layout, **kw)
+        HL.check_workspace(need, launches)
+        for l in launches:
+            if l.kind in kinds:
+                yield (op, dtype, kinds[l.kind], HL.ROLES[l.roles]), HL.TILES[l.tile], l
+
+
+def test_sizes_take_every_shape():
+    """The sizes that the GPU tests run take every tile shape, so that a constant of
+    the planner cannot change and leave one untested."""
+    taken = {}
+    for case in SH.SHAPES:
+        for product, tile, _ in _products(*case):
+            taken.setdefault(product, set()).add(tile)
+    for product, tiles in TAKEN.items():
+        assert set(tiles.split()) <= taken[product], (product, set(tiles.split()) - taken[product])
+
+
+@pytest.mark.parametrize("slabs,case", list(enumerate(SH.LAST_PIECES, 1)), ids=str)
+def test_last_pieces_of_a_few_slabs(slabs, case):
+    got = [(tile, l) for p, tile, l in _products("head", "16", *case, "dense") if p[2:] == ("parts", "NN")]
+    assert len(got) > 1 and all(tile == "256" for tile, _ in got)
+    assert got[-1][1].accumulate and got[-1][1].slabs == slabs
+
+
+@pytest.mark.parametrize("case", SH.COPIED, ids=str)
+def test_weights_copied_in_pieces(case):
+    dtype, m, k, v, layout = case
+    for f in (HL.head_loss, HL.head_loss_backward):
+        need, launches = f("bf16" if dtype == "16" else dtype, m, k, v, layout)
+        HL.check_workspace(need, launches)
+        packs = [l for l in launches if l.kind == HL.PACK and l.a >= HL.AT["weight"]]
+        pieces = [l for l in launches if l.kind in (HL.STATS, HL.GRAD)]
+        assert len(packs) == len(pieces) == 3 and pieces[-1].n < pieces[0].n
+        assert [p.m for p in packs] == [p.n for p in pieces]
+
+
+@pytest.mark.parametrize("case", SH.STREAMED, ids=str)
+def test_large_outputs_are_stored_past_the_caches(case):
+    need, launches = HL.linear(*case, pre=True)
+    out = [l for l in launches if l.kind == HL.LINEAR]
+    assert len(out) == 1 and out[0].stream
+    assert HL.TILES[out[0].tile] == ("128" if case[0] == "f32" else "256")
