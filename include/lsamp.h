@@ -773,7 +773,9 @@ typedef struct lsamp_dropout_args {
   int32_t dtype;
   float p;              /* [0, 1]                                                */
   uint64_t key;
-  uint64_t offset;      /* another value for every layer and step                */
+  uint64_t offset;      /* offset + *step: another value for every layer and step,
+                           so layers lie further apart than the largest step
+                           (layer << 48), or layer L + 1 repeats L's masks       */
   const uint64_t* step; /* device, or NULL: added to `offset` (a captured graph's
                            counter)                                              */
   const void* x;        /* [rows, cols]                                          */

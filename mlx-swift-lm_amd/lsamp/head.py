@@ -251,7 +251,8 @@ class PreparedHeadLossBackward(PreparedCall):
 class PreparedDropout(PreparedCall):
     """out = residual + dropout(x) (lsamp_dropout).  The same key, offset and
     p drop the same elements: the backward pass is this call on the gradient.
-    `step` (an int64 device tensor of one element) is added to the offset."""
+    `step` (an int64 device tensor of one element) is added to the offset, so the
+    offsets of layers lie further apart than any step (layer << 48)."""
 
     entry = "lsamp_dropout"
 
