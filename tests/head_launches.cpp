@@ -19,6 +19,7 @@ struct Launch {
   int32_t kind, tile, roles, parts;
   int32_t m, n, slabs, slabs_per_part;
   int32_t accumulate, first_col, chunks, stream;
+  int32_t element, unused;         // bytes of the operands' elements
   int64_t a, a_ld, b, b_ld;      // operands (a: what a pass reads)
   int32_t a_rows, a_cols, b_rows, b_cols;
   int64_t out, ld_out, out_bytes;  // what it writes: a range from `out`
@@ -31,9 +32,10 @@ namespace {
 std::vector<Launch> g_launches;
 
 int64_t at(const void* p) { return (int64_t)(intptr_t)p; }
-Launch product(int32_t kind, lsamp::GemmTile tile, const lsamp::GemmPlan& g) {
+Launch product(int32_t kind, lsamp::GemmTile tile, const lsamp::GemmPlan& g, int32_t element) {
   Launch l{};
   l.kind = kind;
+  l.element = element;
   l.tile = tile;
   l.parts = g.parts;
   l.slabs = g.slabs;
@@ -69,7 +71,7 @@ int32_t context_device(const lsamp_context*) { return 0; }
 #define EACH_TYPE(DT, EB)                                                                          \
   template <>                                                                                      \
   int HeadOps<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinear& e, void*) {         \
-    Launch l = product(kLinear, t, g);                                                             \
+    Launch l = product(kLinear, t, g, EB);                                                         \
     l.m = e.m, l.n = e.n, l.stream = e.stream;                                                     \
     writes(&l, e.out, e.ld_out, e.m, e.n, e.wide ? 4 : EB);                                        \
     l.out2 = at(e.pre);                                                                            \
@@ -77,7 +79,7 @@ int32_t context_device(const lsamp_context*) { return 0; }
   }                                                                                                \
   template <>                                                                                      \
   int HeadOps<DT>::gemm_stats(GemmTile t, const GemmPlan& g, const EpiStats& e, void*) {           \
-    Launch l = product(kStats, t, g);                                                              \
+    Launch l = product(kStats, t, g, EB);                                                          \
     l.m = e.m, l.n = e.n, l.first_col = e.first_col;                                               \
     writes(&l, e.part, (int64_t)e.blocks * 2, e.m, (int64_t)e.blocks * 2, 4);                      \
     l.out2 = at(e.target), l.out2_bytes = (int64_t)e.m * 4;                                        \
@@ -85,7 +87,7 @@ int32_t context_device(const lsamp_context*) { return 0; }
   }                                                                                                \
   template <>                                                                                      \
   int HeadOps<DT>::gemm_grad(GemmTile t, const GemmPlan& g, const EpiGrad& e, void*) {             \
-    Launch l = product(kGrad, t, g);                                                               \
+    Launch l = product(kGrad, t, g, EB);                                                           \
     l.m = e.m, l.n = e.n, l.first_col = e.first_col;                                               \
     writes(&l, e.out, e.ld_out, e.m, e.n_pad, EB);                                                 \
     l.out2 = at(e.sums);                                                                           \
@@ -96,7 +98,7 @@ int32_t context_device(const lsamp_context*) { return 0; }
   template <>                                                                                      \
   int HeadOps<DT>::gemm_store(GemmRoles r, GemmTile t, const GemmPlan& g, const EpiStore& e,       \
                               void*) {                                                             \
-    Launch l = product(kStore, t, g);                                                              \
+    Launch l = product(kStore, t, g, EB);                                                          \
     l.roles = r, l.m = e.m, l.n = e.n, l.stream = e.stream;                                        \
     writes(&l, e.out, e.ld_out, e.m, e.n, EB);                                                     \
     return put(l);                                                                                 \
@@ -104,7 +106,7 @@ int32_t context_device(const lsamp_context*) { return 0; }
   template <>                                                                                      \
   int HeadOps<DT>::gemm_partial(GemmRoles r, GemmTile t, const GemmPlan& g, const EpiPartial& e,   \
                                 void*) {                                                           \
-    Launch l = product(kPartial, t, g);                                                            \
+    Launch l = product(kPartial, t, g, EB);                                                        \
     l.roles = r, l.m = e.m, l.n = e.n, l.accumulate = e.accumulate, l.part_stride = e.part_stride; \
     writes(&l, e.out, e.ld, e.m, e.ld, 4);                                                         \
     l.out_bytes += (g.parts - 1) * e.part_stride * 4;                                              \

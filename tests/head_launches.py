@@ -21,7 +21,7 @@ TILES = ("256", "128", "64", "128x2", "64x4", "loose128", "loose64", "loose64x4"
 ROLES = ("NT", "NN", "TN")
 DTYPES = {"f32": (_ffi.DTYPE_F32, 4), "bf16": (_ffi.DTYPE_BF16, 2), "f16": (_ffi.DTYPE_F16, 2)}
 
-_ints = ("kind tile roles parts m n slabs slabs_per_part accumulate first_col chunks stream", c_int32)
+_ints = ("kind tile roles parts m n slabs slabs_per_part accumulate first_col chunks stream element unused", c_int32)
 _fields = [(f, c_int32) for f in _ints[0].split()]
 _fields += [(f, c_int64) for f in "a a_ld b b_ld".split()]
 _fields += [(f, c_int32) for f in "a_rows a_cols b_rows b_cols".split()]
@@ -145,14 +145,16 @@ def head_loss_backward(dtype, m, k, v, layout="dense", *, bias=False, want_x=Tru
 
 def check_workspace(need, launches):
     """Every write to the workspace ends inside it, buffers there do not overlap,
-    and none is read before it was written.  Sums of parts: what is added to was
+    and none is read before, or past what, it was written.  Sums of parts: what is added to was
     written before, every part written is joined, and the parts cover the
     reduction."""
     extent, written, chunks = {}, {}, {}
     for l in launches:
-        for p in (l.a, l.b):
+        for p, rows, ld, cols in ((l.a, l.a_rows, l.a_ld, l.a_cols), (l.b, l.b_rows, l.b_ld, l.b_cols)):
             if WORKSPACE <= p < min(AT.values()):
                 assert p in extent, f"launch of kind {l.kind} reads what nothing has written"
+                if l.element:
+                    assert ((rows - 1) * ld + cols) * l.element <= extent[p], f"kind {l.kind} reads past {p}"
         for p, size in ((l.out, l.out_bytes), (l.out2, l.out2_bytes)):
             if size and WORKSPACE <= p < min(AT.values()):
                 assert p + size <= WORKSPACE + need, (l.kind, p + size - WORKSPACE, need)
