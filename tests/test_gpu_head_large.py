@@ -184,3 +184,49 @@ def test_head_whose_last_piece_is_short(ctx, case):
 def test_head_whose_weight_is_copied_in_pieces(ctx, case):
     print(f"copied pieces {case}", flush=True)
     _head(ctx, *case, sampled=True)
+
+
+def _nonfinite(t, rng):
+    """A NaN in one row and an infinity in another, in the last and first columns."""
+    a, b = (int(i) for i in rng.choice(t.shape[0], 2, replace=False))
+    t[a, -1] = float("nan")
+    t[b, 0] = float("inf")
+    keep = torch.ones(t.shape[0], dtype=torch.bool)
+    keep[[a, b]] = False
+    return a, b, keep.cuda()
+
+
+@pytest.mark.parametrize("case", _typed(c[1:] for c in SH.SHAPES if c[0] == "linear"), ids=_id)
+def test_nonfinite_rows_stay_alone_in_every_shape(ctx, case):
+    print(f"nonfinite {case}", flush=True)
+    dtype, m, k, n, layout = case
+    rng = np.random.default_rng(m + k + n)
+    dt = H.DT[dtype]
+    x, w = matrix(rng, m, k, dt, layout=layout), matrix(rng, n, k, dt, 1 / np.sqrt(k), layout)
+    clean = ctx.linear(x, w)
+    a, b, keep = _nonfinite(x, rng)
+    out = ctx.linear(x, w)
+    assert torch.equal(out[keep], clean[keep])
+    assert torch.isnan(out[a]).all()
+    # (infinity times a weight of 0 is no number)
+    assert torch.equal(torch.isnan(out[b]), w[:, 0] == 0)
+    assert torch.equal(out[b] > 0, w[:, 0] > 0) and torch.isinf(out[b][w[:, 0] != 0]).all()
+
+
+@pytest.mark.parametrize("case", _typed(c[1:] for c in SH.SHAPES if c[0] == "linear_backward"), ids=_id)
+def test_nonfinite_rows_stay_alone_in_d_x(ctx, case):
+    print(f"nonfinite d_out {case}", flush=True)
+    dtype, m, k, n, layout = case
+    rng = np.random.default_rng(m + k + n)
+    dt = H.DT[dtype]
+    x, w = matrix(rng, m, k, dt, layout=layout), matrix(rng, n, k, dt, 1 / np.sqrt(k), layout)
+    d, pre = matrix(rng, m, n, dt, layout=layout), matrix(rng, m, n, torch.float32).abs() + 0.1
+    p = ctx.prepare_linear_backward(d, x, w, pre=pre, activation="relu", want_weight=False)
+    p.launch()
+    clean = p.d_x.clone()
+    a, b, keep = _nonfinite(d, rng)
+    p.launch()
+    assert torch.equal(p.d_x[keep], clean[keep])
+    assert torch.isnan(p.d_x[a]).all()
+    assert torch.equal(torch.isnan(p.d_x[b]), w[0] == 0)
+    assert torch.equal(p.d_x[b] > 0, w[0] > 0)
