@@ -45,7 +45,6 @@ SOURCES_HIP = ["lsamp_topk.hip", "lsamp_rank.hip", "lsamp_commit.hip",
                "lsamp_mask.hip", "lsamp_noalloc.hip", "lsamp_penalize.hip",
                "lsamp_head_passes.hip", "lsamp_dropout.hip"]
 SOURCES_CPP = ["lsamp_api.cpp", "lsamp_head_api.cpp"]
-HEADERS = ["lsamp_internal.h", "lsamp_device.h", "lsamp_head.h", "lsamp_gemm.h"]
 
 
 def run(cmd):

@@ -115,7 +115,7 @@ __device__ __forceinline__ void mma(v4f& acc, const v4i& b, const v4i& a) {
 // Float32 products on the bfloat16 matrix instructions.  A value is split into
 // three bfloat16 parts, a = h + m + l, h its first 8 bits (cut off, so that it is
 // finite), m and l the rest rounded; a b = hh + hm + mh + mm + hl + lh, and what
-// is left out is below 2^-23 |a b|, 2^-25 in the mean, so the sums are those of
+// is left out is below 2^-22 |a b|, 2^-26 in the mean, so the sums are those of
 // float32.  Six instructions of 16 cycles take 32 steps of a 16 x 16 tile, the
 // float32 instruction takes 256 cycles.  The parts end at bfloat16's last step,
 // 2^-133: a value is kept to 24 bits or to 2^-134, whichever is larger, so below

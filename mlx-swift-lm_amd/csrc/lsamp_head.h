@@ -52,7 +52,7 @@ constexpr int kSkinnyRows = 64;
 struct EpiLinear {
   int32_t m, n;
   int32_t activation, wide;  // wide: out is float32
-  int32_t stream;            // out (and pre) are stored past the caches
+  int32_t stream;            // pre, and out unless it is float32, are stored past the caches
   float softcap;
   const void* bias;
   const void* residual;

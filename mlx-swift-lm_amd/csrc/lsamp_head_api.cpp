@@ -206,7 +206,8 @@ bool too_many(const GemmPlan& g) {
 }
 
 // Outputs of more than half the last-level cache (256 MB) only push the operands
-// out of it and are stored past it: 8192 x 4096 x 4096 with kept pre-activations
+// out of it and are stored past it (a float32 `out` is not: 4096 x 2048 x 32000 504
+// us, 481 in 16 bits): 8192 x 4096 x 4096 with kept pre-activations
 // (201 MB) 287 us and 246, 4096 x 2048 x 32000 (262 MB) 490 and 458.  Smaller ones
 // are found there by what reads them next: the head's gradients of 333 x 1000 x
 // 40003 (80 MB) take 138 us, stored past it 152.
