@@ -145,6 +145,7 @@ struct ColSumPlan {  // column sums of a matrix, rows_per_chunk rows a partial s
   float* part;       // [chunks][ld_part], or NULL
   int64_t ld_part;
   void* sums;        // one chunk: the sums themselves
+  int32_t join_wide;  // the chunks are joined by sixteen waves, not four
 };
 
 struct DropoutPlan {

@@ -613,7 +613,7 @@ struct LossBackwardPlan {
   EpiPartial dx_sum, dw_sum;  // float32 sums of d_x (all pieces), of a piece's d_weight
   int32_t dx_parts, dx_slabs_per_part;  // of the first piece, the longest
   bool dx_straight, dw_split;
-  ColSumPlan col;  // d_bias: the joint of the tiles' column sums
+  ColSumPlan col;  // d_bias: the join of the tiles' column sums
   int64_t bytes;
 };
 
@@ -675,6 +675,7 @@ lsamp_status plan_loss_backward(const lsamp_head_loss_backward_args* a, void* ba
   if (a->d_bias) {
     P.col.chunks = (int32_t)ceil_div(m, side) * kTileWavesM[P.grad.tile];
     P.col.ld_part = round_up(cols, 4);
+    P.col.join_wide = P.col.chunks > 256;
     P.col.part = ws.take<float>((int64_t)P.col.chunks * P.col.ld_part * 4);
   }
   P.bytes = ws.used;

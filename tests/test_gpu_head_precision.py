@@ -196,7 +196,8 @@ def test_a_bias_of_minus_infinity_under_a_cap(ctx, dtype):
 # ------------------------------------------------------------------------ column sums
 @pytest.mark.parametrize("m,v,layout", [(1, 300, "dense"), (40, 1003, "dense"), (64, 777, "odd"),
                                         (300, 2100, "dense"), (1100, 5000, "dense"),
-                                        (300, 1999, "odd"), (2050, 70001, "dense")])
+                                        (300, 1999, "odd"), (2050, 70001, "dense"),
+                                        (20011, 333, "dense")])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_head_bias_gradient_sums_in_float32(ctx, dtype, m, v, layout):
     """d_bias adds up the gradient at the logits before it is rounded for the products."""

@@ -40,6 +40,13 @@ def test_products_follow_the_pass_that_writes_what_they_read(m, n, bias):
         assert len(read) == 2 and all(p == dz for p in read)
 
 
+def test_sums_of_many_rows_are_joined_by_more_waves():
+    """The size of test_head_bias_gradient_sums_in_float32 with the most rows."""
+    need, launches = HL.head_loss_backward("bf16", 20011, 72, 333, bias=True)
+    HL.check_workspace(need, launches)
+    assert [l.chunks for l in launches if l.kind == HL.COL_SUM_JOIN][0] > 256
+
+
 def _log_int(rng, low, high):
     return int(round(low * (high / low) ** rng.random()))
 
