@@ -605,12 +605,12 @@ lsamp_status lsamp_mask_assemble(lsamp_context* ctx, const lsamp_mask_assemble_a
  *
  * Every matrix is rows of elements of `dtype` with its own distance between
  * rows (`*_stride`, in elements); any distance and any element-aligned address
- * is taken.  Products run on the matrix cores with float32 sums (float32 operands
- * of more than 64 rows to 24 bits or 2^-134, whichever is larger).  Rows that do
- * not start at multiples of 16 bytes, or whose length is no multiple of 16
- * bytes, are read as they are in small products; where it is quicker they are
- * first copied to the workspace by the call.  Up to 2^27 rows (a loss: 2^23)
- * and 2^22 features or vocabulary ids.
+ * is taken.  Products run on the matrix cores with float32 sums.  (They take
+ * float32 operands to 24 bits or 2^-134, whichever is larger; forward products of
+ * up to 64 rows take them as they are.)  Rows that do not start at multiples of 16
+ * bytes, or whose length is no multiple of 16 bytes, are read as they are in small
+ * products; where it is quicker they are first copied to the workspace by the
+ * call.  Up to 2^27 rows (a loss: 2^23) and 2^22 features or vocabulary ids.
  *
  * `workspace` is device memory of at least the bytes that the matching
  * *_workspace function returns for the same arguments (its pointers included:
