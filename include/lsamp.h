@@ -788,6 +788,151 @@ typedef struct lsamp_dropout_args {
 
 lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* args, void* stream);
 
+/* Layer norm of every row, with float32 statistics:
+ *   mean = sum x / cols;  rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps);
+ *   out = (x - mean) rstd weight + bias.
+ * `out` may be x itself (same address, stride and type) where no gradient is
+ * taken.  A NaN or an infinity makes its row NaN and changes no other. */
+typedef struct lsamp_layer_norm_args {
+  int32_t rows;
+  int32_t cols;
+  int32_t dtype;      /* of x, weight, bias and out                              */
+  float eps;          /* positive                                                */
+  const void* x;      /* [rows, cols]                                            */
+  int64_t x_stride;
+  const void* weight; /* [cols] or NULL (1)                                      */
+  const void* bias;   /* [cols] or NULL (0)                                      */
+  void* out;          /* [rows, cols]                                            */
+  int64_t out_stride;
+  float* mean;        /* [rows] out or NULL                                      */
+  float* rstd;        /* [rows] out or NULL                                      */
+} lsamp_layer_norm_args;
+
+lsamp_status lsamp_layer_norm(lsamp_context* ctx, const lsamp_layer_norm_args* args, void* stream);
+
+/* Its gradients.  With xh = (x - mean) rstd and g = d_out weight,
+ *   d_x = rstd (g - mean(g) - xh mean(g xh)) + residual,
+ *   d_weight = column sums of d_out xh,  d_bias = column sums of d_out,
+ * the sums in float32, in a fixed order, each result rounded once.  `residual` is
+ * the gradient that reaches x past the norm (a block's skip path); d_x may be the
+ * residual or d_out itself (same address, stride and type). */
+typedef struct lsamp_layer_norm_backward_args {
+  int32_t rows;
+  int32_t cols;
+  int32_t dtype;
+  const void* x;        /* [rows, cols]                                          */
+  int64_t x_stride;
+  const void* weight;   /* [cols] or NULL (1)                                    */
+  const float* mean;    /* [rows] from lsamp_layer_norm, as rstd                 */
+  const float* rstd;
+  const void* d_out;    /* [rows, cols]                                          */
+  int64_t d_out_stride;
+  const void* residual; /* [rows, cols] or NULL; needs d_x                       */
+  int64_t residual_stride;
+  void* d_x;            /* [rows, cols] out or NULL                              */
+  int64_t d_x_stride;
+  void* d_weight;       /* [cols] out or NULL                                    */
+  void* d_bias;         /* [cols] out or NULL                                    */
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_layer_norm_backward_args;
+
+int64_t lsamp_layer_norm_backward_workspace(const lsamp_layer_norm_backward_args* args);
+lsamp_status lsamp_layer_norm_backward(lsamp_context* ctx,
+                                       const lsamp_layer_norm_backward_args* args, void* stream);
+
+/* Rows of 8-bit integers with a float32 scale each, x ~ scale q:
+ *   scale = max(max |x| (1/127), 2^-126), 1/127 and the product in float32,
+ *   q = x / scale to the nearest whole number (the exact quotient; ties to the even
+ *   one), at most 127 in magnitude.
+ * A row with a NaN or an infinity has scale NaN and q = 0.  Weights are quantised
+ * with it once, a scale for each output channel. */
+typedef struct lsamp_quantize_rows_args {
+  int32_t rows;
+  int32_t cols;
+  int32_t dtype;
+  const void* x;    /* [rows, cols]                                              */
+  int64_t x_stride;
+  int8_t* q;        /* [rows, cols] out                                          */
+  int64_t q_stride;
+  float* scale;     /* [rows] out                                                */
+} lsamp_quantize_rows_args;
+
+lsamp_status lsamp_quantize_rows(lsamp_context* ctx, const lsamp_quantize_rows_args* args,
+                                 void* stream);
+
+/* out = act(x weight^T + bias) + residual with 8-bit operands: x ~ x_scale q for
+ * each row (token), weight ~ weight_scale q for each output channel,
+ *   x weight^T = x_scale[r] weight_scale[c] sum_k qx[r][k] qw[c][k],
+ * the sums exact (in_features up to 131,071).  Without x_scale x is of `dtype`, and
+ * the call quantises its rows as lsamp_quantize_rows does. */
+typedef struct lsamp_linear_int8_args {
+  int32_t rows;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;        /* of bias, residual, and of x without x_scale           */
+  int32_t activation;   /* lsamp_activation                                      */
+  float softcap;        /* > 0 with LSAMP_ACT_SOFTCAP, else ignored              */
+  int32_t out_dtype;    /* dtype, or LSAMP_DTYPE_F32                             */
+  const void* x;        /* [rows, in_features] of dtype, or int8 with x_scale    */
+  int64_t x_stride;
+  const float* x_scale; /* [rows] or NULL                                        */
+  const int8_t* weight; /* [out_features, in_features]                           */
+  int64_t weight_stride;
+  const float* weight_scale; /* [out_features]                                   */
+  const void* bias;     /* [out_features] or NULL                                */
+  const void* residual; /* [rows, out_features] or NULL                          */
+  int64_t residual_stride;
+  void* out;            /* [rows, out_features] of out_dtype                     */
+  int64_t out_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_linear_int8_args;
+
+int64_t lsamp_linear_int8_workspace(const lsamp_linear_int8_args* args);
+lsamp_status lsamp_linear_int8(lsamp_context* ctx, const lsamp_linear_int8_args* args, void* stream);
+
+/* An update made nearly orthogonal, as the Muon optimiser does to a momentum:
+ *   X = G / (|G|_F + eps);  for each step with coefficients (a, b, c)
+ *     A = X X^T,  X <- a X + (b A + c A A) X    (rows <= cols; else with X^T X)
+ *   out = scale X + keep base
+ * for each of `batch` matrices.  With the weights as base and out, scale = -rate and
+ * keep = 1 - rate * decay it is the optimiser's step.  Coefficients that would take
+ * singular values of up to 1 past 8, or b t + c t^2 past 128 on their squares t, are refused.
+ *
+ * A float32 or float16 out is computed in float32; a bfloat16 out with products of
+ * float16 operands, X in two parts: off by about 1e-3 of the result's norm before
+ * its rounding (bfloat16's own is 1.7e-3).  A matrix with a NaN or an infinity, or
+ * whose steps meet one, becomes NaN; the others of the batch do not change.
+ * `out` may be `base` itself (same address, strides and type). */
+typedef struct lsamp_orthogonalize_args {
+  int32_t batch;
+  int32_t rows;
+  int32_t cols;
+  int32_t in_dtype;   /* of x                                                    */
+  int32_t out_dtype;  /* of base and out                                         */
+  int32_t steps;      /* 1 .. 64                                                 */
+  const float* coefficients; /* [steps][3] host                                  */
+  float eps;          /* positive                                                */
+  float scale;
+  float keep;         /* ignored without base                                    */
+  const void* x;      /* [batch, rows, cols]                                     */
+  int64_t x_stride;
+  int64_t x_batch_stride; /* elements between matrices (batch > 1)               */
+  const void* base;   /* [batch, rows, cols] or NULL                             */
+  int64_t base_stride;
+  int64_t base_batch_stride;
+  void* out;          /* [batch, rows, cols]                                     */
+  int64_t out_stride;
+  int64_t out_batch_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+} lsamp_orthogonalize_args;
+
+int64_t lsamp_orthogonalize_workspace(const lsamp_orthogonalize_args* args);
+lsamp_status lsamp_orthogonalize(lsamp_context* ctx, const lsamp_orthogonalize_args* args,
+                                 void* stream);
+
 /* ---- host-side parameter resolution (no device work) ---------------------- */
 
 /* GenerateParameters subset that drives the mlx-lm sampler/processor factory

@@ -39,12 +39,13 @@ DEVICE = [
     "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-# compiled once per element type (LSAMP_DT = 0, 1, 2), in parallel
-SOURCES_HIP_DT = ["lsamp_kernels.hip", "lsamp_head.hip"]
+# compiled once per element type (LSAMP_DT: float32 0, bfloat16 1, float16 2), in parallel
+SOURCES_HIP_DT = {"lsamp_kernels.hip": (0, 1, 2), "lsamp_head.hip": (0, 1, 2),
+                  "lsamp_int8.hip": (0, 1, 2), "lsamp_orth.hip": (0, 2)}
 SOURCES_HIP = ["lsamp_topk.hip", "lsamp_rank.hip", "lsamp_commit.hip",
                "lsamp_mask.hip", "lsamp_noalloc.hip", "lsamp_penalize.hip",
-               "lsamp_head_passes.hip", "lsamp_dropout.hip"]
-SOURCES_CPP = ["lsamp_api.cpp", "lsamp_head_api.cpp"]
+               "lsamp_head_passes.hip", "lsamp_dropout.hip", "lsamp_norm.hip"]
+SOURCES_CPP = ["lsamp_api.cpp", "lsamp_head_api.cpp", "lsamp_blocks_api.cpp"]
 
 
 def run(cmd):
@@ -57,8 +58,8 @@ def build_lib(verbose_asm: bool = False, jobs: int = 0) -> str:
     link liblsamp.so."""
     os.makedirs(LIB_DIR, exist_ok=True)
     cmds, objs = [], []
-    for src in SOURCES_HIP_DT:
-        for dt in range(3):
+    for src, dts in SOURCES_HIP_DT.items():
+        for dt in dts:
             obj = os.path.join(LIB_DIR, src.replace(".hip", f"_{dt}.o"))
             cmds.append([HIPCC, "-x", "hip", *COMMON, *DEVICE, f"-DLSAMP_DT={dt}", "-c",
                          os.path.join(CSRC, src), "-o", obj])

@@ -495,6 +495,12 @@ int64_t lsamp_abi_sizeof(const char* name) {
   if (!strcmp(name, "lsamp_head_loss_backward_args"))
     return (int64_t)sizeof(lsamp_head_loss_backward_args);
   if (!strcmp(name, "lsamp_dropout_args")) return (int64_t)sizeof(lsamp_dropout_args);
+  if (!strcmp(name, "lsamp_layer_norm_args")) return (int64_t)sizeof(lsamp_layer_norm_args);
+  if (!strcmp(name, "lsamp_layer_norm_backward_args"))
+    return (int64_t)sizeof(lsamp_layer_norm_backward_args);
+  if (!strcmp(name, "lsamp_quantize_rows_args")) return (int64_t)sizeof(lsamp_quantize_rows_args);
+  if (!strcmp(name, "lsamp_linear_int8_args")) return (int64_t)sizeof(lsamp_linear_int8_args);
+  if (!strcmp(name, "lsamp_orthogonalize_args")) return (int64_t)sizeof(lsamp_orthogonalize_args);
   return -1;
 }
 

@@ -1,0 +1,461 @@
+// lsamp_blocks_api.cpp — the C entry points of a block's other operators: layer
+// norm and its gradients, rows of 8-bit integers and their products, and the
+// orthogonalised update.
+#include "lsamp_head_plan.h"
+#include "lsamp_orth.h"
+
+using namespace lsamp;
+
+namespace {
+
+constexpr int32_t kMaxInt8Features = (1 << 17) - 1;  // (2^14 k below 2^31)
+
+lsamp_status check_positive(const char* what, float v) {
+  if (!(v > 0.f && std::isfinite(v)))
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "%s %g must be positive and finite", what, v);
+  return LSAMP_OK;
+}
+
+// ------------------------------------------------------------------ layer norm
+lsamp_status plan_norm(const lsamp_layer_norm_args* a, NormPlan* out) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
+  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  LSAMP_CHECK(check_positive("eps", a->eps));
+  const int eb = element_bytes(a->dtype);
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, a->rows, a->cols, eb));
+  LSAMP_CHECK(check_matrix("out", a->out, a->out_stride, a->rows, a->cols, eb));
+  LSAMP_CHECK(check_vector("weight", a->weight, eb, false));
+  LSAMP_CHECK(check_vector("bias", a->bias, eb, false));
+  LSAMP_CHECK(check_vector("mean", a->mean, 4, false));
+  LSAMP_CHECK(check_vector("rstd", a->rstd, 4, false));
+  *out = NormPlan{a->rows,   a->cols, a->eps,
+                  a->x,      stride_of(a->x_stride, a->rows, a->cols),
+                  a->weight, a->bias,
+                  a->out,    stride_of(a->out_stride, a->rows, a->cols),
+                  a->mean,   a->rstd};
+  return LSAMP_OK;
+}
+
+lsamp_status plan_norm_backward(const lsamp_layer_norm_backward_args* a, void* base,
+                                NormBackwardPlan* out, int64_t* bytes) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
+  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  const int eb = element_bytes(a->dtype);
+  const int32_t m = a->rows, n = a->cols;
+  if (!a->d_x && !a->d_weight && !a->d_bias)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, m, n, eb));
+  LSAMP_CHECK(check_matrix("d_out", a->d_out, a->d_out_stride, m, n, eb));
+  LSAMP_CHECK(check_vector("weight", a->weight, eb, false));
+  LSAMP_CHECK(check_vector("mean", a->mean, 4, true));
+  LSAMP_CHECK(check_vector("rstd", a->rstd, 4, true));
+  if (a->residual && !a->d_x)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "a residual without d_x to add it to");
+  if (a->residual)
+    LSAMP_CHECK(check_matrix("residual", a->residual, a->residual_stride, m, n, eb));
+  if (a->d_x) LSAMP_CHECK(check_matrix("d_x", a->d_x, a->d_x_stride, m, n, eb));
+  LSAMP_CHECK(check_vector("d_weight", a->d_weight, eb, false));
+  LSAMP_CHECK(check_vector("d_bias", a->d_bias, eb, false));
+  NormBackwardPlan P{};
+  Arena ws(base);
+  P.rows = m;
+  P.cols = n;
+  P.x = a->x;
+  P.ld_x = stride_of(a->x_stride, m, n);
+  P.weight = a->weight;
+  P.mean = a->mean;
+  P.rstd = a->rstd;
+  P.d_out = a->d_out;
+  P.ld_d = stride_of(a->d_out_stride, m, n);
+  P.residual = a->residual;
+  P.ld_residual = stride_of(a->residual_stride, m, n);
+  P.d_x = a->d_x;
+  P.ld_dx = stride_of(a->d_x_stride, m, n);
+  P.d_weight = a->d_weight;
+  P.d_bias = a->d_bias;
+  if (a->d_weight || a->d_bias) {
+    P.chunks = norm_chunks(m, n);
+    P.ld_part = round_up(n, 8);
+    P.part = ws.take<float>((int64_t)P.chunks * 2 * P.ld_part * 4);
+  }
+  *out = P;
+  *bytes = ws.used;
+  return LSAMP_OK;
+}
+
+// ------------------------------------------------------------- 8-bit integers
+lsamp_status check_quantized(const char* what, const void* p, int64_t ld, int32_t rows, int32_t cols) {
+  return check_matrix(what, p, ld, rows, cols, 1);
+}
+
+struct LinearInt8Plan {
+  bool quantize;
+  QuantizePlan quant;
+  Operand x, w;
+  Choice choice;
+  GemmPlan gemm;
+  EpiPartial partial;
+  EpiLinearInt8 epi;
+  int64_t bytes;
+};
+
+lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, LinearInt8Plan* out) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
+  LSAMP_CHECK(check_dims("in_features", a->in_features, kMaxInt8Features));
+  LSAMP_CHECK(check_dims("out_features", a->out_features));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  if (a->out_dtype != a->dtype && a->out_dtype != LSAMP_DTYPE_F32)
+    return set_error(LSAMP_ERR_DTYPE, "out_dtype %d must be the dtype %d or float32", a->out_dtype,
+                     a->dtype);
+  LSAMP_CHECK(check_activation(a->activation, a->softcap));
+  const int eb = element_bytes(a->dtype), ob = element_bytes(a->out_dtype);
+  const int32_t m = a->rows, n = a->out_features, k = a->in_features;
+  const bool given = a->x_scale != nullptr;
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, m, k, given ? 1 : eb));
+  LSAMP_CHECK(check_vector("x_scale", a->x_scale, 4, false));
+  LSAMP_CHECK(check_quantized("weight", a->weight, a->weight_stride, n, k));
+  LSAMP_CHECK(check_vector("weight_scale", a->weight_scale, 4, true));
+  LSAMP_CHECK(check_matrix("out", a->out, a->out_stride, m, n, ob));
+  LSAMP_CHECK(check_vector("bias", a->bias, eb, false));
+  if (a->residual)
+    LSAMP_CHECK(check_matrix("residual", a->residual, a->residual_stride, m, n, eb));
+
+  LinearInt8Plan P{};
+  Arena ws(base);
+  const int64_t ld_x = stride_of(a->x_stride, m, k);
+  const float* x_scale = a->x_scale;
+  if (given) {
+    P.x = operand(a->x, ld_x, m, k, 1);
+  } else {
+    // (rows of whole chunks, zeros behind their ends)
+    const int64_t pitch = row_pitch(k, 1);
+    const int32_t wide = (int32_t)row_chunks(k, 1);
+    int8_t* const q = ws.take<int8_t>((int64_t)m * pitch);
+    float* const s = ws.take<float>((int64_t)m * 4);
+    P.quantize = true;
+    P.quant = QuantizePlan{m, k, wide, a->x, ld_x, q, pitch, s};
+    P.x.ref = MatrixRef{q, pitch, m, wide};
+    P.x.chunked = true;
+    x_scale = s;
+  }
+  P.w = operand(a->weight, stride_of(a->weight_stride, n, k), n, k, 1);
+  MatrixRef x = P.x.ref, w = P.w.ref;
+  if (m <= kSkinnyRows) {
+    P.choice = choose_skinny(m, n, false);
+    if (m > kLooseRows) x = packed(ws, P.x, 1);
+  } else {
+    // (an instruction's slab of bytes takes what one of 16-bit elements does)
+    P.choice = choose_rows(m, n, slabs_of(k, 1), LSAMP_DTYPE_BF16, ob + (a->residual ? eb : 0),
+                           pack_all(P.x, P.w, 1));
+    if (!is_loose(P.choice)) {
+      x = packed(ws, P.x, 1);
+      w = packed(ws, P.w, 1);
+    }
+  }
+  P.gemm = plan_gemm(P.choice, x, w, m, n, k, 1);
+  if (too_many(P.gemm))
+    return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
+  if (P.gemm.parts > 1) P.partial = take_partial(ws, m, n, P.gemm.parts);
+  EpiLinearInt8& e = P.epi;
+  e.m = m;
+  e.n = n;
+  e.activation = a->activation;
+  e.softcap = a->softcap;
+  e.wide = a->out_dtype == LSAMP_DTYPE_F32;
+  e.stream = streams((int64_t)m * n * ob);
+  e.bias = a->bias;
+  e.residual = a->residual;
+  e.ld_residual = stride_of(a->residual_stride, m, n);
+  e.out = a->out;
+  e.ld_out = stride_of(a->out_stride, m, n);
+  e.x_scale = x_scale;
+  e.w_scale = a->weight_scale;
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+#define INT8_OP(dtype, call)                                              \
+  ((dtype) == LSAMP_DTYPE_F32    ? Int8Ops<LSAMP_DTYPE_F32>::call         \
+   : (dtype) == LSAMP_DTYPE_BF16 ? Int8Ops<LSAMP_DTYPE_BF16>::call        \
+                                 : Int8Ops<LSAMP_DTYPE_F16>::call)
+
+// --------------------------------------------------------- orthogonalised update
+// What the steps' matrices hold at most: singular values start at most at 1, and a
+// step takes s to |a s + b s^3 + c s^5|.  The largest |B| is that of b t + c t^2 over
+// the squares t.
+constexpr double kMostValue = 8.0, kMostPoly = 128.0;
+constexpr int kMaxSteps = 64;
+lsamp_status check_steps(const float* coefficients, int32_t steps) {
+  if (steps < 1 || steps > kMaxSteps)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "steps %d out of range [1, %d]", steps, kMaxSteps);
+  if (!coefficients) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "coefficients is required");
+  double top = 1.0;
+  for (int i = 0; i < steps; ++i) {
+    const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    const auto p = [&](double t) { return std::sqrt(t) * std::fabs(a + b * t + c * t * t); };
+    const auto q = [&](double t) { return std::fabs(b * t + c * t * t); };
+    const double end = top * top;
+    double most = p(end), poly = q(end);
+    const auto at = [&](double t) {  // a place where a slope may be 0
+      if (!(t > 0.0 && t < end)) return;
+      most = std::max(most, p(t));
+      poly = std::max(poly, q(t));
+    };
+    if (c != 0.0) {
+      const double d = 9.0 * b * b - 20.0 * a * c;
+      if (d >= 0.0) {
+        at((-3.0 * b + std::sqrt(d)) / (10.0 * c));
+        at((-3.0 * b - std::sqrt(d)) / (10.0 * c));
+      }
+      at(-b / (2.0 * c));
+    } else if (b != 0.0) {
+      at(-a / (3.0 * b));
+    }
+    if (!(most <= kMostValue && poly <= kMostPoly))
+      return set_error(LSAMP_ERR_INVALID_ARGUMENT,
+                       "coefficients of step %d take singular values of up to %g to %g", i, top, most);
+    top = most;
+  }
+  return LSAMP_OK;
+}
+
+struct OrthPlan {
+  bool half, tall;
+  OrthStart start;
+  Choice gram, poly, update;
+  BatchPlan g_gram, g_poly, g_update;  // (of the first step: X is in the first buffer)
+  void* x[2][2];                       // [buffer][hi, lo]
+  EpiSymmetric e_gram, e_poly;
+  EpiOrthUpdate e_update;
+  int64_t bytes;
+};
+
+lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* out) {
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("batch", a->batch, 65535));
+  LSAMP_CHECK(check_dims("rows", a->rows));
+  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dtype(a->in_dtype));
+  LSAMP_CHECK(check_dtype(a->out_dtype));
+  LSAMP_CHECK(check_positive("eps", a->eps));
+  if (!std::isfinite(a->scale) || !std::isfinite(a->keep))
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "scale %g and keep %g must be finite", a->scale,
+                     a->keep);
+  LSAMP_CHECK(check_steps(a->coefficients, a->steps));
+  const int ib = element_bytes(a->in_dtype), ob = element_bytes(a->out_dtype);
+  const int32_t batch = a->batch, m = a->rows, n = a->cols;
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, m, n, ib));
+  LSAMP_CHECK(check_matrix("out", a->out, a->out_stride, m, n, ob));
+  if (a->base) LSAMP_CHECK(check_matrix("base", a->base, a->base_stride, m, n, ob));
+  const int64_t ld_out = stride_of(a->out_stride, m, n);
+  const int64_t most = (int64_t)1 << 40;
+  if (batch > 1) {
+    if (a->out_batch_stride < (int64_t)(m - 1) * ld_out + n || a->out_batch_stride > most)
+      return set_error(LSAMP_ERR_SHAPE, "out batch stride %lld is below a matrix or out of range",
+                       (long long)a->out_batch_stride);
+    if (a->x_batch_stride < 0 || a->x_batch_stride > most ||
+        (a->base && (a->base_batch_stride < 0 || a->base_batch_stride > most)))
+      return set_error(LSAMP_ERR_SHAPE, "a batch stride is out of range");
+  }
+
+  OrthPlan P{};
+  Arena ws(base);
+  P.half = a->out_dtype == LSAMP_DTYPE_BF16;
+  P.tall = m > n;
+  const int dt = P.half ? LSAMP_DTYPE_F16 : LSAMP_DTYPE_F32, eb = P.half ? 2 : 4;
+  const int32_t p = std::min(m, n), q = std::max(m, n);
+  const int64_t ld_x = row_pitch(n, eb), ld_a = row_pitch(p, eb);
+  const int64_t step_x = (int64_t)m * ld_x, step_a = (int64_t)p * ld_a;
+  const int32_t wide_x = (int32_t)round_up(n, 8), wide_a = (int32_t)round_up(p, 8);
+
+  OrthStart& s = P.start;
+  s.rows = m;
+  s.cols = n;
+  s.parts = std::min(m, std::max(1, 1024 / batch));
+  s.eps = a->eps;
+  s.x = a->x;
+  s.ld_x = stride_of(a->x_stride, m, n);
+  s.step_x = batch > 1 ? a->x_batch_stride * ib : 0;
+  s.part = ws.take<double>((int64_t)batch * s.parts * 8);
+  s.left = ws.take<float>((int64_t)batch * 4);
+  for (auto& buffer : P.x)
+    for (int i = 0; i < (P.half ? 2 : 1); ++i) buffer[i] = ws.take(batch * step_x * eb);
+  s.hi = P.x[0][0];
+  s.lo = P.x[0][1];
+  s.ld = ld_x;
+  s.step = step_x;
+  void* const gram = ws.take(batch * step_a * eb);
+  void* const poly = ws.take(batch * step_a * eb);
+  float* const diagonal = P.half ? ws.take<float>((int64_t)batch * ld_a * 4) : nullptr;
+
+  P.gram = choose(p, p, slabs_of(q, eb), dt, eb, false, kChunked, batch, true);
+  P.poly = choose(p, p, slabs_of(p, eb), dt, 2 * eb, false, kChunked, batch, true);
+  P.update = choose(m, n, slabs_of(p, eb), dt, 4 * eb, false, kChunked, batch);
+  const MatrixRef x{P.x[0][0], ld_x, m, wide_x}, A{gram, ld_a, p, wide_a}, B{poly, ld_a, p, wide_a};
+  const auto batched = [&](const Choice& c, const MatrixRef& l, const MatrixRef& r, int64_t rows,
+                           int64_t cols, int64_t k, int64_t step_l, int64_t step_r, bool symmetric) {
+    BatchPlan g{};
+    static_cast<GemmPlan&>(g) = plan_gemm(c, l, r, rows, cols, k, eb);
+    g.parts = batch;
+    g.step_a = step_l * eb;
+    g.step_b = step_r * eb;
+    g.symmetric = symmetric;
+    return g;
+  };
+  P.g_gram = batched(P.gram, x, x, p, p, q, step_x, step_x, true);
+  P.g_poly = batched(P.poly, A, A, p, p, p, step_a, step_a, true);
+  P.g_update = P.tall ? batched(P.update, x, B, m, n, p, step_x, step_a, false)
+                      : batched(P.update, B, x, m, n, p, step_a, step_x, false);
+  if (too_many(P.g_gram) || too_many(P.g_poly) || too_many(P.g_update))
+    return set_error(LSAMP_ERR_SHAPE, "%d matrices %d x %d are too large for one call", batch, m, n);
+
+  P.e_gram.n = P.e_poly.n = p;
+  P.e_gram.out = gram;
+  P.e_poly.in = gram;
+  P.e_poly.out = poly;
+  P.e_gram.ld = P.e_poly.ld = ld_a;
+  P.e_gram.step = P.e_poly.step = step_a;
+  P.e_poly.diagonal = diagonal;
+  P.e_poly.step_d = ld_a;
+  EpiOrthUpdate& e = P.e_update;
+  e.m = m;
+  e.n = n;
+  e.tall = P.tall;
+  e.out_dtype = a->out_dtype;
+  e.diagonal = diagonal;
+  e.step_d = ld_a;
+  e.ld = ld_x;
+  e.step = step_x;
+  P.bytes = ws.used;
+  *out = P;
+  return LSAMP_OK;
+}
+
+#define ORTH_OP(half, call) \
+  ((half) ? OrthOps<LSAMP_DTYPE_F16>::call : OrthOps<LSAMP_DTYPE_F32>::call)
+
+}  // namespace
+
+lsamp_status lsamp_layer_norm(lsamp_context* ctx, const lsamp_layer_norm_args* a, void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  NormPlan P;
+  LSAMP_CHECK(plan_norm(a, &P));
+  OnDevice guard(context_device(ctx));
+  LSAMP_TRY(launch_norm(P, a->dtype, stream));
+  return clear_error();
+}
+
+int64_t lsamp_layer_norm_backward_workspace(const lsamp_layer_norm_backward_args* a) {
+  NormBackwardPlan P;
+  int64_t bytes = 0;
+  const lsamp_status st = plan_norm_backward(a, nullptr, &P, &bytes);
+  return needed(st, bytes);
+}
+
+lsamp_status lsamp_layer_norm_backward(lsamp_context* ctx, const lsamp_layer_norm_backward_args* a,
+                                       void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  NormBackwardPlan P;
+  int64_t bytes = 0;
+  LSAMP_CHECK(plan_norm_backward(a, a ? a->workspace : nullptr, &P, &bytes));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, bytes));
+  OnDevice guard(context_device(ctx));
+  LSAMP_TRY(launch_norm_backward(P, a->dtype, stream));
+  return clear_error();
+}
+
+lsamp_status lsamp_quantize_rows(lsamp_context* ctx, const lsamp_quantize_rows_args* a,
+                                 void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
+  LSAMP_CHECK(check_dims("rows", a->rows, kMaxDim));
+  LSAMP_CHECK(check_dims("cols", a->cols));
+  LSAMP_CHECK(check_dtype(a->dtype));
+  LSAMP_CHECK(check_matrix("x", a->x, a->x_stride, a->rows, a->cols, element_bytes(a->dtype)));
+  LSAMP_CHECK(check_quantized("q", a->q, a->q_stride, a->rows, a->cols));
+  LSAMP_CHECK(check_vector("scale", a->scale, 4, true));
+  const QuantizePlan P{a->rows, a->cols, a->cols,
+                       a->x,    stride_of(a->x_stride, a->rows, a->cols),
+                       a->q,    stride_of(a->q_stride, a->rows, a->cols),
+                       a->scale};
+  OnDevice guard(context_device(ctx));
+  LSAMP_TRY(launch_quantize(P, a->dtype, stream));
+  return clear_error();
+}
+
+int64_t lsamp_linear_int8_workspace(const lsamp_linear_int8_args* a) {
+  LinearInt8Plan P;
+  const lsamp_status st = plan_linear_int8(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_linear_int8(lsamp_context* ctx, const lsamp_linear_int8_args* a, void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  LinearInt8Plan P;
+  LSAMP_CHECK(plan_linear_int8(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  if (P.quantize) LSAMP_TRY(launch_quantize(P.quant, a->dtype, stream));
+  LSAMP_TRY(lay_out(P.x, 1, stream));
+  LSAMP_TRY(lay_out(P.w, 1, stream));
+  if (P.gemm.parts == 1) {
+    LSAMP_TRY(INT8_OP(a->dtype, gemm_linear(P.choice.tile, P.gemm, P.epi, stream)));
+  } else {
+    LSAMP_TRY(launch_partial_int8(P.choice.tile, P.gemm, P.partial, stream));
+    LSAMP_TRY(INT8_OP(a->dtype, join_linear(P.partial, P.gemm.parts, P.epi, stream)));
+  }
+  return clear_error();
+}
+
+int64_t lsamp_orthogonalize_workspace(const lsamp_orthogonalize_args* a) {
+  OrthPlan P;
+  const lsamp_status st = plan_orth(a, nullptr, &P);
+  return needed(st, st == LSAMP_OK ? P.bytes : 0);
+}
+
+lsamp_status lsamp_orthogonalize(lsamp_context* ctx, const lsamp_orthogonalize_args* a,
+                                 void* stream) {
+  if (!ctx) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "context is NULL");
+  OrthPlan P;
+  LSAMP_CHECK(plan_orth(a, a ? a->workspace : nullptr, &P));
+  LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
+  OnDevice guard(context_device(ctx));
+  LSAMP_TRY(ORTH_OP(P.half, start(P.start, a->batch, a->in_dtype, stream)));
+  const int ob = element_bytes(a->out_dtype);
+  for (int i = 0; i < a->steps; ++i) {
+    const float* const c = a->coefficients + 3 * i;
+    void* const* const now = P.x[i & 1];
+    void* const* const next = P.x[~i & 1];
+    P.g_gram.a.p = P.g_gram.b.p = now[0];
+    (P.tall ? P.g_update.a : P.g_update.b).p = now[0];
+    P.e_gram.left = P.e_update.left = i == 0 ? P.start.left : nullptr;
+    P.e_poly.b3 = c[1];
+    P.e_poly.c3 = c[2];
+    EpiOrthUpdate& e = P.e_update;
+    e.a1 = c[0];
+    e.x_hi = now[0];
+    e.x_lo = now[1];
+    e.to_hi = next[0];
+    e.to_lo = next[1];
+    if (i + 1 == a->steps) {
+      e.out = a->out;
+      e.ld_out = stride_of(a->out_stride, a->rows, a->cols);
+      e.step_out = a->batch > 1 ? a->out_batch_stride * ob : 0;
+      e.base = a->base;
+      e.ld_base = stride_of(a->base_stride, a->rows, a->cols);
+      e.step_base = a->batch > 1 ? a->base_batch_stride * ob : 0;
+      e.scale = a->scale;
+      e.keep = a->keep;
+    }
+    LSAMP_TRY(ORTH_OP(P.half, gram(P.tall, P.gram.tile, P.g_gram, P.e_gram, stream)));
+    LSAMP_TRY(ORTH_OP(P.half, poly(P.poly.tile, P.g_poly, P.e_poly, stream)));
+    LSAMP_TRY(ORTH_OP(P.half, update(P.tall, P.update.tile, P.g_update, e, stream)));
+  }
+  return clear_error();
+}

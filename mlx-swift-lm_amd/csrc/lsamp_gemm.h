@@ -76,6 +76,15 @@ struct El<LSAMP_DTYPE_F16> {
   using S = _Float16;
   static constexpr int kBytes = 2;
 };
+// Whole numbers of 8 bits: an operand type of row-major products only, summed in 32 bits.
+constexpr int kInt8 = 3;
+template <>
+struct El<kInt8> {
+  using S = int8_t;
+  static constexpr int kBytes = 1;
+};
+template <int DT>
+using Sum = std::conditional_t<DT == kInt8, v4i, v4f>;  // four sums of a lane
 template <int DT>
 constexpr int kChunkOf = 16 / El<DT>::kBytes;  // elements of a 16-byte chunk
 template <int DT>
@@ -92,13 +101,15 @@ __device__ __forceinline__ void barrier() {
 }
 
 // acc += 16 x 16 products over the reduction steps of one chunk per lane
-// (32 steps of 16-bit elements, 16 of float32).  Lane l holds row l & 15 and the
+// (64 steps of 8-bit elements, 32 of 16-bit ones, 16 of float32).  Lane l holds row l & 15 and the
 // chunk of steps l >> 4.  The float32 instruction takes one step of a lane at a
 // time: step j of every lane's chunk, which is a different set of reduction steps
 // on both sides alike.
 template <int DT>
-__device__ __forceinline__ void mma(v4f& acc, const v4i& b, const v4i& a) {
-  if constexpr (DT == LSAMP_DTYPE_BF16) {
+__device__ __forceinline__ void mma(Sum<DT>& acc, const v4i& b, const v4i& a) {
+  if constexpr (DT == kInt8) {
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, acc, 0, 0, 0);
+  } else if constexpr (DT == LSAMP_DTYPE_BF16) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, b),
                                                   __builtin_bit_cast(v8bf, a), acc, 0, 0, 0);
   } else if constexpr (DT == LSAMP_DTYPE_F16) {
@@ -423,6 +434,26 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
   return t;
 }
 
+// The same for a batch of equal products: `part` is the product.  Of a symmetric one
+// (C = C^T) only the tiles at or right of the diagonal are computed, column after
+// column.
+__device__ __forceinline__ TileAt tile_at(int bid, const BatchPlan& g) {
+  const int each = g.symmetric ? g.tiles_n * (g.tiles_n + 1) / 2 : g.tiles_m * g.tiles_n;
+  if (!g.symmetric) return tile_at(bid, g.tiles_m, g.tiles_n, g.parts);
+  const int total = each * g.parts;
+  const int xcd = bid & 7, q = total >> 3, rem = total & 7;
+  int i = xcd * q + (xcd < rem ? xcd : rem) + (bid >> 3);
+  TileAt t;
+  t.part = i / each;
+  i -= t.part * each;
+  int n = (int)((__builtin_sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
+  n += (n + 1) * (n + 2) / 2 <= i ? 1 : 0;  // (the root is off by less than one)
+  n -= n * (n + 1) / 2 > i ? 1 : 0;
+  t.n = n;
+  t.m = i - n * (n + 1) / 2;
+  return t;
+}
+
 // One tile.  Epi: what happens to the sums, with kBarriers barriers; called by the
 // waves that hold them with
 //   run(acc, m0, n0, at, wave-in-M, wave-in-N, lane, lds)
@@ -449,8 +480,9 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
 // registers: after that barrier slab t + 2 may overwrite it, and slab t + 1
 // (loaded a whole slab ago) is complete.
 template <int DT, bool AK, bool BK, int BM, int BN, int WM, int WN, int STAGES, int GROUPS, bool LOOSE,
-          class Epi>
-__global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, Epi epi) {
+          class Epi, class Plan = GemmPlan>
+__global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi epi) {
+  constexpr bool kBatch = std::is_same_v<Plan, BatchPlan>;
   constexpr int kWaves = WM * WN;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   using A = std::conditional_t<LOOSE, LooseSide<DT, AK, BM, kWaves>, Side<DT, AK, BM, kWaves>>;
@@ -462,10 +494,20 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
   const int lane = threadIdx.x & (kWave - 1);
   const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wave = wave_all % kWaves, group = wave_all / kWaves;
-  const TileAt at = tile_at((int)blockIdx.x, g.tiles_m, g.tiles_n, g.parts);
+  TileAt at;
+  int slab0, slabs;
+  if constexpr (kBatch) {
+    at = tile_at((int)blockIdx.x, g);
+    g.a.p = (const char*)g.a.p + at.part * g.step_a;
+    g.b.p = (const char*)g.b.p + at.part * g.step_b;
+    slab0 = 0;
+    slabs = g.slabs;
+  } else {
+    at = tile_at((int)blockIdx.x, g.tiles_m, g.tiles_n, g.parts);
+    slab0 = at.part * g.slabs_per_part;
+    slabs = min(g.slabs_per_part, g.slabs - slab0);
+  }
   const int m0 = at.m * BM, n0 = at.n * BN;
-  const int slab0 = at.part * g.slabs_per_part;
-  const int slabs = min(g.slabs_per_part, g.slabs - slab0);
   const int wm = wave % WM, wn = wave / WM;
 
   A a;
@@ -483,11 +525,12 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
   const int last_a = (AK ? g.a.rows : g.a.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
   const int last_b = (BK ? g.b.rows : g.b.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
 
-  v4f acc[FN][FM];
+  using V = Sum<DT>;
+  V acc[FN][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FM; ++j) acc[i][j] = V{0, 0, 0, 0};
 
   const uint32_t lds0 = lds_address(lds);
   const auto fetch_full = [&](int buffer) {
@@ -648,7 +691,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
-          for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < FM; ++j) acc[i][j] = V{0, 0, 0, 0};
         reduce(std::true_type{});
       }
     }
@@ -656,7 +699,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(GemmPlan g, E
       // [group - 1][fragment][lane] of every wave; the first group adds them up in order
       constexpr int kFrags = FM * FN;
       __syncthreads();
-      v4f* sums = (v4f*)lds;
+      V* sums = (V*)lds;
       static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + WN * BM * 8 <= (int)sizeof(lds),
                     "the sums and an epilogue's pair of floats for every row and wave");
       static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + kWaves * FN * 1024 <= (int)sizeof(lds),

@@ -26,6 +26,12 @@ struct GemmPlan {
   int32_t slabs, slabs_per_part;  // 128-byte slabs of the reduction
 };
 
+// `parts` equal products, one after another in memory.
+struct BatchPlan : GemmPlan {
+  int64_t step_a, step_b;  // bytes
+  int32_t symmetric;       // the result is: tiles left of the diagonal are left out
+};
+
 // Which operand is read along the reduction's rows (lsamp_gemm.h).
 enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
 // Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
@@ -162,6 +168,52 @@ struct DropoutPlan {
   int64_t ld_out;
 };
 
+struct EpiLinearInt8 : EpiLinear {
+  const float* x_scale;  // [m]
+  const float* w_scale;  // [n]
+};
+
+struct NormPlan {
+  int32_t rows, cols;
+  float eps;
+  const void* x;
+  int64_t ld_x;
+  const void* weight;  // or NULL, as bias
+  const void* bias;
+  void* out;
+  int64_t ld_out;
+  float* mean;  // or NULL, as rstd
+  float* rstd;
+};
+struct NormBackwardPlan {
+  int32_t rows, cols;
+  int32_t chunks;  // shares of the columns' sums (norm_chunks)
+  const void* x;
+  int64_t ld_x;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  const void* d_out;
+  int64_t ld_d;
+  const void* residual;  // or NULL: added to d_x
+  int64_t ld_residual;
+  void* d_x;  // or NULL
+  int64_t ld_dx;
+  void* d_weight;  // or NULL
+  void* d_bias;
+  float* part;  // [chunks][2][ld_part], NULL without d_weight and d_bias
+  int64_t ld_part;  // a multiple of 8
+};
+struct QuantizePlan {
+  int32_t rows, cols;
+  int32_t out_cols;  // columns cols .. out_cols - 1 of q are written as zero
+  const void* x;
+  int64_t ld_x;
+  int8_t* q;
+  int64_t ld_q;
+  float* scale;
+};
+
 // One set of these for each element type; 0 or a hipError_t.
 template <int DT>
 struct HeadOps {
@@ -179,8 +231,21 @@ struct HeadOps {
   static int col_sum(const ColSumPlan& p, void* stream);
   static int col_sum_join(const ColSumPlan& p, void* out, const float* scale, void* stream);
 };
+// One set for each element type of bias, residual and out.  Tiles: not kTile* for rows
+// that are no chunks.
+template <int DT>
+struct Int8Ops {
+  static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinearInt8& e, void* stream);
+  static int join_linear(const EpiPartial& from, int parts, const EpiLinearInt8& e, void* stream);
+};
+// Sums of parts as whole numbers of 32 bits.
+int launch_partial_int8(GemmTile tile, const GemmPlan& g, const EpiPartial& e, void* stream);
+int norm_chunks(int rows, int cols);
+int launch_norm(const NormPlan& p, int dtype, void* stream);
+int launch_norm_backward(const NormBackwardPlan& p, int dtype, void* stream);
+int launch_quantize(const QuantizePlan& p, int dtype, void* stream);
 int launch_dropout(const DropoutPlan& p, int dtype, void* stream);
-// Element size 2 or 4.
+// Element size 1, 2 or 4.
 int launch_pack(const PackPlan& p, int element_bytes, void* stream);
 int launch_join_stats(const JoinStatsPlan& p, void* stream);
 int launch_grad_scale(const GradScalePlan& p, void* stream);

@@ -139,7 +139,9 @@ int launch_pack(const PackPlan& p, int element_bytes, void* stream) {
   const dim3 grid((unsigned)((chunks + kThreads - 1) / kThreads),
                   (unsigned)(p.rows < 32768 ? p.rows : 32768));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (element_bytes == 2)
+  if (element_bytes == 1)
+    hipLaunchKernelGGL((k_pack<uint8_t>), grid, dim3(kThreads), 0, st, p);
+  else if (element_bytes == 2)
     hipLaunchKernelGGL((k_pack<uint16_t>), grid, dim3(kThreads), 0, st, p);
   else
     hipLaunchKernelGGL((k_pack<uint32_t>), grid, dim3(kThreads), 0, st, p);

@@ -1,0 +1,529 @@
+// lsamp_norm.hip — layer norm over the rows of a matrix, its gradients, and rows
+// quantised to 8-bit integers.
+//
+//   y = (x - mean) rstd w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   d_x = rstd (g - mean(g) - xh mean(g xh)) + residual,  g = d w,  xh = (x - mean) rstd
+//   d_w = sum over rows of d xh,  d_b = sum over rows of d
+//   q = rint(x / s),  s = max |x| / 127 (as a product with 1 / 127)
+//
+// All are bound by memory: a row of up to 16,384 elements is read once, into
+// registers, eight elements of a thread in each of V groups; the variance is that
+// of the centred values (their squares do not cancel).  Longer rows are read
+// again for every sum.  All sums are float32.
+#include <hip/hip_runtime.h>
+
+#include "lsamp_head.h"
+
+namespace lsamp {
+namespace {
+
+constexpr int kWave = 64;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename E>
+struct __attribute__((packed, aligned(sizeof(E)))) Any16 {  // 16 bytes of any alignment
+  u32x4 v;
+};
+struct Eight {
+  float v[8];
+};
+// Eight elements, `valid` of them in the row, the others zero.
+template <typename E>
+__device__ __forceinline__ Eight load8(const E* p, int valid) {
+  Eight o;
+  if (valid >= 8) {
+    E e[8];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
+      const u32x4 q = ((const Any16<E>*)p)[i].v;
+      __builtin_memcpy((char*)e + 16 * i, &q, 16);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.v[k] = (float)e[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.v[k] = k < valid ? (float)p[k] : 0.f;
+  }
+  return o;
+}
+template <typename E>
+__device__ __forceinline__ void store8(E* p, const Eight& x, int valid) {
+  E e[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) e[k] = (E)x.v[k];
+  if (valid >= 8) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
+      u32x4 q;
+      __builtin_memcpy(&q, (const char*)e + 16 * i, 16);
+      ((Any16<E>*)p)[i].v = q;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < valid) p[k] = e[k];
+  }
+}
+
+// Sums (or maxima) of N values over the THREADS threads of a row: a wave, or a
+// work-group.  Every thread gets them.  `red` has 2 N floats a wave: a row's
+// exchange may begin while the one before is still read.
+template <int THREADS, int N, bool MAX = false>
+__device__ __forceinline__ void join(float (&s)[N], float* red, int& turn) {
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float o = __shfl_xor(s[i], d);
+      s[i] = MAX ? fmaxf(s[i], o) : s[i] + o;
+    }
+  if constexpr (THREADS > kWave) {
+    constexpr int kWaves = THREADS / kWave;
+    const int wave = (int)threadIdx.x / kWave;
+    float* const at = red + turn * (kWaves * N);
+    turn ^= 1;
+    if ((threadIdx.x & (kWave - 1)) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) at[wave * N + i] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float t = at[i];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) t = MAX ? fmaxf(t, at[w * N + i]) : t + at[w * N + i];
+      s[i] = t;
+    }
+  }
+}
+
+constexpr int kBlock = 256;  // threads of a work-group whose rows are a wave's
+
+// A row's threads and the rows of a work-group.
+template <int THREADS>
+struct Rows {
+  static constexpr int kPer = THREADS < kBlock ? kBlock / THREADS : 1;
+  static constexpr int kGroup = THREADS < kBlock ? kBlock : THREADS;
+  int first, step, t;  // the thread's first row, the distance to the next, its place in the row
+  __device__ __forceinline__ Rows()
+      : first((int)blockIdx.x * kPer + (int)threadIdx.x / THREADS), step((int)gridDim.x * kPer),
+        t((int)threadIdx.x % THREADS) {}
+};
+
+// LONG: rows of any length, read three times.
+template <typename E, int THREADS, int V, bool LONG>
+__global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
+  __shared__ float red[2 * THREADS / kWave];
+  const Rows<THREADS> rows;
+  int turn = 0;
+  const float per = 1.f / (float)p.cols;
+  const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
+  for (int64_t r = rows.first; r < p.rows; r += rows.step) {
+    const E* const x = (const E*)p.x + r * p.ld_x;
+    Eight a[V];
+    const auto fetch = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = ((s * V + i) * THREADS + rows.t) * 8;
+        if (LONG || c < p.cols) a[i] = load8(x + c, p.cols - c);
+      }
+    };
+    float sum[1] = {0.f};
+    for (int s = 0; s < span; ++s) {
+      fetch(s);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (((s * V + i) * THREADS + rows.t) * 8 < p.cols)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum[0] += a[i].v[k];
+    }
+    join<THREADS>(sum, red, turn);
+    const float mean = sum[0] * per;
+    float sq[1] = {0.f};
+    for (int s = 0; s < span; ++s) {
+      if (LONG) fetch(s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int valid = p.cols - ((s * V + i) * THREADS + rows.t) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < valid) {
+            const float d = a[i].v[k] - mean;
+            sq[0] += d * d;
+          }
+      }
+    }
+    join<THREADS>(sq, red, turn);
+    const float rstd = 1.f / sqrtf(sq[0] * per + p.eps);
+    if (rows.t == 0) {
+      if (p.mean) p.mean[r] = mean;
+      if (p.rstd) p.rstd[r] = rstd;
+    }
+    for (int s = 0; s < span; ++s) {
+      if (LONG) fetch(s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = ((s * V + i) * THREADS + rows.t) * 8, valid = p.cols - c;
+        if (valid <= 0) continue;
+        Eight y;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y.v[k] = (a[i].v[k] - mean) * rstd;
+        if (p.weight) {
+          const Eight w = load8((const E*)p.weight + c, valid);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y.v[k] *= w.v[k];
+        }
+        if (p.bias) {
+          const Eight b = load8((const E*)p.bias + c, valid);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y.v[k] += b.v[k];
+        }
+        store8((E*)p.out + r * p.ld_out + c, y, valid);
+      }
+    }
+  }
+}
+
+// A row's gradient, and (SUMS) the work-group's share of the columns' sums, which
+// stay in registers over its rows.  LONG: d_x only, each row read twice.
+template <typename E, int THREADS, int V, bool SUMS, bool LONG>
+__global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBackwardPlan p) {
+  static_assert(!(SUMS && LONG), "a long row's sums are another kernel's");
+  constexpr int kPer = Rows<THREADS>::kPer;
+  __shared__ float red[4 * THREADS / kWave];
+  const Rows<THREADS> rows;
+  int turn = 0;
+  const float per = 1.f / (float)p.cols;
+  const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
+  Eight sum_w[SUMS ? V : 1], sum_b[SUMS ? V : 1], w[V];
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum_w[i].v[k] = sum_b[i].v[k] = 0.f;
+  }
+  const auto col = [&](int s, int i) { return ((s * V + i) * THREADS + rows.t) * 8; };
+  const auto weights = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = col(s, i);
+      if (p.weight) {
+        w[i] = load8((const E*)p.weight + c, p.cols - c);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[i].v[k] = 1.f;
+      }
+    }
+  };
+  if (!LONG) weights(0);
+  for (int64_t r = rows.first; r < p.rows; r += rows.step) {
+    const E* const x = (const E*)p.x + r * p.ld_x;
+    const E* const d = (const E*)p.d_out + r * p.ld_d;
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    Eight xh[V], g[V], res[V];
+    const auto fetch = [&](int s, bool last) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = col(s, i), valid = p.cols - c;
+        xh[i] = load8(x + c, valid);
+        g[i] = load8(d + c, valid);
+        if (last && p.residual) res[i] = load8((const E*)p.residual + r * p.ld_residual + c, valid);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int valid = p.cols - col(s, i);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) xh[i].v[k] = k < valid ? (xh[i].v[k] - mean) * rstd : 0.f;
+      }
+    };
+    float c12[2] = {0.f, 0.f};
+    for (int s = 0; s < span; ++s) {
+      if (LONG) weights(s);
+      fetch(s, !LONG);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (SUMS) {
+            sum_w[i].v[k] += g[i].v[k] * xh[i].v[k];
+            sum_b[i].v[k] += g[i].v[k];
+          }
+          g[i].v[k] *= w[i].v[k];
+          c12[0] += g[i].v[k];
+          c12[1] += g[i].v[k] * xh[i].v[k];
+        }
+    }
+    if (!p.d_x) continue;  // (the same for every thread)
+    join<THREADS>(c12, red, turn);
+    const float c1 = c12[0] * per, c2 = c12[1] * per;
+    for (int s = 0; s < span; ++s) {
+      if (LONG) {
+        weights(s);
+        fetch(s, true);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = col(s, i), valid = p.cols - c;
+        if (valid <= 0) continue;
+        Eight y;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float gk = LONG ? g[i].v[k] * w[i].v[k] : g[i].v[k];
+          y.v[k] = rstd * (gk - c1 - xh[i].v[k] * c2);
+          if (p.residual) y.v[k] += res[i].v[k];
+        }
+        store8((E*)p.d_x + r * p.ld_dx + c, y, valid);
+      }
+    }
+  }
+  if constexpr (SUMS) {
+    // [work-group][2][ld_part]; rows of a wave each are joined first
+    if constexpr (kPer > 1) {
+      __shared__ float both[kPer - 1][V][8][2][kWave];
+      const int wave = (int)threadIdx.x / kWave;
+      if (wave > 0)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            both[wave - 1][i][k][0][rows.t] = sum_w[i].v[k];
+            both[wave - 1][i][k][1][rows.t] = sum_b[i].v[k];
+          }
+      __syncthreads();
+      if (wave > 0) return;
+      for (int o = 0; o < kPer - 1; ++o)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            sum_w[i].v[k] += both[o][i][k][0][rows.t];
+            sum_b[i].v[k] += both[o][i][k][1][rows.t];
+          }
+    }
+    float* const part = p.part + (int64_t)blockIdx.x * 2 * p.ld_part;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = col(0, i);
+      if (c >= p.cols) continue;  // (rows of sums are whole groups of eight)
+      store8(part + c, sum_w[i], 8);
+      store8(part + p.ld_part + c, sum_b[i], 8);
+    }
+  }
+}
+
+// Column sums of long rows: a column a thread, a chunk of rows a work-group.
+template <typename E>
+__global__ __launch_bounds__(kBlock) void k_norm_sums(NormBackwardPlan p) {
+  const int c = (int)blockIdx.x * kBlock + (int)threadIdx.x;
+  if (c >= p.cols) return;
+  const int per = (p.rows + p.chunks - 1) / p.chunks;
+  const int r0 = (int)blockIdx.y * per, r1 = min(p.rows, r0 + per);
+  float w = 0.f, b = 0.f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const float d = (float)((const E*)p.d_out)[r * p.ld_d + c];
+    const float xh = ((float)((const E*)p.x)[r * p.ld_x + c] - p.mean[r]) * p.rstd[r];
+    w += d * xh;
+    b += d;
+  }
+  float* const part = p.part + (int64_t)blockIdx.y * 2 * p.ld_part;
+  part[c] = w;
+  part[p.ld_part + c] = b;
+}
+
+// The work-groups' shares, joined in their order: 64 columns a work-group of
+// sixteen waves, the waves taking shares in turn.
+constexpr int kJoinWaves = 16;
+template <typename E>
+__global__ __launch_bounds__(kJoinWaves* kWave) void k_norm_join(NormBackwardPlan p) {
+  __shared__ float red[kJoinWaves][kWave];
+  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
+  const int c = (int)blockIdx.x * kWave + lane, which = (int)blockIdx.y;
+  E* const out = (E*)(which ? p.d_bias : p.d_weight);
+  if (!out) return;
+  float s = 0.f;
+  if (c < p.cols) {
+#pragma unroll 8
+    for (int i = wave; i < p.chunks; i += kJoinWaves) s += p.part[((int64_t)i * 2 + which) * p.ld_part + c];
+  }
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= p.cols) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) s += red[w][lane];
+  out[c] = (E)s;
+}
+
+// x / s to the nearest whole number, ties to the even one, from the product with
+// 1 / s, which is off by one at most: e = x - q s is exact (one fma of values that
+// are multiples of the smaller one's last place), and where it is more than half
+// a step, or half a step and q odd, the neighbour is taken.
+__device__ __forceinline__ int nearest(float x, float s, float inverse) {
+  float q = rintf(x * inverse);
+  const float e = fmaf(-q, s, x), half = 0.5f * s;
+  const bool odd = ((int)q & 1) != 0;
+  if (e > half || (e == half && odd)) q += 1.f;
+  else if (e < -half || (e == -half && odd)) q -= 1.f;
+  return (int)fminf(fmaxf(q, -127.f), 127.f);
+}
+
+constexpr float kPart = 1.f / 127.f;
+template <typename E, int THREADS, int V, bool LONG>
+__global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan p) {
+  __shared__ float red[4 * THREADS / kWave];
+  const Rows<THREADS> rows;
+  int turn = 0;
+  const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
+  for (int64_t r = rows.first; r < p.rows; r += rows.step) {
+    const E* const x = (const E*)p.x + r * p.ld_x;
+    Eight a[V];
+    const auto fetch = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = ((s * V + i) * THREADS + rows.t) * 8;
+        a[i] = load8(x + c, p.cols - c);
+      }
+    };
+    float top[2] = {0.f, 0.f};  // the largest magnitude; 1 where a value is not finite
+    for (int s = 0; s < span; ++s) {
+      fetch(s);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float m = fabsf(a[i].v[k]);
+          top[0] = fmaxf(top[0], m);
+          top[1] = m < INFINITY ? top[1] : 1.f;
+        }
+    }
+    join<THREADS, 2, true>(top, red, turn);
+    const bool finite = top[1] == 0.f;
+    const float scale = finite ? fmaxf(top[0] * kPart, 1.17549435e-38f) : NAN;
+    const float inverse = 1.f / scale;
+    if (rows.t == 0) p.scale[r] = scale;
+    for (int s = 0; s < span; ++s) {
+      if (LONG) fetch(s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = ((s * V + i) * THREADS + rows.t) * 8, valid = p.out_cols - c;
+        if (valid <= 0) continue;
+        int8_t q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)  // (past the row's end a value is 0)
+          q[k] = finite ? (int8_t)nearest(a[i].v[k], scale, inverse) : (int8_t)0;
+        int8_t* const to = p.q + r * p.ld_q + c;
+        if (valid >= 8) {
+          struct __attribute__((packed)) Any8 {
+            uint64_t v;
+          };
+          uint64_t word;
+          __builtin_memcpy(&word, q, 8);
+          ((Any8*)to)->v = word;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < valid) to[k] = q[k];
+        }
+      }
+    }
+  }
+}
+
+// The shape of a row of `cols` elements: a wave, 256 or 1024 threads, one, two or
+// four groups of eight of a thread.  Few rows take more threads a row.
+enum Shape { kWave1, kWave2, kWave4, kBlock1, kBlock2, kWide2, kLong };
+Shape shape_of(int rows, int cols) {
+  if (cols <= 2048 && rows >= 1024) return cols <= 512 ? kWave1 : cols <= 1024 ? kWave2 : kWave4;
+  if (cols <= 512) return kWave1;
+  if (cols <= 2048) return kBlock1;
+  if (cols <= 4096) return kBlock2;
+  return cols <= 16384 ? kWide2 : kLong;
+}
+int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
+int threads_of(Shape s) { return s == kWide2 || s == kLong ? 1024 : kBlock; }
+
+#define LSAMP_SHAPES(s, K, ARGS)        \
+  switch (s) {                          \
+    case kWave1: K(64, 1, false); break;  \
+    case kWave2: K(64, 2, false); break;  \
+    case kWave4: K(64, 4, false); break;  \
+    case kBlock1: K(256, 1, false); break; \
+    case kBlock2: K(256, 2, false); break; \
+    case kWide2: K(1024, 2, false); break; \
+    default: K(1024, 1, true); break;     \
+  }
+
+template <typename E>
+int norm(const NormPlan& p, hipStream_t st) {
+  const Shape s = shape_of(p.rows, p.cols);
+  const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
+  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536)), block((unsigned)threads_of(s));
+#define K(T, V, L) hipLaunchKernelGGL((k_norm<E, T, V, L>), grid, block, 0, st, p)
+  LSAMP_SHAPES(s, K, )
+#undef K
+  return (int)hipGetLastError();
+}
+
+template <typename E>
+int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
+  const Shape s = shape_of(p.rows, p.cols);
+  const bool sums = p.part != nullptr;
+  const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
+  const dim3 grid((unsigned)(sums && s != kLong ? p.chunks : groups < 65536 ? groups : 65536));
+  const dim3 block((unsigned)threads_of(s));
+  if (s == kLong) {
+    if (p.d_x) hipLaunchKernelGGL((k_norm_backward<E, 1024, 1, false, true>), grid, block, 0, st, p);
+    if (sums)
+      hipLaunchKernelGGL((k_norm_sums<E>),
+                         dim3((unsigned)((p.cols + kBlock - 1) / kBlock), (unsigned)p.chunks),
+                         dim3(kBlock), 0, st, p);
+  } else if (sums) {
+#define K(T, V, L) hipLaunchKernelGGL((k_norm_backward<E, T, V, !(L), L>), grid, block, 0, st, p)
+    LSAMP_SHAPES(s, K, )
+#undef K
+  } else {
+#define K(T, V, L) hipLaunchKernelGGL((k_norm_backward<E, T, V, false, L>), grid, block, 0, st, p)
+    LSAMP_SHAPES(s, K, )
+#undef K
+  }
+  if (sums)
+    hipLaunchKernelGGL((k_norm_join<E>), dim3((unsigned)((p.cols + kWave - 1) / kWave), 2),
+                       dim3(kJoinWaves * kWave), 0, st, p);
+  return (int)hipGetLastError();
+}
+
+template <typename E>
+int quantize(const QuantizePlan& p, hipStream_t st) {
+  const Shape s = shape_of(p.rows, p.cols);
+  const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
+  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536)), block((unsigned)threads_of(s));
+#define K(T, V, L) hipLaunchKernelGGL((k_quantize<E, T, V, L>), grid, block, 0, st, p)
+  LSAMP_SHAPES(s, K, )
+#undef K
+  return (int)hipGetLastError();
+}
+
+#define LSAMP_EACH_TYPE(call)                                 \
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);     \
+  switch (dtype) {                                            \
+    case LSAMP_DTYPE_F32: return call<float>(p, st);          \
+    case LSAMP_DTYPE_BF16: return call<__bf16>(p, st);        \
+    default: return call<_Float16>(p, st);                    \
+  }
+
+}  // namespace
+
+// Shares of the columns' sums: a work-group's.
+int norm_chunks(int rows, int cols) {
+  const Shape s = shape_of(rows, cols);
+  if (s == kLong) return rows < 64 ? 1 : rows / 32 < 256 ? rows / 32 : 256;
+  const int groups = (rows + rows_per_group(s) - 1) / rows_per_group(s);
+  const int most = s == kWide2 ? 256 : 512;
+  return groups < most ? groups : most;
+}
+
+int launch_norm(const NormPlan& p, int dtype, void* stream) { LSAMP_EACH_TYPE(norm) }
+int launch_norm_backward(const NormBackwardPlan& p, int dtype, void* stream) {
+  LSAMP_EACH_TYPE(norm_backward)
+}
+int launch_quantize(const QuantizePlan& p, int dtype, void* stream) { LSAMP_EACH_TYPE(quantize) }
+
+}  // namespace lsamp

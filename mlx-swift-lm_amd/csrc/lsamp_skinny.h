@@ -61,11 +61,12 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
   const char* const x_base = x.base;
   char* const mine = lds + wave * 2 * X::kBytes;
 
-  v4f acc[NF][MF];
+  using V = Sum<DT>;
+  V acc[NF][MF];
 #pragma unroll
   for (int i = 0; i < NF; ++i)
 #pragma unroll
-    for (int j = 0; j < MF; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MF; ++j) acc[i][j] = V{0, 0, 0, 0};
 
   struct Step {
     v4i w[NF][2], x[2];
@@ -167,14 +168,14 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
   }
 
   if constexpr (kStaged) __syncthreads();  // (the sums take the slabs' place)
-  v4f* sums = (v4f*)lds;                   // [wave][fragment][lane]
+  V* sums = (V*)lds;                       // [wave][fragment][lane]
 #pragma unroll
   for (int i = 0; i < NF; ++i)
 #pragma unroll
     for (int j = 0; j < MF; ++j) sums[(wave * kFrags + i * MF + j) * kWave + lane] = acc[i][j];
   __syncthreads();
   const auto total = [&](int frag, int l) {
-    v4f v = sums[frag * kWave + l];
+    V v = sums[frag * kWave + l];
 #pragma unroll
     for (int k = 1; k < WK; ++k) v += sums[(k * kFrags + frag) * kWave + l];
     return v;
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(WK* kWave, 2) void k_skinny(GemmPlan g, Epi epi) {
         epi.put(r, n0 + c, total(c / 16 * MF + r / 16, (r & 15) + (c % 16) * 4), 0);
     }
   } else {
-    v4f part[1][MF];
+    V part[1][MF];
 #pragma unroll
     for (int j = 0; j < MF; ++j) part[0][j] = total(wave * MF + j, lane);
     epi.template run<MF, 1, MF * 16, NF * 16, 1, NF>(part, 0, n0, TileAt{0, (int)blockIdx.x, 0}, 0,

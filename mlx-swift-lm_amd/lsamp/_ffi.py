@@ -406,6 +406,110 @@ class DropoutArgs(Structure):
     ]
 
 
+class LayerNormArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("dtype", c_int32),
+        ("eps", c_float),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("bias", c_void_p),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("mean", c_void_p),
+        ("rstd", c_void_p),
+    ]
+
+
+class LayerNormBackwardArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("dtype", c_int32),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("weight", c_void_p),
+        ("mean", c_void_p),
+        ("rstd", c_void_p),
+        ("d_out", c_void_p),
+        ("d_out_stride", c_int64),
+        ("residual", c_void_p),
+        ("residual_stride", c_int64),
+        ("d_x", c_void_p),
+        ("d_x_stride", c_int64),
+        ("d_weight", c_void_p),
+        ("d_bias", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class QuantizeRowsArgs(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("dtype", c_int32),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("q", c_void_p),
+        ("q_stride", c_int64),
+        ("scale", c_void_p),
+    ]
+
+
+class LinearInt8Args(Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("in_features", c_int32),
+        ("out_features", c_int32),
+        ("dtype", c_int32),
+        ("activation", c_int32),
+        ("softcap", c_float),
+        ("out_dtype", c_int32),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("x_scale", c_void_p),
+        ("weight", c_void_p),
+        ("weight_stride", c_int64),
+        ("weight_scale", c_void_p),
+        ("bias", c_void_p),
+        ("residual", c_void_p),
+        ("residual_stride", c_int64),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class OrthogonalizeArgs(Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("in_dtype", c_int32),
+        ("out_dtype", c_int32),
+        ("steps", c_int32),
+        ("coefficients", c_void_p),
+        ("eps", c_float),
+        ("scale", c_float),
+        ("keep", c_float),
+        ("x", c_void_p),
+        ("x_stride", c_int64),
+        ("x_batch_stride", c_int64),
+        ("base", c_void_p),
+        ("base_stride", c_int64),
+        ("base_batch_stride", c_int64),
+        ("out", c_void_p),
+        ("out_stride", c_int64),
+        ("out_batch_stride", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
 class LibraryMissing(RuntimeError):
     pass
 
@@ -466,13 +570,18 @@ def load_library(path: str | None = None):
     for name, args in (("lsamp_linear", LinearArgs),
                        ("lsamp_linear_backward", LinearBackwardArgs),
                        ("lsamp_head_loss", HeadLossArgs),
-                       ("lsamp_head_loss_backward", HeadLossBackwardArgs)):
+                       ("lsamp_head_loss_backward", HeadLossBackwardArgs),
+                       ("lsamp_layer_norm_backward", LayerNormBackwardArgs),
+                       ("lsamp_linear_int8", LinearInt8Args),
+                       ("lsamp_orthogonalize", OrthogonalizeArgs)):
         getattr(lib, name).argtypes = [c_void_p, POINTER(args), c_void_p]
         getattr(lib, name).restype = c_int32
         getattr(lib, name + "_workspace").argtypes = [POINTER(args)]
         getattr(lib, name + "_workspace").restype = c_int64
-    lib.lsamp_dropout.argtypes = [c_void_p, POINTER(DropoutArgs), c_void_p]
-    lib.lsamp_dropout.restype = c_int32
+    for name, args in (("lsamp_dropout", DropoutArgs), ("lsamp_layer_norm", LayerNormArgs),
+                       ("lsamp_quantize_rows", QuantizeRowsArgs)):
+        getattr(lib, name).argtypes = [c_void_p, POINTER(args), c_void_p]
+        getattr(lib, name).restype = c_int32
     lib.lsamp_resolve_generate_parameters.argtypes = [
         POINTER(GenerateParameters), POINTER(RowParams), POINTER(c_int32)]
     lib.lsamp_resolve_generate_parameters.restype = c_int32

@@ -354,6 +354,57 @@ class Context:
         p.launch()
         return p.out
 
+    def prepare_layer_norm(self, x: torch.Tensor, **kw) -> "head.PreparedLayerNorm":
+        """(x - mean) rstd weight + bias over every row (lsamp_layer_norm).
+        Keywords: weight, bias, eps, want_stats, out."""
+        return head.PreparedLayerNorm(self, x, **kw)
+
+    def layer_norm(self, x: torch.Tensor, **kw) -> torch.Tensor:
+        p = self.prepare_layer_norm(x, **kw)
+        p.launch()
+        return p.out
+
+    def prepare_layer_norm_backward(self, d_out: torch.Tensor, x: torch.Tensor, *,
+                                    mean: torch.Tensor, rstd: torch.Tensor,
+                                    **kw) -> "head.PreparedLayerNormBackward":
+        """Its gradients.  Keywords: weight, residual, want_x, want_weight,
+        want_bias, d_x."""
+        return head.PreparedLayerNormBackward(self, d_out, x, mean=mean, rstd=rstd, **kw)
+
+    def prepare_quantize_rows(self, x: torch.Tensor, **kw) -> "head.PreparedQuantizeRows":
+        """Rows of 8-bit integers with a scale each (lsamp_quantize_rows): a
+        layer's weights (a scale an output channel), or tokens.  Keyword: q."""
+        return head.PreparedQuantizeRows(self, x, **kw)
+
+    def quantize_rows(self, x: torch.Tensor, **kw):
+        """(q, scale)."""
+        p = self.prepare_quantize_rows(x, **kw)
+        p.launch()
+        return p.q, p.scale
+
+    def prepare_linear_int8(self, x: torch.Tensor, weight: torch.Tensor,
+                            weight_scale: torch.Tensor, **kw) -> "head.PreparedLinearInt8":
+        """The linear block on 8-bit operands (lsamp_linear_int8).  Keywords:
+        x_scale, bias, residual, activation, softcap, out_dtype, out."""
+        return head.PreparedLinearInt8(self, x, weight, weight_scale, **kw)
+
+    def linear_int8(self, x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                    **kw) -> torch.Tensor:
+        p = self.prepare_linear_int8(x, weight, weight_scale, **kw)
+        p.launch()
+        return p.out
+
+    def prepare_orthogonalize(self, x: torch.Tensor, **kw) -> "head.PreparedOrthogonalize":
+        """scale orth(x) + keep base, by Newton-Schulz steps
+        (lsamp_orthogonalize).  Keywords: steps, coefficients, eps, base, scale,
+        keep, out_dtype, out."""
+        return head.PreparedOrthogonalize(self, x, **kw)
+
+    def orthogonalize(self, x: torch.Tensor, **kw) -> torch.Tensor:
+        p = self.prepare_orthogonalize(x, **kw)
+        p.launch()
+        return p.out
+
 
 class PreparedSample:
     """A fully bound lsamp_sample call: every input and output buffer is a

@@ -1,5 +1,6 @@
 """Prepared calls of the hidden-state operators (include/lsamp.h): linear
-blocks, the vocabulary head's cross entropy, their gradients, and dropout.
+blocks, the vocabulary head's cross entropy, layer norm, their gradients,
+dropout, products of 8-bit integers, and orthogonalised updates.
 
 Made by the Context methods of the same names (`Context.prepare_linear`, ...).
 A prepared call holds its inputs, outputs and workspace; `launch()` is one C
@@ -62,7 +63,7 @@ class PreparedCall:
             raise ValueError(f"{name} rows must be contiguous")
         if dtype is not None and t.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-        if t.dtype not in DTYPES:
+        if t.dtype not in DTYPES and dtype is None:
             raise ValueError(f"{name}: {t.dtype} is not float32, bfloat16 or float16")
         if t.device != self.device:
             raise ValueError(f"{name} must be on {self.device}")
@@ -270,6 +271,193 @@ class PreparedDropout(PreparedCall):
         self.out = self._empty(tuple(x.shape), x.dtype) if out is None else out
         a.out, a.out_stride = self._matrix("out", self.out, *x.shape, x.dtype)
         self._bind(a)
+
+    def outputs(self) -> dict:
+        return {"out": self.out}
+
+
+class PreparedLayerNorm(PreparedCall):
+    """out = (x - mean) rstd weight + bias over every row (lsamp_layer_norm);
+    `mean` and `rstd` hold the rows' statistics where asked for."""
+
+    entry = "lsamp_layer_norm"
+
+    def __init__(self, ctx, x, *, weight=None, bias=None, eps=1e-5, want_stats=False, out=None):
+        super().__init__(ctx, x.device)
+        a = _ffi.LayerNormArgs()
+        a.x, a.x_stride = self._matrix("x", x)
+        rows, n = x.shape
+        a.rows, a.cols, a.dtype, a.eps = rows, n, DTYPES[x.dtype], eps
+        if weight is not None:
+            a.weight = self._vector("weight", weight, n, x.dtype)
+        if bias is not None:
+            a.bias = self._vector("bias", bias, n, x.dtype)
+        self.out = self._empty((rows, n), x.dtype) if out is None else out
+        a.out, a.out_stride = self._matrix("out", self.out, rows, n, x.dtype)
+        self.mean = self._empty(rows, torch.float32) if want_stats else None
+        self.rstd = self._empty(rows, torch.float32) if want_stats else None
+        if want_stats:
+            a.mean, a.rstd = self.mean.data_ptr(), self.rstd.data_ptr()
+        self._bind(a)
+
+    def outputs(self) -> dict:
+        o = {"out": self.out, "mean": self.mean, "rstd": self.rstd}
+        return {k: v for k, v in o.items() if v is not None}
+
+
+class PreparedLayerNormBackward(PreparedCall):
+    """The gradients of a layer norm at d_out (lsamp_layer_norm_backward);
+    `mean` and `rstd` are the forward call's, `residual` is added to d_x."""
+
+    entry = "lsamp_layer_norm_backward"
+
+    def __init__(self, ctx, d_out, x, *, mean, rstd, weight=None, residual=None, want_x=True,
+                 want_weight=True, want_bias=False, d_x=None):
+        super().__init__(ctx, x.device)
+        a = _ffi.LayerNormBackwardArgs()
+        a.x, a.x_stride = self._matrix("x", x)
+        rows, n = x.shape
+        dt = x.dtype
+        a.rows, a.cols, a.dtype = rows, n, DTYPES[dt]
+        a.d_out, a.d_out_stride = self._matrix("d_out", d_out, rows, n, dt)
+        if weight is not None:
+            a.weight = self._vector("weight", weight, n, dt)
+        a.mean = self._vector("mean", mean, rows, torch.float32)
+        a.rstd = self._vector("rstd", rstd, rows, torch.float32)
+        if residual is not None:
+            a.residual, a.residual_stride = self._matrix("residual", residual, rows, n, dt)
+        self.d_x = self._empty((rows, n), dt) if want_x and d_x is None else d_x
+        self.d_weight = self._empty(n, dt) if want_weight else None
+        self.d_bias = self._empty(n, dt) if want_bias else None
+        if self.d_x is not None:
+            a.d_x, a.d_x_stride = self._matrix("d_x", self.d_x, rows, n, dt)
+        if want_weight:
+            a.d_weight = self.d_weight.data_ptr()
+        if want_bias:
+            a.d_bias = self.d_bias.data_ptr()
+        self._bind(a)
+
+    def outputs(self) -> dict:
+        o = {"d_x": self.d_x, "d_weight": self.d_weight, "d_bias": self.d_bias}
+        return {k: v for k, v in o.items() if v is not None}
+
+
+class PreparedQuantizeRows(PreparedCall):
+    """x ~ scale q, a row at a time (lsamp_quantize_rows): `q` in int8, `scale`
+    in float32."""
+
+    entry = "lsamp_quantize_rows"
+
+    def __init__(self, ctx, x, *, q=None):
+        super().__init__(ctx, x.device)
+        a = _ffi.QuantizeRowsArgs()
+        a.x, a.x_stride = self._matrix("x", x)
+        rows, n = x.shape
+        a.rows, a.cols, a.dtype = rows, n, DTYPES[x.dtype]
+        self.q = self._empty((rows, n), torch.int8) if q is None else q
+        a.q, a.q_stride = self._matrix("q", self.q, rows, n, torch.int8)
+        self.scale = self._empty(rows, torch.float32)
+        a.scale = self.scale.data_ptr()
+        self._bind(a)
+
+    def outputs(self) -> dict:
+        return {"q": self.q, "scale": self.scale}
+
+
+class PreparedLinearInt8(PreparedCall):
+    """out = act(x weight^T + bias) + residual with 8-bit operands
+    (lsamp_linear_int8).  `weight` and `weight_scale` are a quantize_rows'
+    outputs; so are x and `x_scale`, or x is left to the call to quantise.  A
+    quantised x takes the type of the block from bias, residual, out or
+    out_dtype."""
+
+    entry = "lsamp_linear_int8"
+
+    def __init__(self, ctx, x, weight, weight_scale, *, x_scale=None, bias=None, residual=None,
+                 activation="none", softcap=0.0, out_dtype=None, out=None):
+        super().__init__(ctx, x.device)
+        a = _ffi.LinearInt8Args()
+        rows, k = x.shape if x.dim() == 2 else (0, 0)
+        if x_scale is None:
+            a.x, a.x_stride = self._matrix("x", x)
+            dt = x.dtype
+        else:
+            a.x, a.x_stride = self._matrix("x", x, dtype=torch.int8)
+            a.x_scale = self._vector("x_scale", x_scale, rows, torch.float32)
+            typed = [t.dtype for t in (bias, residual) if t is not None]
+            if out_dtype is None and out is not None:
+                out_dtype = out.dtype
+            dt = typed[0] if typed else out_dtype or torch.bfloat16
+        a.weight, a.weight_stride = self._matrix("weight", weight, cols=k, dtype=torch.int8)
+        n = weight.shape[0]
+        a.weight_scale = self._vector("weight_scale", weight_scale, n, torch.float32)
+        a.rows, a.in_features, a.out_features = rows, k, n
+        if dt not in DTYPES:
+            raise ValueError(f"{dt} is not float32, bfloat16 or float16")
+        a.dtype = DTYPES[dt]
+        a.activation, a.softcap = _activation(activation), softcap
+        out_dtype = (out.dtype if out is not None else dt) if out_dtype is None else out_dtype
+        if out_dtype not in (dt, torch.float32):
+            raise ValueError(f"out_dtype must be {dt} or float32")
+        a.out_dtype = DTYPES[out_dtype]
+        if bias is not None:
+            a.bias = self._vector("bias", bias, n, dt)
+        if residual is not None:
+            a.residual, a.residual_stride = self._matrix("residual", residual, rows, n, dt)
+        self.out = self._empty((rows, n), out_dtype) if out is None else out
+        a.out, a.out_stride = self._matrix("out", self.out, rows, n, out_dtype)
+        self._bind(a)
+
+    def outputs(self) -> dict:
+        return {"out": self.out}
+
+
+# The quintic of the Newton-Schulz steps: its slope at 0 is as steep as it gets while
+# every singular value ends within (0.7, 1.2).
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+class PreparedOrthogonalize(PreparedCall):
+    """out = scale orth(x) + keep base (lsamp_orthogonalize) for a matrix or a
+    stack of them.  `coefficients`: (a, b, c), or one of these for each step.  An
+    optimiser's step has the weights as `base` and `out`."""
+
+    entry = "lsamp_orthogonalize"
+
+    def __init__(self, ctx, x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7, base=None,
+                 scale=1.0, keep=1.0, out_dtype=None, out=None):
+        super().__init__(ctx, x.device)
+        a = _ffi.OrthogonalizeArgs()
+        if x.dim() not in (2, 3) or 0 in x.shape:
+            raise ValueError(f"x must be a matrix or a stack of matrices, got {tuple(x.shape)}")
+        a.batch = x.shape[0] if x.dim() == 3 else 1
+        a.rows, a.cols = x.shape[-2:]
+        given = [t.dtype for t in (out, base) if t is not None]
+        out_dtype = (given[0] if given else x.dtype) if out_dtype is None else out_dtype
+        if x.dtype not in DTYPES or out_dtype not in DTYPES:
+            raise ValueError(f"{x.dtype} or {out_dtype} is not float32, bfloat16 or float16")
+        a.in_dtype, a.out_dtype = DTYPES[x.dtype], DTYPES[out_dtype]
+        rows = [coefficients] if not hasattr(coefficients[0], "__len__") else list(coefficients)
+        rows = rows * steps if len(rows) == 1 else rows
+        if len(rows) != steps or any(len(r) != 3 for r in rows):
+            raise ValueError(f"coefficients must be three numbers, or {steps} times three")
+        self.coefficients = (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+        a.steps = steps
+        a.coefficients = ctypes.cast(self.coefficients, ctypes.c_void_p)
+        a.eps, a.scale, a.keep = eps, scale, keep
+        a.x, a.x_stride, a.x_batch_stride = self._stack("x", x, x.shape, x.dtype)
+        if base is not None:
+            a.base, a.base_stride, a.base_batch_stride = self._stack("base", base, x.shape,
+                                                                     out_dtype)
+        self.out = self._empty(tuple(x.shape), out_dtype) if out is None else out
+        a.out, a.out_stride, a.out_batch_stride = self._stack("out", self.out, x.shape, out_dtype)
+        self._bind(a)
+
+    def _stack(self, name, t, shape, dtype):
+        if t.shape != shape:
+            raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        p, stride = self._matrix(name, t if t.dim() == 2 else t[0], dtype=dtype)
+        return p, stride, t.stride(0) if t.dim() == 3 else 0
 
     def outputs(self) -> dict:
         return {"out": self.out}
