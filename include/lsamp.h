@@ -900,9 +900,11 @@ lsamp_status lsamp_linear_int8(lsamp_context* ctx, const lsamp_linear_int8_args*
  * keep = 1 - rate * decay it is the optimiser's step.  Coefficients that would take
  * singular values of up to 1 past 8, or b t + c t^2 past 128 on their squares t, are refused.
  *
- * A float32 or float16 out is computed in float32; a bfloat16 out with products of
- * float16 operands, X in two parts: off by about 1e-3 of the result's norm before
- * its rounding (bfloat16's own is 1.7e-3).  A matrix with a NaN or an infinity, or
+ * The products take float16 operands with float32 sums.  For a bfloat16 out X is held
+ * in two parts, and the result is off by about 1e-3 of its norm before its rounding
+ * (bfloat16's own is 1.7e-3); for a float32 or float16 out all operands are in two
+ * parts, 22 bits: 3e-7 to 2e-6 of its norm in five steps.  (Elements of X below 2^-35
+ * are 0.)  A matrix with a NaN or an infinity, or
  * whose steps meet one, becomes NaN; the others of the batch do not change.
  * `out` may be `base` itself (same address, strides and type). */
 typedef struct lsamp_orthogonalize_args {

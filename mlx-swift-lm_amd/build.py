@@ -41,7 +41,7 @@ DEVICE = [
 ]
 # compiled once per element type (LSAMP_DT: float32 0, bfloat16 1, float16 2), in parallel
 SOURCES_HIP_DT = {"lsamp_kernels.hip": (0, 1, 2), "lsamp_head.hip": (0, 1, 2),
-                  "lsamp_int8.hip": (0, 1, 2), "lsamp_orth.hip": (0, 2)}
+                  "lsamp_int8.hip": (0, 1, 2), "lsamp_orth.hip": (2,)}
 SOURCES_HIP = ["lsamp_topk.hip", "lsamp_rank.hip", "lsamp_commit.hip",
                "lsamp_mask.hip", "lsamp_noalloc.hip", "lsamp_penalize.hip",
                "lsamp_head_passes.hip", "lsamp_dropout.hip", "lsamp_norm.hip"]

@@ -226,15 +226,29 @@ lsamp_status check_steps(const float* coefficients, int32_t steps) {
 }
 
 struct OrthPlan {
-  bool half, tall;
+  bool wide, tall;
   OrthStart start;
   Choice gram, poly, update;
   BatchPlan g_gram, g_poly, g_update;  // (of the first step: X is in the first buffer)
-  void* x[2][2];                       // [buffer][hi, lo]
+  void* x[2][2];                       // [buffer][part]
   EpiSymmetric e_gram, e_poly;
   EpiOrthUpdate e_update;
   int64_t bytes;
 };
+
+// The tile shape for `batch` products of m x n over `slabs` slabs, one round of the
+// device after the other (see choose).  192 x 192 tiles, 0.95 us a slab, are for symmetric
+// products that they spread over the device (4096: 253 tiles).
+Choice choose_batch(int64_t m, int64_t n, int64_t slabs, double bytes, int64_t batch, bool symmetric) {
+  Choice best = choose(m, n, slabs, LSAMP_DTYPE_F16, bytes, false, kChunked, batch, symmetric);
+  if (symmetric) {
+    const int64_t across = ceil_div(n, kTileSide[kTile192]);
+    const double rounds = (double)ceil_div(batch * (across * (across + 1) / 2), 256);
+    const double us = rounds * (0.95 * (double)slabs + 2.0 + 192.0 * 192.0 * bytes * 256.0 / 5e6);
+    if (us < best.us) best = Choice{kTile192, 1, us};
+  }
+  return best;
+}
 
 lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* out) {
   if (!a) return set_error(LSAMP_ERR_INVALID_ARGUMENT, "args is NULL");
@@ -266,18 +280,19 @@ lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* 
 
   OrthPlan P{};
   Arena ws(base);
-  P.half = a->out_dtype == LSAMP_DTYPE_BF16;
+  P.wide = a->out_dtype != LSAMP_DTYPE_BF16;
   P.tall = m > n;
-  const int dt = P.half ? LSAMP_DTYPE_F16 : LSAMP_DTYPE_F32, eb = P.half ? 2 : 4;
-  const int32_t p = std::min(m, n), q = std::max(m, n);
-  const int64_t ld_x = row_pitch(n, eb), ld_a = row_pitch(p, eb);
-  const int64_t step_x = (int64_t)m * ld_x, step_a = (int64_t)p * ld_a;
-  const int32_t wide_x = (int32_t)round_up(n, 8), wide_a = (int32_t)round_up(p, 8);
+  const int eb = 2;
+  const int32_t M = (int32_t)round_up(m, 64), N = (int32_t)round_up(n, 64);
+  const int32_t p = std::min(M, N), q = std::max(M, N);
+  const int64_t step_x = (int64_t)M * N, step_a = (int64_t)p * p;
 
   OrthStart& s = P.start;
   s.rows = m;
   s.cols = n;
-  s.parts = std::min(m, std::max(1, 1024 / batch));
+  s.all_rows = M;
+  while (s.log_x < 8 && (8 << s.log_x) < N) ++s.log_x;
+  s.parts = (int32_t)std::min<int64_t>(ceil_div(M, 256 >> s.log_x), std::max(1, 2048 / batch));
   s.eps = a->eps;
   s.x = a->x;
   s.ld_x = stride_of(a->x_stride, m, n);
@@ -285,60 +300,73 @@ lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* 
   s.part = ws.take<double>((int64_t)batch * s.parts * 8);
   s.left = ws.take<float>((int64_t)batch * 4);
   for (auto& buffer : P.x)
-    for (int i = 0; i < (P.half ? 2 : 1); ++i) buffer[i] = ws.take(batch * step_x * eb);
+    for (auto& part : buffer) part = ws.take(batch * step_x * eb);
   s.hi = P.x[0][0];
   s.lo = P.x[0][1];
-  s.ld = ld_x;
+  s.ld = N;
   s.step = step_x;
-  void* const gram = ws.take(batch * step_a * eb);
-  void* const poly = ws.take(batch * step_a * eb);
-  float* const diagonal = P.half ? ws.take<float>((int64_t)batch * ld_a * 4) : nullptr;
+  void *gram[2] = {}, *poly[2] = {};
+  for (int i = 0; i < (P.wide ? 2 : 1); ++i) {
+    gram[i] = ws.take(batch * step_a * eb);
+    poly[i] = ws.take(batch * step_a * eb);
+  }
+  float* const diagonal = ws.take<float>((int64_t)batch * p * 4);
 
-  P.gram = choose(p, p, slabs_of(q, eb), dt, eb, false, kChunked, batch, true);
-  P.poly = choose(p, p, slabs_of(p, eb), dt, 2 * eb, false, kChunked, batch, true);
-  P.update = choose(m, n, slabs_of(p, eb), dt, 4 * eb, false, kChunked, batch);
-  const MatrixRef x{P.x[0][0], ld_x, m, wide_x}, A{gram, ld_a, p, wide_a}, B{poly, ld_a, p, wide_a};
+  const int64_t turns = P.wide ? 3 : 1;  // (products of parts)
+  const double parts = P.wide ? 2.0 : 1.0;
+  P.gram = choose_batch(p, p, turns * slabs_of(q, eb), 2 * eb * parts, batch, true);
+  P.poly = choose_batch(p, p, turns * slabs_of(p, eb), 3 * eb * parts, batch, true);
+  P.update = choose_batch(M, N, turns * slabs_of(p, eb), 4 * eb, batch, false);
+  const MatrixRef x{P.x[0][0], N, M, N}, A{gram[0], p, p, p}, B{poly[0], p, p, p};
+  const int64_t rest_x = (char*)P.x[0][1] - (char*)P.x[0][0];
+  const auto rest = [&](void* const* two) { return (char*)two[1] - (char*)two[0]; };
   const auto batched = [&](const Choice& c, const MatrixRef& l, const MatrixRef& r, int64_t rows,
-                           int64_t cols, int64_t k, int64_t step_l, int64_t step_r, bool symmetric) {
+                           int64_t cols, int64_t k, int64_t step_l, int64_t step_r, int64_t rest_l,
+                           int64_t rest_r, bool symmetric) {
     BatchPlan g{};
     static_cast<GemmPlan&>(g) = plan_gemm(c, l, r, rows, cols, k, eb);
     g.parts = batch;
     g.step_a = step_l * eb;
     g.step_b = step_r * eb;
     g.symmetric = symmetric;
+    if (P.wide) {
+      g.rest_a = rest_l;
+      g.rest_b = rest_r;
+    }
     return g;
   };
-  P.g_gram = batched(P.gram, x, x, p, p, q, step_x, step_x, true);
-  P.g_poly = batched(P.poly, A, A, p, p, p, step_a, step_a, true);
-  P.g_update = P.tall ? batched(P.update, x, B, m, n, p, step_x, step_a, false)
-                      : batched(P.update, B, x, m, n, p, step_a, step_x, false);
+  P.g_gram = batched(P.gram, x, x, p, p, q, step_x, step_x, rest_x, rest_x, true);
+  P.g_poly = batched(P.poly, A, A, p, p, p, step_a, step_a, rest(gram), rest(gram), true);
+  P.g_update = P.tall ? batched(P.update, x, B, M, N, p, step_x, step_a, rest_x, rest(poly), false)
+                      : batched(P.update, B, x, M, N, p, step_a, step_x, rest(poly), rest_x, false);
   if (too_many(P.g_gram) || too_many(P.g_poly) || too_many(P.g_update))
     return set_error(LSAMP_ERR_SHAPE, "%d matrices %d x %d are too large for one call", batch, m, n);
 
   P.e_gram.n = P.e_poly.n = p;
-  P.e_gram.out = gram;
-  P.e_poly.in = gram;
-  P.e_poly.out = poly;
-  P.e_gram.ld = P.e_poly.ld = ld_a;
+  P.e_gram.out = gram[0];
+  P.e_gram.out_lo = gram[1];
+  P.e_poly.in = gram[0];
+  P.e_poly.in_lo = gram[1];
+  P.e_poly.out = poly[0];
+  P.e_poly.out_lo = poly[1];
   P.e_gram.step = P.e_poly.step = step_a;
   P.e_poly.diagonal = diagonal;
-  P.e_poly.step_d = ld_a;
   EpiOrthUpdate& e = P.e_update;
   e.m = m;
   e.n = n;
+  e.all_m = M;
   e.tall = P.tall;
   e.out_dtype = a->out_dtype;
   e.diagonal = diagonal;
-  e.step_d = ld_a;
-  e.ld = ld_x;
+  e.step_d = p;
+  e.ld = N;
   e.step = step_x;
   P.bytes = ws.used;
   *out = P;
   return LSAMP_OK;
 }
 
-#define ORTH_OP(half, call) \
-  ((half) ? OrthOps<LSAMP_DTYPE_F16>::call : OrthOps<LSAMP_DTYPE_F32>::call)
+#define ORTH_OP(wide, call) ((wide) ? OrthOps<true>::call : OrthOps<false>::call)
 
 }  // namespace
 
@@ -426,7 +454,7 @@ lsamp_status lsamp_orthogonalize(lsamp_context* ctx, const lsamp_orthogonalize_a
   LSAMP_CHECK(plan_orth(a, a ? a->workspace : nullptr, &P));
   LSAMP_CHECK(check_workspace(a->workspace, a->workspace_bytes, P.bytes));
   OnDevice guard(context_device(ctx));
-  LSAMP_TRY(ORTH_OP(P.half, start(P.start, a->batch, a->in_dtype, stream)));
+  LSAMP_TRY(launch_orth_start(P.start, a->batch, a->in_dtype, stream));
   const int ob = element_bytes(a->out_dtype);
   for (int i = 0; i < a->steps; ++i) {
     const float* const c = a->coefficients + 3 * i;
@@ -453,9 +481,9 @@ lsamp_status lsamp_orthogonalize(lsamp_context* ctx, const lsamp_orthogonalize_a
       e.scale = a->scale;
       e.keep = a->keep;
     }
-    LSAMP_TRY(ORTH_OP(P.half, gram(P.tall, P.gram.tile, P.g_gram, P.e_gram, stream)));
-    LSAMP_TRY(ORTH_OP(P.half, poly(P.poly.tile, P.g_poly, P.e_poly, stream)));
-    LSAMP_TRY(ORTH_OP(P.half, update(P.tall, P.update.tile, P.g_update, e, stream)));
+    LSAMP_TRY(ORTH_OP(P.wide, gram(P.tall, P.gram.tile, P.g_gram, P.e_gram, stream)));
+    LSAMP_TRY(ORTH_OP(P.wide, poly(P.poly.tile, P.g_poly, P.e_poly, stream)));
+    LSAMP_TRY(ORTH_OP(P.wide, update(P.tall, P.update.tile, P.g_update, e, stream)));
   }
   return clear_error();
 }

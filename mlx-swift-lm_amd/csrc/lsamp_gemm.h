@@ -222,6 +222,15 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
 }
 #pragma clang diagnostic pop
 
+// A pointer that is the same for the wave, in scalar registers also where the compiler
+// took it through vector ones.
+__device__ __forceinline__ const char* scalar(const char* p) {
+  const uint64_t v = (uint64_t)p;
+  const uint32_t low = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t high = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+  return (const char*)((uint64_t)high << 32 | low);
+}
+
 // 16 bytes from an address aligned to elements only.
 template <int DT>
 __device__ __forceinline__ v4i load_chunk(const char* p) {
@@ -449,8 +458,8 @@ __device__ __forceinline__ TileAt tile_at(int bid, const BatchPlan& g) {
   int n = (int)((__builtin_sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
   n += (n + 1) * (n + 2) / 2 <= i ? 1 : 0;  // (the root is off by less than one)
   n -= n * (n + 1) / 2 > i ? 1 : 0;
-  t.n = n;
-  t.m = i - n * (n + 1) / 2;
+  t.n = __builtin_amdgcn_readfirstlane(n);  // (a vector unit took the root)
+  t.m = i - t.n * (t.n + 1) / 2;
   return t;
 }
 
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
     g.a.p = (const char*)g.a.p + at.part * g.step_a;
     g.b.p = (const char*)g.b.p + at.part * g.step_b;
     slab0 = 0;
-    slabs = g.slabs;
+    slabs = g.rest_a ? 3 * g.slabs : g.slabs;
   } else {
     at = tile_at((int)blockIdx.x, g.tiles_m, g.tiles_n, g.parts);
     slab0 = at.part * g.slabs_per_part;
@@ -520,7 +529,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
       b.step *= GROUPS;
     }
   };
-  start();
+  if constexpr (!kBatch) start();
   // reduction steps of this part's last slab
   const int last_a = (AK ? g.a.rows : g.a.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
   const int last_b = (BK ? g.b.rows : g.b.cols) - (slab0 + slabs - 1) * kSlabOf<DT>;
@@ -533,6 +542,22 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
     for (int j = 0; j < FM; ++j) acc[i][j] = V{0, 0, 0, 0};
 
   const uint32_t lds0 = lds_address(lds);
+  // Batches: slab t of the reduction, which goes over the operands' parts in turn.
+  const char *base_a = nullptr, *base_b = nullptr;
+  if constexpr (kBatch) {
+    a.init(g.a, m0, 0, wave, lane);
+    b.init(g.b, n0, 0, wave, lane);
+    base_a = a.base;
+    base_b = b.base;
+  }
+  const auto seek = [&](int t) {
+    if constexpr (kBatch) {
+      const int turn = (t >= g.slabs) + (t >= 2 * g.slabs);
+      const int64_t at_slab = t - turn * g.slabs;
+      a.base = scalar(base_a + at_slab * a.step + (turn == 2 ? g.rest_a : 0));
+      b.base = scalar(base_b + at_slab * b.step + (turn == 1 ? g.rest_b : 0));
+    }
+  };
   const auto fetch_full = [&](int buffer) {
     if constexpr (!LOOSE) {
       const uint32_t dst = lds0 + buffer * kStage;
@@ -544,6 +569,9 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
     if constexpr (LOOSE) {
       a.hold(slab0 + slab, g.a.rows, wave, lane);
       b.hold(slab0 + slab, g.b.rows, wave, lane);
+    } else if constexpr (kBatch) {
+      seek(slab);
+      fetch_full(buffer);
     } else if (slab + 1 < slabs) {
       fetch_full(buffer);
     } else {
@@ -614,9 +642,12 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
     for (; t + 3 < slabs; ++t) {
       half(fa[1], fb[1], t & 1, 1, fa[0], fb[0], std::false_type{}, 0);
       settle();
+      seek(t + 2);
       half(fa[0], fb[0], (t + 1) & 1, 0, fa[1], fb[1], std::true_type{}, t & 1);
-      a.base += a.step;
-      b.base += b.step;
+      if constexpr (!kBatch) {
+        a.base += a.step;
+        b.base += b.step;
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     for (; t < slabs; ++t) {

@@ -26,18 +26,22 @@ struct GemmPlan {
   int32_t slabs, slabs_per_part;  // 128-byte slabs of the reduction
 };
 
-// `parts` equal products, one after another in memory.
+// `parts` equal products, one after another in memory, of operands in whole slabs.
 struct BatchPlan : GemmPlan {
   int64_t step_a, step_b;  // bytes
   int32_t symmetric;       // the result is: tiles left of the diagonal are left out
+  // Operands in two parts, `rest_*` bytes from a's and b's first to its second: the
+  // sums are those of first first + first second + second first.  Else 0.
+  int64_t rest_a, rest_b;
 };
 
 // Which operand is read along the reduction's rows (lsamp_gemm.h).
 enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
 // Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
 // slabs of the reduction at a time, for launches of at most a tile a CU; loose ones
-// for operands whose rows are no 16-byte chunks; and the products of at most
-// 16, 32 or 64 rows (lsamp_skinny.h), 64 or 16 columns a work-group.
+// for operands whose rows are no 16-byte chunks; the products of at most 16, 32 or 64
+// rows (lsamp_skinny.h), 64 or 16 columns a work-group; and 192 x 192 for symmetric
+// products.
 enum GemmTile {
   kTile256,
   kTile128,
@@ -49,9 +53,10 @@ enum GemmTile {
   kLoose64x4,
   kSkinny64,
   kSkinny16,
+  kTile192,
 };
-constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16};
-constexpr int kTileWavesM[] = {2, 2, 2, 2, 2, 2, 2, 2, 1, 1};  // waves that share a tile's rows
+constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16, 192};
+constexpr int kTileWavesM[] = {2, 2, 2, 2, 2, 2, 2, 2, 1, 1, 2};  // waves that share a tile's rows
 constexpr int kSkinnyRows = 64;
 
 // Epilogues.  `m`, `n`: rows and columns that exist.

@@ -7,9 +7,12 @@
 
 namespace lsamp {
 
-// Steps are in elements where they are of the workspace's matrices, else in bytes.
+// Matrices of the workspace are float16, in one part or two (lo: the rest); their rows
+// and columns are multiples of 64.  Steps are in elements there, else in bytes.
 struct OrthStart {
-  int32_t rows, cols, parts;  // work-groups of a matrix
+  int32_t rows, cols, all_rows;
+  int32_t parts;  // work-groups of a matrix
+  int32_t log_x;  // 2^log_x threads a row
   float eps;
   const void* x;
   int64_t ld_x, step_x;
@@ -20,17 +23,18 @@ struct OrthStart {
   int64_t ld, step;
 };
 struct EpiSymmetric {  // A, or B
-  int32_t n;
+  int32_t n;           // rows, columns and their distance
+  float b3, c3;
   const float* left;  // of the first step's A, else NULL
   const void* in;     // B: A
+  const void* in_lo;
   void* out;
-  int64_t ld, step;
-  float b3, c3;
-  float* diagonal;  // [batch][step_d] B's, where it is kept apart
-  int64_t step_d;
+  void* out_lo;
+  int64_t step;
+  float* diagonal;  // [batch][n] B's
 };
 struct EpiOrthUpdate {
-  int32_t m, n;
+  int32_t m, n, all_m;
   int32_t tall;
   int32_t out_dtype;
   float a1;
@@ -49,11 +53,12 @@ struct EpiOrthUpdate {
   float scale, keep;
 };
 
-// LSAMP_DTYPE_F32 or LSAMP_DTYPE_F16: what the products are taken in.  Tiles: 128 and
-// 64, alone or grouped; 256 for float16.
-template <int DT>
+int launch_orth_start(const OrthStart& p, int batch, int in_dtype, void* stream);
+
+// WIDE: A and B in two parts.  Tiles: 256, 128 and 64, the latter grouped too; 192 for
+// gram and poly.
+template <bool WIDE>
 struct OrthOps {
-  static int start(const OrthStart& p, int batch, int in_dtype, void* stream);
   static int gram(bool tall, GemmTile tile, const BatchPlan& g, const EpiSymmetric& e, void* stream);
   static int poly(GemmTile tile, const BatchPlan& g, const EpiSymmetric& e, void* stream);
   static int update(bool tall, GemmTile tile, const BatchPlan& g, const EpiOrthUpdate& e,

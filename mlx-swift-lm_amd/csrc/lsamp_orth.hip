@@ -4,25 +4,27 @@
 //
 // for a wide or square matrix (rows <= columns), X X^T the smaller Gram matrix; for
 // a tall one A = X^T X and X <- a X + X B.  An odd polynomial of the singular
-// values, a step at a time, without taking the matrix apart.  Compiled once per
-// type that the products are taken in (LSAMP_DT):
+// values, a step at a time, without taking the matrix apart.
 //
-// float32: X, A and B are float32, the products those of lsamp_gemm.h (24 bits).
+// The products are float16's, at the full rate of the matrix instructions.  What a
+// rounding of X does grows with the polynomial's slope at 0 in every step (485 times in
+// five of Muon's), and near-singular momenta are the rule: X in float16 alone leaves
+// 1e-2 of such a result's norm, in bfloat16 1e-1.  So X has two float16 parts, x = hi +
+// lo, 22 bits: the products take hi, the linear term a X both.  Then B's rounding is
+// the largest; its diagonal (about -2.7 once the singular values are near 1, against
+// an off-diagonal part of 0.3) is kept apart in float32 and joins the linear term.
+// What is left is 4e-4 to 1.1e-3 of the result's norm in five steps, below
+// bfloat16's own 1.7e-3.
 //
-// float16 (for bfloat16 results): the products are float16's, at the full rate.  What
-// a rounding of X does grows with the polynomial's slope at 0 in every step (485
-// times in five of Muon's), and near-singular momenta are the rule: X alone in
-// float16 leaves 1e-2 of such a result's norm, in bfloat16 1e-1.  So X has two
-// float16 parts, x = hi + lo: the products take hi, the linear term a X both.  Then B's
-// rounding is the largest; its diagonal (about -2.7 once the singular values are
-// near 1, against an off-diagonal part of 0.3) is kept apart in float32 and joins the
-// linear term.  What is left is 4e-4 to 1.1e-3 of the result's norm in five steps,
-// below bfloat16's own 1.7e-3.  X is held times 2^10, A and B times 2^8, so that
-// small elements stay normal numbers and the largest (singular values up to 8,
-// |B| up to 128: the entry point checks the polynomials) stay finite.
+// WIDE (float32 and float16 results): A and B have two parts too, and a product is
+// three, hi hi + hi lo + lo hi, one after the other into the same float32 sums: 3e-7 to 2e-6
+// in five steps, float32's own steps 2e-7 to 1.3e-6.
 //
-// Of A and A A, which are symmetric, only the tiles at and right of the diagonal
-// are computed, and stored on both sides.
+// X is held times 2^10, A and B times 2^8, so that small elements stay normal numbers
+// and the largest (singular values up to 8, |B| up to 128: the entry point checks the
+// polynomials) stay finite.  All matrices are held with zeros up to multiples of 64
+// rows and columns, which the products keep.  Of A and A A, which are symmetric, only
+// the tiles at and right of the diagonal are computed, and stored on both sides.
 #include <hip/hip_runtime.h>
 
 #include "lsamp_epilogue.h"
@@ -33,15 +35,39 @@ namespace lsamp {
 namespace gemm {
 namespace {
 
-constexpr bool kHalf = DT == LSAMP_DTYPE_F16;
-constexpr float kOfX = kHalf ? 1024.f : 1.f;  // what X, and what A and B are held times
-constexpr float kOfA = kHalf ? 256.f : 1.f;
+static_assert(DT == LSAMP_DTYPE_F16, "the products' type");
+constexpr float kOfX = 1024.f, kOfA = 256.f;
 constexpr int kThreads = 256;
+typedef _Float16 v8e __attribute__((ext_vector_type(8)));
 
 // ----------------------------------------------------------------- the start
+// Eight elements of a row, `valid` of them in it.
 template <int IN>
-__device__ __forceinline__ float element(const void* p, int64_t i) {
-  return (float)((const typename El<IN>::S*)p)[i];
+__device__ __forceinline__ void load8(float (&v)[8], const char* row, int c, int valid) {
+  using T = typename El<IN>::S;
+  constexpr int N = kChunkOf<IN>;
+  if (valid >= 8) {
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+      const v4i q = load_chunk<IN>(row + (int64_t)(c + i * N) * El<IN>::kBytes);
+      T e[N];
+      __builtin_memcpy(e, &q, 16);
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[i * N + k] = (float)e[k];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < valid ? (float)((const T*)row)[c + k] : 0.f;
+  }
+}
+__device__ __forceinline__ double block_sum(double s, double* red) {
+  for (int d = 32; d > 0; d /= 2) s += __shfl_xor(s, d);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+  __syncthreads();
+  s = red[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / kWave; ++w) s += red[w];
+  return s;
 }
 
 // Sums of squares in 64 bits, which neither overflow nor underflow: a work-group's
@@ -51,19 +77,18 @@ __global__ __launch_bounds__(kThreads) void k_norm2(OrthStart p) {
   __shared__ double red[kThreads / kWave];
   const int matrix = (int)blockIdx.y;
   const char* const x = (const char*)p.x + (int64_t)matrix * p.step_x;
+  const int lane = (int)threadIdx.x & ((1 << p.log_x) - 1), per = kThreads >> p.log_x;
   double s = 0.0;
-  for (int r = (int)blockIdx.x; r < p.rows; r += (int)gridDim.x)
-    for (int c = (int)threadIdx.x; c < p.cols; c += kThreads) {
-      const double v = (double)element<IN>(x, (int64_t)r * p.ld_x + c);
-      s += v * v;
+  for (int r = (int)blockIdx.x * per + ((int)threadIdx.x >> p.log_x); r < p.rows;
+       r += (int)gridDim.x * per)
+    for (int c = lane * 8; c < p.cols; c += 8 << p.log_x) {
+      float v[8];
+      load8<IN>(v, x + (int64_t)r * p.ld_x * El<IN>::kBytes, c, p.cols - c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fma((double)v[k], (double)v[k], s);
     }
-  for (int d = 32; d > 0; d /= 2) s += __shfl_xor(s, d);
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / kWave; ++w) s += red[w];
-    p.part[(int64_t)matrix * p.parts + blockIdx.x] = s;
-  }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) p.part[(int64_t)matrix * p.parts + blockIdx.x] = s;
 }
 
 // X0 = G 2^-e with 2^e <= |G|_F + eps < 2^(e + 1): no rounding of 16-bit values, and
@@ -75,96 +100,121 @@ __global__ __launch_bounds__(kThreads) void k_start(OrthStart p) {
   double s = 0.0;
   for (int i = (int)threadIdx.x; i < p.parts; i += kThreads)
     s += p.part[(int64_t)matrix * p.parts + i];
-  for (int d = 32; d > 0; d /= 2) s += __shfl_xor(s, d);
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
-  __syncthreads();
-  s = red[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / kWave; ++w) s += red[w];
-  const double norm = sqrt(s) + (double)p.eps;
+  const double norm = sqrt(block_sum(s, red)) + (double)p.eps;
   const bool finite = norm < INFINITY;
   const int e = finite ? ilogb(norm) : 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.left[matrix] = finite ? (float)(ldexp(1.0, e) / norm) : NAN;
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    p.left[matrix] = finite ? (float)(ldexp(1.0, e) / norm) : NAN;
   const char* const x = (const char*)p.x + (int64_t)matrix * p.step_x;
-  const double scale = ldexp((double)kOfX, -e);
+  // (in two factors: the scale of a tiny matrix is beyond float32)
+  const float scale = ldexpf(kOfX, -e / 2), scale2 = ldexpf(1.f, -(e - e / 2));
   S* const hi = (S*)p.hi + (int64_t)matrix * p.step;
-  S* const lo = kHalf ? (S*)p.lo + (int64_t)matrix * p.step : nullptr;
-  const int wide = (p.cols + 7) / 8 * 8;
-  for (int r = (int)blockIdx.x; r < p.rows; r += (int)gridDim.x)
-    for (int c = (int)threadIdx.x; c < wide; c += kThreads) {
-      // (a product of doubles: the scale of a tiny matrix is beyond float32)
-      const float v =
-          c < p.cols ? (float)((double)element<IN>(x, (int64_t)r * p.ld_x + c) * scale) : 0.f;
-      const S h = (S)v;
-      hi[(int64_t)r * p.ld + c] = h;
-      if constexpr (kHalf) lo[(int64_t)r * p.ld + c] = (S)(v - (float)h);
+  S* const lo = (S*)p.lo + (int64_t)matrix * p.step;
+  const int lane = (int)threadIdx.x & ((1 << p.log_x) - 1), per = kThreads >> p.log_x;
+  for (int r = (int)blockIdx.x * per + ((int)threadIdx.x >> p.log_x); r < p.all_rows;
+       r += (int)gridDim.x * per)
+    for (int c = lane * 8; c < p.ld; c += 8 << p.log_x) {
+      float v[8];
+      load8<IN>(v, x + (int64_t)r * p.ld_x * El<IN>::kBytes, c, r < p.rows ? p.cols - c : 0);
+      v8e h, l;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = v[k] * scale * scale2;
+        h[k] = (S)f;
+        l[k] = (S)(f - (float)h[k]);
+      }
+      *(v8e*)(hi + (int64_t)r * p.ld + c) = h;
+      *(v8e*)(lo + (int64_t)r * p.ld + c) = l;
     }
 }
 
 // ----------------------------------------------------------------- epilogues
-// Sums and the same tile's mirror image: what is stored at (r, c) is stored at
-// (c, r) too, unless the tile lies on the diagonal.  `value(r, c, sums)` gives four
-// columns' results, zero past the last.
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+// Four columns of a row a lane -> four rows of a column, among four lanes whose rows
+// follow one another: two exchanges of a 32-bit word.
+__device__ __forceinline__ v4e turned(v4e in, int lane) {
+  const v2u w = __builtin_bit_cast(v2u, in);
+  const bool high = lane & 2, odd = lane & 1;
+  // the columns 0, 1 (high: 2, 3) of the rows l & 1 and (l & 1) + 2
+  const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(high ? w[0] : w[1]), 0x4E, 0xf, 0xf, false);
+  const uint32_t r0 = high ? got : w[0], r2 = high ? w[1] : got;
+  const uint32_t lower = (r0 & 0xffffu) | (r2 << 16), upper = (r0 >> 16) | (r2 & 0xffff0000u);
+  const uint32_t rest = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? lower : upper), 0xB1, 0xf, 0xf, false);
+  const uint32_t mine = odd ? upper : lower;
+  // rows 0 .. 3: an even lane has 0 and 2, an odd one 1 and 3
+  const uint32_t a = odd ? rest : mine, b = odd ? mine : rest;
+  v2u o;
+  o[0] = (a & 0xffffu) | (b << 16);
+  o[1] = (a >> 16) | (b & 0xffff0000u);
+  return __builtin_bit_cast(v4e, o);
+}
+
+// A tile and its mirror image: what is stored at (r, c) is stored at (c, r) too,
+// unless the tile lies on the diagonal.  `value(r, c, sums)` gives four columns' results.
+template <bool WIDE>
 struct Symmetric : EpiSymmetric {
   static constexpr int kBarriers = 0;
   template <int FM, int FN, int BM, int BN, int WM, int WN, class F>
-  __device__ __forceinline__ void store(v4f (&acc)[FN][FM], S* to, int m0, int n0, TileAt at, int wm,
-                                        int wn, int lane, F value) const {
-    const int r0 = m0 + wm * (FM * 16) + (lane & 15);
-    const int c0 = n0 + wn * (FN * 16) + (lane >> 4) * 4;
-    const int wide = (n + 7) / 8 * 8;
+  __device__ __forceinline__ void store(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
+                                        int lane, F value) const {
+    S* const to = (S*)out + at.part * step;
+    S* const rest = WIDE ? (S*)out_lo + at.part * step : nullptr;
+    const int r0 = m0 + wm * (FM * 16), c0 = n0 + wn * (FN * 16);
+    const int row = lane & 15, quad = (lane >> 4) * 4;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      const int r = r0 + j * 16;
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        const int c = c0 + i * 16;
-        if (r >= n || c >= wide) continue;
-        const v4f v = value(r, c, acc[i][j]);
-        v4e e;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = c + k < n ? (S)v[k] : (S)0.f;
-        *(v4e*)(to + (int64_t)r * ld + c) = e;
-        if (at.m != at.n) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (c + k < n) to[(int64_t)(c + k) * ld + r] = e[k];
+        const int rb = r0 + j * 16, cb = c0 + i * 16;  // (the same for the wave; n is a multiple of 64)
+        if (rb >= n || cb >= n) continue;
+        const v4f v = value(rb + row, cb + quad, acc[i][j]);
+        const v4e e = __builtin_convertvector(v, v4e);
+        const int64_t here = (int64_t)(rb + row) * n + cb + quad;
+        const int64_t there = (int64_t)(cb + quad + (lane & 3)) * n + rb + (row & 12);
+        *(v4e*)(to + here) = e;
+        if (at.m != at.n) *(v4e*)(to + there) = turned(e, lane);
+        if constexpr (WIDE) {
+          const v4e l = __builtin_convertvector(v - __builtin_convertvector(e, v4f), v4e);
+          *(v4e*)(rest + here) = l;
+          if (at.m != at.n) *(v4e*)(rest + there) = turned(l, lane);
         }
       }
     }
   }
 };
 
-struct Gram : Symmetric {
+template <bool WIDE>
+struct Gram : Symmetric<WIDE> {
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char*) const {
-    const float s = left ? left[at.part] : 1.f;
+    const float s = this->left ? this->left[at.part] : 1.f;
     const float f = s * s * (kOfA / (kOfX * kOfX));
-    store<FM, FN, BM, BN, WM, WN>(acc, (S*)out + at.part * step, m0, n0, at, wm, wn, lane,
-                                  [&](int, int, v4f v) { return v * f; });
+    this->template store<FM, FN, BM, BN, WM, WN>(acc, m0, n0, at, wm, wn, lane,
+                                                 [&](int, int, v4f v) { return v * f; });
   }
 };
 
-struct Poly : Symmetric {
+template <bool WIDE>
+struct Poly : Symmetric<WIDE> {
   template <int FM, int FN, int BM, int BN, int WM, int WN>
   __device__ __forceinline__ void run(v4f (&acc)[FN][FM], int m0, int n0, TileAt at, int wm, int wn,
                                       int lane, char*) const {
-    const S* const g = (const S*)in + at.part * step;
-    float* const d = kHalf ? diagonal + at.part * step_d : nullptr;
-    const float fc = c3 / kOfA;
-    store<FM, FN, BM, BN, WM, WN>(
-        acc, (S*)out + at.part * step, m0, n0, at, wm, wn, lane, [&](int r, int c, v4f v) {
-          const v4e a = *(const v4e*)(g + (int64_t)r * ld + c);  // (whole quads of a row)
+    const int n = this->n;
+    const S* const g = (const S*)this->in + at.part * this->step;
+    const S* const gl = WIDE ? (const S*)this->in_lo + at.part * this->step : nullptr;
+    float* const d = this->diagonal + (int64_t)at.part * n;
+    const float b = this->b3, c3 = this->c3 * (1.f / kOfA);
+    this->template store<FM, FN, BM, BN, WM, WN>(
+        acc, m0, n0, at, wm, wn, lane, [&](int r, int c, v4f v) {
+          v4f a = __builtin_convertvector(*(const v4e*)(g + (int64_t)r * n + c), v4f);
+          if constexpr (WIDE) a += __builtin_convertvector(*(const v4e*)(gl + (int64_t)r * n + c), v4f);
+          v = b * a + c3 * v;
+          const int k = r - c;
+          if ((unsigned)k < 4u) {
+            d[r] = (k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3]) * (1.f / kOfA);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = b3 * (float)a[k] + fc * v[k];
-          if constexpr (kHalf) {
-            const int k = r - c;
-            if ((unsigned)k < 4u) {
-              d[r] = (k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3]) * (1.f / kOfA);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) v[q] = q == k ? 0.f : v[q];
-            }
+            for (int q = 0; q < 4; ++q) v[q] = q == k ? 0.f : v[q];
           }
           return v;
         });
@@ -172,6 +222,7 @@ struct Poly : Symmetric {
 };
 
 // X' = (a + diagonal) X + sums, as the next X or, at the last step, the result.
+template <bool WIDE>
 struct Update : EpiOrthUpdate {
   static constexpr int kBarriers = 0;
   template <int FM, int FN, int BM, int BN, int WM, int WN>
@@ -180,13 +231,13 @@ struct Update : EpiOrthUpdate {
     const Along<FN> along(lane);
     char* const mine = lds + (wn * WM + wm) * (FN * 1024);
     const int r0 = m0 + wm * (FM * 16) + along.row, c = n0 + wn * (FN * 16) + along.col;
-    const int wide = (n + 7) / 8 * 8, valid = n - c;
+    if (c >= ld) return;  // (ld: a multiple of 64, as every wave's columns)
     const float s = left ? left[at.part] : 1.f;
     const S* const hi = (const S*)x_hi + at.part * step;
-    const S* const lo = kHalf ? (const S*)x_lo + at.part * step : nullptr;
-    const float* const d = kHalf ? diagonal + at.part * step_d : nullptr;
+    const S* const lo = (const S*)x_lo + at.part * step;
+    const float* const d = diagonal + at.part * step_d;
     v4f by_col = {a1, a1, a1, a1};
-    if (kHalf && tall && c < n) by_col += load4f(d + c, valid);
+    if (tall) by_col += *(const v4f*)(d + c);
 #pragma unroll 1
     for (int j = 0; j < FM; ++j) {
       v4f v[FN];
@@ -200,27 +251,19 @@ struct Update : EpiOrthUpdate {
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int r = r0 + j * 16 + i * along.kRows;
-        if (r >= m || c >= wide) continue;
-        const v4e h = *(const v4e*)(hi + (int64_t)r * ld + c);
-        v4f x = __builtin_convertvector(h, v4f);
-        v4f f = by_col;
-        if constexpr (kHalf) {
-          x += __builtin_convertvector(*(const v4e*)(lo + (int64_t)r * ld + c), v4f);
-          if (!tall) f += d[r];
-        }
-        v4f y = (x * f + v[i] * (1.f / kOfA)) * s;
+        if (r >= all_m) continue;
+        const int64_t here = (int64_t)r * ld + c;
+        const v4f x = __builtin_convertvector(*(const v4e*)(hi + here), v4f) +
+                      __builtin_convertvector(*(const v4e*)(lo + here), v4f);
+        const v4f f = tall ? by_col : by_col + d[r];
+        const v4f y = (x * f + v[i] * (1.f / kOfA)) * s;
         if (!out) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = k < valid ? y[k] : 0.f;
           const v4e top = __builtin_convertvector(y, v4e);
-          *(v4e*)((S*)to_hi + at.part * step + (int64_t)r * ld + c) = top;
-          if constexpr (kHalf) {
-            const v4f rest = y - __builtin_convertvector(top, v4f);
-            *(v4e*)((S*)to_lo + at.part * step + (int64_t)r * ld + c) =
-                __builtin_convertvector(rest, v4e);
-          }
-        } else if (valid > 0) {
-          finish(at.part, r, c, y * (scale / kOfX), valid);
+          *(v4e*)((S*)to_hi + at.part * step + here) = top;
+          *(v4e*)((S*)to_lo + at.part * step + here) =
+              __builtin_convertvector(y - __builtin_convertvector(top, v4f), v4e);
+        } else if (r < m && c < n) {
+          finish(at.part, r, c, y * (scale / kOfX), n - c);
         }
       }
     }
@@ -243,7 +286,7 @@ struct Update : EpiOrthUpdate {
     }
   }
   __device__ __forceinline__ void finish(int64_t matrix, int r, int c, v4f v, int valid) const {
-    if constexpr (kHalf)
+    if constexpr (!WIDE)
       finish_as<__bf16>(matrix, r, c, v, valid);
     else if (out_dtype == LSAMP_DTYPE_F32)
       finish_as<float>(matrix, r, c, v, valid);
@@ -270,16 +313,17 @@ int launch(GemmTile tile, const BatchPlan& g, const E& e, void* stream) {
   const dim3 grid((unsigned)(tiles * g.parts));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (tile) {
-    case kTile256:
-      if constexpr (kHalf) {
-        LSAMP_TILE(512, 256, 256, 2, 4, 0, 1, false);
-        break;
-      }
-      return (int)hipErrorInvalidValue;
+    case kTile256: LSAMP_TILE(512, 256, 256, 2, 4, 0, 1, false); break;
     case kTile128: LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, false); break;
     case kTile64: LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, false); break;
     case kTile128x2: LSAMP_TILE(512, 128, 128, 2, 2, 2, 2, false); break;
     case kTile64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, false); break;
+    case kTile192:
+      if constexpr (std::is_base_of_v<EpiSymmetric, E>) {
+        LSAMP_TILE(512, 192, 192, 2, 4, 0, 1, false);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
     default: return (int)hipErrorInvalidValue;
   }
   return (int)hipGetLastError();
@@ -290,8 +334,7 @@ int launch(GemmTile tile, const BatchPlan& g, const E& e, void* stream) {
 
 using namespace gemm;
 
-template <>
-int OrthOps<DT>::start(const OrthStart& p, int batch, int in_dtype, void* stream) {
+int launch_orth_start(const OrthStart& p, int batch, int in_dtype, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)p.parts, (unsigned)batch);
 #define LSAMP_START(IN)                                                     \
@@ -304,19 +347,22 @@ int OrthOps<DT>::start(const OrthStart& p, int batch, int in_dtype, void* stream
   }
   return (int)hipGetLastError();
 }
-template <>
-int OrthOps<DT>::gram(bool tall, GemmTile t, const BatchPlan& g, const EpiSymmetric& p, void* st) {
-  const Gram e = with<Gram>(p);
+template <bool WIDE>
+int OrthOps<WIDE>::gram(bool tall, GemmTile t, const BatchPlan& g, const EpiSymmetric& p, void* st) {
+  const Gram<WIDE> e = with<Gram<WIDE>>(p);
   return tall ? launch<true, true>(t, g, e, st) : launch<false, false>(t, g, e, st);
 }
-template <>
-int OrthOps<DT>::poly(GemmTile t, const BatchPlan& g, const EpiSymmetric& p, void* st) {
-  return launch<false, false>(t, g, with<Poly>(p), st);
+template <bool WIDE>
+int OrthOps<WIDE>::poly(GemmTile t, const BatchPlan& g, const EpiSymmetric& p, void* st) {
+  return launch<false, false>(t, g, with<Poly<WIDE>>(p), st);
 }
-template <>
-int OrthOps<DT>::update(bool tall, GemmTile t, const BatchPlan& g, const EpiOrthUpdate& p, void* st) {
-  const Update e = with<Update>(p);
+template <bool WIDE>
+int OrthOps<WIDE>::update(bool tall, GemmTile t, const BatchPlan& g, const EpiOrthUpdate& p,
+                          void* st) {
+  const Update<WIDE> e = with<Update<WIDE>>(p);
   return tall ? launch<false, false>(t, g, e, st) : launch<false, true>(t, g, e, st);
 }
+template struct OrthOps<false>;
+template struct OrthOps<true>;
 
 }  // namespace lsamp

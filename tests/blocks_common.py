@@ -125,7 +125,8 @@ def _two_parts(t, scale):
 def orth64(x, steps, coefficients, eps, arithmetic="exact"):
     """One matrix.  "exact": in 64 bits.  "f16": with the roundings that a bfloat16 result's
     steps make (X in two float16 parts of which products take the first, A and B in
-    float16, B's diagonal apart; sums in 64 bits).  "f32": X, A and B rounded to float32."""
+    float16, B's diagonal apart; sums in 64 bits).  "two": with those of float32 and float16
+    results (X, A and B in two float16 parts, whose last products are left out)."""
     G = d64(x)
     tall = G.shape[0] > G.shape[1]
     if tall:
@@ -134,7 +135,10 @@ def orth64(x, steps, coefficients, eps, arithmetic="exact"):
     rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
     X, s = G, 1 / norm
     f16 = lambda t: (t * 256).half().double() / 256  # noqa: E731
-    f32 = lambda t: t.float().double()  # noqa: E731
+
+    def times(l, r):  # of two parts each
+        return l[0] @ (r[0] + r[1]) + l[1] @ r[0]
+
     for i, (a, b, c) in enumerate(rows):
         a, b, c = (float(np.float32(v)) for v in (a, b, c))
         if arithmetic == "f16":
@@ -151,10 +155,14 @@ def orth64(x, steps, coefficients, eps, arithmetic="exact"):
             X = s * (a * (h + lo) + diag @ (h + lo) + f16(B - diag) @ h)
         else:
             X = X * s if i == 0 else X
-            if arithmetic == "f32":
-                X = f32(X)
-                A = f32(X @ X.t())
-                X = a * X + f32(b * A + c * (A @ A)) @ X
+            if arithmetic == "two":
+                x2 = _two_parts(X, 1024)
+                A = times(x2, [v.t() for v in x2])
+                a2 = _two_parts(A, 256)
+                B = b * (a2[0] + a2[1]) + c * times(a2, a2)
+                diag = torch.diag(B.diagonal())
+                X = sum(x2)
+                X = a * X + diag @ X + times(_two_parts(B - diag, 256), x2)
             else:
                 A = X @ X.t()
                 X = a * X + (b * A + c * (A @ A)) @ X
@@ -169,15 +177,17 @@ def orth_strict(x, steps, coefficients, eps, half):
       A: X's first parts (half: u = 2^-11), a sum of K products, A's rounding;
       B: what A's error makes of b A + c A A, its own sum, its rounding;
       X: B's error, the product with X's first part, its sum, the rounding of the result
-    (half: A and B round by 2^-11, X with its second part by 2^-22; all have an absolute
-    floor, half of float16's last step)."""
+    (half: A and B round by 2^-11, X with its second part by 2^-22; not half: two parts, 2^-22,
+    and products without that of the second ones, 2^-22 each of both operands.  All have an
+    absolute floor, half of float16's last step, 2^-25, over the 2^8 or more that they are
+    held times: 2^-33 an element)."""
     G = d64(x)
     if G.shape[0] > G.shape[1]:
         G = G.t()
     p, q = G.shape
     X = G / (float(G.norm()) + float(np.float32(eps)))
-    u, ux, ust = (2.0 ** -11, 2.0 ** -11, 2.0 ** -22) if half else (E, 0.0, E)
-    floor = 2.0 ** -33 if half else 0.0
+    u, ux, ust = (2.0 ** -11, 2.0 ** -11, 2.0 ** -22) if half else (2.0 ** -22,) * 3
+    floor = 2.0 ** -33
     e = 4 * E * float(X.norm()) + (floor * np.sqrt(p * q))
     rows = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
     for a, b, c in rows:
@@ -203,8 +213,8 @@ def check_orth(got, x, steps, coefficients, eps, base=None, scale=1.0, keep=1.0,
     from tight, so from 32 x 32 on (more than a thousand roundings of A and of B, whose norm is
     then near its mean) also twice what the emulated arithmetic is off by: the kernel's
     roundings are the same ones, but fall elsewhere where a float32 sum decides them (K
-    roundings of random sign, sqrt(K) E of its terms: in float32 the sums' share, sqrt(K)
-    times a rounding's).  The result's own rounding, and those of scale and keep, come on top."""
+    roundings of random sign, sqrt(K) E of its terms: beside parts that round by 2^-22 = 4 E
+    the sums' share is sqrt(K) / 4).  The result's own rounding, and those of scale and keep, come on top."""
     dt = got.dtype
     half = dt == torch.bfloat16
     xs, gs = (x[None], got[None]) if x.dim() == 2 else (x, got)
@@ -213,9 +223,9 @@ def check_orth(got, x, steps, coefficients, eps, base=None, scale=1.0, keep=1.0,
         want = orth64(xs[i], steps, coefficients, eps)
         bound = orth_strict(xs[i], steps, coefficients, eps, half)
         if min(want.shape) >= 32:
-            model = orth64(xs[i], steps, coefficients, eps, "f16" if half else "f32")
+            model = orth64(xs[i], steps, coefficients, eps, "f16" if half else "two")
             off = float((model - want).norm())
-            bound = min(bound, off * (2.0 if half else 2.0 + np.sqrt(max(want.shape))))
+            bound = min(bound, off * (2.0 if half else 2.0 + np.sqrt(max(want.shape)) / 4))
         kept = keep * d64(bs[i]) if bs is not None else torch.zeros_like(want)
         y = scale * want + kept
         bound = (abs(scale) * bound + U[dt] * (float(y.norm()) + abs(scale) * bound)
