@@ -161,13 +161,20 @@ struct Symmetric : EpiSymmetric {
     S* const rest = WIDE ? (S*)out_lo + at.part * step : nullptr;
     const int r0 = m0 + wm * (FM * 16), c0 = n0 + wn * (FN * 16);
     const int row = lane & 15, quad = (lane >> 4) * 4;
+    // (all values before the first store, which the compiler moves no load past)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+        if (r0 + j * 16 < n && c0 + i * 16 < n)  // (the same for the wave; n is a multiple of 64)
+          acc[i][j] = value(r0 + j * 16 + row, c0 + i * 16 + quad, acc[i][j]);
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
-        const int rb = r0 + j * 16, cb = c0 + i * 16;  // (the same for the wave; n is a multiple of 64)
+        const int rb = r0 + j * 16, cb = c0 + i * 16;
         if (rb >= n || cb >= n) continue;
-        const v4f v = value(rb + row, cb + quad, acc[i][j]);
+        const v4f v = acc[i][j];
         const v4e e = __builtin_convertvector(v, v4e);
         const int64_t here = (int64_t)(rb + row) * n + cb + quad;
         const int64_t there = (int64_t)(cb + quad + (lane & 3)) * n + rb + (row & 12);
@@ -238,24 +245,43 @@ struct Update : EpiOrthUpdate {
     const float* const d = diagonal + at.part * step_d;
     v4f by_col = {a1, a1, a1, a1};
     if (tall) by_col += *(const v4f*)(d + c);
+    // (the next rows' X on its way while these are stored: the compiler does not move
+    // loads past stores that may be to their memory)
+    v4e nh[FN], nl[FN];
+    float nd[FN];
+    const auto fetch = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const int r = min(r0 + j * 16 + i * along.kRows, all_m - 1);
+        nh[i] = *(const v4e*)(hi + (int64_t)r * ld + c);
+        nl[i] = *(const v4e*)(lo + (int64_t)r * ld + c);
+        nd[i] = tall ? 0.f : d[r];
+      }
+    };
+    fetch(0);
 #pragma unroll 1
     for (int j = 0; j < FM; ++j) {
       v4f v[FN];
+      v4e h[FN], l[FN];
+      float dr[FN];
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         v[i] = acc[i][0];
 #pragma unroll
         for (int k = 0; k + 1 < FM; ++k) acc[i][k] = acc[i][k + 1];
+        h[i] = nh[i];
+        l[i] = nl[i];
+        dr[i] = nd[i];
       }
+      if (j + 1 < FM) fetch(j + 1);
       exchange<FN>(v, mine, lane);
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
         const int r = r0 + j * 16 + i * along.kRows;
         if (r >= all_m) continue;
         const int64_t here = (int64_t)r * ld + c;
-        const v4f x = __builtin_convertvector(*(const v4e*)(hi + here), v4f) +
-                      __builtin_convertvector(*(const v4e*)(lo + here), v4f);
-        const v4f f = tall ? by_col : by_col + d[r];
+        const v4f x = __builtin_convertvector(h[i], v4f) + __builtin_convertvector(l[i], v4f);
+        const v4f f = by_col + dr[i];
         const v4f y = (x * f + v[i] * (1.f / kOfA)) * s;
         if (!out) {
           const v4e top = __builtin_convertvector(y, v4e);
