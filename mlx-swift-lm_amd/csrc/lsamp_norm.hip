@@ -27,25 +27,29 @@ struct __attribute__((packed, aligned(sizeof(E)))) Any16 {  // 16 bytes of any a
 struct Eight {
   float v[8];
 };
-// Eight elements, `valid` of them in the row, the others zero.
+// Eight elements of a row as they lie in memory, `valid` of them in the row, the others
+// zero.
 template <typename E>
-__device__ __forceinline__ Eight load8(const E* p, int valid) {
-  Eight o;
-  if (valid >= 8) {
-    E e[8];
+struct Raw {
+  E e[8];
+  __device__ __forceinline__ void load(const E* p, int valid) {
+    if (valid >= 8) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
-      const u32x4 q = ((const Any16<E>*)p)[i].v;
-      __builtin_memcpy((char*)e + 16 * i, &q, 16);
+      for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
+        const u32x4 q = ((const Any16<E>*)p)[i].v;
+        __builtin_memcpy((char*)e + 16 * i, &q, 16);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = k < valid ? p[k] : (E)0.f;
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o.v[k] = (float)e[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o.v[k] = k < valid ? (float)p[k] : 0.f;
   }
-  return o;
-}
+  __device__ __forceinline__ float at(int k) const { return (float)e[k]; }
+  __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = (E)v;
+  }
+};
 template <typename E>
 __device__ __forceinline__ void store8(E* p, const Eight& x, int valid) {
   E e[8];
@@ -96,6 +100,7 @@ __device__ __forceinline__ void join(float (&s)[N], float* red, int& turn) {
   }
 }
 
+constexpr int kStay = 2048;
 constexpr int kBlock = 256;  // threads of a work-group whose rows are a wave's
 
 // A row's threads and the rows of a work-group.
@@ -109,6 +114,21 @@ struct Rows {
         t((int)threadIdx.x % THREADS) {}
 };
 
+// A thread's groups of a row: group i of span s (one span unless LONG).
+template <int THREADS, int V>
+__device__ __forceinline__ int col_of(int t, int s, int i) {
+  return ((s * V + i) * THREADS + t) * 8;
+}
+template <int THREADS, int V, typename E>
+__device__ __forceinline__ void fetch(Raw<E> (&a)[V], const void* p, int64_t row, int cols, int t, int s) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = col_of<THREADS, V>(t, s, i);
+    a[i].load((const E*)p + row + c, cols - c);
+  }
+}
+
+// The next row is on its way while one is summed; weight and bias stay in registers.
 // LONG: rows of any length, read three times.
 template <typename E, int THREADS, int V, bool LONG>
 __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
@@ -117,39 +137,44 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
   int turn = 0;
   const float per = 1.f / (float)p.cols;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
+  const auto col = [&](int s, int i) { return col_of<THREADS, V>(rows.t, s, i); };
+  Raw<E> a[V], next[LONG ? 1 : V], w[V], b[V];
+  const auto vectors = [&](int s) {
+    if (p.weight) fetch<THREADS, V>(w, p.weight, 0, p.cols, rows.t, s);
+    if (p.bias) fetch<THREADS, V>(b, p.bias, 0, p.cols, rows.t, s);
+  };
+  if constexpr (!LONG) {
+    if (rows.first < p.rows) fetch<THREADS, V>(next, p.x, rows.first * p.ld_x, p.cols, rows.t, 0);
+    vectors(0);
+  }
   for (int64_t r = rows.first; r < p.rows; r += rows.step) {
-    const E* const x = (const E*)p.x + r * p.ld_x;
-    Eight a[V];
-    const auto fetch = [&](int s) {
+    if constexpr (!LONG) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = ((s * V + i) * THREADS + rows.t) * 8;
-        if (LONG || c < p.cols) a[i] = load8(x + c, p.cols - c);
-      }
-    };
+      for (int i = 0; i < V; ++i) a[i] = next[i];
+      if (r + rows.step < p.rows)
+        fetch<THREADS, V>(next, p.x, (r + rows.step) * p.ld_x, p.cols, rows.t, 0);
+    }
     float sum[1] = {0.f};
     for (int s = 0; s < span; ++s) {
-      fetch(s);
+      if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (((s * V + i) * THREADS + rows.t) * 8 < p.cols)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sum[0] += a[i].v[k];
+        for (int k = 0; k < 8; ++k) sum[0] += a[i].at(k);
     }
     join<THREADS>(sum, red, turn);
     const float mean = sum[0] * per;
     float sq[1] = {0.f};
     for (int s = 0; s < span; ++s) {
-      if (LONG) fetch(s);
+      if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int valid = p.cols - ((s * V + i) * THREADS + rows.t) * 8;
+        const int valid = p.cols - col(s, i);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < valid) {
-            const float d = a[i].v[k] - mean;
-            sq[0] += d * d;
-          }
+        for (int k = 0; k < 8; ++k) {
+          const float d = a[i].at(k) - mean;
+          sq[0] += k < valid ? d * d : 0.f;
+        }
       }
     }
     join<THREADS>(sq, red, turn);
@@ -159,23 +184,24 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
       if (p.rstd) p.rstd[r] = rstd;
     }
     for (int s = 0; s < span; ++s) {
-      if (LONG) fetch(s);
+      if (LONG) {
+        fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
+        vectors(s);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int c = ((s * V + i) * THREADS + rows.t) * 8, valid = p.cols - c;
+        const int c = col(s, i), valid = p.cols - c;
         if (valid <= 0) continue;
         Eight y;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y.v[k] = (a[i].v[k] - mean) * rstd;
+        for (int k = 0; k < 8; ++k) y.v[k] = (a[i].at(k) - mean) * rstd;
         if (p.weight) {
-          const Eight w = load8((const E*)p.weight + c, valid);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y.v[k] *= w.v[k];
+          for (int k = 0; k < 8; ++k) y.v[k] *= w[i].at(k);
         }
         if (p.bias) {
-          const Eight b = load8((const E*)p.bias + c, valid);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y.v[k] += b.v[k];
+          for (int k = 0; k < 8; ++k) y.v[k] += b[i].at(k);
         }
         store8((E*)p.out + r * p.ld_out + c, y, valid);
       }
@@ -184,7 +210,8 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
 }
 
 // A row's gradient, and (SUMS) the work-group's share of the columns' sums, which
-// stay in registers over its rows.  LONG: d_x only, each row read twice.
+// stay in registers over its rows; the next row is on its way meanwhile.  LONG: d_x
+// only, each row read twice.
 template <typename E, int THREADS, int V, bool SUMS, bool LONG>
 __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBackwardPlan p) {
   static_assert(!(SUMS && LONG), "a long row's sums are another kernel's");
@@ -194,63 +221,67 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBac
   int turn = 0;
   const float per = 1.f / (float)p.cols;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
-  Eight sum_w[SUMS ? V : 1], sum_b[SUMS ? V : 1], w[V];
+  const auto col = [&](int s, int i) { return col_of<THREADS, V>(rows.t, s, i); };
+  Eight sum_w[SUMS ? V : 1], sum_b[SUMS ? V : 1];
   if constexpr (SUMS) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum_w[i].v[k] = sum_b[i].v[k] = 0.f;
   }
-  const auto col = [&](int s, int i) { return ((s * V + i) * THREADS + rows.t) * 8; };
+  struct Row {
+    Raw<E> x[V], d[V], res[V];
+    float mean, rstd;
+  };
+  const auto load = [&](Row& o, int64_t r, int s, bool residual) {
+    fetch<THREADS, V>(o.x, p.x, r * p.ld_x, p.cols, rows.t, s);
+    fetch<THREADS, V>(o.d, p.d_out, r * p.ld_d, p.cols, rows.t, s);
+    if (residual) fetch<THREADS, V>(o.res, p.residual, r * p.ld_residual, p.cols, rows.t, s);
+    o.mean = p.mean[r];
+    o.rstd = p.rstd[r];
+  };
+  Raw<E> w[V];
   const auto weights = [&](int s) {
+    if (p.weight) {
+      fetch<THREADS, V>(w, p.weight, 0, p.cols, rows.t, s);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = col(s, i);
-      if (p.weight) {
-        w[i] = load8((const E*)p.weight + c, p.cols - c);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[i].v[k] = 1.f;
-      }
+      for (int i = 0; i < V; ++i) w[i].fill(1.f);
     }
   };
-  if (!LONG) weights(0);
+  const bool has_residual = p.residual != nullptr;
+  Row row, next;
+  if constexpr (!LONG) {
+    if (rows.first < p.rows) load(next, rows.first, 0, has_residual);
+    weights(0);
+  }
   for (int64_t r = rows.first; r < p.rows; r += rows.step) {
-    const E* const x = (const E*)p.x + r * p.ld_x;
-    const E* const d = (const E*)p.d_out + r * p.ld_d;
-    const float mean = p.mean[r], rstd = p.rstd[r];
-    Eight xh[V], g[V], res[V];
-    const auto fetch = [&](int s, bool last) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = col(s, i), valid = p.cols - c;
-        xh[i] = load8(x + c, valid);
-        g[i] = load8(d + c, valid);
-        if (last && p.residual) res[i] = load8((const E*)p.residual + r * p.ld_residual + c, valid);
+    if constexpr (!LONG) {
+      row = next;
+      if (r + rows.step < p.rows) load(next, r + rows.step, 0, has_residual);
+    }
+    float c12[2] = {0.f, 0.f};
+    for (int s = 0; s < span; ++s) {
+      if (LONG) {
+        weights(s);
+        load(row, r, s, false);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int valid = p.cols - col(s, i);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) xh[i].v[k] = k < valid ? (xh[i].v[k] - mean) * rstd : 0.f;
-      }
-    };
-    float c12[2] = {0.f, 0.f};
-    for (int s = 0; s < span; ++s) {
-      if (LONG) weights(s);
-      fetch(s, !LONG);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-#pragma unroll
         for (int k = 0; k < 8; ++k) {
+          // (past the row's end d is 0, and so is every term)
+          const float d = row.d[i].at(k), xh = (row.x[i].at(k) - row.mean) * row.rstd;
+          const float dx = k < valid ? d * xh : 0.f;
           if constexpr (SUMS) {
-            sum_w[i].v[k] += g[i].v[k] * xh[i].v[k];
-            sum_b[i].v[k] += g[i].v[k];
+            sum_w[i].v[k] += dx;
+            sum_b[i].v[k] += d;
           }
-          g[i].v[k] *= w[i].v[k];
-          c12[0] += g[i].v[k];
-          c12[1] += g[i].v[k] * xh[i].v[k];
+          c12[0] += d * w[i].at(k);
+          c12[1] += dx * w[i].at(k);
         }
+      }
     }
     if (!p.d_x) continue;  // (the same for every thread)
     join<THREADS>(c12, red, turn);
@@ -258,7 +289,7 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBac
     for (int s = 0; s < span; ++s) {
       if (LONG) {
         weights(s);
-        fetch(s, true);
+        load(row, r, s, has_residual);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -267,9 +298,13 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBac
         Eight y;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float gk = LONG ? g[i].v[k] * w[i].v[k] : g[i].v[k];
-          y.v[k] = rstd * (gk - c1 - xh[i].v[k] * c2);
-          if (p.residual) y.v[k] += res[i].v[k];
+          const float g = row.d[i].at(k) * w[i].at(k);
+          const float xh = (row.x[i].at(k) - row.mean) * row.rstd;
+          y.v[k] = row.rstd * (g - c1 - xh * c2);
+        }
+        if (has_residual) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) y.v[k] += row.res[i].at(k);
         }
         store8((E*)p.d_x + r * p.ld_dx + c, y, valid);
       }
@@ -372,24 +407,25 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan
   const Rows<THREADS> rows;
   int turn = 0;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
+  Raw<E> a[V], next[LONG ? 1 : V];
+  if constexpr (!LONG) {
+    if (rows.first < p.rows) fetch<THREADS, V>(next, p.x, rows.first * p.ld_x, p.cols, rows.t, 0);
+  }
   for (int64_t r = rows.first; r < p.rows; r += rows.step) {
-    const E* const x = (const E*)p.x + r * p.ld_x;
-    Eight a[V];
-    const auto fetch = [&](int s) {
+    if constexpr (!LONG) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int c = ((s * V + i) * THREADS + rows.t) * 8;
-        a[i] = load8(x + c, p.cols - c);
-      }
-    };
+      for (int i = 0; i < V; ++i) a[i] = next[i];
+      if (r + rows.step < p.rows)
+        fetch<THREADS, V>(next, p.x, (r + rows.step) * p.ld_x, p.cols, rows.t, 0);
+    }
     float top[2] = {0.f, 0.f};  // the largest magnitude; 1 where a value is not finite
     for (int s = 0; s < span; ++s) {
-      fetch(s);
+      if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float m = fabsf(a[i].v[k]);
+          const float m = fabsf(a[i].at(k));
           top[0] = fmaxf(top[0], m);
           top[1] = m < INFINITY ? top[1] : 1.f;
         }
@@ -400,15 +436,15 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan
     const float inverse = 1.f / scale;
     if (rows.t == 0) p.scale[r] = scale;
     for (int s = 0; s < span; ++s) {
-      if (LONG) fetch(s);
+      if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int c = ((s * V + i) * THREADS + rows.t) * 8, valid = p.out_cols - c;
+        const int c = col_of<THREADS, V>(rows.t, s, i), valid = p.out_cols - c;
         if (valid <= 0) continue;
         int8_t q[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k)  // (past the row's end a value is 0)
-          q[k] = finite ? (int8_t)nearest(a[i].v[k], scale, inverse) : (int8_t)0;
+          q[k] = finite ? (int8_t)nearest(a[i].at(k), scale, inverse) : (int8_t)0;
         int8_t* const to = p.q + r * p.ld_q + c;
         if (valid >= 8) {
           struct __attribute__((packed)) Any8 {
@@ -440,6 +476,9 @@ Shape shape_of(int rows, int cols) {
 int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
 int threads_of(Shape s) { return s == kWide2 || s == kLong ? 1024 : kBlock; }
 
+// Work-groups that stay, each for several rows of a long matrix.
+unsigned launched(int64_t groups) { return (unsigned)(groups < kStay ? groups : kStay); }
+
 #define LSAMP_SHAPES(s, K, ARGS)        \
   switch (s) {                          \
     case kWave1: K(64, 1, false); break;  \
@@ -455,7 +494,7 @@ template <typename E>
 int norm(const NormPlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536)), block((unsigned)threads_of(s));
+  const dim3 grid(launched(groups)), block((unsigned)threads_of(s));
 #define K(T, V, L) hipLaunchKernelGGL((k_norm<E, T, V, L>), grid, block, 0, st, p)
   LSAMP_SHAPES(s, K, )
 #undef K
@@ -467,7 +506,7 @@ int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const bool sums = p.part != nullptr;
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  const dim3 grid((unsigned)(sums && s != kLong ? p.chunks : groups < 65536 ? groups : 65536));
+  const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups));
   const dim3 block((unsigned)threads_of(s));
   if (s == kLong) {
     if (p.d_x) hipLaunchKernelGGL((k_norm_backward<E, 1024, 1, false, true>), grid, block, 0, st, p);
@@ -494,7 +533,7 @@ template <typename E>
 int quantize(const QuantizePlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  const dim3 grid((unsigned)(groups < 65536 ? groups : 65536)), block((unsigned)threads_of(s));
+  const dim3 grid(launched(groups)), block((unsigned)threads_of(s));
 #define K(T, V, L) hipLaunchKernelGGL((k_quantize<E, T, V, L>), grid, block, 0, st, p)
   LSAMP_SHAPES(s, K, )
 #undef K
