@@ -80,7 +80,7 @@ lsamp_status plan_norm_backward(const lsamp_layer_norm_backward_args* a, void* b
   if (a->d_weight || a->d_bias) {
     P.chunks = norm_chunks(m, n);
     P.ld_part = round_up(n, 8);
-    P.part = ws.take<float>((int64_t)P.chunks * 2 * P.ld_part * 4);
+    if (P.chunks) P.part = ws.take<float>((int64_t)P.chunks * 2 * P.ld_part * 4);
   }
   *out = P;
   *bytes = ws.used;

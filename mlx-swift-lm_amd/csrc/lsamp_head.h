@@ -192,7 +192,7 @@ struct NormPlan {
 };
 struct NormBackwardPlan {
   int32_t rows, cols;
-  int32_t chunks;  // shares of the columns' sums (norm_chunks)
+  int32_t chunks;  // shares of the columns' sums (norm_chunks), 0 where there are none
   const void* x;
   int64_t ld_x;
   const void* weight;
@@ -206,7 +206,7 @@ struct NormBackwardPlan {
   int64_t ld_dx;
   void* d_weight;  // or NULL
   void* d_bias;
-  float* part;  // [chunks][2][ld_part], NULL without d_weight and d_bias
+  float* part;  // [chunks][2][ld_part]
   int64_t ld_part;  // a multiple of 8
 };
 struct QuantizePlan {

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include "lsamp_head.h"
+#include "lsamp_quant.h"
 
 namespace lsamp {
 namespace {
@@ -69,22 +70,21 @@ __device__ __forceinline__ void store8(E* p, const Eight& x, int valid) {
   }
 }
 
-// Sums (or maxima) of N values over the THREADS threads of a row: a wave, or a
-// work-group.  Every thread gets them.  `red` has 2 N floats a wave: a row's
+// Sums of N values (maxima of whole numbers) over the THREADS threads of a row: a wave,
+// or a work-group.  Every thread gets them.  `red` has 2 N of them a wave: a row's
 // exchange may begin while the one before is still read.
-template <int THREADS, int N, bool MAX = false>
-__device__ __forceinline__ void join(float (&s)[N], float* red, int& turn) {
+__device__ __forceinline__ float joined(float a, float b) { return a + b; }
+__device__ __forceinline__ uint32_t joined(uint32_t a, uint32_t b) { return max(a, b); }
+template <int THREADS, int N, typename T>
+__device__ __forceinline__ void join(T (&s)[N], T* red, int& turn) {
 #pragma unroll
   for (int d = 32; d > 0; d /= 2)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float o = __shfl_xor(s[i], d);
-      s[i] = MAX ? fmaxf(s[i], o) : s[i] + o;
-    }
+    for (int i = 0; i < N; ++i) s[i] = joined(s[i], (T)__shfl_xor(s[i], d));
   if constexpr (THREADS > kWave) {
     constexpr int kWaves = THREADS / kWave;
     const int wave = (int)threadIdx.x / kWave;
-    float* const at = red + turn * (kWaves * N);
+    T* const at = red + turn * (kWaves * N);
     turn ^= 1;
     if ((threadIdx.x & (kWave - 1)) == 0)
 #pragma unroll
@@ -92,15 +92,15 @@ __device__ __forceinline__ void join(float (&s)[N], float* red, int& turn) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float t = at[i];
+      T t = at[i];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) t = MAX ? fmaxf(t, at[w * N + i]) : t + at[w * N + i];
+      for (int w = 1; w < kWaves; ++w) t = joined(t, at[w * N + i]);
       s[i] = t;
     }
   }
 }
 
-constexpr int kStay = 2048;
+constexpr int kStay = 2048, kFew = 512;
 constexpr int kBlock = 256;  // threads of a work-group whose rows are a wave's
 
 // A row's threads and the rows of a work-group.
@@ -109,8 +109,8 @@ struct Rows {
   static constexpr int kPer = THREADS < kBlock ? kBlock / THREADS : 1;
   static constexpr int kGroup = THREADS < kBlock ? kBlock : THREADS;
   int first, step, t;  // the thread's first row, the distance to the next, its place in the row
-  __device__ __forceinline__ Rows()
-      : first((int)blockIdx.x * kPer + (int)threadIdx.x / THREADS), step((int)gridDim.x * kPer),
+  __device__ __forceinline__ Rows(int group, int groups)
+      : first(group * kPer + (int)threadIdx.x / THREADS), step(groups * kPer),
         t((int)threadIdx.x % THREADS) {}
 };
 
@@ -133,7 +133,7 @@ __device__ __forceinline__ void fetch(Raw<E> (&a)[V], const void* p, int64_t row
 template <typename E, int THREADS, int V, bool LONG>
 __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
   __shared__ float red[2 * THREADS / kWave];
-  const Rows<THREADS> rows;
+  const Rows<THREADS> rows((int)blockIdx.x, (int)gridDim.x);
   int turn = 0;
   const float per = 1.f / (float)p.cols;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
@@ -213,11 +213,10 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
 // stay in registers over its rows; the next row is on its way meanwhile.  LONG: d_x
 // only, each row read twice.
 template <typename E, int THREADS, int V, bool SUMS, bool LONG>
-__global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBackwardPlan p) {
+__device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const Rows<THREADS>& rows) {
   static_assert(!(SUMS && LONG), "a long row's sums are another kernel's");
   constexpr int kPer = Rows<THREADS>::kPer;
   __shared__ float red[4 * THREADS / kWave];
-  const Rows<THREADS> rows;
   int turn = 0;
   const float per = 1.f / (float)p.cols;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
@@ -345,6 +344,11 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBac
   }
 }
 
+template <typename E, int THREADS, int V, bool SUMS, bool LONG>
+__global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm_backward(NormBackwardPlan p) {
+  backward_rows<E, THREADS, V, SUMS, LONG>(p, Rows<THREADS>((int)blockIdx.x, (int)gridDim.x));
+}
+
 // Column sums of long rows: a column a thread, a chunk of rows a work-group.
 template <typename E>
 __global__ __launch_bounds__(kBlock) void k_norm_sums(NormBackwardPlan p) {
@@ -362,6 +366,44 @@ __global__ __launch_bounds__(kBlock) void k_norm_sums(NormBackwardPlan p) {
   float* const part = p.part + (int64_t)blockIdx.y * 2 * p.ld_part;
   part[c] = w;
   part[p.ld_part + c] = b;
+}
+
+// Few rows: one launch, whose first `rows_groups` work-groups take rows and the others
+// 16 columns each, which they read from the L2 once more: 16 threads a column take rows
+// in turn.
+template <typename E>
+__device__ __forceinline__ void columns(const NormBackwardPlan& p, int group) {
+  __shared__ float red[2][16][17];
+  const int lane = (int)threadIdx.x & 15, part = (int)threadIdx.x >> 4;
+  const int c = group * 16 + lane;
+  float w = 0.f, b = 0.f;
+  if (c < p.cols) {
+#pragma unroll 8
+    for (int r = part; r < p.rows; r += 16) {
+      const float d = (float)((const E*)p.d_out)[(int64_t)r * p.ld_d + c];
+      const float xh = ((float)((const E*)p.x)[(int64_t)r * p.ld_x + c] - p.mean[r]) * p.rstd[r];
+      w += d * xh;
+      b += d;
+    }
+  }
+  red[0][part][lane] = w;
+  red[1][part][lane] = b;
+  __syncthreads();
+  if (part > 1 || c >= p.cols) return;
+  float s = red[part][0][lane];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[part][i][lane];
+  E* const out = (E*)(part ? p.d_bias : p.d_weight);
+  if (out) out[c] = (E)s;
+}
+
+template <typename E, int THREADS, int V>
+__global__ __launch_bounds__(kBlock) void k_norm_backward_few(NormBackwardPlan p, int row_groups) {
+  const int group = (int)blockIdx.x;
+  if (group < row_groups)
+    backward_rows<E, THREADS, V, false, false>(p, Rows<THREADS>(group, row_groups));
+  else
+    columns<E>(p, group - row_groups);
 }
 
 // The work-groups' shares, joined in their order: 64 columns a work-group of
@@ -387,24 +429,10 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void k_norm_join(NormBackwardPla
   out[c] = (E)s;
 }
 
-// x / s to the nearest whole number, ties to the even one, from the product with
-// 1 / s, which is off by one at most: e = x - q s is exact (one fma of values that
-// are multiples of the smaller one's last place), and where it is more than half
-// a step, or half a step and q odd, the neighbour is taken.
-__device__ __forceinline__ int nearest(float x, float s, float inverse) {
-  float q = rintf(x * inverse);
-  const float e = fmaf(-q, s, x), half = 0.5f * s;
-  const bool odd = ((int)q & 1) != 0;
-  if (e > half || (e == half && odd)) q += 1.f;
-  else if (e < -half || (e == -half && odd)) q -= 1.f;
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
-}
-
-constexpr float kPart = 1.f / 127.f;
 template <typename E, int THREADS, int V, bool LONG>
 __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan p) {
-  __shared__ float red[4 * THREADS / kWave];
-  const Rows<THREADS> rows;
+  __shared__ uint32_t red[2 * THREADS / kWave];
+  const Rows<THREADS> rows((int)blockIdx.x, (int)gridDim.x);
   int turn = 0;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
   Raw<E> a[V], next[LONG ? 1 : V];
@@ -418,45 +446,37 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan
       if (r + rows.step < p.rows)
         fetch<THREADS, V>(next, p.x, (r + rows.step) * p.ld_x, p.cols, rows.t, 0);
     }
-    float top[2] = {0.f, 0.f};  // the largest magnitude; 1 where a value is not finite
+    uint32_t top[1] = {0};
     for (int s = 0; s < span; ++s) {
       if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float m = fabsf(a[i].at(k));
-          top[0] = fmaxf(top[0], m);
-          top[1] = m < INFINITY ? top[1] : 1.f;
-        }
+        for (int k = 0; k < 8; ++k) top[0] = max(top[0], magnitude(a[i].at(k)));
     }
-    join<THREADS, 2, true>(top, red, turn);
-    const bool finite = top[1] == 0.f;
-    const float scale = finite ? fmaxf(top[0] * kPart, 1.17549435e-38f) : NAN;
-    const float inverse = 1.f / scale;
+    join<THREADS>(top, red, turn);
+    const float scale = row_scale(top[0]), inverse = 1.f / scale;
     if (rows.t == 0) p.scale[r] = scale;
     for (int s = 0; s < span; ++s) {
       if (LONG) fetch<THREADS, V>(a, p.x, r * p.ld_x, p.cols, rows.t, s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int c = col_of<THREADS, V>(rows.t, s, i), valid = p.out_cols - c;
-        if (valid <= 0) continue;
-        int8_t q[8];
+        float v[8];  // (past the row's end 0)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // (past the row's end a value is 0)
-          q[k] = finite ? (int8_t)nearest(a[i].at(k), scale, inverse) : (int8_t)0;
+        for (int k = 0; k < 8; ++k) v[k] = a[i].at(k);
+        const uint64_t word = quantize8(v, scale, inverse);
+        if (valid <= 0) continue;
         int8_t* const to = p.q + r * p.ld_q + c;
         if (valid >= 8) {
           struct __attribute__((packed)) Any8 {
             uint64_t v;
           };
-          uint64_t word;
-          __builtin_memcpy(&word, q, 8);
           ((Any8*)to)->v = word;
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (k < valid) to[k] = q[k];
+            if (k < valid) to[k] = (int8_t)(word >> (8 * k));
         }
       }
     }
@@ -473,6 +493,8 @@ Shape shape_of(int rows, int cols) {
   if (cols <= 4096) return kBlock2;
   return cols <= 16384 ? kWide2 : kLong;
 }
+// Whether the columns' sums are taken beside the rows, in the same launch.
+bool few(int rows, int cols) { return rows <= kFew && cols <= 4096; }
 int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
 int threads_of(Shape s) { return s == kWide2 || s == kLong ? 1024 : kBlock; }
 
@@ -504,8 +526,20 @@ int norm(const NormPlan& p, hipStream_t st) {
 template <typename E>
 int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
-  const bool sums = p.part != nullptr;
+  const bool sums = p.d_weight || p.d_bias;
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
+  if (sums && few(p.rows, p.cols)) {
+    const int row_groups = p.d_x ? (int)groups : 0;
+    const dim3 all((unsigned)(row_groups + (p.cols + 15) / 16));
+#define K(T, V) hipLaunchKernelGGL((k_norm_backward_few<E, T, V>), all, dim3(kBlock), 0, st, p, row_groups)
+    switch (s) {
+      case kWave1: K(64, 1); break;
+      case kBlock1: K(256, 1); break;
+      default: K(256, 2); break;
+    }
+#undef K
+    return (int)hipGetLastError();
+  }
   const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups));
   const dim3 block((unsigned)threads_of(s));
   if (s == kLong) {
@@ -552,6 +586,7 @@ int quantize(const QuantizePlan& p, hipStream_t st) {
 
 // Shares of the columns' sums: a work-group's.
 int norm_chunks(int rows, int cols) {
+  if (few(rows, cols)) return 0;
   const Shape s = shape_of(rows, cols);
   if (s == kLong) return rows < 64 ? 1 : rows / 32 < 256 ? rows / 32 : 256;
   const int groups = (rows + rows_per_group(s) - 1) / rows_per_group(s);
