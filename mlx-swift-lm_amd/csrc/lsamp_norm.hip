@@ -210,8 +210,10 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
 }
 
 // A row's gradient, and (SUMS) the work-group's share of the columns' sums, which
-// stay in registers over its rows; the next row is on its way meanwhile.  LONG: d_x
-// only, each row read twice.
+// stay in registers over its rows; the next row is on its way meanwhile.  1024 threads
+// have 128 registers each: their sums lie in LDS, a thread's own 16 bytes beside its
+// neighbours', and float32 rows are not fetched ahead (4096 x 16384 bf16: 433 us with the
+// sums in registers, spilled; 111 so).  LONG: d_x only, each row read twice.
 template <typename E, int THREADS, int V, bool SUMS, bool LONG>
 __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const Rows<THREADS>& rows) {
   static_assert(!(SUMS && LONG), "a long row's sums are another kernel's");
@@ -221,6 +223,9 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
   const float per = 1.f / (float)p.cols;
   const int span = LONG ? (p.cols + V * THREADS * 8 - 1) / (V * THREADS * 8) : 1;
   const auto col = [&](int s, int i) { return col_of<THREADS, V>(rows.t, s, i); };
+  constexpr bool kInLds = SUMS && THREADS == 1024;
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  __shared__ f32x4 kept[kInLds ? V * 4 : 1][kInLds ? THREADS : 1];
   Eight sum_w[SUMS ? V : 1], sum_b[SUMS ? V : 1];
   if constexpr (SUMS) {
 #pragma unroll
@@ -228,6 +233,14 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
 #pragma unroll
       for (int k = 0; k < 8; ++k) sum_w[i].v[k] = sum_b[i].v[k] = 0.f;
   }
+  if constexpr (kInLds) {
+#pragma unroll
+    for (int i = 0; i < V * 4; ++i) kept[i][rows.t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // four terms of group i's sums (which: of d xh, of d), its half h
+  const auto add = [&](int i, int which, int h, const f32x4& v) {
+    if constexpr (kInLds) kept[(i * 2 + which) * 2 + h][rows.t] += v;
+  };
   struct Row {
     Raw<E> x[V], d[V], res[V];
     float mean, rstd;
@@ -249,15 +262,18 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
     }
   };
   const bool has_residual = p.residual != nullptr;
+  constexpr bool kAhead = !LONG && (THREADS < 1024 || V == 1);
   Row row, next;
-  if constexpr (!LONG) {
+  if constexpr (kAhead) {
     if (rows.first < p.rows) load(next, rows.first, 0, has_residual);
-    weights(0);
   }
+  if (!LONG) weights(0);
   for (int64_t r = rows.first; r < p.rows; r += rows.step) {
-    if constexpr (!LONG) {
+    if constexpr (kAhead) {
       row = next;
       if (r + rows.step < p.rows) load(next, r + rows.step, 0, has_residual);
+    } else if constexpr (!LONG) {
+      load(row, r, 0, has_residual);
     }
     float c12[2] = {0.f, 0.f};
     for (int s = 0; s < span; ++s) {
@@ -269,16 +285,25 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
       for (int i = 0; i < V; ++i) {
         const int valid = p.cols - col(s, i);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          // (past the row's end d is 0, and so is every term)
-          const float d = row.d[i].at(k), xh = (row.x[i].at(k) - row.mean) * row.rstd;
-          const float dx = k < valid ? d * xh : 0.f;
-          if constexpr (SUMS) {
-            sum_w[i].v[k] += dx;
-            sum_b[i].v[k] += d;
+        for (int h = 0; h < 2; ++h) {
+          f32x4 tw, tb;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            // (past the row's end d is 0, and so is every term)
+            const int k = h * 4 + q;
+            const float d = row.d[i].at(k), xh = (row.x[i].at(k) - row.mean) * row.rstd;
+            const float dx = k < valid ? d * xh : 0.f;
+            if constexpr (SUMS && !kInLds) {
+              sum_w[i].v[k] += dx;
+              sum_b[i].v[k] += d;
+            }
+            tw[q] = dx;
+            tb[q] = d;
+            c12[0] += d * w[i].at(k);
+            c12[1] += dx * w[i].at(k);
           }
-          c12[0] += d * w[i].at(k);
-          c12[1] += dx * w[i].at(k);
+          add(i, 0, h, tw);
+          add(i, 1, h, tb);
         }
       }
     }
@@ -308,6 +333,15 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
         store8((E*)p.d_x + r * p.ld_dx + c, y, valid);
       }
     }
+  }
+  if constexpr (kInLds) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sum_w[i].v[k] = kept[i * 4 + k / 4][rows.t][k % 4];
+        sum_b[i].v[k] = kept[i * 4 + 2 + k / 4][rows.t][k % 4];
+      }
   }
   if constexpr (SUMS) {
     // [work-group][2][ld_part]; rows of a wave each are joined first
@@ -485,21 +519,24 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_quantize(QuantizePlan
 
 // The shape of a row of `cols` elements: a wave, 256 or 1024 threads, one, two or
 // four groups of eight of a thread.  Few rows take more threads a row.
-enum Shape { kWave1, kWave2, kWave4, kBlock1, kBlock2, kWide2, kLong };
+enum Shape { kWave1, kWave2, kWave4, kBlock1, kBlock2, kWide1, kWide2, kLong };
 Shape shape_of(int rows, int cols) {
   if (cols <= 2048 && rows >= 1024) return cols <= 512 ? kWave1 : cols <= 1024 ? kWave2 : kWave4;
   if (cols <= 512) return kWave1;
   if (cols <= 2048) return kBlock1;
   if (cols <= 4096) return kBlock2;
-  return cols <= 16384 ? kWide2 : kLong;
+  return cols <= 8192 ? kWide1 : cols <= 16384 ? kWide2 : kLong;
 }
 // Whether the columns' sums are taken beside the rows, in the same launch.
 bool few(int rows, int cols) { return rows <= kFew && cols <= 4096; }
 int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
-int threads_of(Shape s) { return s == kWide2 || s == kLong ? 1024 : kBlock; }
+int threads_of(Shape s) { return s >= kWide1 ? 1024 : kBlock; }
 
 // Work-groups that stay, each for several rows of a long matrix.
-unsigned launched(int64_t groups) { return (unsigned)(groups < kStay ? groups : kStay); }
+unsigned launched(int64_t groups, Shape s) {
+  const int64_t most = s >= kWide1 ? kStay / 4 : kStay;
+  return (unsigned)(groups < most ? groups : most);
+}
 
 #define LSAMP_SHAPES(s, K, ARGS)        \
   switch (s) {                          \
@@ -508,6 +545,7 @@ unsigned launched(int64_t groups) { return (unsigned)(groups < kStay ? groups : 
     case kWave4: K(64, 4, false); break;  \
     case kBlock1: K(256, 1, false); break; \
     case kBlock2: K(256, 2, false); break; \
+    case kWide1: K(1024, 1, false); break; \
     case kWide2: K(1024, 2, false); break; \
     default: K(1024, 1, true); break;     \
   }
@@ -516,7 +554,7 @@ template <typename E>
 int norm(const NormPlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  const dim3 grid(launched(groups)), block((unsigned)threads_of(s));
+  const dim3 grid(launched(groups, s)), block((unsigned)threads_of(s));
 #define K(T, V, L) hipLaunchKernelGGL((k_norm<E, T, V, L>), grid, block, 0, st, p)
   LSAMP_SHAPES(s, K, )
 #undef K
@@ -540,7 +578,7 @@ int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
 #undef K
     return (int)hipGetLastError();
   }
-  const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups));
+  const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups, s));
   const dim3 block((unsigned)threads_of(s));
   if (s == kLong) {
     if (p.d_x) hipLaunchKernelGGL((k_norm_backward<E, 1024, 1, false, true>), grid, block, 0, st, p);
@@ -567,7 +605,7 @@ template <typename E>
 int quantize(const QuantizePlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  const dim3 grid(launched(groups)), block((unsigned)threads_of(s));
+  const dim3 grid(launched(groups, s)), block((unsigned)threads_of(s));
 #define K(T, V, L) hipLaunchKernelGGL((k_quantize<E, T, V, L>), grid, block, 0, st, p)
   LSAMP_SHAPES(s, K, )
 #undef K
