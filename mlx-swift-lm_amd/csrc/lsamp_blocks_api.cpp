@@ -9,6 +9,7 @@ using namespace lsamp;
 namespace {
 
 constexpr int32_t kMaxInt8Features = (1 << 17) - 1;  // (2^14 k below 2^31)
+constexpr int64_t kKeptBytes = 128 << 10;  // x in LDS (ResidentPlan)
 
 lsamp_status check_positive(const char* what, float v) {
   if (!(v > 0.f && std::isfinite(v)))
@@ -93,7 +94,8 @@ lsamp_status check_quantized(const char* what, const void* p, int64_t ld, int32_
 }
 
 struct LinearInt8Plan {
-  bool quantize;
+  bool quantize, kept;
+  ResidentPlan resident;  // (kept)
   QuantizePlan quant;
   Operand x, w;
   Choice choice;
@@ -129,12 +131,14 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
   Arena ws(base);
   const int64_t ld_x = stride_of(a->x_stride, m, k);
   const float* x_scale = a->x_scale;
-  if (given) {
-    P.x = operand(a->x, ld_x, m, k, 1);
+  P.kept = m <= kSkinnyRows && k >= 16 && m * round_up(k, 128) <= kKeptBytes;
+  const bool fused = P.kept && !given && m <= 4 && m * (int64_t)k <= 8192;
+  if (given || fused) {
+    P.x = operand(a->x, ld_x, m, k, given ? 1 : eb);
   } else {
-    // (rows of whole chunks, zeros behind their ends)
+    // (rows of whole chunks, or slabs, zeros behind their ends)
     const int64_t pitch = row_pitch(k, 1);
-    const int32_t wide = (int32_t)row_chunks(k, 1);
+    const int32_t wide = P.kept ? (int32_t)pitch : (int32_t)row_chunks(k, 1);
     int8_t* const q = ws.take<int8_t>((int64_t)m * pitch);
     float* const s = ws.take<float>((int64_t)m * 4);
     P.quantize = true;
@@ -145,7 +149,15 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
   }
   P.w = operand(a->weight, stride_of(a->weight_stride, n, k), n, k, 1);
   MatrixRef x = P.x.ref, w = P.w.ref;
-  if (m <= kSkinnyRows) {
+  if (P.kept) {
+    if (given && !(P.x.chunked && k % 128 == 0)) x = packed(ws, P.x, 1, true);
+    ResidentPlan& g = P.resident;
+    g = ResidentPlan{m, k, 0, 0, fused, x.p, x.ld, w.p, w.ld};
+    // (a work-group a CU, or two of little LDS)
+    const int64_t most = m * round_up(k, 128) <= 16 << 10 ? 512 : 256, blocks = ceil_div(n, 16);
+    g.shared = blocks < 8 * most;
+    g.groups = (int32_t)std::min(most, g.shared ? blocks : ceil_div(blocks, 8));
+  } else if (m <= kSkinnyRows) {
     P.choice = choose_skinny(m, n, false);
     if (m > kLooseRows) x = packed(ws, P.x, 1);
   } else {
@@ -157,10 +169,12 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
       w = packed(ws, P.w, 1);
     }
   }
-  P.gemm = plan_gemm(P.choice, x, w, m, n, k, 1);
-  if (too_many(P.gemm))
-    return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
-  if (P.gemm.parts > 1) P.partial = take_partial(ws, m, n, P.gemm.parts);
+  if (!P.kept) {
+    P.gemm = plan_gemm(P.choice, x, w, m, n, k, 1);
+    if (too_many(P.gemm))
+      return set_error(LSAMP_ERR_SHAPE, "%d rows of %d outputs are too many for one call", m, n);
+    if (P.gemm.parts > 1) P.partial = take_partial(ws, m, n, P.gemm.parts);
+  }
   EpiLinearInt8& e = P.epi;
   e.m = m;
   e.n = n;
@@ -432,7 +446,9 @@ lsamp_status lsamp_linear_int8(lsamp_context* ctx, const lsamp_linear_int8_args*
   if (P.quantize) LSAMP_TRY(launch_quantize(P.quant, a->dtype, stream));
   LSAMP_TRY(lay_out(P.x, 1, stream));
   LSAMP_TRY(lay_out(P.w, 1, stream));
-  if (P.gemm.parts == 1) {
+  if (P.kept) {
+    LSAMP_TRY(INT8_OP(a->dtype, resident_linear(P.resident, P.epi, stream)));
+  } else if (P.gemm.parts == 1) {
     LSAMP_TRY(INT8_OP(a->dtype, gemm_linear(P.choice.tile, P.gemm, P.epi, stream)));
   } else {
     LSAMP_TRY(launch_partial_int8(P.choice.tile, P.gemm, P.partial, stream));

@@ -178,6 +178,19 @@ struct EpiLinearInt8 : EpiLinear {
   const float* w_scale;  // [n]
 };
 
+// A product of few rows that are kept in LDS: up to 64, of 128 KB in slabs of 128 bytes.
+struct ResidentPlan {
+  int32_t m, k;
+  int32_t groups;  // work-groups
+  int32_t shared;  // the waves of one share a block of columns
+  int32_t fused;   // x is of the block's type (at most 8,192 values), else 8-bit integers in
+                   // aligned rows of whole slabs, zero behind their ends
+  const void* x;
+  int64_t ld_x;
+  const void* w;
+  int64_t ld_w;
+};
+
 struct NormPlan {
   int32_t rows, cols;
   float eps;
@@ -241,6 +254,7 @@ struct HeadOps {
 template <int DT>
 struct Int8Ops {
   static int gemm_linear(GemmTile tile, const GemmPlan& g, const EpiLinearInt8& e, void* stream);
+  static int resident_linear(const ResidentPlan& g, const EpiLinearInt8& e, void* stream);
   static int join_linear(const EpiPartial& from, int parts, const EpiLinearInt8& e, void* stream);
 };
 // Sums of parts as whole numbers of 32 bits.

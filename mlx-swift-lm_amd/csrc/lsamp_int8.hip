@@ -14,6 +14,7 @@
 #include "lsamp_epilogue.h"
 #include "lsamp_gemm.h"
 #include "lsamp_head.h"
+#include "lsamp_quant.h"
 #include "lsamp_skinny.h"
 
 namespace lsamp {
@@ -122,6 +123,221 @@ int launch_skinny(const GemmPlan& g, const LinearInt8& e, void* stream) {
   return (int)hipGetLastError();
 }
 
+// ------------------------------------------------------------ x kept in LDS
+// Up to 64 rows whose 8-bit values fit in LDS (128 KB: 64 x 2048, 16 x 8192): a work-group
+// brings x there once, and its eight waves read nothing but W, chunks of 16 bytes of
+// 16 of its rows straight into fragments, kDepth slabs ahead and from one block of 16
+// columns to the next (k_skinny reads a slab of x beside every slab of W).  WK 1: a wave
+// has blocks of its own, for outputs that are many of them for all waves; 8: the waves
+// share a block, its slabs in turn, and join their sums.
+//
+// A row of W ends anywhere: the last slab's chunks are read from the row's last 16 bytes
+// where they would pass its end, and moved down; what lies behind meets zeros of x.
+//
+// FUSED: x is of the block's own type, and every work-group quantises it as it brings
+// it (a launch less, for one row or few: 2 to 3 us).
+constexpr int kResidentWaves = 8;
+__device__ __forceinline__ v4i moved_down(v4i v, int bytes) {
+  unsigned __int128 w;
+  __builtin_memcpy(&w, &v, 16);
+  w >>= 8 * bytes;
+  __builtin_memcpy(&v, &w, 16);
+  return v;
+}
+
+template <int MF, int WK, int KB, bool FUSED>
+__global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentPlan g, LinearInt8 e) {
+  constexpr int kThreads = kResidentWaves * kWave;
+  constexpr int kDepth = WK == 1 ? 8 : 4;
+  __shared__ __attribute__((aligned(1024))) char xs[KB * 1024];
+  __shared__ float scales[MF * 16];
+  __shared__ v4i sums[WK > 1 ? WK - 1 : 1][WK > 1 ? MF : 1][kWave];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int slabs = (g.k + 127) / 128, pitch = slabs * 128;
+  const auto place = [&](int r, int chunk) { return r * pitch + ((chunk & ~7) | ((chunk ^ r) & 7)) * 16; };
+
+  // This wave's blocks of 16 columns, and its slabs of one: first, first + WK, ...
+  const int blocks = (e.n + 15) / 16;
+  const int block0 = WK == 1 ? (int)blockIdx.x * kResidentWaves + wave : (int)blockIdx.x;
+  const int block_step = WK == 1 ? (int)gridDim.x * kResidentWaves : (int)gridDim.x;
+  const int first = WK == 1 ? 0 : wave;
+  const int steps = slabs > first ? (slabs - first + WK - 1) / WK : 0;
+  const int turns = (steps + kDepth - 1) / kDepth;
+  const int row = lane & 15, at = (lane >> 4) * 16;
+
+  v4i ring[kDepth][2];
+  // (always loads, so that the compiler counts what is under way: past the last step the
+  // last one's bytes again)
+  const auto load = [&](v4i (&to)[2], int block, int step) {
+    const int slab = first + WK * min(step, max(steps - 1, 0));
+    const int64_t r = min(min(block, blocks - 1) * 16 + row, e.n - 1);
+    const char* const p = (const char*)g.w + r * g.ld_w;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      to[kk] = load_chunk<kInt8>(p + min(slab * 128 + kk * 64 + at, g.k - 16));
+  };
+#pragma unroll
+  for (int u = 0; u < kDepth; ++u) load(ring[u], block0, u);
+
+  if constexpr (FUSED) {
+    __shared__ uint32_t tops[2][kResidentWaves];
+    constexpr int kChunks = 2;  // of eight values a thread: 8,192 in all
+    constexpr int kPer = 8 / kChunkOf<DT>;
+    for (int r = 0; r < g.m; ++r) {
+      const char* const x = (const char*)g.x + (int64_t)r * g.ld_x * El<DT>::kBytes;
+      v4i raw[kChunks][kPer];
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+          const int c = (i * kThreads + (int)threadIdx.x) * 8 + h * kChunkOf<DT>;
+          raw[i][h] = v4i{0, 0, 0, 0};
+          if (c + kChunkOf<DT> <= g.k) raw[i][h] = load_chunk<DT>(x + (int64_t)c * El<DT>::kBytes);
+        }
+      if (g.k % kChunkOf<DT>) {  // (where the row ends)
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+          for (int h = 0; h < kPer; ++h) {
+            const int c = (i * kThreads + (int)threadIdx.x) * 8 + h * kChunkOf<DT>;
+            if (c < g.k && c + kChunkOf<DT> > g.k) raw[i][h] = load_chunk_end<DT>(x, c, g.k);
+          }
+      }
+      float v[kChunks][8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        S el[8];
+        __builtin_memcpy(el, raw[i], 16 * kPer);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          v[i][k] = (float)el[k];
+          top = max(top, magnitude(v[i][k]));
+        }
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d /= 2) top = max(top, (uint32_t)__shfl_xor(top, d));
+      if (lane == 0) tops[r & 1][wave] = top;
+      __syncthreads();  // (a row's tops are read before the next but one's are written)
+#pragma unroll
+      for (int i = 0; i < kResidentWaves; ++i) top = max(top, tops[r & 1][i]);
+      const float scale = row_scale(top), inverse = 1.f / scale;
+      if (threadIdx.x == 0) scales[r] = scale;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = (i * kThreads + (int)threadIdx.x) * 8;
+        if (i * kThreads * 8 < pitch) {
+          const uint64_t q = quantize8(v[i], scale, inverse);
+          if (c < pitch) *(uint64_t*)(xs + place(r, c / 16) + c % 16) = q;
+        }
+      }
+    }
+  } else {
+    // (rows of whole slabs, straight to LDS: 64 chunks in order an instruction, so the
+    // chunks that the order asks for are read)
+    const int chunks = pitch / 16, last = g.m * chunks - 1;
+    for (int u = wave; u * kWave <= last; u += kResidentWaves) {
+      const int i = min(u * kWave + lane, last), r = i / chunks, c = i - r * chunks;
+      __builtin_amdgcn_global_load_lds(
+          LSAMP_GLOBAL((const char*)g.x + (int64_t)r * g.ld_x + ((c & ~7) | ((c ^ r) & 7)) * 16),
+          LSAMP_LDS(xs + u * 1024), 16, 0, 0);
+    }
+    if ((int)threadIdx.x < g.m) scales[threadIdx.x] = e.x_scale[threadIdx.x];
+    __builtin_amdgcn_sched_barrier(0);
+    wait_loads<0>();
+  }
+  __syncthreads();
+
+  v4i acc[MF];
+#pragma unroll
+  for (int j = 0; j < MF; ++j) acc[j] = v4i{0, 0, 0, 0};
+  // (rows past the last repeat it)
+  int x_row[MF];
+#pragma unroll
+  for (int j = 0; j < MF; ++j) x_row[j] = min(j * 16 + row, g.m - 1);
+  // What fragment j's end needs: on its way from the block's start.
+  struct Ends {
+    v4f ws, b, res[WK == 1 ? MF : 1];
+  };
+  const auto ends = [&](int block, int j0) {
+    Ends o;
+    const int c = block * 16 + (lane >> 4) * 4;
+    o.ws = c < e.n ? e.w_at(c) : v4f{0.f, 0.f, 0.f, 0.f};
+    o.b = c < e.n ? e.bias_at(c) : v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < (WK == 1 ? MF : 1); ++j)
+      o.res[j] = c < e.n ? e.residual_at((j0 + j) * 16 + row, c) : v4f{0.f, 0.f, 0.f, 0.f};
+    return o;
+  };
+  const auto put = [&](int j, int block, v4i v, const Ends& o, v4f res) {
+    const int r = j * 16 + row, c = block * 16 + (lane >> 4) * 4;
+    if (r < g.m && c < e.n) e.finish(r, c, e.scaled(v, scales[r], o.ws), o.b, res);
+  };
+  for (int block = block0; block < blocks; block += block_step) {
+    Ends o;
+    if (WK == 1 || wave < MF) o = ends(block, WK == 1 ? 0 : wave);
+    for (int turn = 0; turn < turns; ++turn) {
+      const bool next = turn + 1 < turns;
+      const int to_block = next ? block : block + block_step, to_turn = next ? turn + 1 : 0;
+#pragma unroll
+      for (int u = 0; u < kDepth; ++u) {
+        const int step = turn * kDepth + u;
+        if (step < steps) {  // (the same for the wave)
+          const int slab = first + WK * step;
+          v4i w[2] = {ring[u][0], ring[u][1]};
+          if ((slab + 1) * 128 > g.k) {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+              const int over = slab * 128 + kk * 64 + at + 16 - g.k;
+              w[kk] = moved_down(w[kk], min(max(over, 0), 15));
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int j = 0; j < MF; ++j) {
+              const v4i x = *(const v4i*)(xs + place(x_row[j], slab * 8 + kk * 4 + (lane >> 4)));
+              mma<kInt8>(acc[j], w[kk], x);
+            }
+        }
+        load(ring[u], to_block, to_turn * kDepth + u);
+      }
+    }
+    if constexpr (WK == 1) {
+#pragma unroll
+      for (int j = 0; j < MF; ++j) put(j, block, acc[j], o, o.res[j]);
+    } else {
+      // (wave j adds up the rows of fragment j, its own sums among them)
+#pragma unroll
+      for (int j = 0; j < MF; ++j)
+        if (wave != j) sums[wave - (wave > j)][j][lane] = acc[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < MF; ++j)
+        if (wave == j) {
+          v4i v = acc[j];
+#pragma unroll
+          for (int k = 0; k < WK - 1; ++k) v += sums[k][j][lane];
+          put(j, block, v, o, o.res[0]);
+        }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < MF; ++j) acc[j] = v4i{0, 0, 0, 0};
+  }
+}
+
+template <int MF, int KB, bool FUSED>
+int launch_resident(const ResidentPlan& g, const LinearInt8& e, hipStream_t st) {
+  const dim3 grid((unsigned)g.groups), threads(kResidentWaves * kWave);
+  if (g.shared)
+    hipLaunchKernelGGL((k_resident<MF, 8, KB, FUSED>), grid, threads, 0, st, g, e);
+  else
+    hipLaunchKernelGGL((k_resident<MF, 1, KB, FUSED>), grid, threads, 0, st, g, e);
+  return (int)hipGetLastError();
+}
+
 // The parts of a split reduction added up, and the epilogue: a quad of columns a thread.
 __global__ __launch_bounds__(256) void k_join_int8(EpiPartial from, int parts, LinearInt8 e) {
   const int quads = (e.n + 3) / 4;
@@ -156,6 +372,16 @@ int Int8Ops<DT>::gemm_linear(GemmTile t, const GemmPlan& g, const EpiLinearInt8&
   if (t == kSkinny64) return launch_skinny<4, 4>(g, e, st);
   if (t == kSkinny16) return launch_skinny<1, 8>(g, e, st);
   return launch(t, g, e, st);
+}
+template <>
+int Int8Ops<DT>::resident_linear(const ResidentPlan& g, const EpiLinearInt8& p, void* stream) {
+  const LinearInt8 e = epilogue(p);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool small = (int64_t)g.m * ((g.k + 127) / 128 * 128) <= 16 << 10;
+  if (g.m > 32) return launch_resident<4, 128, false>(g, e, st);
+  if (g.m > 16) return launch_resident<2, 128, false>(g, e, st);
+  if (!small) return launch_resident<1, 128, false>(g, e, st);
+  return g.fused ? launch_resident<1, 16, true>(g, e, st) : launch_resident<1, 16, false>(g, e, st);
 }
 template <>
 int Int8Ops<DT>::join_linear(const EpiPartial& from, int parts, const EpiLinearInt8& p, void* st) {
