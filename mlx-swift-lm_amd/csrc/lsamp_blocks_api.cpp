@@ -9,7 +9,7 @@ using namespace lsamp;
 namespace {
 
 constexpr int32_t kMaxInt8Features = (1 << 17) - 1;  // (2^14 k below 2^31)
-constexpr int64_t kKeptBytes = 128 << 10;  // x in LDS (ResidentPlan)
+constexpr int64_t kKeptBytes = 128 << 10, kKeptRow = 256;  // x in LDS (ResidentPlan)
 
 lsamp_status check_positive(const char* what, float v) {
   if (!(v > 0.f && std::isfinite(v)))
@@ -131,13 +131,14 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
   Arena ws(base);
   const int64_t ld_x = stride_of(a->x_stride, m, k);
   const float* x_scale = a->x_scale;
-  P.kept = m <= kSkinnyRows && k >= 16 && m * round_up(k, 128) <= kKeptBytes;
+  const int64_t kept_bytes = m * round_up(k, kKeptRow);
+  P.kept = m <= kSkinnyRows && k >= 16 && kept_bytes <= kKeptBytes;
   const bool fused = P.kept && !given && m <= 4 && m * (int64_t)k <= 8192;
   if (given || fused) {
     P.x = operand(a->x, ld_x, m, k, given ? 1 : eb);
   } else {
-    // (rows of whole chunks, or slabs, zeros behind their ends)
-    const int64_t pitch = row_pitch(k, 1);
+    // (rows of whole chunks, or as they are kept, zeros behind their ends)
+    const int64_t pitch = P.kept ? round_up(k, kKeptRow) : row_pitch(k, 1);
     const int32_t wide = P.kept ? (int32_t)pitch : (int32_t)row_chunks(k, 1);
     int8_t* const q = ws.take<int8_t>((int64_t)m * pitch);
     float* const s = ws.take<float>((int64_t)m * 4);
@@ -150,11 +151,11 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
   P.w = operand(a->weight, stride_of(a->weight_stride, n, k), n, k, 1);
   MatrixRef x = P.x.ref, w = P.w.ref;
   if (P.kept) {
-    if (given && !(P.x.chunked && k % 128 == 0)) x = packed(ws, P.x, 1, true);
+    if (given && !(P.x.chunked && k % kKeptRow == 0)) x = packed(ws, P.x, 1, kKeptRow);
     ResidentPlan& g = P.resident;
     g = ResidentPlan{m, k, 0, 0, fused, x.p, x.ld, w.p, w.ld};
-    // (a work-group a CU, or two of little LDS)
-    const int64_t most = m * round_up(k, 128) <= 16 << 10 ? 512 : 256, blocks = ceil_div(n, 16);
+    // (a work-group a CU, of little LDS two)
+    const int64_t most = kept_bytes <= 16 << 10 ? 512 : 256, blocks = ceil_div(n, 16);
     g.shared = blocks < 8 * most;
     g.groups = (int32_t)std::min(most, g.shared ? blocks : ceil_div(blocks, 8));
   } else if (m <= kSkinnyRows) {

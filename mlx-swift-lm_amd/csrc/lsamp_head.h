@@ -178,13 +178,13 @@ struct EpiLinearInt8 : EpiLinear {
   const float* w_scale;  // [n]
 };
 
-// A product of few rows that are kept in LDS: up to 64, of 128 KB in slabs of 128 bytes.
+// A product of few rows that are kept in LDS: up to 64, of 128 KB in rows of 256 bytes.
 struct ResidentPlan {
   int32_t m, k;
   int32_t groups;  // work-groups
   int32_t shared;  // the waves of one share a block of columns
   int32_t fused;   // x is of the block's type (at most 8,192 values), else 8-bit integers in
-                   // aligned rows of whole slabs, zero behind their ends
+                   // aligned rows of multiples of 256 bytes, zero behind their ends
   const void* x;
   int64_t ld_x;
   const void* w;

@@ -84,15 +84,15 @@ Operand operand(const void* p, int64_t ld, int32_t rows, int32_t cols, int eb) {
 // us with rows 8,208 bytes apart, 128 with rows 8,320 apart).
 int64_t row_chunks(int64_t cols, int eb) { return round_up(cols, 16 / eb); }
 int64_t row_pitch(int64_t cols, int eb) { return round_up(cols, 128 / eb); }
-// Lays the operand out, if it has to be; `slabs`: in rows of whole slabs, also where
-// its own are chunks.
-MatrixRef packed(Arena& ws, Operand& o, int eb, bool slabs = false) {
-  if ((!o.chunked || slabs) && !o.packed) {
-    const int64_t pitch = row_pitch(o.ref.cols, eb);
+// Lays the operand out, if it has to be; `rows_of`: in rows of so many bytes, zeros
+// behind their ends, also where its own are chunks.
+MatrixRef packed(Arena& ws, Operand& o, int eb, int64_t rows_of = 0) {
+  if ((!o.chunked || rows_of) && !o.packed) {
+    const int64_t pitch = rows_of ? round_up(o.ref.cols, rows_of / eb) : row_pitch(o.ref.cols, eb);
     void* dst = ws.take((int64_t)o.ref.rows * pitch * eb);
     o.packed = true;
     o.pack = PackPlan{o.ref.p,    o.ref.ld,   dst, pitch, o.ref.rows,
-                      o.ref.cols, (int32_t)(slabs ? pitch : row_chunks(o.ref.cols, eb))};
+                      o.ref.cols, (int32_t)(rows_of ? pitch : row_chunks(o.ref.cols, eb))};
   }
   return o.packed ? MatrixRef{o.pack.dst, o.pack.dst_ld, o.pack.rows, o.pack.dst_cols} : o.ref;
 }

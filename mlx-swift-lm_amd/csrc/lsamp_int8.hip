@@ -28,6 +28,10 @@ struct LinearInt8 : Linear {
   __device__ __forceinline__ v4f scaled(v4i v, float xs, v4f ws) const {
     return __builtin_convertvector(v, v4f) * (ws * xs);
   }
+  __device__ __forceinline__ v4f result(v4f v, v4f b, v4f res) const {
+    v = activate(activation, softcap, v + b);
+    return residual ? v + res : v;
+  }
   __device__ __forceinline__ void put(int r, int c, v4i v, int) const {
     finish(r, c, scaled(v, x_scale[r], w_at(c)), bias_at(c), residual_at(r, c));
   }
@@ -129,7 +133,13 @@ int launch_skinny(const GemmPlan& g, const LinearInt8& e, void* stream) {
 // 16 of its rows straight into fragments, kDepth slabs ahead and from one block of 16
 // columns to the next (k_skinny reads a slab of x beside every slab of W).  WK 1: a wave
 // has blocks of its own, for outputs that are many of them for all waves; 8: the waves
-// share a block, its slabs in turn, and join their sums.
+// share a block, its slabs in turn, and join their sums.  ONCE: every work-group has one
+// block, and a wave at most kDepth slabs.
+//
+// LINES: the eight waves' blocks lie side by side, and rows of 128 columns are stored
+// together, from LDS, and past the L2: left there, 19 MB of them are written back when the
+// kernel ends, after the last of W has been read (64 x 2048 x 151936: 74 us so, stored
+// past it 66; 56 without any stores).
 //
 // A row of W ends anywhere: the last slab's chunks are read from the row's last 16 bytes
 // where they would pass its end, and moved down; what lies behind meets zeros of x.
@@ -145,17 +155,22 @@ __device__ __forceinline__ v4i moved_down(v4i v, int bytes) {
   return v;
 }
 
-template <int MF, int WK, int KB, bool FUSED>
+template <int MF, int WK, int KB, bool FUSED, bool ONCE, bool LINES>
 __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentPlan g, LinearInt8 e) {
   constexpr int kThreads = kResidentWaves * kWave;
-  constexpr int kDepth = WK == 1 ? 8 : 4;
+  constexpr int kDepth = WK == 1 || ONCE ? 8 : 4;
+  constexpr int kLine = kResidentWaves * 16 + 8;  // elements of a row of results in LDS
+  static_assert(!LINES || (WK == 1 && DT != LSAMP_DTYPE_F32), "blocks of 16-bit elements side by side");
+  __shared__ __attribute__((aligned(16))) S lines[LINES ? MF * 16 : 1][LINES ? kLine : 1];
   __shared__ __attribute__((aligned(1024))) char xs[KB * 1024];
   __shared__ float scales[MF * 16];
   __shared__ v4i sums[WK > 1 ? WK - 1 : 1][WK > 1 ? MF : 1][kWave];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int slabs = (g.k + 127) / 128, pitch = slabs * 128;
-  const auto place = [&](int r, int chunk) { return r * pitch + ((chunk & ~7) | ((chunk ^ r) & 7)) * 16; };
+  const int slabs = (g.k + 127) / 128, pitch = (g.k + 255) / 256 * 256;
+  // (16 rows' chunks of one number fall on all banks)
+  const auto turned = [](int r, int chunk) { return (chunk & ~15) | ((chunk ^ r) & 15); };
+  const auto place = [&](int r, int chunk) { return r * pitch + turned(r, chunk) * 16; };
 
   // This wave's blocks of 16 columns, and its slabs of one: first, first + WK, ...
   const int blocks = (e.n + 15) / 16;
@@ -177,23 +192,24 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
     for (int kk = 0; kk < 2; ++kk)
       to[kk] = load_chunk<kInt8>(p + min(slab * 128 + kk * 64 + at, g.k - 16));
   };
+  const auto fill = [&] {
 #pragma unroll
-  for (int u = 0; u < kDepth; ++u) load(ring[u], block0, u);
-
+    for (int u = 0; u < kDepth; ++u)
+      if (!ONCE || u < steps) load(ring[u], block0, u);
+  };
   if constexpr (FUSED) {
     __shared__ uint32_t tops[2][kResidentWaves];
     constexpr int kChunks = 2;  // of eight values a thread: 8,192 in all
     constexpr int kPer = 8 / kChunkOf<DT>;
-    for (int r = 0; r < g.m; ++r) {
+    v4i raw[kChunks][kPer];
+    const auto fetch = [&](int r) {
       const char* const x = (const char*)g.x + (int64_t)r * g.ld_x * El<DT>::kBytes;
-      v4i raw[kChunks][kPer];
 #pragma unroll
       for (int i = 0; i < kChunks; ++i)
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
           const int c = (i * kThreads + (int)threadIdx.x) * 8 + h * kChunkOf<DT>;
-          raw[i][h] = v4i{0, 0, 0, 0};
-          if (c + kChunkOf<DT> <= g.k) raw[i][h] = load_chunk<DT>(x + (int64_t)c * El<DT>::kBytes);
+          raw[i][h] = load_chunk<DT>(x + (int64_t)min(c, g.k - kChunkOf<DT>) * El<DT>::kBytes);
         }
       if (g.k % kChunkOf<DT>) {  // (where the row ends)
 #pragma unroll
@@ -204,6 +220,14 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
             if (c < g.k && c + kChunkOf<DT> > g.k) raw[i][h] = load_chunk_end<DT>(x, c, g.k);
           }
       }
+    };
+    const auto value = [&](int i, int k, S v) {  // (0 past the row's end)
+      return (i * kThreads + (int)threadIdx.x) * 8 + k < g.k ? (float)v : 0.f;
+    };
+    // (x first: loads are waited for in their order, and W's come from far)
+    fetch(0);
+    fill();
+    for (int r = 0; r < g.m; ++r) {
       float v[kChunks][8];
       uint32_t top = 0;
 #pragma unroll
@@ -212,7 +236,7 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
         __builtin_memcpy(el, raw[i], 16 * kPer);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          v[i][k] = (float)el[k];
+          v[i][k] = value(i, k, el[k]);
           top = max(top, magnitude(v[i][k]));
         }
       }
@@ -232,15 +256,17 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
           if (c < pitch) *(uint64_t*)(xs + place(r, c / 16) + c % 16) = q;
         }
       }
+      if (r + 1 < g.m) fetch(r + 1);
     }
   } else {
-    // (rows of whole slabs, straight to LDS: 64 chunks in order an instruction, so the
+    fill();
+    // (rows of 256 bytes, straight to LDS: 64 chunks in order an instruction, so the
     // chunks that the order asks for are read)
     const int chunks = pitch / 16, last = g.m * chunks - 1;
     for (int u = wave; u * kWave <= last; u += kResidentWaves) {
       const int i = min(u * kWave + lane, last), r = i / chunks, c = i - r * chunks;
       __builtin_amdgcn_global_load_lds(
-          LSAMP_GLOBAL((const char*)g.x + (int64_t)r * g.ld_x + ((c & ~7) | ((c ^ r) & 7)) * 16),
+          LSAMP_GLOBAL((const char*)g.x + (int64_t)r * g.ld_x + turned(r, c) * 16),
           LSAMP_LDS(xs + u * 1024), 16, 0, 0);
     }
     if ((int)threadIdx.x < g.m) scales[threadIdx.x] = e.x_scale[threadIdx.x];
@@ -274,7 +300,8 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
     const int r = j * 16 + row, c = block * 16 + (lane >> 4) * 4;
     if (r < g.m && c < e.n) e.finish(r, c, e.scaled(v, scales[r], o.ws), o.b, res);
   };
-  for (int block = block0; block < blocks; block += block_step) {
+  // (LINES: every wave stays until the last of them has stored)
+  for (int block = block0; (LINES ? block - wave : block) < blocks; block += block_step) {
     Ends o;
     if (WK == 1 || wave < MF) o = ends(block, WK == 1 ? 0 : wave);
     for (int turn = 0; turn < turns; ++turn) {
@@ -294,17 +321,40 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
             }
           }
 #pragma unroll
-          for (int kk = 0; kk < 2; ++kk)
+          for (int kk = 0; kk < 2; ++kk) {
+            v4i x[MF];
 #pragma unroll
-            for (int j = 0; j < MF; ++j) {
-              const v4i x = *(const v4i*)(xs + place(x_row[j], slab * 8 + kk * 4 + (lane >> 4)));
-              mma<kInt8>(acc[j], w[kk], x);
-            }
+            for (int j = 0; j < MF; ++j)
+              x[j] = *(const v4i*)(xs + place(x_row[j], slab * 8 + kk * 4 + (lane >> 4)));
+#pragma unroll
+            for (int j = 0; j < MF; ++j) mma<kInt8>(acc[j], w[kk], x[j]);
+          }
         }
-        load(ring[u], to_block, to_turn * kDepth + u);
+        if constexpr (!ONCE) load(ring[u], to_block, to_turn * kDepth + u);
       }
     }
-    if constexpr (WK == 1) {
+    if constexpr (LINES) {
+#pragma unroll
+      for (int j = 0; j < MF; ++j) {
+        const v4f v = e.result(e.scaled(acc[j], scales[x_row[j]], o.ws), o.b, o.res[j]);
+        *(v4e*)&lines[j * 16 + row][wave * 16 + (lane >> 4) * 4] = __builtin_convertvector(v, v4e);
+      }
+      __syncthreads();
+      const int c0 = (block - wave) * 16;
+#pragma unroll
+      for (int i = 0; i < MF * 16 * 16 / kThreads + (MF == 1); ++i) {
+        const int q = i * kThreads + (int)threadIdx.x, r = q / 16, c = q % 16 * 8;
+        if (r >= g.m || c0 + c >= e.n) continue;
+        S* const to = (S*)e.out + (int64_t)r * e.ld_out + c0 + c;
+        if (c0 + c + 8 <= e.n) {
+          const v4i v = *(const v4i*)&lines[r][c];
+          asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1 nt" : : "v"(to), "v"(v) : "memory");
+        } else {
+          for (int k = 0; c0 + c + k < e.n; ++k) to[k] = lines[r][c + k];
+        }
+      }
+      __syncthreads();
+    } else if constexpr (WK == 1) {
 #pragma unroll
       for (int j = 0; j < MF; ++j) put(j, block, acc[j], o, o.res[j]);
     } else {
@@ -331,10 +381,21 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
 template <int MF, int KB, bool FUSED>
 int launch_resident(const ResidentPlan& g, const LinearInt8& e, hipStream_t st) {
   const dim3 grid((unsigned)g.groups), threads(kResidentWaves * kWave);
-  if (g.shared)
-    hipLaunchKernelGGL((k_resident<MF, 8, KB, FUSED>), grid, threads, 0, st, g, e);
-  else
-    hipLaunchKernelGGL((k_resident<MF, 1, KB, FUSED>), grid, threads, 0, st, g, e);
+  const bool once = g.groups >= (e.n + 15) / 16 && g.k <= 8 * 8 * 128;
+  if (g.shared) {
+    if (once)
+      hipLaunchKernelGGL((k_resident<MF, 8, KB, FUSED, true, false>), grid, threads, 0, st, g, e);
+    else
+      hipLaunchKernelGGL((k_resident<MF, 8, KB, FUSED, false, false>), grid, threads, 0, st, g, e);
+    return (int)hipGetLastError();
+  }
+  if constexpr (DT != LSAMP_DTYPE_F32 && KB == 128) {
+    if (!e.wide) {
+      hipLaunchKernelGGL((k_resident<MF, 1, KB, FUSED, false, true>), grid, threads, 0, st, g, e);
+      return (int)hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((k_resident<MF, 1, KB, FUSED, false, false>), grid, threads, 0, st, g, e);
   return (int)hipGetLastError();
 }
 
@@ -377,7 +438,7 @@ template <>
 int Int8Ops<DT>::resident_linear(const ResidentPlan& g, const EpiLinearInt8& p, void* stream) {
   const LinearInt8 e = epilogue(p);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const bool small = (int64_t)g.m * ((g.k + 127) / 128 * 128) <= 16 << 10;
+  const bool small = (int64_t)g.m * ((g.k + 255) / 256 * 256) <= 16 << 10;
   if (g.m > 32) return launch_resident<4, 128, false>(g, e, st);
   if (g.m > 16) return launch_resident<2, 128, false>(g, e, st);
   if (!small) return launch_resident<1, 128, false>(g, e, st);

@@ -82,9 +82,9 @@ def test_norm_backward_workspace(lib):
 def test_linear_int8_refusals(lib):
     assert lib.lsamp_linear_int8_workspace(None) == I
     assert int8(lib) == 0 and int8(lib, rows=8) >= 8 * 64 + 8 * 4
-    # (few rows are kept on the chip in rows of whole slabs of 128 bytes)
-    assert int8(lib, x_scale=P, in_features=128, x_stride=128, weight_stride=128) == 0
-    assert int8(lib, x_scale=P) >= 4 * 128
+    # (few rows are kept on the chip in rows of multiples of 256 bytes)
+    assert int8(lib, x_scale=P, in_features=256, x_stride=256, weight_stride=256) == 0
+    assert int8(lib, x_scale=P) >= 4 * 256
     for kw, want in [(dict(rows=0), S), (dict(in_features=0), S), (dict(out_features=0), S),
                      (dict(in_features=131072, x_stride=131072, weight_stride=131072), S),
                      (dict(dtype=3), D), (dict(out_dtype=_ffi.DTYPE_F16), D),
