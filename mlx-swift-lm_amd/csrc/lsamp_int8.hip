@@ -174,13 +174,6 @@ int launch_skinny(const GemmPlan& g, const LinearInt8& e, void* stream) {
 // FUSED: x is of the block's own type, and every work-group quantises it as it brings
 // it (a launch less, for one row or few: 2 to 3 us).
 constexpr int kResidentWaves = 8;
-__device__ __forceinline__ v4i moved_down(v4i v, int bytes) {
-  unsigned __int128 w;
-  __builtin_memcpy(&w, &v, 16);
-  w >>= 8 * bytes;
-  __builtin_memcpy(&v, &w, 16);
-  return v;
-}
 
 template <int MF, int WK, int KB, bool FUSED, bool ONCE, bool LINES>
 __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentPlan g, LinearInt8 e) {

@@ -453,6 +453,11 @@ class PreparedOrthogonalize(PreparedCall):
         a.out, a.out_stride, a.out_batch_stride = self._stack("out", self.out, x.shape, out_dtype)
         self._bind(a)
 
+    def weigh(self, *, scale: float, keep: float) -> None:
+        """Another scale and keep for the launches that follow (a learning rate's
+        schedule; a captured graph keeps those of its capture)."""
+        self.args.scale, self.args.keep = scale, keep
+
     def _stack(self, name, t, shape, dtype):
         if t.shape != shape:
             raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
