@@ -254,7 +254,15 @@ struct OrthPlan {
 // The tile shape for `batch` products of m x n over `slabs` slabs, one round of the
 // device after the other (see choose).  192 x 192 tiles, 0.95 us a slab, are for symmetric
 // products that they spread over the device (4096: 253 tiles).
-Choice choose_batch(int64_t m, int64_t n, int64_t slabs, double bytes, int64_t batch, bool symmetric) {
+// A launch of few tiles is bound by what a CU loads, some 70 GB/s: 32 x 32 tiles, where
+// there is a CU for each, have half the bytes of 64 x 64 ones (`rows_out`: both operands
+// have rows along the output; the A of four 256 x 256 float32
+// ones 7.8 us and 5.4).
+Choice choose_batch(int64_t m, int64_t n, int64_t slabs, double bytes, int64_t batch, bool symmetric,
+                    bool rows_out) {
+  const int64_t fine = ceil_div(n, kTileSide[kTile32x8]);
+  if (rows_out && batch * (symmetric ? fine * (fine + 1) / 2 : ceil_div(m, kTileSide[kTile32x8]) * fine) <= 256)
+    return Choice{kTile32x8, 1, 0.0};
   Choice best = choose(m, n, slabs, LSAMP_DTYPE_F16, bytes, false, kChunked, batch, symmetric);
   if (symmetric) {
     const int64_t across = ceil_div(n, kTileSide[kTile192]);
@@ -329,9 +337,9 @@ lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* 
 
   const int64_t turns = P.wide ? 3 : 1;  // (products of parts)
   const double parts = P.wide ? 2.0 : 1.0;
-  P.gram = choose_batch(p, p, turns * slabs_of(q, eb), 2 * eb * parts, batch, true);
-  P.poly = choose_batch(p, p, turns * slabs_of(p, eb), 3 * eb * parts, batch, true);
-  P.update = choose_batch(M, N, turns * slabs_of(p, eb), 4 * eb, batch, false);
+  P.gram = choose_batch(p, p, turns * slabs_of(q, eb), 2 * eb * parts, batch, true, !P.tall);
+  P.poly = choose_batch(p, p, turns * slabs_of(p, eb), 3 * eb * parts, batch, true, true);
+  P.update = choose_batch(M, N, turns * slabs_of(p, eb), 4 * eb, batch, false, P.tall);
   const MatrixRef x{P.x[0][0], N, M, N}, A{gram[0], p, p, p}, B{poly[0], p, p, p};
   const int64_t rest_x = (char*)P.x[0][1] - (char*)P.x[0][0];
   const auto rest = [&](void* const* two) { return (char*)two[1] - (char*)two[0]; };

@@ -90,6 +90,11 @@ constexpr int kChunkOf = 16 / El<DT>::kBytes;  // elements of a 16-byte chunk
 template <int DT>
 constexpr int kSlabOf = kSlabBytes / El<DT>::kBytes;  // reduction steps of a slab
 
+// Waits until none of this wave's LDS operations are under way.
+__device__ __forceinline__ void wait_lds() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // (lgkmcnt 0; the others at their most)
+}
+
 // Every wave's barrier, with no memory access moved across it by the compiler
 // (and no wait: what has to be done by then is waited for by wait_loads).
 __device__ __forceinline__ void barrier() {
@@ -278,6 +283,7 @@ struct Side {
   static constexpr int kUnits = ROWS / 8 / WAVES;
   static constexpr int kBytes = ROWS * kSlabBytes;
   static_assert(ROWS % (8 * WAVES) == 0, "whole units a wave");
+  static_assert(!KMAJ || ROWS % kSlab == 0, "whole blocks of 128 bytes of columns");
 
   const char* base;         // the slab's first element (the same for every lane)
   int64_t step;             // bytes from slab to slab
@@ -418,6 +424,9 @@ struct LooseSide : Side<DT, KMAJ, ROWS, WAVES> {
   }
   // Slab `slab` to registers; `rows`: k-major rows in all.
   __device__ __forceinline__ void hold(int slab, int rows, int wave, int lane) {
+    hold(held, slab, rows, wave, lane);
+  }
+  __device__ __forceinline__ void hold(v4i (&held)[kUnits], int slab, int rows, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       if constexpr (!KMAJ) {
@@ -430,7 +439,8 @@ struct LooseSide : Side<DT, KMAJ, ROWS, WAVES> {
       }
     }
   }
-  __device__ __forceinline__ void place(char* lds, int wave, int lane) {
+  __device__ __forceinline__ void place(char* lds, int wave, int lane) { place(held, lds, wave, lane); }
+  __device__ __forceinline__ void place(const v4i (&held)[kUnits], char* lds, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i)
       *(v4i*)(lds + (wave * kUnits + i) * 1024 + lane * 16) = held[i];
@@ -491,6 +501,8 @@ __device__ __forceinline__ TileAt tile_at(int bid, const BatchPlan& g) {
 // GROUPS: so many slabs are multiplied at a time, each by its own WM x WN waves,
 // and the groups' sums joined through LDS at the end: for products with fewer
 // tiles than the device has CUs, whose time is the length of the reduction.
+// STAGES 3: two slabs of a group on their way, for short reductions, whose time is the
+// latency of their loads one after the other (8-bit 301 x 1537 x 2053 18.4 -> 16.7 us).
 // LOOSE: operands that are no 16-byte chunks, through registers (301 x 1537 x 2053
 // f16: 16 us; 304 x 1536 x 2048 of whole chunks 10).
 // Measured, bf16: the 256 x 256 tile without an epilogue 1.47 PFLOP/s on random
@@ -511,7 +523,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
   using A = std::conditional_t<LOOSE, LooseSide<DT, AK, BM, kWaves>, Side<DT, AK, BM, kWaves>>;
   using B = std::conditional_t<LOOSE, LooseSide<DT, BK, BN, kWaves>, Side<DT, BK, BN, kWaves>>;
-  static_assert(!LOOSE || STAGES == 2, "two buffers");
+  static_assert(!LOOSE || STAGES >= 2, "two buffers");
   constexpr int kStage = A::kBytes + B::kBytes;
   __shared__ __attribute__((aligned(1024))) char lds[2 * GROUPS * kStage];
 
@@ -616,6 +628,41 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
       for (int i = 0; i < FN; ++i) mma<DT>(acc[i][j], fb[i], fa[j]);
   };
 
+  // The groups' sums to the first one's waves, and the epilogue.
+  const auto join_groups = [&] {
+    if constexpr (GROUPS > 1) {
+      // [group - 1][fragment][lane] of every wave; the first group adds them up in order
+      constexpr int kFrags = FM * FN;
+      __syncthreads();
+      V* sums = (V*)lds;
+      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + WN * BM * 8 <= (int)sizeof(lds),
+                    "the sums and an epilogue's pair of floats for every row and wave");
+      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + kWaves * FN * 1024 <= (int)sizeof(lds),
+                    "the sums and an epilogue's 16 rows for every wave");
+      if (group > 0) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            sums[(((group - 1) * kWaves + wave) * kFrags + i * FM + j) * kWave + lane] = acc[i][j];
+      }
+      __syncthreads();
+      if (group > 0) {
+        for (int k = 0; k < Epi::kBarriers; ++k) __syncthreads();  // (those of the epilogue)
+        return;
+      }
+      for (int k = 0; k < GROUPS - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            acc[i][j] += sums[((k * kWaves + wave) * kFrags + i * FM + j) * kWave + lane];
+      epi.template run<FM, FN, BM, BN, WM, WN>(
+          acc, m0, n0, at, wm, wn, lane,
+          lds + (GROUPS - 1) * kWaves * kFrags * kWave * 16);
+    }
+  };
+
   if constexpr (STAGES == 0) {
     const auto settle = [] {
       __builtin_amdgcn_sched_barrier(0);
@@ -673,6 +720,68 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
       if (t + 1 < slabs) read(fa[0], fb[0], (t + 1) & 1, 0);
       multiply(fa[1], fb[1]);
     }
+  } else if constexpr (STAGES == 3) {
+    static_assert(DT != LSAMP_DTYPE_F32 && GROUPS > 1, "the products of a slab at once");
+    const auto step = [&](int buffer) {
+      v4i fa[2][FM], fb[2][FN];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) read(fa[kk], fb[kk], buffer, kk);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) multiply(fa[kk], fb[kk]);
+    };
+    // (every wave makes as many turns as the first group: their barriers)
+    if constexpr (LOOSE) {
+      v4i ha[2][A::kUnits], hb[2][B::kUnits];
+      const auto hold = [&](int t, int set) {
+        a.hold(ha[set], slab0 + t, g.a.rows, wave, lane);
+        b.hold(hb[set], slab0 + t, g.b.rows, wave, lane);
+      };
+      const auto put = [&](int buffer, int set) {
+        a.place(ha[set], lds + buffer * kStage, wave, lane);
+        b.place(hb[set], lds + buffer * kStage + A::kBytes, wave, lane);
+      };
+      // slab t is in LDS, t + GROUPS in set `set`, t + 2 GROUPS in the other
+      const auto turn = [&](int t, int buffer, int set) {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lds();
+        barrier();
+        if (t < slabs) step(buffer);
+        const int other = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
+        if (t + GROUPS < slabs) put(other, set);
+        if (t + 3 * GROUPS < slabs) hold(t + 3 * GROUPS, set);
+      };
+      if (group < slabs) hold(group, 0);
+      if (group + GROUPS < slabs) hold(group + GROUPS, 1);
+      if (group < slabs) put(group, 0);
+      if (group + 2 * GROUPS < slabs) hold(group + 2 * GROUPS, 0);
+      for (int t = group; t - group < slabs; t += 2 * GROUPS) {
+        turn(t, group, 1);
+        if (t + GROUPS - group < slabs) turn(t + GROUPS, group + GROUPS, 0);
+      }
+    } else {
+      constexpr int kFetch = A::kUnits + B::kUnits;
+      if (group < slabs) fetch(group, group);
+      if (group + GROUPS < slabs) fetch(group + GROUPS, group + GROUPS);
+      int buffer = group;
+      for (int t = group; t - group < slabs; t += GROUPS) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + GROUPS < slabs)
+          wait_loads<kFetch>();
+        else
+          wait_loads<0>();
+        barrier();
+        if (t < slabs) step(buffer);
+        if (t + 2 * GROUPS - group < slabs) {  // (the same for all: the buffer is read by then)
+          __builtin_amdgcn_sched_barrier(0);
+          wait_lds();
+          barrier();
+          if (t + 2 * GROUPS < slabs) fetch(t + 2 * GROUPS, buffer);
+        }
+        buffer = buffer < GROUPS ? buffer + GROUPS : buffer - GROUPS;
+      }
+    }
+    join_groups();
+    return;
   } else {
     // ANY: float32 values that may not be finite.
     const auto reduce = [&](auto any) {
@@ -742,35 +851,7 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
       }
     }
     if constexpr (GROUPS > 1) {
-      // [group - 1][fragment][lane] of every wave; the first group adds them up in order
-      constexpr int kFrags = FM * FN;
-      __syncthreads();
-      V* sums = (V*)lds;
-      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + WN * BM * 8 <= (int)sizeof(lds),
-                    "the sums and an epilogue's pair of floats for every row and wave");
-      static_assert((GROUPS - 1) * kWaves * kFrags * kWave * 16 + kWaves * FN * 1024 <= (int)sizeof(lds),
-                    "the sums and an epilogue's 16 rows for every wave");
-      if (group > 0) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FM; ++j)
-            sums[(((group - 1) * kWaves + wave) * kFrags + i * FM + j) * kWave + lane] = acc[i][j];
-      }
-      __syncthreads();
-      if (group > 0) {
-        for (int k = 0; k < Epi::kBarriers; ++k) __syncthreads();  // (those of the epilogue)
-        return;
-      }
-      for (int k = 0; k < GROUPS - 1; ++k)
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FM; ++j)
-            acc[i][j] += sums[((k * kWaves + wave) * kFrags + i * FM + j) * kWave + lane];
-      epi.template run<FM, FN, BM, BN, WM, WN>(
-          acc, m0, n0, at, wm, wn, lane,
-          lds + (GROUPS - 1) * kWaves * kFrags * kWave * 16);
+      join_groups();
       return;
     }
   }

@@ -40,8 +40,8 @@ enum GemmRoles { kRolesNT = 0, kRolesNN = 1, kRolesTN = 2 };
 // Tile shapes.  256 x 256, 128 x 128 and 64 x 64; 128 and 64 with two and four
 // slabs of the reduction at a time, for launches of at most a tile a CU; loose ones
 // for operands whose rows are no 16-byte chunks; the products of at most 16, 32 or 64
-// rows (lsamp_skinny.h), 64 or 16 columns a work-group; and 192 x 192 for symmetric
-// products.
+// rows (lsamp_skinny.h), 64 or 16 columns a work-group; 192 x 192 for symmetric products,
+// and 32 x 32 with eight slabs at a time for batches of at most one such tile a CU.
 enum GemmTile {
   kTile256,
   kTile128,
@@ -54,9 +54,10 @@ enum GemmTile {
   kSkinny64,
   kSkinny16,
   kTile192,
+  kTile32x8,
 };
-constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16, 192};
-constexpr int kTileWavesM[] = {2, 2, 2, 2, 2, 2, 2, 2, 1, 1, 2};  // waves that share a tile's rows
+constexpr int kTileSide[] = {256, 128, 64, 128, 64, 128, 64, 64, 64, 16, 192, 32};
+constexpr int kTileWavesM[] = {2, 2, 2, 2, 2, 2, 2, 2, 1, 1, 2, 1};  // waves that share a tile's rows
 constexpr int kSkinnyRows = 64;
 
 // Epilogues.  `m`, `n`: rows and columns that exist.

@@ -132,10 +132,10 @@ int launch(GemmTile tile, const GemmPlan& g, const E& e, void* stream) {
     case kTile128: LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, false); break;
     case kTile64: LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, false); break;
     case kTile128x2: LSAMP_TILE(512, 128, 128, 2, 2, 2, 2, false); break;
-    case kTile64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, false); break;
+    case kTile64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 3, 4, false); break;
     case kLoose128: LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, true); break;
     case kLoose64: LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, true); break;
-    case kLoose64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, true); break;
+    case kLoose64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 3, 4, true); break;
     default: return (int)hipErrorInvalidValue;
   }
   return (int)hipGetLastError();

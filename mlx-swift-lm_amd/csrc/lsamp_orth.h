@@ -55,7 +55,8 @@ struct EpiOrthUpdate {
 
 int launch_orth_start(const OrthStart& p, int batch, int in_dtype, void* stream);
 
-// WIDE: A and B in two parts.  Tiles: 256, 128 and 64, the latter grouped too; 192 for
+// WIDE: A and B in two parts.  Tiles: 256, 128 and 64, the latter grouped too; 32x8 where
+// both operands have rows along the output (not a tall gram, not a wide update); 192 for
 // gram and poly.
 template <bool WIDE>
 struct OrthOps {

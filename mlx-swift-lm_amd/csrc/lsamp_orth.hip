@@ -343,7 +343,13 @@ int launch(GemmTile tile, const BatchPlan& g, const E& e, void* stream) {
     case kTile128: LSAMP_TILE(256, 128, 128, 2, 2, 2, 1, false); break;
     case kTile64: LSAMP_TILE(256, 64, 64, 2, 2, 2, 1, false); break;
     case kTile128x2: LSAMP_TILE(512, 128, 128, 2, 2, 2, 2, false); break;
-    case kTile64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 2, 4, false); break;
+    case kTile64x4: LSAMP_TILE(1024, 64, 64, 2, 2, 3, 4, false); break;
+    case kTile32x8:
+      if constexpr (!AK && !BK) {
+        LSAMP_TILE(512, 32, 32, 1, 1, 3, 8, false);
+        break;
+      }
+      return (int)hipErrorInvalidValue;
     case kTile192:
       if constexpr (std::is_base_of_v<EpiSymmetric, E>) {
         LSAMP_TILE(512, 192, 192, 2, 4, 0, 1, false);
