@@ -527,8 +527,9 @@ Shape shape_of(int rows, int cols) {
   if (cols <= 4096) return kBlock2;
   return cols <= 8192 ? kWide1 : cols <= 16384 ? kWide2 : kLong;
 }
-// Whether the columns' sums are taken beside the rows, in the same launch.
-bool few(int rows, int cols) { return rows <= kFew && cols <= 4096; }
+// Whether the columns' sums are taken beside the rows, in the same launch: not where the
+// rows' gradients are written over the d_out that the columns read.
+bool few(int rows, int cols, bool in_place) { return rows <= kFew && cols <= 4096 && !in_place; }
 int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
 int threads_of(Shape s) { return s >= kWide1 ? 1024 : kBlock; }
 
@@ -566,7 +567,7 @@ int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
   const Shape s = shape_of(p.rows, p.cols);
   const bool sums = p.d_weight || p.d_bias;
   const int64_t groups = ((int64_t)p.rows + rows_per_group(s) - 1) / rows_per_group(s);
-  if (sums && few(p.rows, p.cols)) {
+  if (sums && !p.chunks) {
     const int row_groups = p.d_x ? (int)groups : 0;
     const dim3 all((unsigned)(row_groups + (p.cols + 15) / 16));
 #define K(T, V) hipLaunchKernelGGL((k_norm_backward_few<E, T, V>), all, dim3(kBlock), 0, st, p, row_groups)
@@ -581,11 +582,12 @@ int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
   const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups, s));
   const dim3 block((unsigned)threads_of(s));
   if (s == kLong) {
-    if (p.d_x) hipLaunchKernelGGL((k_norm_backward<E, 1024, 1, false, true>), grid, block, 0, st, p);
+    // (the sums first: d_x may be d_out itself)
     if (sums)
       hipLaunchKernelGGL((k_norm_sums<E>),
                          dim3((unsigned)((p.cols + kBlock - 1) / kBlock), (unsigned)p.chunks),
                          dim3(kBlock), 0, st, p);
+    if (p.d_x) hipLaunchKernelGGL((k_norm_backward<E, 1024, 1, false, true>), grid, block, 0, st, p);
   } else if (sums) {
 #define K(T, V, L) hipLaunchKernelGGL((k_norm_backward<E, T, V, !(L), L>), grid, block, 0, st, p)
     LSAMP_SHAPES(s, K, )
@@ -623,8 +625,8 @@ int quantize(const QuantizePlan& p, hipStream_t st) {
 }  // namespace
 
 // Shares of the columns' sums: a work-group's.
-int norm_chunks(int rows, int cols) {
-  if (few(rows, cols)) return 0;
+int norm_chunks(int rows, int cols, bool in_place) {
+  if (few(rows, cols, in_place)) return 0;
   const Shape s = shape_of(rows, cols);
   if (s == kLong) return rows < 64 ? 1 : rows / 32 < 256 ? rows / 32 : 256;
   const int groups = (rows + rows_per_group(s) - 1) / rows_per_group(s);

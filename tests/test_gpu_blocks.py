@@ -114,9 +114,10 @@ def test_layer_norm_nan_and_infinity_stay_in_their_rows(ctx, rows, n):
     assert torch.equal(got[keep], y[keep])
 
 
-def test_layer_norm_in_place(ctx):
+@pytest.mark.parametrize("rows,n", [(50, 777), (600, 4000), (1200, 300), (20, 9000), (40, 17000)])
+def test_layer_norm_in_place(ctx, rows, n):
     rng = np.random.default_rng(8)
-    x, r = (H.matrix(rng, 50, 777, torch.float16) for _ in range(2))
+    x, r = (H.matrix(rng, rows, n, torch.float16) for _ in range(2))
     p = ctx.prepare_layer_norm(x, want_stats=True)
     p.launch()
     d = p.out.clone()
@@ -128,7 +129,8 @@ def test_layer_norm_in_place(ctx):
     into = d.clone()
     s = ctx.prepare_layer_norm_backward(into, x, mean=p.mean, rstd=p.rstd, residual=r, d_x=into)
     s.launch()
-    assert torch.equal(into, q.d_x) and torch.equal(s.d_weight, q.d_weight)
+    assert torch.equal(into, q.d_x)
+    H.check(s.d_weight, B.norm_grads64(d, x, p.mean, p.rstd, None, r)["d_weight"])
     z = x.clone()
     ctx.layer_norm(z, out=z)
     assert torch.equal(z, p.out)
@@ -221,6 +223,18 @@ INT8 = [
     (70, 8209, 72, "gelu", True, True, "odd"),
     (2100, 160, 2100, "none", True, True, "dense"),
     (2051, 2049, 2053, "silu", True, True, "dense"),
+    (3, 1001, 200, "gelu", True, True, "odd"),       # (quantised by every work-group)
+    (4, 1100, 16, "none", True, False, "dense"),
+    (1, 8192, 40, "none", True, False, "dense"),
+    (1, 100, 65700, "silu", True, True, "odd"),      # (a wave's own columns)
+    (9, 300, 65601, "none", True, False, "pad"),
+    (13, 1500, 32801, "silu", True, True, "odd"),    # (lines of eight waves' columns)
+    (17, 260, 33000, "relu", True, True, "dense"),
+    (64, 130, 40003, "none", False, True, "odd"),
+    (64, 2100, 300, "none", True, True, "odd"),      # (too long to be kept)
+    (40, 5000, 130, "silu", True, False, "dense"),
+    (16, 9000, 70, "none", False, False, "odd"),
+    (50, 3100, 16400, "none", True, True, "dense"),
 ]
 
 
@@ -260,7 +274,11 @@ def test_linear_int8(ctx, case, dtype):
     odd = torch.full((rows, k + 3), 9, dtype=torch.int8, device="cuda")[:, 1:1 + k]
     odd.copy_(gq)
     assert torch.equal(ctx.linear_int8(odd, w, ws, x_scale=gs, out_dtype=dt, **kw), first)
-    # float32 out, into a padded buffer whose rest is left alone
+    # into padded buffers whose rest is left alone; float32 out
+    into = torch.full((rows, n + 5), 7.0, dtype=dt, device="cuda")
+    ctx.linear_int8(x, w, ws, out=into[:, 3:3 + n], **kw)
+    assert torch.equal(into[:, 3:3 + n], first)
+    assert (into[:, :3] == 7).all() and (into[:, 3 + n:] == 7).all()
     wide = torch.full((rows, n + 5), 7.0, device="cuda")
     ctx.linear_int8(x, w, ws, out=wide[:, 2:2 + n], **kw)
     H.check(wide[:, 2:2 + n], B.int8_64(q, xs, w, ws, b, res, act, 5.0, dt, torch.float32), "float32")
@@ -309,12 +327,14 @@ def test_linear_int8_follows_linear(ctx):
     assert (off.abs() <= 1.001 * bound).all()
 
 
-def test_linear_int8_residual_in_place(ctx):
+@pytest.mark.parametrize("rows,k,n", [(40, 96, 96), (1, 96, 300), (20, 600, 33000), (300, 64, 700),
+                                      (2000, 300, 2000)])
+def test_linear_int8_residual_in_place(ctx, rows, k, n):
     rng = np.random.default_rng(5)
-    x = H.matrix(rng, 40, 96, torch.bfloat16)
-    w, ws = _quantized(rng, 96, 96, "dense")
-    y = ctx.linear_int8(x, w, ws, activation="silu", residual=x)
-    z = x.clone()
+    x, r = H.matrix(rng, rows, k, torch.bfloat16), H.matrix(rng, rows, n, torch.bfloat16)
+    w, ws = _quantized(rng, n, k, "dense")
+    y = ctx.linear_int8(x, w, ws, activation="silu", residual=r)
+    z = r.clone()
     ctx.linear_int8(x, w, ws, activation="silu", residual=z, out=z)
     assert torch.equal(y, z)
 
