@@ -133,7 +133,9 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
   const float* x_scale = a->x_scale;
   const int64_t kept_bytes = m * round_up(k, kKeptRow);
   P.kept = m <= kSkinnyRows && k >= 16 && kept_bytes <= kKeptBytes;
-  const bool fused = P.kept && !given && m <= 4 && m * (int64_t)k <= 8192;
+  // (two rows of 2048, to 2048: quantised by every work-group 5.3 us, by a launch of its own
+  // 6.1; three 6.2, four 7.1)
+  const bool fused = P.kept && !given && m <= 2 && m * (int64_t)k <= 8192;
   if (given || fused) {
     P.x = operand(a->x, ld_x, m, k, given ? 1 : eb);
   } else {
@@ -154,7 +156,8 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
     if (given && !(P.x.chunked && k % kKeptRow == 0)) x = packed(ws, P.x, 1, kKeptRow);
     ResidentPlan& g = P.resident;
     g = ResidentPlan{m, k, 0, 0, fused, x.p, x.ld, w.p, w.ld};
-    // (a work-group a CU, of little LDS two)
+    // (a work-group a CU, of little LDS two; waves share blocks that are fewer than they: one
+    // row over 16,384 columns of 4096 16 us, 1,024 work-groups of a block each 22)
     const int64_t most = kept_bytes <= 16 << 10 ? 512 : 256, blocks = ceil_div(n, 16);
     g.shared = blocks < 8 * most;
     g.groups = (int32_t)std::min(most, g.shared ? blocks : ceil_div(blocks, 8));

@@ -8,7 +8,9 @@
 // are multiplied first, another.  The tiles are lsamp_gemm.h's and lsamp_skinny.h's:
 // a slab of 128 bytes is 128 steps, an instruction takes 64 steps of a 16 x 16 tile in
 // the time that it takes 32 of 16-bit elements, so a product moves half the bytes
-// and takes half the time of a 16-bit one on either side of the roofline.
+// and takes half the time of a 16-bit one on either side of the roofline: 8192 x 4096 x
+// 4096 133 us without a residual (2.07 POP/s; a library product 127), 64 x 2048 x 151936 66,
+// one row of it 55 (5.7 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "lsamp_epilogue.h"
@@ -172,7 +174,7 @@ int launch_skinny(const GemmPlan& g, const LinearInt8& e, void* stream) {
 // where they would pass its end, and moved down; what lies behind meets zeros of x.
 //
 // FUSED: x is of the block's own type, and every work-group quantises it as it brings
-// it (a launch less, for one row or few: 2 to 3 us).
+// it (a launch less, for one row or two: 1 x 2048 x 2048 7.3 -> 4.7 us).
 constexpr int kResidentWaves = 8;
 
 template <int MF, int WK, int KB, bool FUSED, bool ONCE, bool LINES>

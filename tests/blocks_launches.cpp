@@ -70,7 +70,7 @@ namespace lsamp {
 lsamp_status set_error(lsamp_status st, const char*, ...) { return st; }
 lsamp_status clear_error() { return LSAMP_OK; }
 int32_t context_device(const lsamp_context*) { return 0; }
-int norm_chunks(int rows, int cols, bool in_place) { return rows <= 512 && cols <= 4096 && !in_place ? 0 : 5; }
+int norm_chunks(int rows, int cols, bool in_place) { return rows <= 768 && cols <= 4096 && !in_place ? 0 : 5; }
 
 int launch_norm(const NormPlan& p, int dtype, void*) {
   const int eb = bytes_of(dtype);

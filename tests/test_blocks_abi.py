@@ -81,7 +81,7 @@ def test_norm_backward_workspace(lib):
 
 def test_linear_int8_refusals(lib):
     assert lib.lsamp_linear_int8_workspace(None) == I
-    assert int8(lib) == 0 and int8(lib, rows=8) >= 8 * 64 + 8 * 4
+    assert int8(lib, rows=1) == 0 and int8(lib, rows=8) >= 8 * 64 + 8 * 4
     # (few rows are kept on the chip in rows of multiples of 256 bytes)
     assert int8(lib, x_scale=P, in_features=256, x_stride=256, weight_stride=256) == 0
     assert int8(lib, x_scale=P) >= 4 * 256

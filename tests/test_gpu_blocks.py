@@ -223,7 +223,8 @@ INT8 = [
     (70, 8209, 72, "gelu", True, True, "odd"),
     (2100, 160, 2100, "none", True, True, "dense"),
     (2051, 2049, 2053, "silu", True, True, "dense"),
-    (3, 1001, 200, "gelu", True, True, "odd"),       # (quantised by every work-group)
+    (2, 1001, 200, "gelu", True, True, "odd"),       # (quantised by every work-group)
+    (2, 4096, 16, "none", True, False, "dense"),
     (4, 1100, 16, "none", True, False, "dense"),
     (1, 8192, 40, "none", True, False, "dense"),
     (1, 100, 65700, "silu", True, True, "odd"),      # (a wave's own columns)
