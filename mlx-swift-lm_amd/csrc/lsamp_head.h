@@ -194,6 +194,7 @@ struct ResidentPlan {
 
 struct NormPlan {
   int32_t rows, cols;
+  int32_t stream;  // out is stored past the caches
   float eps;
   const void* x;
   int64_t ld_x;
@@ -207,6 +208,7 @@ struct NormPlan {
 struct NormBackwardPlan {
   int32_t rows, cols;
   int32_t chunks;  // shares of the columns' sums (norm_chunks), 0 where there are none
+  int32_t stream;  // d_x is stored past the caches
   const void* x;
   int64_t ld_x;
   const void* weight;

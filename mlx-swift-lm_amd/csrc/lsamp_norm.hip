@@ -51,8 +51,9 @@ struct Raw {
     for (int k = 0; k < 8; ++k) e[k] = (E)v;
   }
 };
+// `stream`: past the caches.
 template <typename E>
-__device__ __forceinline__ void store8(E* p, const Eight& x, int valid) {
+__device__ __forceinline__ void store8(E* p, const Eight& x, int valid, bool stream = false) {
   E e[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) e[k] = (E)x.v[k];
@@ -61,7 +62,10 @@ __device__ __forceinline__ void store8(E* p, const Eight& x, int valid) {
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
       u32x4 q;
       __builtin_memcpy(&q, (const char*)e + 16 * i, 16);
-      ((Any16<E>*)p)[i].v = q;
+      if (stream)  // (as a builtin it would be joined with the other store, and lost)
+        asm volatile("global_store_dwordx4 %0, %1, off nt" : : "v"((char*)p + 16 * i), "v"(q) : "memory");
+      else
+        ((Any16<E>*)p)[i].v = q;
     }
   } else {
 #pragma unroll
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) y.v[k] += b[i].at(k);
         }
-        store8((E*)p.out + r * p.ld_out + c, y, valid);
+        store8((E*)p.out + r * p.ld_out + c, y, valid, p.stream);
       }
     }
   }
@@ -332,7 +336,7 @@ __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const R
 #pragma unroll
           for (int k = 0; k < 8; ++k) y.v[k] += row.res[i].at(k);
         }
-        store8((E*)p.d_x + r * p.ld_dx + c, y, valid);
+        store8((E*)p.d_x + r * p.ld_dx + c, y, valid, p.stream);
       }
     }
   }

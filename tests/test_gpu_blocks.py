@@ -591,3 +591,30 @@ def test_refusals(ctx):
                 lambda: ctx.orthogonalize(x, coefficients=(3.4445, 4.7750, 2.0315))):
         with pytest.raises(_ffi.LsampError):
             bad()
+
+
+def test_layer_norm_larger_than_the_caches(ctx):
+    """Results of 256 MiB and more, stored past the caches, equal those of their parts."""
+    rng = np.random.default_rng(41)
+    rows, n = 32800, 4100
+    part = H.matrix(rng, 1025, n, torch.bfloat16)
+    x = part.repeat(32, 1)
+    assert x.shape[0] == rows
+    d = x.flip(1).contiguous()
+    w, b = (H.matrix(rng, 1, n, torch.bfloat16)[0] for _ in range(2))
+    p = ctx.prepare_layer_norm(x, weight=w, bias=b, want_stats=True)
+    p.launch()
+    q = ctx.prepare_layer_norm_backward(d, x, mean=p.mean, rstd=p.rstd, weight=w, residual=x)
+    q.launch()
+    few = ctx.prepare_layer_norm(part, weight=w, bias=b, want_stats=True)
+    few.launch()
+    back = ctx.prepare_layer_norm_backward(d[:1025], part, mean=few.mean, rstd=few.rstd, weight=w,
+                                           residual=part)
+    back.launch()
+    assert torch.equal(p.out.view(32, 1025, n), few.out.expand(32, 1025, n))
+    assert torch.equal(q.d_x.view(32, 1025, n), back.d_x.expand(32, 1025, n))
+    # 32 equal parts: 32 times their sum, with norm_grads64's roundings of all rows
+    D = H.d64(d[:1025])
+    terms = D * (H.d64(part) - H.d64(few.mean)[:, None]) * H.d64(few.rstd)[:, None]
+    err = (64 + rows // 256 + 64 + 4) * H.E * 32 * terms.abs().sum(0)
+    H.check(q.d_weight, B.rounded(32 * terms.sum(0), err, torch.bfloat16), "d_weight")
