@@ -227,13 +227,13 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, const char* p) {
 }
 #pragma clang diagnostic pop
 
-// A pointer that is the same for the wave, in scalar registers also where the compiler
-// took it through vector ones.
-__device__ __forceinline__ const char* scalar(const char* p) {
-  const uint64_t v = (uint64_t)p;
-  const uint32_t low = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-  const uint32_t high = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
-  return (const char*)((uint64_t)high << 32 | low);
+// Two bases that load_to_lds may read at once.  A vector instruction that writes a scalar
+// register has to be five wait states ahead of a memory instruction that reads it; the
+// compiler sees to that for its own loads, but does not look into the text above.  Nothing
+// but scalar arithmetic is meant to make these; should the compiler take some of it through
+// vector registers, it reads them back ahead of the wait.
+__device__ __forceinline__ void settled(const char*& a, const char*& b) {
+  asm volatile("s_nop 4" : "+s"(a), "+s"(b));
 }
 
 // 16 bytes from an address aligned to elements only.
@@ -473,18 +473,25 @@ __device__ __forceinline__ TileAt tile_at(int bid, int tm, int tn, int parts) {
 // column.
 __device__ __forceinline__ TileAt tile_at(int bid, const BatchPlan& g) {
   const int each = g.symmetric ? g.tiles_n * (g.tiles_n + 1) / 2 : g.tiles_m * g.tiles_n;
-  if (!g.symmetric) return tile_at(bid, g.tiles_m, g.tiles_n, g.parts);
-  const int total = each * g.parts;
-  const int xcd = bid & 7, q = total >> 3, rem = total & 7;
-  int i = xcd * q + (xcd < rem ? xcd : rem) + (bid >> 3);
   TileAt t;
-  t.part = i / each;
-  i -= t.part * each;
-  int n = (int)((__builtin_sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
-  n += (n + 1) * (n + 2) / 2 <= i ? 1 : 0;  // (the root is off by less than one)
-  n -= n * (n + 1) / 2 > i ? 1 : 0;
-  t.n = __builtin_amdgcn_readfirstlane(n);  // (a vector unit took the root)
-  t.m = i - t.n * (t.n + 1) / 2;
+  if (!g.symmetric) {
+    t = tile_at(bid, g.tiles_m, g.tiles_n, g.parts);
+  } else {
+    const int total = each * g.parts;
+    const int xcd = bid & 7, q = total >> 3, rem = total & 7;
+    int i = xcd * q + (xcd < rem ? xcd : rem) + (bid >> 3);
+    t.part = i / each;
+    i -= t.part * each;
+    int n = (int)((__builtin_sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
+    n += (n + 1) * (n + 2) / 2 <= i ? 1 : 0;  // (the root is off by less than one)
+    n -= n * (n + 1) / 2 > i ? 1 : 0;
+    t.n = n;
+    t.m = i - n * (n + 1) / 2;
+  }
+  // (vector units took the quotients and the root: back to scalars, for all that follows)
+  t.m = __builtin_amdgcn_readfirstlane(t.m);
+  t.n = __builtin_amdgcn_readfirstlane(t.n);
+  t.part = __builtin_amdgcn_readfirstlane(t.part);
   return t;
 }
 
@@ -579,10 +586,12 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
   }
   const auto seek = [&](int t) {
     if constexpr (kBatch) {
-      const int turn = (t >= g.slabs) + (t >= 2 * g.slabs);
-      const int64_t at_slab = t - turn * g.slabs;
-      a.base = scalar(base_a + at_slab * a.step + (turn == 2 ? g.rest_a : 0));
-      b.base = scalar(base_b + at_slab * b.step + (turn == 1 ? g.rest_b : 0));
+      const bool second = t >= g.slabs, third = t >= 2 * g.slabs;
+      // (a slab is at most 64 rows of 2^22 elements: a step has 32 bits)
+      const uint64_t at_slab = (uint32_t)(t - (third ? 2 * g.slabs : second ? g.slabs : 0));
+      a.base = base_a + at_slab * (uint32_t)a.step + (third ? g.rest_a : 0);
+      b.base = base_b + at_slab * (uint32_t)b.step + (third ? 0 : second ? g.rest_b : 0);
+      settled(a.base, b.base);
     }
   };
   const auto fetch_full = [&](int buffer) {

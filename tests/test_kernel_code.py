@@ -1,0 +1,17 @@
+"""CPU tests of the compiled kernels: hazards that the compiler does not see, because the
+instruction that has to wait is written as inline assembly."""
+from __future__ import annotations
+
+import kernel_code as K
+from lsamp import _ffi
+
+
+def test_scalar_addresses_of_loads_to_lds():
+    """A vector instruction that writes a scalar register is five wait states ahead of a
+    load that takes its address from there, on every path."""
+    loads, stale = 0, []
+    for f in K.functions(_ffi.LIB_PATH, "global_load_lds"):
+        loads += sum(c.op.startswith("global_load_lds") for c in f.code)
+        stale += [(f.name, f.code[i]) for i in K.stale_addresses(f)]
+    assert loads > 1000, "the library's loads to LDS were not found"
+    assert not stale, f"{len(stale)} loads, the first {stale[0]}"
