@@ -294,6 +294,11 @@ lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* 
   if (!std::isfinite(a->scale) || !std::isfinite(a->keep))
     return set_error(LSAMP_ERR_INVALID_ARGUMENT, "scale %g and keep %g must be finite", a->scale,
                      a->keep);
+  if (a->fast != 0 && a->fast != 1)
+    return set_error(LSAMP_ERR_INVALID_ARGUMENT, "fast %d must be 0 or 1", a->fast);
+  if (a->fast && a->out_dtype != LSAMP_DTYPE_BF16)
+    return set_error(LSAMP_ERR_DTYPE, "fast products are for a bfloat16 out, not dtype %d",
+                     a->out_dtype);
   LSAMP_CHECK(check_steps(a->coefficients, a->steps));
   const int ib = element_bytes(a->in_dtype), ob = element_bytes(a->out_dtype);
   const int32_t batch = a->batch, m = a->rows, n = a->cols;
@@ -313,7 +318,7 @@ lsamp_status plan_orth(const lsamp_orthogonalize_args* a, void* base, OrthPlan* 
 
   OrthPlan P{};
   Arena ws(base);
-  P.wide = a->out_dtype != LSAMP_DTYPE_BF16;
+  P.wide = !a->fast;
   P.tall = m > n;
   const int eb = 2;
   const int32_t M = (int32_t)round_up(m, 64), N = (int32_t)round_up(n, 64);

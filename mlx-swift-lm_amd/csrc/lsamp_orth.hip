@@ -9,16 +9,18 @@
 // The products are float16's, at the full rate of the matrix instructions.  What a
 // rounding of X does grows with the polynomial's slope at 0 in every step (485 times in
 // five of Muon's), and near-singular momenta are the rule: X in float16 alone leaves
-// 1e-2 of such a result's norm, in bfloat16 1e-1.  So X has two float16 parts, x = hi +
-// lo, 22 bits: the products take hi, the linear term a X both.  Then B's rounding is
+// 1e-2 of such a result's norm, in bfloat16 1e-1.  So X, A and B have two float16 parts, x
+// = hi + lo, 22 bits, and a product is three, hi hi + hi lo + lo hi, one after the other
+// into the same float32 sums (WIDE): 3e-7 to 2e-6 of the result's norm in five steps of
+// falling spectra and 1.3e-5 of a matrix of rank 8, float32's own steps 2e-7 to 1.3e-6 and
+// 2.5e-5.
+//
+// Not WIDE, where the caller of a bfloat16 result asks for it: X has two parts, of which
+// products take hi and the linear term a X both; A and B have one.  Then B's rounding is
 // the largest; its diagonal (about -2.7 once the singular values are near 1, against
 // an off-diagonal part of 0.3) is kept apart in float32 and joins the linear term.
 // What is left is 4e-4 to 1.1e-3 of the result's norm in five steps, below
-// bfloat16's own 1.7e-3.
-//
-// WIDE (float32 and float16 results): A and B have two parts too, and a product is
-// three, hi hi + hi lo + lo hi, one after the other into the same float32 sums: 3e-7 to 2e-6
-// in five steps, float32's own steps 2e-7 to 1.3e-6.
+// bfloat16's own 1.7e-3; in ten, 1e-2 to 5e-2 of a spectrum down to 1e-6.
 //
 // X is held times 2^10, A and B times 2^8, so that small elements stay normal numbers
 // and the largest (singular values up to 8, |B| up to 128: the entry point checks the
@@ -315,7 +317,7 @@ struct Update : EpiOrthUpdate {
     }
   }
   __device__ __forceinline__ void finish(int64_t matrix, int r, int c, v4f v, int valid) const {
-    if constexpr (!WIDE)
+    if (!WIDE || out_dtype == LSAMP_DTYPE_BF16)
       finish_as<__bf16>(matrix, r, c, v, valid);
     else if (out_dtype == LSAMP_DTYPE_F32)
       finish_as<float>(matrix, r, c, v, valid);

@@ -496,6 +496,7 @@ class OrthogonalizeArgs(Structure):
         ("eps", c_float),
         ("scale", c_float),
         ("keep", c_float),
+        ("fast", c_int32),
         ("x", c_void_p),
         ("x_stride", c_int64),
         ("x_batch_stride", c_int64),

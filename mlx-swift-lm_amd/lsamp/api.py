@@ -397,7 +397,7 @@ class Context:
     def prepare_orthogonalize(self, x: torch.Tensor, **kw) -> "head.PreparedOrthogonalize":
         """scale orth(x) + keep base, by Newton-Schulz steps
         (lsamp_orthogonalize).  Keywords: steps, coefficients, eps, base, scale,
-        keep, out_dtype, out."""
+        keep, out_dtype, out, fast."""
         return head.PreparedOrthogonalize(self, x, **kw)
 
     def orthogonalize(self, x: torch.Tensor, **kw) -> torch.Tensor:

@@ -420,12 +420,13 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 class PreparedOrthogonalize(PreparedCall):
     """out = scale orth(x) + keep base (lsamp_orthogonalize) for a matrix or a
     stack of them.  `coefficients`: (a, b, c), or one of these for each step.  An
-    optimiser's step has the weights as `base` and `out`."""
+    optimiser's step has the weights as `base` and `out`.  `fast`, for a bfloat16 out:
+    a third of the products, and about 1e-3 of the result's norm off in five steps."""
 
     entry = "lsamp_orthogonalize"
 
     def __init__(self, ctx, x, *, steps=5, coefficients=COEFFICIENTS, eps=1e-7, base=None,
-                 scale=1.0, keep=1.0, out_dtype=None, out=None):
+                 scale=1.0, keep=1.0, out_dtype=None, out=None, fast=False):
         super().__init__(ctx, x.device)
         a = _ffi.OrthogonalizeArgs()
         if x.dim() not in (2, 3) or 0 in x.shape:
@@ -444,7 +445,7 @@ class PreparedOrthogonalize(PreparedCall):
         self.coefficients = (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
         a.steps = steps
         a.coefficients = ctypes.cast(self.coefficients, ctypes.c_void_p)
-        a.eps, a.scale, a.keep = eps, scale, keep
+        a.eps, a.scale, a.keep, a.fast = eps, scale, keep, fast
         a.x, a.x_stride, a.x_batch_stride = self._stack("x", x, x.shape, x.dtype)
         if base is not None:
             a.base, a.base_stride, a.base_batch_stride = self._stack("base", base, x.shape,
