@@ -601,7 +601,9 @@ __global__ __launch_bounds__(WM* WN* GROUPS* kWave, 2) void k_gemm(Plan g, Epi e
       b.template load<false>(dst + A::kBytes, 0, wave, lane);
     }
   };
-  const auto fetch = [&](int slab, int buffer) {
+  // (inlined: called, it would keep both sides and what they hold in scratch memory, and
+  // wait there for a slab's loads before its products)
+  const auto fetch = [&](int slab, int buffer) __attribute__((always_inline)) {
     if constexpr (LOOSE) {
       a.hold(slab0 + slab, g.a.rows, wave, lane);
       b.hold(slab0 + slab, g.b.rows, wave, lane);

@@ -1,5 +1,5 @@
-"""The instructions of liblsamp.so's kernels, for tests of what inline assembly leaves to its
-author."""
+"""The compiled kernels of liblsamp.so as text: what each needs of the device, and its
+instructions, for tests of what inline assembly leaves to its author."""
 from __future__ import annotations
 
 import os
@@ -7,7 +7,7 @@ import re
 import struct
 import subprocess
 import tempfile
-from typing import Iterator, List, NamedTuple, Tuple
+from typing import Dict, Iterator, List, NamedTuple, Tuple
 
 LLVM = "/opt/rocm/llvm/bin"
 MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
@@ -34,6 +34,27 @@ def code_objects(library: str) -> Iterator[bytes]:
 def _run(tool: str, *args: str) -> str:
     return subprocess.run([os.path.join(LLVM, tool), *args], check=True, capture_output=True,
                           text=True).stdout
+
+
+def scratch_bytes(library: str) -> Dict[str, int]:
+    """Bytes of scratch memory a thread, for each kernel (mangled names)."""
+    out = {}
+    with tempfile.TemporaryDirectory() as d:
+        path = os.path.join(d, "code")
+        for code in code_objects(library):
+            with open(path, "wb") as f:
+                f.write(code)
+            name = None
+            for line in _run("llvm-readelf", "--notes", path).splitlines():
+                m = re.match(r"\s+(?:- )?\.(name|private_segment_fixed_size):\s+(\S+)", line)
+                if not m:
+                    continue
+                # (an argument's name is indented further, and no kernel's)
+                if m[1] == "name" and m[2].startswith("_Z"):
+                    name = m[2]
+                elif m[1] == "private_segment_fixed_size":
+                    out[name] = int(m[2])
+    return out
 
 
 class Instruction(NamedTuple):

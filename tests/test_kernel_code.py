@@ -1,5 +1,5 @@
 """CPU tests of the compiled kernels: hazards that the compiler does not see, because the
-instruction that has to wait is written as inline assembly."""
+instruction that has to wait is written as inline assembly, and scratch memory."""
 from __future__ import annotations
 
 import kernel_code as K
@@ -15,3 +15,14 @@ def test_scalar_addresses_of_loads_to_lds():
         stale += [(f.name, f.code[i]) for i in K.stale_addresses(f)]
     assert loads > 1000, "the library's loads to LDS were not found"
     assert not stale, f"{len(stale)} loads, the first {stale[0]}"
+
+
+def test_blocks_operators_use_no_scratch_memory():
+    """8-bit products, norms and orthogonalised updates: no spills, and no called function
+    whose state would lie there."""
+    scratch = K.scratch_bytes(_ffi.LIB_PATH)
+    ours = [k for k in scratch if any(part in k for part in (
+        "k_gemmILi3E", "k_skinnyILi3E", "k_resident", "k_join_int8", "k_norm", "k_quantize",
+        "BatchPlan", "k_start"))]
+    assert len(ours) > 150
+    assert not [(k, scratch[k]) for k in ours if scratch[k]]
