@@ -172,9 +172,13 @@ lsamp_status plan_linear_int8(const lsamp_linear_int8_args* a, void* base, Linea
     P.choice = choose_skinny(m, n, false);
     if (m > kLooseRows) x = packed(ws, P.x, 1);
   } else {
-    // (an instruction's slab of bytes takes what one of 16-bit elements does)
+    // (an instruction's slab of bytes takes what one of 16-bit elements does.  A loose 128 x
+    // 128 tile, every chunk of which may end its row, takes over twice an aligned one's, and
+    // copies are cheaper than pack_us has them: 3.2 keeps it where W is large beside the
+    // products.  So and copied: 301 x 1537 x 32003 92 us and 56, 700 x 1537 x 8195 47 and
+    // 35, 73 x 24997 x 3643 90 and 58; 100 x 300 x 60001 21 and 39, 108 x 933 x 27106 32 and 35)
     P.choice = choose_rows(m, n, slabs_of(k, 1), LSAMP_DTYPE_BF16, ob + (a->residual ? eb : 0),
-                           pack_all(P.x, P.w, 1));
+                           pack_all(P.x, P.w, 1), 3.2);
     if (!is_loose(P.choice)) {
       x = packed(ws, P.x, 1);
       w = packed(ws, P.w, 1);

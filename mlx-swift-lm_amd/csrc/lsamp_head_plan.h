@@ -174,12 +174,14 @@ bool is_loose(const Choice& c) {
   return c.tile == kLoose128 || c.tile == kLoose64 || c.tile == kLoose64x4;
 }
 // For operands of which some are no chunks: loose tiles (about 1.4 times an
-// aligned one's time), or any tile after `pack` microseconds of copies.
-Choice choose_rows(int64_t m, int64_t n, int64_t slabs, int dtype, double bytes, double pack) {
+// aligned one's time; `loose128`: the large one's), or any tile after `pack` microseconds
+// of copies.
+Choice choose_rows(int64_t m, int64_t n, int64_t slabs, int dtype, double bytes, double pack,
+                   double loose128 = 1.4) {
   const Choice best = choose(m, n, slabs, dtype, bytes, true);
   if (pack == 0.0) return best;
   const Choice any = choose(m, n, slabs, dtype, bytes, true, kLooseSmall);
-  return any.us * 1.4 < best.us + pack ? any : best;
+  return any.us * (any.tile == kLoose128 ? loose128 : 1.4) < best.us + pack ? any : best;
 }
 // At most 64 rows are bound by reading the other operand, which the kernels of
 // lsamp_skinny.h do without a detour: 64 columns a work-group where that leaves
