@@ -90,7 +90,9 @@ class Int8DraftHead(DraftHead):
 
     def __init__(self, m: DraftHead):
         self.ctx, self.hidden, self.vocab, self.dtype = m.ctx, m.hidden, m.vocab, m.dtype
-        self.biases, self.norms = m.biases, m.norms
+        # (copies: training goes on in the vectors of the head that it was made from)
+        self.biases = [b.clone() for b in m.biases]
+        self.norms = [(w.clone(), b.clone()) for w, b in m.norms]
         self.weights = [self.ctx.quantize_rows(w) for w in m.weights]
         self.head = self.ctx.quantize_rows(m.head)
 
@@ -100,6 +102,9 @@ class Int8DraftHead(DraftHead):
 
     def logits(self, x: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return self.ctx.linear_int8(self.forward(x), *self.head, out_dtype=dtype)
+
+    def quantized(self) -> "Int8DraftHead":
+        raise TypeError("a quantised head is one already")
 
     def training(self, rows: int) -> "Training":
         raise TypeError("a quantised head is not trained: train the one it was made from")
