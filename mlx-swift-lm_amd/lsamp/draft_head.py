@@ -207,6 +207,19 @@ class Training:
             w.add_(self.grads[f"norm_weight{i}"], alpha=-rate)
             b.add_(self.grads[f"norm_bias{i}"], alpha=-rate)
 
+    def prepare_orthogonal(self, *, fast: bool = False) -> None:
+        """The momenta of update_orthogonal, zero, and its calls (`fast`: as
+        Context.prepare_orthogonalize has it).  The first update makes them; one that is
+        captured into a graph, where every replay would clear them, needs them made
+        before."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("momenta are made outside a capture: call prepare_orthogonal before")
+        m = self.model
+        self.momenta = [torch.zeros(w.shape, device=w.device) for w in m.weights]
+        self.nesterov = [torch.empty_like(v) for v in self.momenta]
+        self.orth = [m.ctx.prepare_orthogonalize(v, base=w, out=w, fast=fast)
+                     for v, w in zip(self.nesterov, m.weights)]
+
     def update_orthogonal(self, rate: float, *, plain_rate: float, momentum: float = 0.95,
                           decay: float = 0.0) -> None:
         """A step with orthogonalised momenta (Muon's) of the blocks' matrices:
@@ -214,11 +227,8 @@ class Training:
             W <- (1 - rate decay) W - rate orth(gradient + momentum M)
         and plain descent of the rest at `plain_rate`."""
         m = self.model
-        if not self.orth:
-            self.momenta = [torch.zeros(w.shape, device=w.device) for w in m.weights]
-            self.nesterov = [torch.empty_like(v) for v in self.momenta]
-            self.orth = [m.ctx.prepare_orthogonalize(v, base=w, out=w)
-                         for v, w in zip(self.nesterov, m.weights)]
+        if not self.orth and m.weights:
+            self.prepare_orthogonal()
         for i, call in enumerate(self.orth):
             grad = self.grads[f"weight{i}"].float()
             self.momenta[i].mul_(momentum).add_(grad)
