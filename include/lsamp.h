@@ -815,7 +815,7 @@ lsamp_status lsamp_layer_norm(lsamp_context* ctx, const lsamp_layer_norm_args* a
  *   d_weight = column sums of d_out xh,  d_bias = column sums of d_out,
  * the sums in float32, in a fixed order, each result rounded once.  `residual` is
  * the gradient that reaches x past the norm (a block's skip path); d_x may be the
- * residual or d_out itself (same address, stride and type). */
+ * residual, d_out or x itself (same address, stride and type). */
 typedef struct lsamp_layer_norm_backward_args {
   int32_t rows;
   int32_t cols;

@@ -86,7 +86,7 @@ lsamp_status plan_norm_backward(const lsamp_layer_norm_backward_args* a, void* b
   P.d_weight = a->d_weight;
   P.d_bias = a->d_bias;
   if (a->d_weight || a->d_bias) {
-    P.chunks = norm_chunks(m, n, a->d_x == a->d_out);
+    P.chunks = norm_chunks(m, n, a->d_x && (a->d_x == a->d_out || a->d_x == a->x));
     P.ld_part = round_up(n, 8);
     if (P.chunks) P.part = ws.take<float>((int64_t)P.chunks * 2 * P.ld_part * 4);
   }

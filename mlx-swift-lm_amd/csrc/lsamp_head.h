@@ -262,7 +262,7 @@ struct Int8Ops {
 };
 // Sums of parts as whole numbers of 32 bits.
 int launch_partial_int8(GemmTile tile, const GemmPlan& g, const EpiPartial& e, void* stream);
-int norm_chunks(int rows, int cols, bool in_place);  // in_place: d_x is d_out
+int norm_chunks(int rows, int cols, bool in_place);  // in_place: d_x is d_out or x
 int launch_norm(const NormPlan& p, int dtype, void* stream);
 int launch_norm_backward(const NormBackwardPlan& p, int dtype, void* stream);
 int launch_quantize(const QuantizePlan& p, int dtype, void* stream);

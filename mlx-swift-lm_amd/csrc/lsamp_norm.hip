@@ -538,8 +538,8 @@ Shape shape_of(int rows, int cols) {
 }
 // Whether the columns' sums are taken beside the rows, in the same launch (forward and
 // gradients of 700 x 4096 16.0 us, with shares and their join 19.6; 768 x 1024 10.9 and 15.6;
-// 1000 x 4096 24 and 21): not where the rows' gradients are written over the d_out that
-// the columns read.
+// 1000 x 4096 24 and 21): not where the rows' gradients are written over the d_out or the x
+// that the columns read.
 bool few(int rows, int cols, bool in_place) { return rows <= kFew && cols <= 4096 && !in_place; }
 int rows_per_group(Shape s) { return s <= kWave4 ? kBlock / kWave : 1; }
 int threads_of(Shape s) { return s >= kWide1 ? 1024 : kBlock; }
@@ -593,7 +593,7 @@ int norm_backward(const NormBackwardPlan& p, hipStream_t st) {
   const dim3 grid(sums && s != kLong ? (unsigned)p.chunks : launched(groups, s));
   const dim3 block((unsigned)threads_of(s));
   if (s == kLong) {
-    // (the sums first: d_x may be d_out itself)
+    // (the sums first: d_x may be d_out or x itself)
     if (sums)
       hipLaunchKernelGGL((k_norm_sums<E>),
                          dim3((unsigned)((p.cols + kBlock - 1) / kBlock), (unsigned)p.chunks),
