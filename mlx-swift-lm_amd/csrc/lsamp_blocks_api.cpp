@@ -231,21 +231,20 @@ lsamp_status check_steps(const float* coefficients, int32_t steps) {
     const auto q = [&](double t) { return std::fabs(b * t + c * t * t); };
     const double end = top * top;
     double most = p(end), poly = q(end);
-    const auto at = [&](double t) {  // a place where a slope may be 0
+    const auto at = [&](double t) {  // a place where a slope may be 0, if it is one
       if (!(t > 0.0 && t < end)) return;
       most = std::max(most, p(t));
       poly = std::max(poly, q(t));
     };
-    if (c != 0.0) {
-      const double d = 9.0 * b * b - 20.0 * a * c;
-      if (d >= 0.0) {
-        at((-3.0 * b + std::sqrt(d)) / (10.0 * c));
-        at((-3.0 * b - std::sqrt(d)) / (10.0 * c));
-      }
-      at(-b / (2.0 * c));
-    } else if (b != 0.0) {
-      at(-a / (3.0 * b));
+    // (the roots of a + 3 b t + 5 c t^2 without a difference of near values, which a small c
+    // would lose one to; 0 or none of them where c is 0)
+    const double d = 9.0 * b * b - 20.0 * a * c;
+    if (d >= 0.0) {
+      const double sum = -0.5 * (3.0 * b + std::copysign(std::sqrt(d), b));
+      at(sum / (5.0 * c));
+      at(a / sum);
     }
+    at(-b / (2.0 * c));
     if (!(most <= kMostValue && poly <= kMostPoly))
       return set_error(LSAMP_ERR_INVALID_ARGUMENT,
                        "coefficients of step %d take singular values of up to %g to %g", i, top, most);
