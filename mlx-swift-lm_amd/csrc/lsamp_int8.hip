@@ -5,8 +5,8 @@
 // Compiled once per element type of bias, residual and out (LSAMP_DT).  The sums
 // are whole numbers of 32 bits (127^2 k, exact for the lengths that the entry
 // point takes); one becomes float32 with a rounding of 2^-24, and its two scales
-// are multiplied first, another.  The tiles are lsamp_gemm.h's and lsamp_skinny.h's:
-// a slab of 128 bytes is 128 steps, an instruction takes 64 steps of a 16 x 16 tile in
+// are multiplied first, another, where that gives a normal number.  The tiles are
+// lsamp_gemm.h's and lsamp_skinny.h's: a slab of 128 bytes is 128 steps, an instruction takes 64 steps of a 16 x 16 tile in
 // the time that it takes 32 of 16-bit elements, so a product moves half the bytes
 // and takes half the time of a 16-bit one on either side of the roofline: 8192 x 4096 x
 // 4096 133 us without a residual (2.07 POP/s; a library product 127), 64 x 2048 x 151936 66,
@@ -27,8 +27,41 @@ struct LinearInt8 : Linear {
   const float* x_scale;
   const float* w_scale;
   __device__ __forceinline__ v4f w_at(int c) const { return load4f(w_scale + c, n - c); }
-  __device__ __forceinline__ v4f scaled(v4i v, float xs, v4f ws) const {
-    return __builtin_convertvector(v, v4f) * (ws * xs);
+  // The smallest and largest magnitude of four scales (past the last column they are 0).
+  struct Range {
+    float low, high;
+  };
+  static __device__ __forceinline__ Range range(v4f ws) {
+    return Range{fminf(fminf(fabsf(ws[0]), fabsf(ws[1])), fminf(fabsf(ws[2]), fabsf(ws[3]))),
+                 fmaxf(fmaxf(fabsf(ws[0]), fabsf(ws[1])), fmaxf(fabsf(ws[2]), fabsf(ws[3])))};
+  }
+  // The sums of N rows by their scales, four columns each.  Two scales of tiny or huge rows
+  // may have a product that is no normal number: the sum then takes the smaller one first,
+  // which leaves it one, for a scale is 2^-126 or more.
+  template <int N>
+  static __device__ __forceinline__ void scale(v4f (&r)[N], const v4i (&v)[N], const float (&xs)[N],
+                                               v4f ws, Range w) {
+    Range x{fabsf(xs[0]), fabsf(xs[0])};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x.low = fminf(x.low, fabsf(xs[i]));
+      x.high = fmaxf(x.high, fabsf(xs[i]));
+      r[i] = __builtin_convertvector(v[i], v4f) * (ws * xs[i]);
+    }
+    if (!(x.low * w.low >= 1.17549435e-38f && x.high * w.high <= 3.4028234e38f)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool less = fabsf(ws[k]) < fabsf(xs[i]);
+          r[i][k] = (float)v[i][k] * (less ? ws[k] : xs[i]) * (less ? xs[i] : ws[k]);
+        }
+    }
+  }
+  static __device__ __forceinline__ v4f scaled(v4i v, float xs, v4f ws) {
+    v4f r[1];
+    scale<1>(r, {v}, {xs}, ws, range(ws));
+    return r[0];
   }
   __device__ __forceinline__ v4f result(v4f v, v4f b, v4f res) const {
     v = activate(activation, softcap, v + b);
@@ -63,6 +96,7 @@ struct LinearInt8 : Linear {
     char* const mine = lds + (wn * WM + wm) * (FN * 1024);
     const int r0 = m0 + wm * (FM * 16) + at.row, c = n0 + wn * (FN * 16) + at.col;
     const v4f b = bias_at(c), ws = c < n ? w_at(c) : v4f{0.f, 0.f, 0.f, 0.f};
+    const Range w = range(ws);
     constexpr int kAhead = 8 / sizeof(S) < FM ? 8 / sizeof(S) : FM;
     Raw res[kAhead][FN];
     float xs[FN];
@@ -94,10 +128,12 @@ struct LinearInt8 : Linear {
       }
       scale_of(j + 1);
       exchange<FN>(v, mine, lane);
+      v4f y[FN];
+      scale<FN>(y, v, s, ws, w);
 #pragma unroll
       for (int i = 0; i < FN; ++i)
         if (r + i * at.kRows < m && c < n)
-          finish(r + i * at.kRows, c, scaled(v[i], s[i], ws), b,
+          finish(r + i * at.kRows, c, y[i], b,
                  __builtin_convertvector(__builtin_bit_cast(v4e, add[i]), v4f));
     }
   }
