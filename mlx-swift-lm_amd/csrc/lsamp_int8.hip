@@ -406,7 +406,12 @@ __global__ __launch_bounds__(kResidentWaves* kWave, 2) void k_resident(ResidentP
         S* const to = (S*)e.out + (int64_t)r * e.ld_out + c0 + c;
         if (c0 + c + 8 <= e.n) {
           const v4i v = *(const v4i*)&lines[r][c];
-          asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1 nt" : : "v"(to), "v"(v) : "memory");
+          // (two wait states before its data may be overwritten, which the compiler does not
+          // know to be a store's)
+          asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1 nt\n\ts_nop 1"
+                       :
+                       : "v"(to), "v"(v)
+                       : "memory");
         } else {
           for (int k = 0; c0 + c + k < e.n; ++k) to[k] = lines[r][c + k];
         }

@@ -63,7 +63,12 @@ __device__ __forceinline__ void store8(E* p, const Eight& x, int valid, bool str
       u32x4 q;
       __builtin_memcpy(&q, (const char*)e + 16 * i, 16);
       if (stream)  // (as a builtin it would be joined with the other store, and lost)
-        asm volatile("global_store_dwordx4 %0, %1, off nt" : : "v"((char*)p + 16 * i), "v"(q) : "memory");
+        // (two wait states before its data may be overwritten, which the compiler does not
+        // know to be a store's)
+        asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1"
+                     :
+                     : "v"((char*)p + 16 * i), "v"(q)
+                     : "memory");
       else
         ((Any16<E>*)p)[i].v = q;
     }

@@ -2,6 +2,7 @@
 instructions, for tests of what inline assembly leaves to its author."""
 from __future__ import annotations
 
+import functools
 import os
 import re
 import struct
@@ -69,8 +70,10 @@ class Function(NamedTuple):
     before: List[List[int]]  # the places an instruction may be reached from
 
 
-def functions(library: str, having: str) -> Iterator[Function]:
-    """The functions of the code objects that have an instruction named `having`."""
+@functools.lru_cache(maxsize=1)
+def _texts(library: str) -> List[Tuple[str, str]]:
+    """Every function's name and instructions."""
+    out = []
     with tempfile.TemporaryDirectory() as d:
         path = os.path.join(d, "code")
         for code in code_objects(library):
@@ -79,8 +82,17 @@ def functions(library: str, having: str) -> Iterator[Function]:
             text = _run("llvm-objdump", "-d", "--no-show-raw-insn", path)
             for part in re.split(r"\n(?=[0-9a-f]{16} <)", text):
                 head = re.match(r"[0-9a-f]{16} <(.*)>:\n", part)
-                if head and having in part:
-                    yield _function(head[1], part[head.end():])
+                if head:
+                    out.append((head[1], part[head.end():]))
+    return out
+
+
+def functions(library: str, having: str, named: str = "") -> Iterator[Function]:
+    """The functions of the code objects that have an instruction named `having`, and `named`
+    in their own names."""
+    for name, text in _texts(library):
+        if having in text and named in name:
+            yield _function(name, text)
 
 
 def _function(name: str, text: str) -> Function:
@@ -154,3 +166,13 @@ def stale_addresses(f: Function, op: str = "global_load_lds", states: int = 5) -
                 if total < states:
                     todo.append((b, total))
     return bad
+
+
+def unsettled_stores(f: Function, flags: Tuple[str, ...], states: int = 2) -> Tuple[int, List[int]]:
+    """The number of stores of 128 bits with these flags, and the places of those that no wait
+    of `states` wait states follows at once: a vector instruction may overwrite their data, if
+    not here then after any change of the code around them."""
+    stores = [i for i, c in enumerate(f.code)
+              if c.op == "global_store_dwordx4" and set(c.args[-1].split()) == {"off", *flags}]
+    return len(stores), [i for i in stores if f.code[i + 1].op != "s_nop"
+                         or waits(f.code[i + 1]) < states]

@@ -17,6 +17,19 @@ def test_scalar_addresses_of_loads_to_lds():
     assert not stale, f"{len(stale)} loads, the first {stale[0]}"
 
 
+def test_data_of_stores_past_the_caches():
+    """A store's data is not overwritten by a vector instruction within two wait states."""
+    for kernels, flags, least in (("k_norm", ("nt",), 50),
+                                  ("k_resident", ("sc0", "sc1", "nt"), 6)):
+        stores, unsettled = 0, []
+        for f in K.functions(_ffi.LIB_PATH, "global_store_dwordx4", kernels):
+            n, bad = K.unsettled_stores(f, flags)
+            stores += n
+            unsettled += [(f.name, f.code[i:i + 2]) for i in bad]
+        assert stores >= least, f"{stores} stores of {kernels} were found"
+        assert not unsettled, f"{len(unsettled)} stores, the first {unsettled[0]}"
+
+
 def test_blocks_operators_use_no_scratch_memory():
     """8-bit products, norms and orthogonalised updates: no spills, and no called function
     whose state would lie there."""
