@@ -6,11 +6,12 @@
 // are whole numbers of 32 bits (127^2 k, exact for the lengths that the entry
 // point takes); one becomes float32 with a rounding of 2^-24, and its two scales
 // are multiplied first, another, where that gives a normal number.  The tiles are
-// lsamp_gemm.h's and lsamp_skinny.h's: a slab of 128 bytes is 128 steps, an instruction takes 64 steps of a 16 x 16 tile in
-// the time that it takes 32 of 16-bit elements, so a product moves half the bytes
-// and takes half the time of a 16-bit one on either side of the roofline: 8192 x 4096 x
-// 4096 133 us without a residual (2.07 POP/s; a library product 127), 64 x 2048 x 151936 66,
-// one row of it 55 (5.7 TB/s).
+// lsamp_gemm.h's and lsamp_skinny.h's: a slab of 128 bytes is 128 steps, an instruction
+// takes 64 steps of a 16 x 16 tile in the time that it takes 32 of 16-bit elements, so a
+// product moves half the bytes and takes half the time of a 16-bit one on either side of
+// the roofline: 8192 x 4096 x 4096 130 to 133 us without a residual (2.1 POP/s; a library
+// product 127), 64 x 2048 x 151936 65, one row of it 55 (5.7 TB/s).  Rows of W that are
+// no 16-byte chunks cost more (301 x 1537 x 2053 12 us, 304 x 1536 x 2048 7).
 #include <hip/hip_runtime.h>
 
 #include "lsamp_epilogue.h"

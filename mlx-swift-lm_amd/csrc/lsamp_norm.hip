@@ -223,8 +223,9 @@ __global__ __launch_bounds__(Rows<THREADS>::kGroup) void k_norm(NormPlan p) {
 // stay in registers over its rows; the next row is on its way meanwhile (16384 x 4096 bf16
 // with a residual 108 us, 4.9 TB/s; 171 without the next row).  1024 threads
 // have 128 registers each: their sums lie in LDS, a thread's own 16 bytes beside its
-// neighbours', and float32 rows are not fetched ahead (4096 x 16384 bf16: 433 us with the
-// sums in registers, spilled; 111 so).  LONG: d_x only, each row read twice.
+// neighbours', and rows of more than 8,192 elements are not fetched ahead (4096 x 16384
+// bf16: 433 us with the sums in registers, spilled; 111 so).  LONG: d_x only, each row
+// read twice.
 template <typename E, int THREADS, int V, bool SUMS, bool LONG>
 __device__ __forceinline__ void backward_rows(const NormBackwardPlan& p, const Rows<THREADS>& rows) {
   static_assert(!(SUMS && LONG), "a long row's sums are another kernel's");
@@ -413,9 +414,9 @@ __global__ __launch_bounds__(kBlock) void k_norm_sums(NormBackwardPlan p) {
   part[p.ld_part + c] = b;
 }
 
-// Few rows (301 x 1537 f16 4.2 us, shares and their join 10.4): one launch, whose first `rows_groups` work-groups take rows and the others
-// 16 columns each, which they read from the L2 once more: 16 threads a column take rows
-// in turn.
+// Few rows (301 x 1537 f16 4.2 us, shares and their join 10.4): one launch, whose first
+// `row_groups` work-groups take rows and the others 16 columns each, which they read from
+// the L2 once more: 16 threads a column take rows in turn.
 template <typename E>
 __device__ __forceinline__ void columns(const NormBackwardPlan& p, int group) {
   __shared__ float red[2][16][17];

@@ -152,9 +152,9 @@ __device__ __forceinline__ v4e turned(v4e in, int lane) {
   return __builtin_bit_cast(v4e, o);
 }
 
-// A tile and its mirror image (A of 4096 x 4096 82 us, of which the products of 64 slabs are
-// 64; B 87): what is stored at (r, c) is stored at (c, r) too,
-// unless the tile lies on the diagonal.  `value(r, c, sums)` gives four columns' results.
+// A tile and its mirror image (A of 4096 x 4096, one part 75 us, two 213; B 80 and 223; A
+// and B of 2048 x 2048 in two parts 60 each): what is stored at (r, c) is stored at (c, r)
+// too, unless the tile lies on the diagonal.  `value(r, c, sums)` gives four columns' results.
 template <bool WIDE>
 struct Symmetric : EpiSymmetric {
   static constexpr int kBarriers = 0;
@@ -233,7 +233,8 @@ struct Poly : Symmetric<WIDE> {
 };
 
 // X' = (a + diagonal) X + sums, as the next X or, at the last step, the result.  4096 x 4096
-// 125 to 135 us: 96 of products, then 134 MB that nothing hides (one tile a CU).
+// of one part 125 us, 96 of them products, then 134 MB that nothing hides (one tile a CU);
+// of two 304.
 template <bool WIDE>
 struct Update : EpiOrthUpdate {
   static constexpr int kBarriers = 0;

@@ -412,8 +412,9 @@ class PreparedLinearInt8(PreparedCall):
         return {"out": self.out}
 
 
-# The quintic of the Newton-Schulz steps: its slope at 0 is as steep as it gets while
-# every singular value ends within (0.7, 1.2).
+# The quintic of the Newton-Schulz steps, steep at 0: in five steps singular values from
+# 0.01 to 1 (of the matrix's norm) end within (0.68, 1.14), one of 0.003 at 1.11, of 0.001 at
+# 0.47 and of 0.0001 at 0.05.
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
