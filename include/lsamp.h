@@ -792,7 +792,8 @@ lsamp_status lsamp_dropout(lsamp_context* ctx, const lsamp_dropout_args* args, v
  *   mean = sum x / cols;  rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps);
  *   out = (x - mean) rstd weight + bias.
  * `out` may be x itself (same address, stride and type) where no gradient is
- * taken.  A NaN or an infinity makes its row NaN and changes no other. */
+ * taken.  A NaN or an infinity makes its row NaN and changes no other.  (A row whose
+ * squared deviations sum to more than float32 holds, as of values past 1e18, has rstd 0.) */
 typedef struct lsamp_layer_norm_args {
   int32_t rows;
   int32_t cols;
